@@ -53,6 +53,8 @@ extern "C" {
 #define STK_STATUS_WAIT_TIMEOUT 1
 #define STK_STATUS_BAD_BLOCK_ID 2
 #define STK_STATUS_SHAPE_OVERFLOW 3
+#define STK_STATUS_BAD_POSITION 4 /* a rotary position outside the table */
+#define STK_STATUS_BAD_LENGTH 5   /* a length outside the request's blocks */
 
 /* block-state job modes */
 #define STK_MODE_FULL 0   /* (m, l, u) per block */
@@ -421,6 +423,70 @@ STK_API int stk_group_attention(const stk_kv* kv, const void* q, int q_dtype, in
  * Replaces kernels.py:553-560 touch_kv() (_touch, kernels.py:250-260).
  * out [rows, s, ceil(b * d / 1024)] FP32. */
 STK_API int stk_touch_kv(const stk_kv* kv, int rows, int hq, const void* ids, int ids64, int s, float* out, void* stream);
+
+/* Rotary position table: cos / sin [max_position, pairs] FP32. Pair p of a
+ * head is its dims (p, p + pairs), or (2p, 2p + 1) with interleaved; dims from
+ * 2 * pairs on are not rotated. axis [pairs] (NULL: one axis) names the row of
+ * positions [axes, T] that turns each pair (time, height, width of a video). */
+typedef struct stk_rotary {
+  const float* cos;
+  const float* sin;
+  int pairs;
+  int max_position;
+  int interleaved;
+  int axes;
+  const uint8_t* axis;
+} stk_rotary;
+
+/* Append T new tokens (packed request after request, request r's at
+ * token_offsets[r] .. token_offsets[r + 1]; NULL: one token per request) to a
+ * paged cache of `pages` pages: request r's new token i becomes token
+ * lengths[r] + i. Keys (and queries q [T, hq, d] into q_out, contiguous) are
+ * rotated on the way by positions [axes, T] (NULL: the token's place), keys
+ * and values [T, hkv, d] are written to their page slots and the bounds lo /
+ * hi of their blocks (NULL: none kept) are folded over the stored keys; a
+ * block's first token resets its bounds. rotary NULL: no rotation. Inputs
+ * have the cache's type and unit stride along d; strides are in elements. A
+ * token beyond its request's blocks is not written and a position outside
+ * the table is taken as 0; both are reported in status. New: the reference
+ * starts from a filled cache. */
+STK_API int stk_append_tokens(const stk_kv* kv, int pages, int R, int total_blocks, int T, const void* k_new,
+                              long long k_token_stride, long long k_head_stride, const void* v_new,
+                              long long v_token_stride, long long v_head_stride, const void* q,
+                              long long q_token_stride, long long q_head_stride, int hq, void* q_out,
+                              const int32_t* lengths, const int32_t* token_offsets, const int32_t* positions,
+                              const stk_rotary* rotary, float* lo, float* hi, int32_t* status, void* stream);
+
+/* Scores of stk_paged_attention: s = scale q.k (scale 0: d^-1/2), then
+ * s = softcap tanh(s / softcap) (0: none), then s -= slopes[h] |pos - j|
+ * (NULL: none), for keys kv_lo[t] <= j < kv_hi[t] (NULL: 0 and pos + 1,
+ * causal), pos = the token's place in its request. */
+typedef struct stk_attention_options {
+  float scale;
+  float softcap;
+  const float* slopes;  /* [hq] */
+  const int32_t* kv_lo; /* [T] */
+  const int32_t* kv_hi; /* [T] */
+} stk_attention_options;
+
+/* Workspace (bytes) for stk_paged_attention of the same sizes. */
+STK_API size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int T, int hq, int has_offsets,
+                                                   int max_length, int prefix);
+
+/* Dense attention of T packed tokens (the last ones of their requests) over a
+ * paged cache that holds lengths[r] tokens of request r, at most max_length:
+ * prompts, pieces of prompts, several drafted tokens or one token per
+ * request. q [T, hq, d] has the cache's type; out [T, hq, d] (contiguous, the
+ * same type) is zero where a row's keys are empty, lse [T, hq] (or NULL) the
+ * log-sum-exp of the row's scores (-inf there). prefix > 0: the first prefix
+ * tokens (whole pages) of every request are the same pages (those of request
+ * 0's table are read), attended once for all requests' tokens and joined
+ * with each request's own rest. New: the reference attends block lists only. */
+STK_API int stk_paged_attention(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
+                                long long q_head_stride, int R, int T, int hq, const int32_t* lengths,
+                                const int32_t* token_offsets, int max_length, int prefix,
+                                const stk_attention_options* options, void* out, float* lse, void* workspace,
+                                size_t workspace_bytes, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

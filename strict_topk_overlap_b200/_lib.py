@@ -35,6 +35,7 @@ SYMBOLS = (
     "stk_decode_step_workspace_bytes", "stk_decode_step", "stk_build_metadata", "stk_append_token",
     "stk_predict", "stk_group_repair_saved_workspace_bytes", "stk_group_repair_saved",
     "stk_group_attention_workspace_bytes", "stk_group_attention", "stk_touch_kv",
+    "stk_append_tokens", "stk_paged_attention_workspace_bytes", "stk_paged_attention",
 )
 
 
@@ -56,10 +57,21 @@ class StkRepairOut(C.Structure):
                 ("extra", C.c_void_p), ("positive_jobs", C.c_void_p), ("total_jobs", C.c_void_p)]
 
 
+class StkRotary(C.Structure):
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("pairs", C.c_int), ("max_position", C.c_int),
+                ("interleaved", C.c_int), ("axes", C.c_int), ("axis", C.c_void_p)]
+
+
+class StkAttentionOptions(C.Structure):
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("slopes", C.c_void_p), ("kv_lo", C.c_void_p),
+                ("kv_hi", C.c_void_p)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _F = C.c_float
 _SZ = C.c_size_t
+_LL = C.c_longlong
 _SIGS = {
     "stk_abi_version": (_I, []),
     "stk_last_error": (C.c_char_p, []),
@@ -98,6 +110,11 @@ _SIGS = {
     "stk_group_attention_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "stk_group_attention": (_I, [C.POINTER(StkKV), _P, _I, _I, _P, _I, _P, _P, _SZ, _P, _P]),
     "stk_touch_kv": (_I, [C.POINTER(StkKV), _I, _I, _P, _I, _I, _P, _P]),
+    "stk_append_tokens": (_I, [C.POINTER(StkKV), _I, _I, _I, _I, _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _I, _P, _P,
+                               _P, _P, C.POINTER(StkRotary), _P, _P, _P, _P]),
+    "stk_paged_attention_workspace_bytes": (_SZ, [C.POINTER(StkKV), _I, _I, _I, _I, _I, _I]),
+    "stk_paged_attention": (_I, [C.POINTER(StkKV), _I, _P, _LL, _LL, _I, _I, _I, _P, _P, _I, _I,
+                                 C.POINTER(StkAttentionOptions), _P, _P, _P, _SZ, _P, _P]),
 }
 
 _lock = threading.Lock()

@@ -12,6 +12,7 @@
 #include <string>
 
 #include "internal.cuh"
+#include "paged_ops.cuh"
 #include "../../include/strict_topk_b200.h"
 
 
@@ -867,4 +868,150 @@ extern "C" int stk_select_topk_static(const void* q, int q_dtype, const float* l
   // shared array has to start at zero.
   return stk_select_topk(q, q_dtype, lo, hi, R, hq, hmeta, n, block_offsets, total_blocks, max_blocks, d, topk,
                          group_select, id_base, ids_out, keys_out, scratch, have, status, stream);
+}
+
+// ----------------------------------------------------------------------------- paged tokens and dense attention
+
+extern "C" int stk_append_tokens(const stk_kv* kv, int pages, int R, int total_blocks, int T, const void* k_new,
+                                 long long k_token_stride, long long k_head_stride, const void* v_new,
+                                 long long v_token_stride, long long v_head_stride, const void* q,
+                                 long long q_token_stride, long long q_head_stride, int hq, void* q_out,
+                                 const int32_t* lengths, const int32_t* token_offsets, const int32_t* positions,
+                                 const stk_rotary* rotary, float* lo, float* hi, int32_t* status, void* stream) {
+  const int rc = check_kv(kv, q ? hq : (kv ? kv->hkv : 1));
+  if (rc) return rc;
+  if (!kv->page_table || !kv->block_offsets) return fail(STK_EINVAL, "a paged cache is expected");
+  if (T > 0 && (!k_new || !v_new || !lengths)) return fail(STK_EINVAL, "null pointer");
+  if (T > 0 && q && !q_out) return fail(STK_EINVAL, "q needs q_out");
+  if ((lo == nullptr) != (hi == nullptr)) return fail(STK_EINVAL, "lo and hi go together");
+  if (pages <= 0 || R <= 0 || T < 0 || total_blocks <= 0 || (!token_offsets && T != R))
+    return fail(STK_EINVAL, "bad append shape R=%d T=%d pages=%d", R, T, pages);
+  if (T == 0) return 0;
+  AppendArgs a{};
+  a.L = make_layout(kv);
+  a.pages = pages; a.R = R; a.T = T; a.hq = hq;
+  a.k = k_new; a.v = v_new; a.q = q; a.q_out = q_out;
+  a.k_ts = k_token_stride; a.k_hs = k_head_stride;
+  a.v_ts = v_token_stride; a.v_hs = v_head_stride;
+  a.q_ts = q_token_stride; a.q_hs = q_head_stride;
+  a.lengths = lengths; a.token_offsets = token_offsets;
+  if (rotary) {
+    if (!rotary->cos || !rotary->sin || rotary->pairs <= 0 || 2 * rotary->pairs > kv->d || rotary->max_position <= 0)
+      return fail(STK_EINVAL, "bad rotary table (pairs=%d of head dim %d)", rotary->pairs, kv->d);
+    if (rotary->axes < 1 || rotary->axes > 255 || (rotary->axis && !positions))
+      return fail(STK_EINVAL, "several rotary axes need positions [axes, T]");
+    a.cos = rotary->cos; a.sin = rotary->sin; a.pairs = rotary->pairs; a.max_position = rotary->max_position;
+    a.interleaved = rotary->interleaved; a.axes = rotary->axes; a.axis = rotary->axis; a.positions = positions;
+  }
+  a.lo = lo; a.hi = hi; a.total = total_blocks; a.status = status;
+  return cuda_status(launch_append_tokens(a, kv->kv_dtype, static_cast<cudaStream_t>(stream)), "append_tokens");
+}
+
+namespace {
+// How a paged attention call runs: one phase over the requests' own keys and,
+// behind a shared prefix, one before it over the prefix; each in nsplit parts
+// of its tiles' key ranges. Everything follows from host sizes, so that the
+// workspace size and the launches agree and a captured graph fits any
+// lengths up to the cache's capacity.
+struct AttnPhase {
+  int nsplit;
+  int span_lo, span_hi, shared;
+};
+struct AttnPlan {
+  AttnPhase phase[2];
+  int phases;
+  bool join;
+  size_t bytes;
+};
+
+int row_splits(int R, int T, int G, bool offsets, bool shared, int hkv, int keys) {
+  const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared, 16)) * hkv;
+  const long long most = (keys + 63) / 64;  // one run of every warp
+  long long n = 2ll * sm_count_current() / tiles;
+  n = n < most ? n : most;
+  return static_cast<int>(n < 1 ? 1 : n);
+}
+
+AttnPlan plan_attention(const stk_kv* kv, int R, int T, int hq, bool offsets, int max_length, int prefix) {
+  AttnPlan p{};
+  const int G = hq / kv->hkv;
+  if (prefix > 0) {
+    // All requests' tokens as one request over the prefix's pages.
+    p.phase[0] = {row_splits(R, T, G, offsets, true, kv->hkv, prefix), 0, prefix, 1};
+    p.phase[1] = {row_splits(R, T, G, offsets, false, kv->hkv, max_length - prefix), prefix, 0x7fffffff, 0};
+    p.phases = 2;
+  } else {
+    p.phase[0] = {row_splits(R, T, G, offsets, false, kv->hkv, max_length), 0, 0x7fffffff, 0};
+    p.phases = 1;
+  }
+  p.join = p.phases > 1 || p.phase[0].nsplit > 1;
+  if (p.join)
+    for (int i = 0; i < p.phases; ++i)
+      p.bytes += static_cast<size_t>(p.phase[i].nsplit) * T * hq * (kv->d + 2) * sizeof(float);
+  return p;
+}
+
+int check_attention(const stk_kv* kv, int R, int T, int hq, bool offsets, int max_length, int prefix) {
+  const int rc = check_kv(kv, hq);
+  if (rc) return rc;
+  if (!kv->page_table || !kv->block_offsets) return fail(STK_EINVAL, "a paged cache is expected");
+  if (R <= 0 || T < 0 || max_length <= 0 || (!offsets && T != R))
+    return fail(STK_EINVAL, "bad attention shape R=%d T=%d max_length=%d", R, T, max_length);
+  if (static_cast<long long>(T) * hq > 0x7fffffff) return fail(STK_EINVAL, "too many query rows");
+  if (prefix < 0 || prefix > max_length || prefix % kv->page_size)
+    return fail(STK_EINVAL, "shared prefix of %d tokens: whole pages of at most %d tokens are expected", prefix,
+                max_length);
+  return 0;
+}
+}  // namespace
+
+extern "C" size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int T, int hq, int has_offsets,
+                                                      int max_length, int prefix) {
+  if (check_attention(kv, R, T, hq, has_offsets != 0, max_length, prefix) || T == 0) return 0;
+  return plan_attention(kv, R, T, hq, has_offsets != 0, max_length, prefix).bytes;
+}
+
+extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
+                                   long long q_head_stride, int R, int T, int hq, const int32_t* lengths,
+                                   const int32_t* token_offsets, int max_length, int prefix,
+                                   const stk_attention_options* options, void* out, float* lse, void* workspace,
+                                   size_t workspace_bytes, int32_t* status, void* stream) {
+  const int rc = check_attention(kv, R, T, hq, token_offsets != nullptr, max_length, prefix);
+  if (rc) return rc;
+  if (T == 0) return 0;
+  if (!q || !lengths || !out || pages <= 0) return fail(STK_EINVAL, "null pointer or empty pool");
+  if (options && (!(options->softcap >= 0.f) || !(options->scale >= 0.f)))
+    return fail(STK_EINVAL, "scale and softcap must not be negative");
+  const AttnPlan p = plan_attention(kv, R, T, hq, token_offsets != nullptr, max_length, prefix);
+  if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return fail(STK_EWS, "attention workspace too small");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  PagedAttnArgs a{};
+  a.L = make_layout(kv);
+  a.pages = pages; a.R = R; a.T = T; a.hq = hq; a.G = hq / kv->hkv; a.d = kv->d;
+  a.q = q; a.q_ts = q_token_stride; a.q_hs = q_head_stride; a.out = out; a.lse = lse;
+  a.lengths = lengths; a.token_offsets = token_offsets;
+  a.scale = attn_scale(kv->d);
+  if (options) {
+    if (options->scale > 0.f) a.scale = options->scale;
+    a.softcap = options->softcap; a.slopes = options->slopes;
+    a.kv_lo = options->kv_lo; a.kv_hi = options->kv_hi;
+  }
+  a.status = status;
+  JoinArgs j{};
+  j.rows = T * hq; j.d = kv->d; j.dtype = kv->kv_dtype; j.out = out; j.lse = lse; j.nsrc = p.phases;
+  float* at = static_cast<float*>(workspace);
+  for (int i = 0; i < p.phases; ++i) {
+    const AttnPhase& ph = p.phase[i];
+    a.span_lo = ph.span_lo; a.span_hi = ph.span_hi; a.shared = ph.shared; a.nsplit = ph.nsplit;
+    if (p.join) {
+      const size_t states = static_cast<size_t>(ph.nsplit) * j.rows;
+      a.part_o = at;
+      a.part_ml = reinterpret_cast<float2*>(at + states * kv->d);
+      at += states * (kv->d + 2);
+      j.src[i] = {a.part_ml, a.part_o, ph.nsplit};
+    }
+    const int r2 = launch_rows_attn(a, kv->kv_dtype, st);
+    if (r2) return cuda_status(r2, "paged attention");
+  }
+  return p.join ? cuda_status(launch_join(j, st), "attention join") : 0;
 }
