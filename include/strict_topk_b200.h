@@ -471,10 +471,11 @@ typedef struct stk_attention_options {
 
 /* Workspace (bytes) for stk_paged_attention of the same sizes. */
 STK_API size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int T, int hq, int has_offsets,
-                                                   int max_length, int prefix);
+                                                   int max_tokens, int max_length, int prefix);
 
 /* Dense attention of T packed tokens (the last ones of their requests) over a
- * paged cache that holds lengths[r] tokens of request r, at most max_length:
+ * paged cache that holds lengths[r] tokens of request r, at most max_length
+ * (a request's new tokens: at most max_tokens, which chooses the kernel):
  * prompts, pieces of prompts, several drafted tokens or one token per
  * request. q [T, hq, d] has the cache's type; out [T, hq, d] (contiguous, the
  * same type) is zero where a row's keys are empty, lse [T, hq] (or NULL) the
@@ -484,7 +485,7 @@ STK_API size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int 
  * with each request's own rest. New: the reference attends block lists only. */
 STK_API int stk_paged_attention(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
                                 long long q_head_stride, int R, int T, int hq, const int32_t* lengths,
-                                const int32_t* token_offsets, int max_length, int prefix,
+                                const int32_t* token_offsets, int max_tokens, int max_length, int prefix,
                                 const stk_attention_options* options, void* out, float* lse, void* workspace,
                                 size_t workspace_bytes, int32_t* status, void* stream);
 

@@ -112,8 +112,8 @@ _SIGS = {
     "stk_touch_kv": (_I, [C.POINTER(StkKV), _I, _I, _P, _I, _I, _P, _P]),
     "stk_append_tokens": (_I, [C.POINTER(StkKV), _I, _I, _I, _I, _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _I, _P, _P,
                                _P, _P, C.POINTER(StkRotary), _P, _P, _P, _P]),
-    "stk_paged_attention_workspace_bytes": (_SZ, [C.POINTER(StkKV), _I, _I, _I, _I, _I, _I]),
-    "stk_paged_attention": (_I, [C.POINTER(StkKV), _I, _P, _LL, _LL, _I, _I, _I, _P, _P, _I, _I,
+    "stk_paged_attention_workspace_bytes": (_SZ, [C.POINTER(StkKV), _I, _I, _I, _I, _I, _I, _I]),
+    "stk_paged_attention": (_I, [C.POINTER(StkKV), _I, _P, _LL, _LL, _I, _I, _I, _P, _P, _I, _I, _I,
                                  C.POINTER(StkAttentionOptions), _P, _P, _P, _SZ, _P, _P]),
 }
 

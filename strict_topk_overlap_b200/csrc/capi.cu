@@ -138,7 +138,8 @@ int stk_device_sm_count(int device) {
 int stk_set_wait_limit_ns(unsigned long long ns) {
   if (ns == 0) return fail(STK_EINVAL, "the wait limit must be positive");
   int (*const setters[])(unsigned long long) = {set_wait_limit_select, set_wait_limit_states, set_wait_limit_repair,
-                                                set_wait_limit_attend, set_wait_limit_group_mma, set_wait_limit_step};
+                                                set_wait_limit_attend, set_wait_limit_group_mma, set_wait_limit_step,
+                                                set_wait_limit_prompt};
   for (auto set : setters) {
     const int rc = set(ns);
     if (rc) return cuda_status(rc, "set wait limit");
@@ -914,6 +915,7 @@ namespace {
 // workspace size and the launches agree and a captured graph fits any
 // lengths up to the cache's capacity.
 struct AttnPhase {
+  bool prompt;  // the tensor-core kernel, else the FP32-unit one
   int nsplit;
   int span_lo, span_hi, shared;
 };
@@ -924,39 +926,47 @@ struct AttnPlan {
   size_t bytes;
 };
 
-int row_splits(int R, int T, int G, bool offsets, bool shared, int hkv, int keys) {
-  const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared, 16)) * hkv;
-  const long long most = (keys + 63) / 64;  // one run of every warp
-  long long n = 2ll * sm_count_current() / tiles;
+AttnPhase plan_phase(int R, int T, int G, bool offsets, bool shared, int hkv, int max_tokens, int keys, bool tensor) {
+  AttnPhase p{};
+  p.shared = shared;
+  // A tile of 16 rows holds a request's rows of one KV head: nothing to gain from 256-row tiles.
+  const long long rows = static_cast<long long>(shared ? T : max_tokens) * G;
+  p.prompt = tensor && rows > 16;
+  const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared, p.prompt ? 256 : 16)) * hkv;
+  const long long ctas = p.prompt ? sm_count_current() : 2ll * sm_count_current();
+  const long long most = p.prompt ? (keys + 255) / 256 : (keys + 63) / 64;
+  long long n = ctas / tiles;
   n = n < most ? n : most;
-  return static_cast<int>(n < 1 ? 1 : n);
+  p.nsplit = static_cast<int>(n < 1 ? 1 : n);
+  return p;
 }
 
-AttnPlan plan_attention(const stk_kv* kv, int R, int T, int hq, bool offsets, int max_length, int prefix) {
+AttnPlan plan_attention(const stk_kv* kv, int R, int T, int hq, bool offsets, int max_tokens, int max_length,
+                        int prefix, bool tensor) {
   AttnPlan p{};
   const int G = hq / kv->hkv;
   if (prefix > 0) {
-    // All requests' tokens as one request over the prefix's pages.
-    p.phase[0] = {row_splits(R, T, G, offsets, true, kv->hkv, prefix), 0, prefix, 1};
-    p.phase[1] = {row_splits(R, T, G, offsets, false, kv->hkv, max_length - prefix), prefix, 0x7fffffff, 0};
-    p.phases = 2;
-  } else {
-    p.phase[0] = {row_splits(R, T, G, offsets, false, kv->hkv, max_length), 0, 0x7fffffff, 0};
+    p.phase[0] = plan_phase(R, T, G, offsets, true, kv->hkv, max_tokens, prefix, tensor);
+    p.phase[0].span_hi = prefix;
     p.phases = 1;
   }
-  p.join = p.phases > 1 || p.phase[0].nsplit > 1;
+  AttnPhase& own = p.phase[p.phases++];
+  own = plan_phase(R, T, G, offsets, false, kv->hkv, max_tokens, max_length - prefix, tensor);
+  own.span_lo = prefix;
+  own.span_hi = 0x7fffffff;
+  p.join = p.phases > 1 || own.nsplit > 1;
   if (p.join)
     for (int i = 0; i < p.phases; ++i)
       p.bytes += static_cast<size_t>(p.phase[i].nsplit) * T * hq * (kv->d + 2) * sizeof(float);
   return p;
 }
 
-int check_attention(const stk_kv* kv, int R, int T, int hq, bool offsets, int max_length, int prefix) {
+int check_attention(const stk_kv* kv, int R, int T, int hq, bool offsets, int max_tokens, int max_length, int prefix) {
   const int rc = check_kv(kv, hq);
   if (rc) return rc;
   if (!kv->page_table || !kv->block_offsets) return fail(STK_EINVAL, "a paged cache is expected");
-  if (R <= 0 || T < 0 || max_length <= 0 || (!offsets && T != R))
-    return fail(STK_EINVAL, "bad attention shape R=%d T=%d max_length=%d", R, T, max_length);
+  if (R <= 0 || T < 0 || max_length <= 0 || (!offsets && T != R) || (T > 0 && (max_tokens <= 0 || max_tokens > T)))
+    return fail(STK_EINVAL, "bad attention shape R=%d T=%d max_tokens=%d max_length=%d", R, T, max_tokens, max_length);
   if (static_cast<long long>(T) * hq > 0x7fffffff) return fail(STK_EINVAL, "too many query rows");
   if (prefix < 0 || prefix > max_length || prefix % kv->page_size)
     return fail(STK_EINVAL, "shared prefix of %d tokens: whole pages of at most %d tokens are expected", prefix,
@@ -966,23 +976,30 @@ int check_attention(const stk_kv* kv, int R, int T, int hq, bool offsets, int ma
 }  // namespace
 
 extern "C" size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int T, int hq, int has_offsets,
-                                                      int max_length, int prefix) {
-  if (check_attention(kv, R, T, hq, has_offsets != 0, max_length, prefix) || T == 0) return 0;
-  return plan_attention(kv, R, T, hq, has_offsets != 0, max_length, prefix).bytes;
+                                                      int max_tokens, int max_length, int prefix) {
+  const bool offsets = has_offsets != 0;
+  if (check_attention(kv, R, T, hq, offsets, max_tokens, max_length, prefix) || T == 0) return 0;
+  // Enough whichever kernel the addresses of the call lead to.
+  const size_t a = plan_attention(kv, R, T, hq, offsets, max_tokens, max_length, prefix, true).bytes;
+  const size_t b = plan_attention(kv, R, T, hq, offsets, max_tokens, max_length, prefix, false).bytes;
+  return a > b ? a : b;
 }
 
 extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
                                    long long q_head_stride, int R, int T, int hq, const int32_t* lengths,
-                                   const int32_t* token_offsets, int max_length, int prefix,
+                                   const int32_t* token_offsets, int max_tokens, int max_length, int prefix,
                                    const stk_attention_options* options, void* out, float* lse, void* workspace,
                                    size_t workspace_bytes, int32_t* status, void* stream) {
-  const int rc = check_attention(kv, R, T, hq, token_offsets != nullptr, max_length, prefix);
+  const int rc = check_attention(kv, R, T, hq, token_offsets != nullptr, max_tokens, max_length, prefix);
   if (rc) return rc;
   if (T == 0) return 0;
   if (!q || !lengths || !out || pages <= 0) return fail(STK_EINVAL, "null pointer or empty pool");
   if (options && (!(options->softcap >= 0.f) || !(options->scale >= 0.f)))
     return fail(STK_EINVAL, "scale and softcap must not be negative");
-  const AttnPlan p = plan_attention(kv, R, T, hq, token_offsets != nullptr, max_length, prefix);
+  const bool tensor =
+      prompt_attn_takes(kv->kv_dtype, kv->d, kv->page_size, kv->k, kv->v, q, q_token_stride, q_head_stride);
+  const AttnPlan p =
+      plan_attention(kv, R, T, hq, token_offsets != nullptr, max_tokens, max_length, prefix, tensor);
   if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return fail(STK_EWS, "attention workspace too small");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   PagedAttnArgs a{};
@@ -1010,7 +1027,7 @@ extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, l
       at += states * (kv->d + 2);
       j.src[i] = {a.part_ml, a.part_o, ph.nsplit};
     }
-    const int r2 = launch_rows_attn(a, kv->kv_dtype, st);
+    const int r2 = ph.prompt ? launch_prompt_attn(a, kv->kv_dtype, st) : launch_rows_attn(a, kv->kv_dtype, st);
     if (r2) return cuda_status(r2, "paged attention");
   }
   return p.join ? cuda_status(launch_join(j, st), "attention join") : 0;

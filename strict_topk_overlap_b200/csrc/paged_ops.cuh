@@ -167,6 +167,11 @@ __device__ __forceinline__ int page_of(const PagedAttnArgs& a, int rp, int j) {
 
 int launch_append_tokens(const AppendArgs& a, int kv_dtype, cudaStream_t stream);
 int launch_rows_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream);
+// Whether the tensor-core kernel takes these types, sizes and addresses.
+bool prompt_attn_takes(int kv_dtype, int d, int page_size, const void* k, const void* v, const void* q, long long q_ts,
+                       long long q_hs);
+int launch_prompt_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream);
+int set_wait_limit_prompt(unsigned long long ns);
 
 // One set of partial softmax states to be joined: part s of row `row` at
 // ml[s * rows + row], o[(s * rows + row) * d].

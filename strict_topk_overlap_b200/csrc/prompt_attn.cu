@@ -1,0 +1,665 @@
+// Dense paged attention of many rows on the tensor cores (tcgen05): prompts,
+// pieces of prompts, and all requests' tokens over a shared prefix.
+//
+// The rows of one KV head (new tokens x query heads of the group, packed) are
+// cut into tiles of 256, two MMA tiles of 128. Per 128 keys:
+//   S = Q K^T          128 x 128, FP32 in tensor memory (TMEM)
+//   P = 2^(c S - m)    one thread per row: cap, bias, mask, running maximum
+//                      and sum in FP32; P rounded to the type, over S in TMEM
+//   O += P V           FP32 in TMEM, P the TMEM operand
+// Warps 0-3 and 4-7 are the softmax of the two MMA tiles, warp 8 issues the
+// MMAs (one tile's products run while the other tile's weights are formed),
+// warp 9 feeds a ring of K and V tiles by TMA, one box per page and 64 dims,
+// swizzled as the MMA reads them.
+//
+// Rounding: P has the type's precision (relative 2^-9 or 2^-12 on average of
+// a weight, about the output's own rounding); the maximum used may be up to
+// 2^8 below the true one, so that O is rescaled only when it grew by more,
+// which leaves P at most 2^8, inside both types' ranges.
+//
+// Tensor-bound in principle: per 128 x 128 x D tile 4 * 128 * 128 * D FLOP.
+//
+// Keys that no row of a tile sees are not read; tiles whose keys all rows see
+// skip the mask. Slots past the request's tokens may hold anything: K's are
+// masked and V's are zeroed in shared memory. A value that is not finite at a
+// key some rows of a tile see and others do not turns the others' sums into
+// NaN (0 * inf); such rows are recomputed one by one from their own keys.
+
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "paged_ops.cuh"
+
+namespace stk {
+
+int set_wait_limit_prompt(unsigned long long ns) { return set_wait_limit_this_unit(ns); }
+
+namespace {
+
+constexpr int kTileM = 128;   // rows of an MMA tile
+constexpr int kTileN = 128;   // keys of a tile
+constexpr int kRows = 256;    // rows of a CTA
+constexpr int kSoftmaxWarps = 8;
+constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLazy = 8.f;  // log2 of the growth of the maximum that is left to P
+
+template <int D>
+struct Plan {
+  static constexpr int kTileBytes = kTileN * D * 2;      // one K or V tile, and one Q tile
+  static constexpr int kRing = D == 128 ? 5 : 10;        // K and V tiles in flight
+  static constexpr int kBytes = (2 + kRing) * kTileBytes + 1024;  // + alignment of the swizzle atoms
+};
+
+// ---------------------------------------------------------------- tcgen05
+__device__ __forceinline__ void tmem_alloc(uint32_t* dst, int columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(columns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, int columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      : "memory");
+}
+
+// 32 consecutive columns of the warp's 32 lanes: element j of lane i is
+// column at + j of TMEM lane 32 (warp % 4) + i.
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The registers of a load, after its wait: keeps their uses behind it.
+__device__ __forceinline__ void tmem_loaded(uint32_t* r) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                      "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+// A bounded wait of a whole warp, converged again on return.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, int* status) {
+  return __all_sync(kFull, mbar_wait(bar, parity, status));
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory matrix descriptor, 128-byte swizzle (rows of 128 bytes,
+// groups of 8 rows 1024 bytes apart); `lead` bytes between the 64-element
+// column groups of an operand whose rows run along the contraction (V).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | static_cast<uint64_t>(lead >> 4) << 16 |
+         static_cast<uint64_t>(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+// Instruction descriptor of kind::f16 with FP32 accumulators.
+template <typename T>
+constexpr uint32_t mma_desc(int m, int n, bool b_along_n) {
+  const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return 1u << 4 | fmt << 7 | fmt << 10 | (b_along_n ? 1u : 0u) << 16 | static_cast<uint32_t>(n >> 3) << 17 |
+         static_cast<uint32_t>(m >> 4) << 24;
+}
+
+__device__ __forceinline__ void tma_load(const CUtensorMap* map, void* dst, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// tanh(x) for capped scores. 1 - 2 / (1 + e^2x) keeps an absolute error of a
+// few 2^-24, which the cap turns into the error of a score.
+__device__ __forceinline__ float cap_tanh(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(x * (2.f * kLog2e))));
+  return fmaf(-2.f, r, 1.f);
+}
+
+struct Shared {
+  uint64_t full[10], empty[10];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint32_t tmem;
+  int kmin[2], kmax[2], lomax[2], himin[2];
+};
+
+// A row recomputed from its own keys [lo, hi), one at a time, by one warp:
+// the definition, for rows whose tile sums met values of other rows' keys
+// that are not finite. On return every lane has m (natural log), l and its
+// D / 32 dims of the sum (dims lane * D / 32 + j).
+template <typename T, int D, int MODE>
+__device__ void single_row(const PagedAttnArgs& a, int rp, int h, const T* q, int lo, int hi, int pos, float slope,
+                           int lane, float& m, float& l, float (&o)[D / 32]) {
+  constexpr int N = D / 32;
+  float x[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    x[j] = to_f32(q[lane * N + j]);
+    o[j] = 0.f;
+  }
+  m = neg_inf();
+  l = 0.f;
+  for (int k = lo; k < hi; ++k) {
+    const int page = page_of(a, rp, k);
+    if (page < 0) continue;
+    const long long at = ((static_cast<long long>(page) * a.L.hkv + h) * a.L.page_size + k % a.L.page_size) * D;
+    const T* kr = static_cast<const T*>(a.L.k) + at + lane * N;
+    const T* vr = static_cast<const T*>(a.L.v) + at + lane * N;
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) s = fmaf(x[j], to_f32(kr[j]), s);
+    s = warp_sum(s) * a.scale;
+    if (MODE & 1) s = a.softcap * tanhf(s / a.softcap);
+    if (MODE & 2) s -= slope * fabsf(static_cast<float>(pos - k));
+    const float mn = fmaxf(m, s);
+    const float base = mn == neg_inf() ? 0.f : mn;
+    const float alpha = expf(m - base), w = expf(s - base);
+    l = l * alpha + w;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = o[j] * alpha + (w == 0.f ? 0.f : w * to_f32(vr[j]));
+    m = mn;
+  }
+}
+
+// MODE: 1 capped scores, 2 biased by distance, 3 both.
+template <typename T, int D, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap,
+                   const __grid_constant__ CUtensorMap vmap) {
+  using P = Plan<D>;
+  constexpr int kHalves = D / 64;
+  constexpr int kHalfBytes = kTileN * 128;
+  extern __shared__ unsigned char raw[];
+  __shared__ Shared sh;
+  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
+  unsigned char* ring = base + 2 * P::kTileBytes;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int h = blockIdx.y;
+  // Later row tiles see more keys under a causal mask: they start first.
+  const int slots = gridDim.x / a.nsplit;
+  const int split = blockIdx.x % a.nsplit;
+  const RowTile t = row_tile<kRows>(a, slots - 1 - static_cast<int>(blockIdx.x) / a.nsplit, lane);
+  if (t.rows == 0) return;
+
+  if (tid == 0) {
+    for (int i = 0; i < P::kRing; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int q = 0; q < 2; ++q) {
+      mbar_init(&sh.q_full[q], kTileM);
+      mbar_init(&sh.s_full[q], 1);
+      mbar_init(&sh.p_full[q], kTileM);
+      mbar_init(&sh.o_full[q], 1);
+      sh.kmin[q] = sh.himin[q] = 0x7fffffff;
+      sh.kmax[q] = sh.lomax[q] = 0;
+    }
+    fence_barrier_init();
+  }
+  if (warp == kSoftmaxWarps) tmem_alloc(&sh.tmem, 512);
+  __syncthreads();
+
+  // ---- the rows' key intervals
+  RowKeys rk{0, 0x7fffffff, 0};
+  const int qt = warp >> 2;                       // softmax warps: MMA tile
+  const int row = tid;                            // and row of the CTA
+  const bool have = tid < kRows && row < t.rows;
+  if (warp < kSoftmaxWarps) {
+    if (have) rk = row_keys(a, t, (t.row0 + row) / a.G);
+    const bool some = have && rk.hi > rk.lo;
+    const int kmin = __reduce_min_sync(kFull, some ? rk.lo : 0x7fffffff);
+    const int kmax = __reduce_max_sync(kFull, some ? rk.hi : 0);
+    const int lomax = __reduce_max_sync(kFull, have ? rk.lo : 0);
+    const int himin = __reduce_min_sync(kFull, have ? rk.hi : 0x7fffffff);
+    if (lane == 0) {
+      atomicMin(&sh.kmin[qt], kmin);
+      atomicMax(&sh.kmax[qt], kmax);
+      atomicMax(&sh.lomax[qt], lomax);
+      atomicMin(&sh.himin[qt], himin);
+    }
+  }
+  __syncthreads();
+  // Tiles [ta, tb) of this CTA's part, and those of each MMA tile.
+  int ta, tb, qa[2], qb[2];
+  {
+    const int kmin = min(sh.kmin[0], sh.kmin[1]), kmax = max(sh.kmax[0], sh.kmax[1]);
+    const int first = kmax > 0 ? kmin / kTileN : 0, last = (kmax + kTileN - 1) / kTileN;
+    const int per = (last - first + a.nsplit - 1) / a.nsplit;
+    ta = min(last, first + split * per);
+    tb = min(last, ta + per);
+    int lo = tb, hi = ta;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      qa[q] = sh.kmax[q] > 0 ? max(ta, sh.kmin[q] / kTileN) : tb;
+      qb[q] = min(tb, (sh.kmax[q] + kTileN - 1) / kTileN);
+      if (qb[q] <= qa[q]) qa[q] = qb[q] = ta;
+      else {
+        lo = min(lo, qa[q]);
+        hi = max(hi, qb[q]);
+      }
+    }
+    ta = lo;
+    tb = max(lo, hi);
+  }
+  const uint32_t tmem = sh.tmem;
+  const int rp = t.r;
+
+  if (warp == kSoftmaxWarps + 1) {
+    // ------------------------------------------------------------ K and V tiles
+    const int bp = min(a.L.page_size, kTileN);  // rows of a box
+    const int boxes = kTileN / bp;
+    const int pages = request_blocks(a.L, rp) * (a.L.b / a.L.page_size);
+    auto page_at = [&](int key) {  // keys past the request's pages, or of a bad entry, read as zeros
+      const int entry = key / a.L.page_size;
+      int page = entry < pages ? page_of(a, rp, key) : -1;
+      return page < 0 ? a.pages : page;
+    };
+    int page = lane < boxes && ta < tb ? page_at(ta * kTileN + lane * bp) : 0;
+    bool ok = true;
+    for (int i = ta; ok && i < tb; ++i) {
+      const int next = lane < boxes && i + 1 < tb ? page_at((i + 1) * kTileN + lane * bp) : 0;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int item = 2 * (i - ta) + kv, slot = item % P::kRing;
+        if (item >= P::kRing) ok = ok && warp_wait(&sh.empty[slot], (item / P::kRing - 1) & 1, a.status);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], P::kTileBytes);
+        __syncwarp();
+        if (lane < boxes) {
+          unsigned char* dst = ring + slot * P::kTileBytes + lane * bp * 128;
+          const int y = (i * kTileN + lane * bp) % a.L.page_size;
+#pragma unroll
+          for (int half = 0; half < kHalves; ++half)
+            tma_load(kv == 0 ? &kmap : &vmap, dst + half * kHalfBytes, &sh.full[slot], half * 64, y, h, page);
+        }
+      }
+      page = next;
+    }
+  } else if (warp == kSoftmaxWarps) {
+    // ------------------------------------------------------------ MMAs
+    constexpr uint32_t qk = mma_desc<T>(kTileM, kTileN, false), pv = mma_desc<T>(kTileM, D, true);
+    const uint32_t sring = smem_u32(ring), sq = smem_u32(base);
+    int n[2] = {0, 0};  // tiles done, per MMA tile
+    bool ok = true;
+    auto wait_full = [&](int item) {
+      ok = ok && warp_wait(&sh.full[item % P::kRing], (item / P::kRing) & 1, a.status);
+    };
+    auto issue_qk = [&](int q, int i) {  // S = Q K^T
+      const uint32_t kt = sring + (2 * (i - ta)) % P::kRing * P::kTileBytes;
+      if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          const uint32_t o = (s >> 2) * kHalfBytes + (s & 3) * 32;
+          mma_ss(tmem + q * kTileN, smem_desc(sq + q * P::kTileBytes + o, 16), smem_desc(kt + o, 16), qk, s > 0);
+        }
+        mma_commit(&sh.s_full[q]);
+      }
+      __syncwarp();
+    };
+    if (ta < tb) {
+      wait_full(0);
+      for (int q = 0; q < 2; ++q) {
+        if (qa[q] < qb[q]) ok = ok && warp_wait(&sh.q_full[q], 0, a.status);
+        fence_after();
+        if (ok && qa[q] == ta && qa[q] < qb[q]) issue_qk(q, ta);
+      }
+      if (lane == 0) mma_commit(&sh.empty[0]);
+      __syncwarp();
+    }
+    for (int i = ta; ok && i < tb; ++i) {
+      const int item = 2 * (i - ta) + 1;
+      wait_full(item);
+      if (!ok) break;
+      unsigned char* vt = ring + item % P::kRing * P::kTileBytes;
+      const int valid = t.len - i * kTileN;
+      if (valid < kTileN) {  // slots past the request's tokens: their values must not meet the zero weights
+        const int fill = min(kTileN, (max(valid, 0) + a.L.page_size - 1) / a.L.page_size * a.L.page_size);
+        const int from = max(valid, 0);
+        for (int x = lane; x < (fill - from) * 8 * kHalves; x += 32) {
+          const int half = x % kHalves, y = x / kHalves;
+          *reinterpret_cast<uint4*>(vt + half * kHalfBytes + (from + y / 8) * 128 + y % 8 * 16) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      if (i + 1 < tb) wait_full(item + 1);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (ok && i >= qa[q] && i < qb[q]) {
+          ok = ok && warp_wait(&sh.p_full[q], n[q] & 1, a.status);
+          fence_after();
+          if (ok && lane == 0) {
+            const uint32_t v = smem_u32(vt);
+#pragma unroll
+            for (int s = 0; s < kTileN / 16; ++s)  // O += P V
+              mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + s * 8, smem_desc(v + s * 2048, kHalfBytes), pv,
+                     n[q] > 0 || s > 0);
+            if (i + 1 == qb[q]) mma_commit(&sh.o_full[q]);
+          }
+          ++n[q];
+          __syncwarp();
+        }
+        if (ok && i + 1 >= qa[q] && i + 1 < qb[q]) issue_qk(q, i + 1);
+      }
+      if (lane == 0) {
+        mma_commit(&sh.empty[item % P::kRing]);
+        if (i + 1 < tb) mma_commit(&sh.empty[(item + 1) % P::kRing]);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int r = tid & (kTileM - 1);  // row of the MMA tile
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
+    const uint32_t ts = tmem + lanes + qt * kTileN, to = tmem + lanes + 2 * kTileN + qt * D;
+    // Q tile, swizzled: 16-byte chunk c of row x at chunk c ^ (x & 7).
+    {
+      unsigned char* dst = base + qt * P::kTileBytes;
+      const T* q = static_cast<const T*>(a.q);
+#pragma unroll 4
+      for (int x = r; x < kTileM * D / 8; x += kTileM) {
+        const int rr = x / (D / 8), c = x % (D / 8);
+        const int cr = qt * kTileM + rr;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (cr < t.rows) {
+          const int tok = (t.row0 + cr) / a.G, g = t.row0 + cr - tok * a.G;
+          w = *reinterpret_cast<const uint4*>(q + (t.t0 + tok) * a.q_ts + (h * a.G + g) * a.q_hs + c * 8);
+        }
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalfBytes + rr * 128 + ((c ^ rr) & 7) * 16) = w;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(&sh.q_full[qt]);
+    }
+    const int tok = have ? (t.row0 + row) / a.G : 0;
+    const int head = h * a.G + (have ? t.row0 + row - tok * a.G : 0);
+    const float slope = (MODE & 2) && a.slopes ? a.slopes[head] : 0.f;
+    const float c1 = (MODE & 1) ? a.scale / a.softcap : a.scale * kLog2e;
+    const float cap2 = a.softcap * kLog2e, slope2 = slope * kLog2e;
+    float m = neg_inf(), l = 0.f;  // in log2 units; m is at most kLazy below the true maximum
+    bool ok = true;
+    for (int i = qa[qt]; i < qb[qt]; ++i) {
+      const int n = i - qa[qt];
+      ok = ok && warp_wait(&sh.s_full[qt], n & 1, a.status);
+      if (!ok) break;
+      fence_after();
+      float s[kTileN];
+#pragma unroll
+      for (int j = 0; j < kTileN; j += 32) tmem_ld32(ts + j, reinterpret_cast<uint32_t*>(s) + j);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < kTileN; j += 32) tmem_loaded(reinterpret_cast<uint32_t*>(s) + j);
+      const int k0 = i * kTileN;
+      const bool full = k0 >= sh.lomax[qt] && k0 + kTileN <= sh.himin[qt];
+      if (MODE != 0) {
+#pragma unroll
+        for (int j = 0; j < kTileN; ++j) {
+          float x = s[j];
+          if (MODE & 1) x = cap2 * cap_tanh(x * c1); else x *= c1;
+          if (MODE & 2) x = fmaf(-slope2, fabsf(static_cast<float>(rk.pos - k0 - j)), x);
+          s[j] = x;
+        }
+      }
+      if (!full) {
+        const int lo = rk.lo - k0, hi = rk.hi - k0;
+#pragma unroll
+        for (int j = 0; j < kTileN; ++j) s[j] = j >= lo && j < hi ? s[j] : neg_inf();
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int j = 1; j < kTileN; ++j) mx = fmaxf(mx, s[j]);
+      const float c = MODE != 0 ? 1.f : c1;
+      mx *= c;
+      const bool grow = mx > m + kLazy || (m == neg_inf() && mx > m);
+      if (__any_sync(kFull, grow && m != neg_inf())) {
+        // O of the warp's rows by 2^(m - mx); the previous product is complete, S comes after it.
+        const float f = grow ? ex2(m - mx) : 1.f;
+        l *= f;
+#pragma unroll 1
+        for (int j = 0; j < D; j += 32) {
+          uint32_t o[32];
+          tmem_ld32(to + j, o);
+          tmem_wait_ld();
+          tmem_loaded(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st32(to + j, o);
+        }
+        tmem_wait_st();
+      }
+      if (grow) m = mx;
+      const float nm = m == neg_inf() ? 0.f : -m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < kTileN; j += 64) {
+        uint32_t p[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float x = ex2(fmaf(s[j + 2 * e], c, nm)), y = ex2(fmaf(s[j + 2 * e + 1], c, nm));
+          sum[(2 * e) & 3] += x;
+          sum[(2 * e + 1) & 3] += y;
+          p[e] = pack2<T>(x, y);
+        }
+        tmem_st32(ts + j / 2, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      fence_before();
+      mbar_arrive(&sh.p_full[qt]);
+    }
+    // ------------------------------------------------------------ output
+    const bool any = qa[qt] < qb[qt];
+    if (any) ok = ok && warp_wait(&sh.o_full[qt], 0, a.status);
+    fence_after();
+    const bool empty = m == neg_inf();
+    const long long orow = static_cast<long long>(t.t0 + tok) * a.hq + head;
+    const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
+    const float inv = empty || a.part_ml ? 1.f : 1.f / l;
+    bool nan = false;
+    if (ok) {
+#pragma unroll 1
+      for (int j = 0; j < D; j += 32) {
+        uint32_t o[32];
+        __syncwarp();
+        if (any) {
+          tmem_ld32(to + j, o);
+          tmem_wait_ld();
+          tmem_loaded(o);
+        }
+        if (!have) continue;
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          f[e] = !any || empty ? 0.f : __uint_as_float(o[e]) * inv;
+          nan = nan || f[e] != f[e];
+        }
+        if (a.part_ml) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(a.part_o + prow * D + j + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        } else {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = pack2<T>(f[2 * e], f[2 * e + 1]);
+          uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + orow * D + j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        }
+      }
+      if (have) {
+        if (a.part_ml) a.part_ml[prow] = make_float2(empty ? neg_inf() : m * kLn2, l);
+        else if (a.lse) a.lse[orow] = empty ? neg_inf() : (m + log2f(l)) * kLn2;
+      }
+      // Rows that met values which are not finite, of keys that they may not see.
+      unsigned redo = __ballot_sync(kFull, nan);
+      while (redo) {
+        const int src = __ffs(redo) - 1;
+        redo &= redo - 1;
+        __syncwarp();
+        const int xtok = __shfl_sync(kFull, tok, src);
+        const int xhead = __shfl_sync(kFull, head, src), xpos = __shfl_sync(kFull, rk.pos, src);
+        const int xlo = max(__shfl_sync(kFull, rk.lo, src), ta * kTileN);
+        const int xhi = min(__shfl_sync(kFull, rk.hi, src), tb * kTileN);
+        const float xslope = __shfl_sync(kFull, slope, src);
+        float xm, xl, xo[D / 32];
+        single_row<T, D, MODE>(a, rp, h, static_cast<const T*>(a.q) + (t.t0 + xtok) * a.q_ts + xhead * a.q_hs, xlo, xhi,
+                               xpos, xslope, lane, xm, xl, xo);
+        const long long xr = static_cast<long long>(t.t0 + xtok) * a.hq + xhead;
+        const long long xp = static_cast<long long>(split) * a.T * a.hq + xr;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const int dd = lane * (D / 32) + j;
+          if (a.part_ml) {
+            a.part_o[xp * D + dd] = xo[j];
+          } else {
+            const float y = xm == neg_inf() ? 0.f : xo[j] / xl;
+            const uint32_t w = pack2<T>(y, 0.f);
+            static_cast<unsigned short*>(a.out)[xr * D + dd] = static_cast<unsigned short>(w & 0xffff);
+          }
+        }
+        if (lane == 0) {
+          if (a.part_ml) a.part_ml[xp] = make_float2(xm, xl);
+          else if (a.lse) a.lse[xr] = xm == neg_inf() ? neg_inf() : xm + logf(xl);
+        }
+      }
+    }
+    fence_before();
+  }
+  __syncthreads();
+  if (warp == kSoftmaxWarps) {
+    fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+template <typename T, int D, int MODE>
+int launch_mode(const PagedAttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t stream) {
+  auto kern = prompt_attn_kernel<T, D, MODE>;
+  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Plan<D>::kBytes));
+  if (rc) return rc;
+  const int slots = row_tile_slots(a.R, a.T, a.G, a.token_offsets != nullptr, a.shared != 0, kRows);
+  kern<<<dim3(static_cast<unsigned>(slots * a.nsplit), static_cast<unsigned>(a.L.hkv)), kThreads, Plan<D>::kBytes,
+         stream>>>(a, km, vm);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, int D>
+int launch_d(const PagedAttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t stream) {
+  switch ((a.softcap > 0.f ? 1 : 0) | (a.slopes ? 2 : 0)) {
+    case 0: return launch_mode<T, D, 0>(a, km, vm, stream);
+    case 1: return launch_mode<T, D, 1>(a, km, vm, stream);
+    case 2: return launch_mode<T, D, 2>(a, km, vm, stream);
+    default: return launch_mode<T, D, 3>(a, km, vm, stream);
+  }
+}
+
+}  // namespace
+
+// A tensor map over a page pool: (64 dims, box_rows tokens) boxes of one KV
+// head's page, 128-byte swizzle.
+int encode_pool_map(CUtensorMap* map, const PagedAttnArgs& a, const void* pool, int kv_dtype, int box_rows) {
+  const EncodeTiled fn = encode_tiled();
+  if (fn == nullptr) return static_cast<int>(cudaErrorNotSupported);
+  const int ps = a.L.page_size;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.d), static_cast<cuuint64_t>(ps),
+                              static_cast<cuuint64_t>(a.L.hkv), static_cast<cuuint64_t>(a.pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(a.d) * 2, static_cast<cuuint64_t>(ps) * a.d * 2,
+                                 static_cast<cuuint64_t>(a.L.hkv) * ps * a.d * 2};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, kv_dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                        const_cast<void*>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : static_cast<int>(cudaErrorInvalidValue);
+}
+
+// 16-bit types, heads of 64 or 128 dims, pages that tile 128 keys (or are
+// tiled by them), 16-byte rows.
+bool prompt_attn_takes(int kv_dtype, int d, int page_size, const void* k, const void* v, const void* q, long long q_ts,
+                       long long q_hs) {
+  const bool pages = page_size >= 8 && (page_size <= kTileN ? kTileN % page_size == 0 : page_size % kTileN == 0);
+  const uintptr_t any = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q) |
+                        static_cast<uintptr_t>(q_ts * 2) | static_cast<uintptr_t>(q_hs * 2);
+  return kv_dtype != kF32 && (d == 64 || d == 128) && pages && any % 16 == 0;
+}
+
+int launch_prompt_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream) {
+  CUtensorMap km, vm;
+  const int rows = a.L.page_size < kTileN ? a.L.page_size : kTileN;
+  int rc = encode_pool_map(&km, a, a.L.k, kv_dtype, rows);
+  if (rc == 0) rc = encode_pool_map(&vm, a, a.L.v, kv_dtype, rows);
+  if (rc) return rc;
+  if (kv_dtype == kBF16)
+    return a.d == 64 ? launch_d<__nv_bfloat16, 64>(a, km, vm, stream) : launch_d<__nv_bfloat16, 128>(a, km, vm, stream);
+  return a.d == 64 ? launch_d<__half, 64>(a, km, vm, stream) : launch_d<__half, 128>(a, km, vm, stream);
+}
+
+}  // namespace stk

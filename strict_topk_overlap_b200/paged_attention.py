@@ -18,10 +18,18 @@ from .paged import PagedKVCache
 from .paged_append import _check_ints, _check_rows
 
 
-def attention_workspace(cache: PagedKVCache, tokens, hq, *, token_offsets=None, prefix=0):
+def _most(max_tokens, tokens, token_offsets):
+    """Bound on a request's new tokens."""
+    if token_offsets is None:
+        return min(1, tokens)
+    return tokens if max_tokens is None else min(int(max_tokens), tokens)
+
+
+def attention_workspace(cache: PagedKVCache, tokens, hq, *, token_offsets=None, max_tokens=None, prefix=0):
     """Workspace for ``attention`` (or, with ``prefix``, ``shared_prefix_attention``) of up to these sizes."""
     need = L.load().stk_paged_attention_workspace_bytes(cache.kv(), cache.requests, tokens, hq,
                                                         int(token_offsets is not None),
+                                                        _most(max_tokens, tokens, token_offsets),
                                                         cache.max_blocks * cache.block_size, prefix)
     return torch.empty((need,), device=cache.k_pages.device, dtype=torch.uint8)
 
@@ -48,19 +56,22 @@ def _attend(q, cache, lengths, token_offsets, max_tokens, kv_lo, kv_hi, softcap,
         raise ValueError("slopes must be contiguous FP32 [Hq] on the cache's device")
     if softcap < 0 or (scale is not None and scale <= 0):
         raise ValueError("softcap must not be negative and scale must be positive")
-    longest = cache.max_blocks * cache.block_size
+    longest, most = cache.max_blocks * cache.block_size, _most(max_tokens, t, token_offsets)
+    if t and most < 1:
+        raise ValueError("max_tokens must be positive")
     if prefix < 0 or prefix % cache.page_size or prefix > longest:
         raise ValueError(f"prefix must be whole pages of {cache.page_size} tokens, at most {longest} tokens")
     out = torch.empty((t, hq, q.shape[2]), dtype=q.dtype, device=dev)
     lse = torch.empty((t, hq), dtype=torch.float32, device=dev) if return_lse else None
     lib, kv = L.load(), cache.kv()
     if workspace is None:
-        need = lib.stk_paged_attention_workspace_bytes(kv, requests, t, hq, int(token_offsets is not None), longest,
+        need = lib.stk_paged_attention_workspace_bytes(kv, requests, t, hq, int(token_offsets is not None), most, longest,
                                                        prefix)
         workspace = torch.empty((need,), device=dev, dtype=torch.uint8)
     options = L.StkAttentionOptions(scale or 0.0, softcap, L.ptr(slopes), L.ptr(kv_lo), L.ptr(kv_hi))
     rc = lib.stk_paged_attention(kv, pool.shape[0], q.data_ptr(), q.stride(0), q.stride(1), requests, t, hq,
-                                 lengths.data_ptr(), L.ptr(token_offsets), longest, prefix, options, out.data_ptr(),
+                                 lengths.data_ptr(), L.ptr(token_offsets), most, longest, prefix, options,
+                                 out.data_ptr(),
                                  L.ptr(lse), workspace.data_ptr(), workspace.numel(), L.status_ptr(), L.stream_of(q))
     L.check(rc, "paged attention")
     return (out, lse) if return_lse else out
