@@ -19,7 +19,7 @@ CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libstk_sm100.so"
 SOURCES = ["select.cu", "states.cu", "repair.cu", "attend.cu", "metadata.cu", "group_mma.cu", "step.cu", "append.cu",
-           "rows_attn.cu", "prompt_attn.cu", "capi.cu"]
+           "rows_attn.cu", "token_attn.cu", "prompt_attn.cu", "capi.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "--extended-lambda",
          "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-diag-suppress", "177,550"]

@@ -139,7 +139,7 @@ int stk_set_wait_limit_ns(unsigned long long ns) {
   if (ns == 0) return fail(STK_EINVAL, "the wait limit must be positive");
   int (*const setters[])(unsigned long long) = {set_wait_limit_select, set_wait_limit_states, set_wait_limit_repair,
                                                 set_wait_limit_attend, set_wait_limit_group_mma, set_wait_limit_step,
-                                                set_wait_limit_prompt};
+                                                set_wait_limit_prompt, set_wait_limit_token};
   for (auto set : setters) {
     const int rc = set(ns);
     if (rc) return cuda_status(rc, "set wait limit");
@@ -914,10 +914,14 @@ namespace {
 // of its tiles' key ranges. Everything follows from host sizes, so that the
 // workspace size and the launches agree and a captured graph fits any
 // lengths up to the cache's capacity.
+enum AttnKind { kAttnRows, kAttnTokens, kAttnPrompt };
+
 struct AttnPhase {
-  bool prompt;  // the tensor-core kernel, else the FP32-unit one
-  int nsplit;
+  AttnKind kind;
+  int nsplit;  // tokens: CTAs
   int span_lo, span_hi, shared;
+  int requests, most_rows;
+  size_t states, bytes;  // partial states; their bytes (and the unit counts'), a multiple of 16
 };
 struct AttnPlan {
   AttnPhase phase[2];
@@ -926,38 +930,50 @@ struct AttnPlan {
   size_t bytes;
 };
 
-AttnPhase plan_phase(int R, int T, int G, bool offsets, bool shared, int hkv, int max_tokens, int keys, bool tensor) {
+AttnPhase plan_phase(const stk_kv* kv, int R, int T, int hq, bool offsets, bool shared, int max_tokens, int keys,
+                     bool prompt_ok, bool token_ok) {
   AttnPhase p{};
+  const int hkv = kv->hkv, G = hq / hkv, sms = sm_count_current();
   p.shared = shared;
-  // A tile of 16 rows holds a request's rows of one KV head: nothing to gain from 256-row tiles.
+  p.requests = shared ? 1 : R;
+  // Up to 16 rows of a KV head share one read of its keys in one tile of the
+  // token kernel; more of them fill the prompt kernel's tiles.
   const long long rows = static_cast<long long>(shared ? T : max_tokens) * G;
-  p.prompt = tensor && rows > 16;
-  const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared, p.prompt ? 256 : 16)) * hkv;
-  const long long ctas = p.prompt ? sm_count_current() : 2ll * sm_count_current();
-  const long long most = p.prompt ? (keys + 255) / 256 : (keys + 63) / 64;
-  long long n = ctas / tiles;
-  n = n < most ? n : most;
-  p.nsplit = static_cast<int>(n < 1 ? 1 : n);
+  p.most_rows = static_cast<int>(rows < 16 ? rows : 16);
+  p.kind = rows <= 16 ? (token_ok ? kAttnTokens : kAttnRows) : (prompt_ok ? kAttnPrompt : kAttnRows);
+  if (p.kind == kAttnTokens) {
+    p.nsplit = 2 * sms;
+    p.states = (static_cast<size_t>(p.nsplit) + static_cast<size_t>(p.requests) * hkv) * p.most_rows;
+    p.bytes = p.states * (kv->d + 2) * sizeof(float) + (p.requests + 1) * sizeof(int);
+  } else {
+    const bool prompt = p.kind == kAttnPrompt;
+    const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared, prompt ? 256 : 16)) * hkv;
+    const long long most = prompt ? (keys + 255) / 256 : (keys + 63) / 64;
+    long long n = (prompt ? sms : 2 * sms) / tiles;
+    n = n < most ? n : most;
+    p.nsplit = static_cast<int>(n < 1 ? 1 : n);
+    p.states = static_cast<size_t>(p.nsplit) * T * hq;
+    p.bytes = p.states * (kv->d + 2) * sizeof(float);
+  }
+  p.bytes = (p.bytes + 15) & ~static_cast<size_t>(15);
   return p;
 }
 
 AttnPlan plan_attention(const stk_kv* kv, int R, int T, int hq, bool offsets, int max_tokens, int max_length,
-                        int prefix, bool tensor) {
+                        int prefix, bool prompt_ok, bool token_ok) {
   AttnPlan p{};
-  const int G = hq / kv->hkv;
   if (prefix > 0) {
-    p.phase[0] = plan_phase(R, T, G, offsets, true, kv->hkv, max_tokens, prefix, tensor);
+    p.phase[0] = plan_phase(kv, R, T, hq, offsets, true, max_tokens, prefix, prompt_ok, token_ok);
     p.phase[0].span_hi = prefix;
     p.phases = 1;
   }
   AttnPhase& own = p.phase[p.phases++];
-  own = plan_phase(R, T, G, offsets, false, kv->hkv, max_tokens, max_length - prefix, tensor);
+  own = plan_phase(kv, R, T, hq, offsets, false, max_tokens, max_length - prefix, prompt_ok, token_ok);
   own.span_lo = prefix;
   own.span_hi = 0x7fffffff;
-  p.join = p.phases > 1 || own.nsplit > 1;
+  p.join = p.phases > 1 || own.kind == kAttnTokens || own.nsplit > 1;
   if (p.join)
-    for (int i = 0; i < p.phases; ++i)
-      p.bytes += static_cast<size_t>(p.phase[i].nsplit) * T * hq * (kv->d + 2) * sizeof(float);
+    for (int i = 0; i < p.phases; ++i) p.bytes += p.phase[i].bytes;
   return p;
 }
 
@@ -979,10 +995,13 @@ extern "C" size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, i
                                                       int max_tokens, int max_length, int prefix) {
   const bool offsets = has_offsets != 0;
   if (check_attention(kv, R, T, hq, offsets, max_tokens, max_length, prefix) || T == 0) return 0;
-  // Enough whichever kernel the addresses of the call lead to.
-  const size_t a = plan_attention(kv, R, T, hq, offsets, max_tokens, max_length, prefix, true).bytes;
-  const size_t b = plan_attention(kv, R, T, hq, offsets, max_tokens, max_length, prefix, false).bytes;
-  return a > b ? a : b;
+  // Enough whichever kernels the addresses of the call lead to.
+  size_t need = 0;
+  for (int ok = 0; ok < 4; ++ok) {
+    const size_t n = plan_attention(kv, R, T, hq, offsets, max_tokens, max_length, prefix, ok & 1, ok & 2).bytes;
+    need = n > need ? n : need;
+  }
+  return need;
 }
 
 extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
@@ -996,10 +1015,10 @@ extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, l
   if (!q || !lengths || !out || pages <= 0) return fail(STK_EINVAL, "null pointer or empty pool");
   if (options && (!(options->softcap >= 0.f) || !(options->scale >= 0.f)))
     return fail(STK_EINVAL, "scale and softcap must not be negative");
-  const bool tensor =
-      prompt_attn_takes(kv->kv_dtype, kv->d, kv->page_size, kv->k, kv->v, q, q_token_stride, q_head_stride);
-  const AttnPlan p =
-      plan_attention(kv, R, T, hq, token_offsets != nullptr, max_tokens, max_length, prefix, tensor);
+  const AttnPlan p = plan_attention(
+      kv, R, T, hq, token_offsets != nullptr, max_tokens, max_length, prefix,
+      prompt_attn_takes(kv->kv_dtype, kv->d, kv->page_size, kv->k, kv->v, q, q_token_stride, q_head_stride),
+      token_attn_takes(kv->kv_dtype, kv->d, kv->page_size, R, kv->k, kv->v, q, q_token_stride, q_head_stride));
   if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return fail(STK_EWS, "attention workspace too small");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   PagedAttnArgs a{};
@@ -1016,18 +1035,22 @@ extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, l
   a.status = status;
   JoinArgs j{};
   j.rows = T * hq; j.d = kv->d; j.dtype = kv->kv_dtype; j.out = out; j.lse = lse; j.nsrc = p.phases;
-  float* at = static_cast<float*>(workspace);
+  j.hq = hq; j.G = a.G; j.token_offsets = token_offsets;
+  unsigned char* at = static_cast<unsigned char*>(workspace);
   for (int i = 0; i < p.phases; ++i) {
     const AttnPhase& ph = p.phase[i];
     a.span_lo = ph.span_lo; a.span_hi = ph.span_hi; a.shared = ph.shared; a.nsplit = ph.nsplit;
+    int* prefix_units = nullptr;
     if (p.join) {
-      const size_t states = static_cast<size_t>(ph.nsplit) * j.rows;
-      a.part_o = at;
-      a.part_ml = reinterpret_cast<float2*>(at + states * kv->d);
-      at += states * (kv->d + 2);
-      j.src[i] = {a.part_ml, a.part_o, ph.nsplit};
+      a.part_o = reinterpret_cast<float*>(at);
+      a.part_ml = reinterpret_cast<float2*>(a.part_o + ph.states * kv->d);
+      if (ph.kind == kAttnTokens) prefix_units = reinterpret_cast<int*>(a.part_ml + ph.states);
+      at += ph.bytes;
+      j.src[i] = {a.part_ml, a.part_o, ph.nsplit, prefix_units, ph.nsplit, ph.most_rows, ph.requests, ph.shared};
     }
-    const int r2 = ph.prompt ? launch_prompt_attn(a, kv->kv_dtype, st) : launch_rows_attn(a, kv->kv_dtype, st);
+    const int r2 = ph.kind == kAttnPrompt   ? launch_prompt_attn(a, kv->kv_dtype, st)
+                   : ph.kind == kAttnTokens ? launch_token_attn(a, kv->kv_dtype, ph.nsplit, ph.most_rows, prefix_units, st)
+                                            : launch_rows_attn(a, kv->kv_dtype, st);
     if (r2) return cuda_status(r2, "paged attention");
   }
   return p.join ? cuda_status(launch_join(j, st), "attention join") : 0;

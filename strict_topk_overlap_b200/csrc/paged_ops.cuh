@@ -173,17 +173,31 @@ bool prompt_attn_takes(int kv_dtype, int d, int page_size, const void* k, const 
 int launch_prompt_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream);
 int set_wait_limit_prompt(unsigned long long ns);
 
-// One set of partial softmax states to be joined: part s of row `row` at
-// ml[s * rows + row], o[(s * rows + row) * d].
+// Few rows per KV head (see token_attn.cu): `ctas` CTAs share the batch's
+// units evenly; CTA c's state of KV head h of request r is partial
+// c + r * hkv + h, most_rows rows each. Writes the units before each request
+// to prefix [requests + 1].
+bool token_attn_takes(int kv_dtype, int d, int page_size, int R, const void* k, const void* v, const void* q,
+                      long long q_ts, long long q_hs);
+int launch_token_attn(const PagedAttnArgs& a, int kv_dtype, int ctas, int most_rows, int* prefix, cudaStream_t stream);
+int set_wait_limit_token(unsigned long long ns);
+
+// One set of partial softmax states to be joined. Without prefix, part s of
+// row `row` is at ml[s * rows + row], o[(s * rows + row) * d]; with it, the
+// parts are those that token_attn wrote.
 struct PartSource {
   const float2* ml;
   const float* o;
   int parts;
+  const int* prefix;
+  int ctas, most_rows, requests, shared;
 };
 
 struct JoinArgs {
   PartSource src[2];
   int nsrc, rows, d, dtype;
+  int hq, G;
+  const int* token_offsets;
   void* out;
   float* lse;
 };

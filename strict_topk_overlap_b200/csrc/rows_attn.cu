@@ -273,25 +273,62 @@ __global__ void __launch_bounds__(128) join_kernel(JoinArgs a) {
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= a.rows) return;
+  // Part s of source k is state base[k] + s * step[k].
+  long long base[2], step[2];
+  int parts[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (k >= a.nsrc) continue;
+    const PartSource& p = a.src[k];
+    base[k] = row;
+    step[k] = a.rows;
+    parts[k] = p.parts;
+    if (p.prefix != nullptr) {
+      const int token = row / a.hq, head = row - token * a.hq, h = head / a.G, hkv = a.hq / a.G;
+      int r = 0, first = 0;
+      if (!p.shared) {
+        r = first = token;
+        if (a.token_offsets != nullptr) {
+          int hi = p.requests;
+          r = 0;
+          while (hi - r > 1) {
+            const int mid = (r + hi) >> 1;
+            if (a.token_offsets[mid] <= token) r = mid; else hi = mid;
+          }
+          first = a.token_offsets[r];
+        }
+      }
+      const long long total = static_cast<long long>(p.prefix[p.requests]) * hkv;
+      const long long per = (total + p.ctas - 1) / p.ctas;
+      const int units = p.prefix[r + 1] - p.prefix[r];
+      const long long u0 = static_cast<long long>(p.prefix[r]) * hkv + static_cast<long long>(h) * units;
+      const int c0 = units ? static_cast<int>(u0 / per) : 0;
+      parts[k] = units ? static_cast<int>((u0 + units - 1) / per) - c0 + 1 : 0;
+      base[k] = (static_cast<long long>(c0) + r * hkv + h) * p.most_rows + (token - first) * a.G + head - h * a.G;
+      step[k] = p.most_rows;
+    }
+  }
   float M = neg_inf();
-  for (int k = 0; k < a.nsrc; ++k)
-    for (int s = lane; s < a.src[k].parts; s += 32)
-      M = fmaxf(M, a.src[k].ml[static_cast<long long>(s) * a.rows + row].x);
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    for (int s = lane; s < parts[k]; s += 32) M = fmaxf(M, a.src[k].ml[base[k] + s * step[k]].x);
   M = warp_max(M);
   float Z = 0.f;
-  for (int k = 0; k < a.nsrc; ++k)
-    for (int s = lane; s < a.src[k].parts; s += 32) {
-      const float2 ml = a.src[k].ml[static_cast<long long>(s) * a.rows + row];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    for (int s = lane; s < parts[k]; s += 32) {
+      const float2 ml = a.src[k].ml[base[k] + s * step[k]];
       if (ml.x != neg_inf()) Z += expf(ml.x - M) * ml.y;
     }
   Z = warp_sum(Z);
   const bool empty = M == neg_inf();
   for (int d0 = lane; d0 < a.d; d0 += 128) {
     float o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < a.nsrc; ++k) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
 #pragma unroll 4
-      for (int s = 0; s < a.src[k].parts; ++s) {
-        const long long at = static_cast<long long>(s) * a.rows + row;
+      for (int s = 0; s < parts[k]; ++s) {
+        const long long at = base[k] + s * step[k];
         const float m = a.src[k].ml[at].x;
         if (m == neg_inf()) continue;
         const float c = expf(m - M);
