@@ -13,11 +13,14 @@
 //
 // HBM-bound for prompts: every q, k, v element is read and written once, plus
 // 8 bytes of table per (token, pair) and 8 bytes of bounds per (block, KV
-// head, dim). One CTA takes the new tokens of one block (request, block), so
-// a block's bounds have one writer and need no atomics; it stages the
-// cosines and sines of its tokens in shared memory once, and each warp then
-// takes whole heads: lanes cover a head's 16-byte vectors, two per lane (the
-// two halves of a pair in one lane, no shuffles), and several tokens at once.
+// head, dim). One CTA takes the new tokens of one block (request, block) and
+// eight heads, so a block's bounds have one writer and need no atomics. It
+// stages the cosines, sines and page slots of its tokens in shared memory
+// once; each warp then takes whole heads: lanes cover a head's 16-byte
+// vectors, two per lane (the two halves of a pair in one lane, no shuffles),
+// and several tokens at once. Bounds of 16-bit keys are kept as packed pairs
+// (the stored values themselves), which halves their registers and leaves
+// three CTAs per SM.
 // Which (request, block) a CTA has follows from token_offsets on the device:
 // request r's blocks start at slot offs[r] / B + 2 r, which leaves room for
 // the ceil of its tokens wherever its first block begins.
@@ -57,13 +60,197 @@ struct alignas(VEC * sizeof(T)) Vec {
   T e[VEC];
 };
 
+// Running minimum and maximum of a lane's 2 VEC stored keys.
+template <typename T, int VEC, bool PACKED = (sizeof(T) == 2 && VEC % 2 == 0)>
+struct Bounds {
+  float lo[2 * VEC], hi[2 * VEC];
+  __device__ __forceinline__ Bounds() {
+#pragma unroll
+    for (int e = 0; e < 2 * VEC; ++e) {
+      lo[e] = __int_as_float(0x7f800000);
+      hi[e] = neg_inf();
+    }
+  }
+  __device__ __forceinline__ void add(const Vec<T, VEC>& x, int half) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float v = to_f32(x.e[e]);
+      lo[half * VEC + e] = min_nan(lo[half * VEC + e], v);
+      hi[half * VEC + e] = max_nan(hi[half * VEC + e], v);
+    }
+  }
+  __device__ __forceinline__ void join(int o) {
+#pragma unroll
+    for (int e = 0; e < 2 * VEC; ++e) {
+      lo[e] = min_nan(lo[e], __shfl_xor_sync(kFull, lo[e], o));
+      hi[e] = max_nan(hi[e], __shfl_xor_sync(kFull, hi[e], o));
+    }
+  }
+  __device__ __forceinline__ float low(int e) const { return lo[e]; }
+  __device__ __forceinline__ float high(int e) const { return hi[e]; }
+};
+
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using type = __half2;
+  static constexpr uint32_t kInf = 0x7c007c00u;
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static constexpr uint32_t kInf = 0x7f807f80u;
+};
+
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(AppendArgs a, int tile_tokens) {
-  // (cos, sin) of pair it * VEC + e of token tk at tk * stride + e * rot_items + it: consecutive lanes read
-  // consecutive entries, and the stride's extra rot_items keep a warp's tokens on different banks.
-  extern __shared__ float2 turn[];
+struct Bounds<T, VEC, true> {
+  using P = typename Pair<T>::type;
+  uint32_t lo[VEC], hi[VEC];  // element e in half e & 1 of word e / 2
+  __device__ __forceinline__ Bounds() {
+#pragma unroll
+    for (int w = 0; w < VEC; ++w) {
+      lo[w] = Pair<T>::kInf;
+      hi[w] = Pair<T>::kInf | 0x80008000u;
+    }
+  }
+  static __device__ __forceinline__ uint32_t least(uint32_t a, uint32_t b) {
+    const P r = __hmin2_nan(*reinterpret_cast<const P*>(&a), *reinterpret_cast<const P*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) {
+    const P r = __hmax2_nan(*reinterpret_cast<const P*>(&a), *reinterpret_cast<const P*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ __forceinline__ void add(const Vec<T, VEC>& x, int half) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      lo[half * VEC / 2 + i] = least(lo[half * VEC / 2 + i], w[i]);
+      hi[half * VEC / 2 + i] = most(hi[half * VEC / 2 + i], w[i]);
+    }
+  }
+  __device__ __forceinline__ void join(int o) {
+#pragma unroll
+    for (int w = 0; w < VEC; ++w) {
+      lo[w] = least(lo[w], __shfl_xor_sync(kFull, lo[w], o));
+      hi[w] = most(hi[w], __shfl_xor_sync(kFull, hi[w], o));
+    }
+  }
+  static __device__ __forceinline__ float element(uint32_t w, int e) {
+    const unsigned short u = static_cast<unsigned short>(e & 1 ? w >> 16 : w & 0xffffu);
+    return to_f32(*reinterpret_cast<const T*>(&u));
+  }
+  __device__ __forceinline__ float low(int e) const { return element(lo[e / 2], e); }
+  __device__ __forceinline__ float high(int e) const { return element(hi[e / 2], e); }
+};
+
+// What a CTA's warps share about a tile of new tokens.
+struct Tile {
+  const float* cosine;     // [nt][pairs]
+  const float* sine;
+  const long long* slot;   // [nt] element of the page slot in its KV head 0, or -1: not stored
+  int nt, pairs, rot_items, tail, D;
+  bool interleaved;
+};
+
+// The rows of one head: rotated (ROT), copied to dst + (slot, or tt * dst_ts),
+// and their bounds taken (BOUNDS).
+template <typename T, int VEC, bool ROT, bool BOUNDS>
+__device__ __forceinline__ void head_rows(const Tile& t, const T* src, long long ts, T* dst, const long long* slot,
+                                          long long dst_ts, int lane, float* lo, float* hi, bool fold) {
+  const int rots = ROT ? t.rot_items : 0, tail = ROT ? t.tail : 0;
+  const int items = rots + (t.D - tail + 2 * VEC - 1) / (2 * VEC);
+  int width = 1;  // lanes along a head's items; the others take further tokens
+  while (width < items && width < 32) width <<= 1;
+  const int step = 32 / width, li = lane & (width - 1), lt = lane / width;
+  for (int it = li; it - li < items; it += width) {
+    const bool active = it < items, turn = ROT && it < rots;
+    int o1, o2;
+    if (turn) {
+      o1 = t.interleaved ? 2 * it * VEC : it * VEC;
+      o2 = t.interleaved ? o1 + VEC : t.pairs + it * VEC;
+    } else {
+      o1 = tail + 2 * (it - rots) * VEC;
+      o2 = o1 + VEC;
+    }
+    const bool second = o2 < t.D;
+    Bounds<T, VEC> bounds;
+    constexpr int U = BOUNDS ? 2 : 4;  // tokens in flight per lane
+    for (int tt = lt; active && tt < t.nt; tt += U * step) {
+      Vec<T, VEC> x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const T* s = src + min(tt + u * step, t.nt - 1) * ts;
+        x[u] = *reinterpret_cast<const Vec<T, VEC>*>(s + o1);
+        y[u] = *reinterpret_cast<const Vec<T, VEC>*>(second ? s + o2 : s + o1);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int tk = tt + u * step;
+        if (tk >= t.nt) break;
+        if (turn) {
+          const float* cs = t.cosine + tk * t.pairs + it * VEC;
+          const float* sn = t.sine + tk * t.pairs + it * VEC;
+          float c[VEC], w[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; e += VEC >= 4 ? 4 : 1) {
+            if constexpr (VEC >= 4) {
+              *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(cs + e);
+              *reinterpret_cast<float4*>(w + e) = *reinterpret_cast<const float4*>(sn + e);
+            } else {
+              c[e] = cs[e];
+              w[e] = sn[e];
+            }
+          }
+          auto pair = [&](T& first, T& other, int e) {
+            const float p = to_f32(first), q = to_f32(other);
+            first = from_f32<T>(__fsub_rn(__fmul_rn(p, c[e]), __fmul_rn(q, w[e])));
+            other = from_f32<T>(__fadd_rn(__fmul_rn(q, c[e]), __fmul_rn(p, w[e])));
+          };
+          if (t.interleaved) {
+            auto at = [&](int i) -> T& { return i < VEC ? x[u].e[i] : y[u].e[i - VEC]; };
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) pair(at(2 * e), at(2 * e + 1), e);
+          } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) pair(x[u].e[e], y[u].e[e], e);
+          }
+        }
+        const long long to = slot ? slot[tk] : tk * dst_ts;
+        if (to < 0) continue;
+        *reinterpret_cast<Vec<T, VEC>*>(dst + to + o1) = x[u];
+        if (second) *reinterpret_cast<Vec<T, VEC>*>(dst + to + o2) = y[u];
+        if constexpr (BOUNDS) {
+          bounds.add(x[u], 0);
+          bounds.add(y[u], 1);
+        }
+      }
+    }
+    if constexpr (BOUNDS) {
+      __syncwarp();
+      for (int o = width; o < 32; o <<= 1) bounds.join(o);
+      if (active && lt == 0) {
+        // The block's first token resets its bounds; later tokens fold into
+        // them (this warp alone writes this head's bounds).
+#pragma unroll
+        for (int e = 0; e < 2 * VEC; ++e) {
+          if (e >= VEC && !second) continue;
+          const int at = e < VEC ? o1 + e : o2 + e - VEC;
+          lo[at] = fold ? min_nan(lo[at], bounds.low(e)) : bounds.low(e);
+          hi[at] = fold ? max_nan(hi[at], bounds.high(e)) : bounds.high(e);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kAppendWarps * 32, VEC > 1 ? 3 : 2) append_kernel(AppendArgs a, int tile_tokens) {
+  extern __shared__ float tables[];  // cosines, then sines, of tile_tokens tokens
+  __shared__ long long slot[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int B = a.L.b, D = a.L.d;
+  const int B = a.L.b, D = a.L.d, hkv = a.L.hkv, ps = a.L.page_size;
   int r, t0, n, f;
   if (a.token_offsets == nullptr) {
     r = blockIdx.x;
@@ -82,159 +269,74 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(AppendArgs a,
     if (tid == 0) report(a.status, kStatusBadLength);
     return;
   }
-  const int j = len / B + f;                                 // block of the request
-  const int begin = max(len, j * B), end = static_cast<int>(min(static_cast<long long>(len) + n, (j + 1ll) * B));
+  const int j = len / B + f;  // block of the request
+  const int begin = max(len, j * B);
+  const int end = static_cast<int>(min(static_cast<long long>(len) + n, (j + 1ll) * B));
   if (begin >= end) return;
   const bool room = j < request_blocks(a.L, r);
   if (!room && tid == 0) report(a.status, kStatusBadLength);
-  const int ppb = B / a.L.page_size;
   const int base = a.L.block_offsets ? a.L.block_offsets[r] : 0;
-  const int* table = a.L.page_table + (static_cast<long long>(base) + j) * ppb;
+  const int* table = a.L.page_table + (static_cast<long long>(base) + j) * (B / ps);
 
-  const int rot_items = a.cos ? a.pairs / VEC : 0;
-  const int stride = a.pairs + rot_items;
-  const int tail0 = a.cos ? 2 * a.pairs : 0;                // first dim that passes through
-  const int row_items = rot_items + (D - tail0 + 2 * VEC - 1) / (2 * VEC);
-  const int copy_items = (D + 2 * VEC - 1) / (2 * VEC);
-  const int heads = (a.q ? a.hq : 0) + 2 * a.L.hkv;
-  const int hq = a.q ? a.hq : 0;
-
+  Tile t;
+  t.pairs = a.cos ? a.pairs : 0;
+  t.rot_items = t.pairs / VEC;
+  t.tail = 2 * t.pairs;
+  t.D = D;
+  t.interleaved = a.interleaved != 0;
+  float* cosine = tables;
+  float* sine = tables + tile_tokens * t.pairs;
+  t.cosine = cosine;
+  t.sine = sine;
+  t.slot = slot;
+  const int hq = a.q ? a.hq : 0, heads = hq + 2 * hkv;
   for (int tile = begin; tile < end; tile += tile_tokens) {
-    const int nt = min(tile_tokens, end - tile);
-    if (a.cos) {
-      if (tile != begin) __syncthreads();
-      for (int i = tid; i < nt * a.pairs; i += blockDim.x) {
-        const int tt = i / a.pairs, p = i - tt * a.pairs;
+    t.nt = min(tile_tokens, end - tile);
+    const int token = t0 + (tile - len);  // packed token of the tile's first
+    if (tile != begin) __syncthreads();
+    if (tid < t.nt) {
+      const int in = tile + tid - j * B, pg = in / ps;
+      const int page = room ? table[pg] : -1;
+      if (room && (page < 0 || page >= a.pages)) report(a.status, kStatusBadBlockId);
+      slot[tid] = page < 0 || page >= a.pages ? -1 : (static_cast<long long>(page) * hkv * ps + (in - pg * ps)) * D;
+    }
+    for (int tt = warp; tt < t.nt; tt += kAppendWarps) {
+      for (int p = lane; p < t.pairs; p += 32) {
         int pos = tile + tt;
         if (a.positions) {
           const int ax = a.axis ? a.axis[p] : 0;
-          pos = ax < a.axes ? a.positions[static_cast<long long>(ax) * a.T + t0 + (tile + tt - len)] : -1;
+          pos = ax < a.axes ? a.positions[static_cast<long long>(ax) * a.T + token + tt] : -1;
         }
         if (pos < 0 || pos >= a.max_position) {
           report(a.status, kStatusBadPosition);
           pos = 0;
         }
-        const long long o = static_cast<long long>(pos) * a.pairs + p;
-        turn[tt * stride + p % VEC * rot_items + p / VEC] = make_float2(a.cos[o], a.sin[o]);
+        const long long o = static_cast<long long>(pos) * t.pairs + p;
+        cosine[tt * t.pairs + p] = a.cos[o];
+        sine[tt * t.pairs + p] = a.sin[o];
       }
-      __syncthreads();
     }
+    __syncthreads();
     for (int hd = blockIdx.y * kAppendWarps + warp; hd < heads; hd += gridDim.y * kAppendWarps) {
-      // kind 0: query head, 1: key head, 2: value head.
-      const int kind = hd < hq ? 0 : hd < hq + a.L.hkv ? 1 : 2;
-      const int h = kind == 0 ? hd : kind == 1 ? hd - hq : hd - hq - a.L.hkv;
-      if (kind != 0 && !room) continue;
-      const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
-                     h * (kind == 0 ? a.q_hs : kind == 1 ? a.k_hs : a.v_hs);
-      const long long ts = kind == 0 ? a.q_ts : kind == 1 ? a.k_ts : a.v_ts;
-      T* dst = static_cast<T*>(kind == 0 ? a.q_out : const_cast<void*>(kind == 1 ? a.L.k : a.L.v));
-      const int items = kind == 2 ? copy_items : row_items;
-      const int rots = kind == 2 ? 0 : rot_items;
-      const int tail = kind == 2 ? 0 : tail0;
-      int width = 1;  // lanes along a head's items; the others take further tokens
-      while (width < items && width < 32) width <<= 1;
-      const int tlanes = 32 / width, li = lane & (width - 1), lt = lane / width;
-      for (int it = li; it - li < items; it += width) {
-        const bool active = it < items;
-        int o1, o2;
-        if (it < rots) {
-          o1 = a.interleaved ? 2 * it * VEC : it * VEC;
-          o2 = a.interleaved ? o1 + VEC : a.pairs + it * VEC;
-        } else {
-          o1 = tail + 2 * (it - rots) * VEC;
-          o2 = o1 + VEC;
-        }
-        const bool second = o2 < D;
-        float mn[2 * VEC], mx[2 * VEC];
-#pragma unroll
-        for (int e = 0; e < 2 * VEC; ++e) {
-          mn[e] = __int_as_float(0x7f800000);
-          mx[e] = neg_inf();
-        }
-        if (active) {
-          constexpr int U = 4;  // tokens in flight per lane
-          for (int tt = lt; tt < nt; tt += U * tlanes) {
-            Vec<T, VEC> x[U], y[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int tk = tt + u * tlanes;
-              if (tk < nt) {
-                const T* s = src + static_cast<long long>(t0 + (tile + tk - len)) * ts;
-                x[u] = *reinterpret_cast<const Vec<T, VEC>*>(s + o1);
-                if (second) y[u] = *reinterpret_cast<const Vec<T, VEC>*>(s + o2); else y[u] = x[u];
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int tk = tt + u * tlanes;
-              if (tk >= nt) continue;
-              const int at = tile + tk;  // the token's place in its request
-              if (it < rots) {
-                const float2* cs = turn + tk * stride + it;
-                auto pair = [&](T& first, T& other, int e) {
-                  const float p = to_f32(first), w = to_f32(other);
-                  const float2 c = cs[e * rot_items];
-                  first = from_f32<T>(__fsub_rn(__fmul_rn(p, c.x), __fmul_rn(w, c.y)));
-                  other = from_f32<T>(__fadd_rn(__fmul_rn(w, c.x), __fmul_rn(p, c.y)));
-                };
-                if (a.interleaved) {
-                  auto at = [&](int i) -> T& { return i < VEC ? x[u].e[i] : y[u].e[i - VEC]; };
-#pragma unroll
-                  for (int e = 0; e < VEC; ++e) pair(at(2 * e), at(2 * e + 1), e);
-                } else {
-#pragma unroll
-                  for (int e = 0; e < VEC; ++e) pair(x[u].e[e], y[u].e[e], e);
-                }
-              }
-              T* d;
-              if (kind == 0) {
-                d = dst + (static_cast<long long>(t0 + (at - len)) * a.hq + h) * D;
-              } else {
-                const int in = at - j * B, pg = in / a.L.page_size;
-                const int page = table[pg];
-                if (page < 0 || page >= a.pages) {
-                  report(a.status, kStatusBadBlockId);
-                  continue;
-                }
-                d = dst + ((static_cast<long long>(page) * a.L.hkv + h) * a.L.page_size + (in - pg * a.L.page_size)) * D;
-              }
-              *reinterpret_cast<Vec<T, VEC>*>(d + o1) = x[u];
-              if (second) *reinterpret_cast<Vec<T, VEC>*>(d + o2) = y[u];
-              if (kind == 1) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                  const float p = to_f32(x[u].e[e]), s = to_f32(y[u].e[e]);
-                  mn[e] = min_nan(mn[e], p);
-                  mx[e] = max_nan(mx[e], p);
-                  mn[VEC + e] = min_nan(mn[VEC + e], s);
-                  mx[VEC + e] = max_nan(mx[VEC + e], s);
-                }
-              }
-            }
-          }
-        }
-        if (kind == 1 && a.lo != nullptr) {
-#pragma unroll
-          for (int e = 0; e < 2 * VEC; ++e) {
-            for (int o = width; o < 32; o <<= 1) {
-              mn[e] = min_nan(mn[e], __shfl_xor_sync(kFull, mn[e], o));
-              mx[e] = max_nan(mx[e], __shfl_xor_sync(kFull, mx[e], o));
-            }
-          }
-          if (active && lt == 0) {
-            // The block's first token resets its bounds; later tokens fold
-            // into them (this warp alone writes this head's bounds).
-            const bool fold = tile > j * B;
-            const long long o = (static_cast<long long>(h) * a.total + base + j) * D;
-#pragma unroll
-            for (int e = 0; e < 2 * VEC; ++e) {
-              if (e >= VEC && !second) continue;
-              const long long at = o + (e < VEC ? o1 + e : o2 + e - VEC);
-              a.lo[at] = fold ? min_nan(a.lo[at], mn[e]) : mn[e];
-              a.hi[at] = fold ? max_nan(a.hi[at], mx[e]) : mx[e];
-            }
-          }
-        }
+      if (hd < hq) {
+        const T* src = static_cast<const T*>(a.q) + token * a.q_ts + hd * a.q_hs;
+        T* dst = static_cast<T*>(a.q_out) + (static_cast<long long>(token) * a.hq + hd) * D;
+        head_rows<T, VEC, true, false>(t, src, a.q_ts, dst, nullptr, static_cast<long long>(a.hq) * D, lane, nullptr,
+                                       nullptr, false);
+      } else if (hd < hq + hkv) {
+        const int h = hd - hq;
+        const T* src = static_cast<const T*>(a.k) + token * a.k_ts + h * a.k_hs;
+        T* dst = static_cast<T*>(const_cast<void*>(a.L.k)) + static_cast<long long>(h) * ps * D;
+        const long long o = (static_cast<long long>(h) * a.total + base + j) * D;
+        if (a.lo != nullptr && room)
+          head_rows<T, VEC, true, true>(t, src, a.k_ts, dst, slot, 0, lane, a.lo + o, a.hi + o, tile > j * B);
+        else
+          head_rows<T, VEC, true, false>(t, src, a.k_ts, dst, slot, 0, lane, nullptr, nullptr, false);
+      } else {
+        const int h = hd - hq - hkv;
+        const T* src = static_cast<const T*>(a.v) + token * a.v_ts + h * a.v_hs;
+        T* dst = static_cast<T*>(const_cast<void*>(a.L.v)) + static_cast<long long>(h) * ps * D;
+        head_rows<T, VEC, false, false>(t, src, a.v_ts, dst, slot, 0, lane, nullptr, nullptr, false);
       }
     }
   }
@@ -247,7 +349,7 @@ static int launch_append_t(const AppendArgs& a, cudaStream_t stream) {
   // 32 tokens of tables per tile up to 128 pairs, fewer for wider heads.
   const int pairs = a.cos ? a.pairs : 0;
   const int tile = pairs <= 128 ? 32 : 8;
-  const size_t smem = static_cast<size_t>(tile) * (pairs + pairs / VEC) * sizeof(float2);
+  const size_t smem = static_cast<size_t>(tile) * pairs * sizeof(float2);
   auto kern = append_kernel<T, VEC>;
   if (smem > 48 * 1024)
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));

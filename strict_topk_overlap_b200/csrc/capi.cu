@@ -1053,5 +1053,5 @@ extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, l
                                             : launch_rows_attn(a, kv->kv_dtype, st);
     if (r2) return cuda_status(r2, "paged attention");
   }
-  return p.join ? cuda_status(launch_join(j, st), "attention join") : 0;
+  return p.join ? cuda_status(launch_join(j, sm_count_current(), st), "attention join") : 0;
 }

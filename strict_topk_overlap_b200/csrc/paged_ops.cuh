@@ -202,6 +202,6 @@ struct JoinArgs {
   float* lse;
 };
 
-int launch_join(const JoinArgs& a, cudaStream_t stream);
+int launch_join(const JoinArgs& a, int sms, cudaStream_t stream);
 
 }  // namespace stk

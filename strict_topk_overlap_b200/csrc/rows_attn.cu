@@ -264,14 +264,21 @@ int launch_rows_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream) 
 }
 
 // ------------------------------------------------------------------ join
-// out = sum_s e^{m_s - M} o_s / sum_s e^{m_s - M} l_s over the parts of a row,
-// in part order; parts without keys have m = -inf. One warp per row; the
-// parts' states are FP32 and read once (L2-resident).
-template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(JoinArgs a) {
+// out = sum_s e^{m_s - M} o_s / sum_s e^{m_s - M} l_s over the parts of a row;
+// parts without keys have m = -inf and are not read. The parts' states are
+// FP32 and read once (L2-resident); the kernel is bound by its few dependent
+// loads. WPR warps share a row: with one, a CTA joins eight rows; where there
+// are too few rows to fill the SMs that way, all eight warps take every eighth
+// part of one row and add up in shared memory, in warp order. Lanes hold V
+// consecutive dims (d = 32 V) or, V = 0, every 32nd.
+constexpr int kJoinWarps = 8;
+
+template <typename T, int V, int WPR>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(JoinArgs a) {
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = WPR == 1 ? blockIdx.x * kJoinWarps + warp : blockIdx.x;
+  const int first_part = WPR == 1 ? 0 : warp;
   if (row >= a.rows) return;
   // Part s of source k is state base[k] + s * step[k].
   long long base[2], step[2];
@@ -313,50 +320,96 @@ __global__ void __launch_bounds__(128) join_kernel(JoinArgs a) {
   for (int k = 0; k < 2; ++k)
     for (int s = lane; s < parts[k]; s += 32) M = fmaxf(M, a.src[k].ml[base[k] + s * step[k]].x);
   M = warp_max(M);
-  float Z = 0.f;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    for (int s = lane; s < parts[k]; s += 32) {
-      const float2 ml = a.src[k].ml[base[k] + s * step[k]];
-      if (ml.x != neg_inf()) Z += expf(ml.x - M) * ml.y;
-    }
-  Z = warp_sum(Z);
   const bool empty = M == neg_inf();
-  for (int d0 = lane; d0 < a.d; d0 += 128) {
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int N = V ? V : 4;
+  __shared__ float sum_o[WPR == 1 ? 1 : kJoinWarps][32 * N + 1];
+  for (int d0 = 0; d0 < a.d; d0 += 32 * N) {
+    float o[N], Z = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = 0.f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-#pragma unroll 4
-      for (int s = 0; s < parts[k]; ++s) {
-        const long long at = base[k] + s * step[k];
-        const float m = a.src[k].ml[at].x;
-        if (m == neg_inf()) continue;
-        const float c = expf(m - M);
-        const float* p = a.src[k].o + at * a.d + d0;
+      // Lane i has the weight of part first_part + WPR (s0 + i).
+      for (int s0 = 0; first_part + WPR * s0 < parts[k]; s0 += 32) {
+        const int s = first_part + WPR * (s0 + lane);
+        float c = 0.f;
+        if (s < parts[k]) {
+          const float2 ml = a.src[k].ml[base[k] + s * step[k]];
+          c = ml.x == neg_inf() ? 0.f : expf(ml.x - M);
+          Z += c == 0.f ? 0.f : c * ml.y;
+        }
+        const int count = min(32, (parts[k] - first_part + WPR - 1) / WPR - s0);
+#pragma unroll 8
+        for (int i = 0; i < count; ++i) {
+          const float w = __shfl_sync(kFull, c, i);
+          if (w == 0.f) continue;  // also a part that was never written
+          const float* p = a.src[k].o + (base[k] + (first_part + WPR * (s0 + i)) * step[k]) * a.d + d0;
+          float x[N];
+          if constexpr (V != 0) {
+            load_vec<float, N>(p + lane * N, x);
+          } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d0 + 32 * j < a.d) o[j] = fmaf(c, p[32 * j], o[j]);
+            for (int j = 0; j < N; ++j) x[j] = d0 + lane + 32 * j < a.d ? p[lane + 32 * j] : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < N; ++j) o[j] = fmaf(w, x[j], o[j]);
+        }
       }
     }
+    Z = warp_sum(Z);
+    if constexpr (WPR > 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (d0 + 32 * j >= a.d) continue;
+      for (int j = 0; j < N; ++j) sum_o[warp][lane * N + j] = o[j];
+      if (lane == 0) sum_o[warp][32 * N] = Z;
+      __syncthreads();
+      if (warp == 0) {
+        Z = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+          Z += sum_o[w][32 * N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) o[j] += sum_o[w][lane * N + j];
+        }
+      }
+      __syncthreads();
+      if (warp != 0) continue;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int dd = d0 + (V ? lane * N + j : lane + 32 * j);
+      if (dd >= a.d) continue;
       const float y = empty ? 0.f : o[j] / Z;
-      T* out = static_cast<T*>(a.out) + static_cast<long long>(row) * a.d + d0 + 32 * j;
+      T* out = static_cast<T*>(a.out) + static_cast<long long>(row) * a.d + dd;
       if constexpr (sizeof(T) == 4) *out = y;
       else if constexpr (std::is_same<T, __half>::value) *out = __float2half_rn(y);
       else *out = __float2bfloat16_rn(y);
     }
+    if (d0 == 0 && lane == 0 && a.lse) a.lse[row] = empty ? neg_inf() : M + logf(Z);
   }
-  if (lane == 0 && a.lse) a.lse[row] = empty ? neg_inf() : M + logf(Z);
 }
 
-int launch_join(const JoinArgs& a, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((a.rows + 3) / 4));
+template <typename T, int V>
+static int launch_join_v(const JoinArgs& a, int sms, cudaStream_t stream) {
+  if (a.rows >= 2 * sms * kJoinWarps)
+    return launch_pdl(join_kernel<T, V, 1>, dim3(static_cast<unsigned>((a.rows + kJoinWarps - 1) / kJoinWarps)),
+                      dim3(kJoinWarps * 32), 0, stream, 0, a);
+  return launch_pdl(join_kernel<T, V, kJoinWarps>, dim3(static_cast<unsigned>(a.rows)), dim3(kJoinWarps * 32), 0,
+                    stream, 0, a);
+}
+
+template <typename T>
+static int launch_join_t(const JoinArgs& a, int sms, cudaStream_t stream) {
+  return a.d == 128 ? launch_join_v<T, 4>(a, sms, stream)
+         : a.d == 64 ? launch_join_v<T, 2>(a, sms, stream) : launch_join_v<T, 0>(a, sms, stream);
+}
+
+int launch_join(const JoinArgs& a, int sms, cudaStream_t stream) {
   switch (a.dtype) {
-    case kF32: return launch_pdl(join_kernel<float>, grid, dim3(128), 0, stream, 0, a);
-    case kF16: return launch_pdl(join_kernel<__half>, grid, dim3(128), 0, stream, 0, a);
-    default: return launch_pdl(join_kernel<__nv_bfloat16>, grid, dim3(128), 0, stream, 0, a);
+    case kF32: return launch_join_t<float>(a, sms, stream);
+    case kF16: return launch_join_t<__half>(a, sms, stream);
+    default: return launch_join_t<__nv_bfloat16>(a, sms, stream);
   }
 }
 
