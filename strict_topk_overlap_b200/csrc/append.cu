@@ -154,6 +154,82 @@ struct Tile {
   bool interleaved;
 };
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// (x, y) -> (x c - y s, y c + x s), each product and sum rounded by itself.
+__device__ __forceinline__ float2 turned(float x, float y, float c, float s) {
+  return make_float2(__fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s)), __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s)));
+}
+
+// Rotates a lane's VEC pairs: element e of x with element e of y, or, when
+// interleaved, the neighbours in x and then in y. 16-bit vectors are taken
+// word by word (two elements), so that nothing is unpacked beyond a pair.
+template <typename T, int VEC>
+__device__ __forceinline__ void turn_pairs(Vec<T, VEC>& x, Vec<T, VEC>& y, const float* cosine, const float* sine,
+                                           bool interleaved) {
+  if constexpr (VEC == 1) {
+    const float2 z = turned(to_f32(x.e[0]), to_f32(y.e[0]), cosine[0], sine[0]);
+    x.e[0] = from_f32<T>(z.x);
+    y.e[0] = from_f32<T>(z.y);
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 c = *reinterpret_cast<const float4*>(cosine), s = *reinterpret_cast<const float4*>(sine);
+    if (interleaved) {
+      float2 z = turned(x.e[0], x.e[1], c.x, s.x), w = turned(x.e[2], x.e[3], c.y, s.y);
+      x = {z.x, z.y, w.x, w.y};
+      z = turned(y.e[0], y.e[1], c.z, s.z);
+      w = turned(y.e[2], y.e[3], c.w, s.w);
+      y = {z.x, z.y, w.x, w.y};
+    } else {
+      const float2 z0 = turned(x.e[0], y.e[0], c.x, s.x), z1 = turned(x.e[1], y.e[1], c.y, s.y);
+      const float2 z2 = turned(x.e[2], y.e[2], c.z, s.z), z3 = turned(x.e[3], y.e[3], c.w, s.w);
+      x = {z0.x, z1.x, z2.x, z3.x};
+      y = {z0.y, z1.y, z2.y, z3.y};
+    }
+  } else {
+    uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
+    uint32_t* yw = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {  // pairs 4q .. 4q + 3
+      const float4 c = *reinterpret_cast<const float4*>(cosine + 4 * q);
+      const float4 s = *reinterpret_cast<const float4*>(sine + 4 * q);
+      if (interleaved) {
+        uint32_t* w = q == 0 ? xw : yw;
+        float2 p = unpack_pair<T>(w[0]), z = turned(p.x, p.y, c.x, s.x);
+        w[0] = pack_pair<T>(z.x, z.y);
+        p = unpack_pair<T>(w[1]), z = turned(p.x, p.y, c.y, s.y);
+        w[1] = pack_pair<T>(z.x, z.y);
+        p = unpack_pair<T>(w[2]), z = turned(p.x, p.y, c.z, s.z);
+        w[2] = pack_pair<T>(z.x, z.y);
+        p = unpack_pair<T>(w[3]), z = turned(p.x, p.y, c.w, s.w);
+        w[3] = pack_pair<T>(z.x, z.y);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 p = unpack_pair<T>(xw[2 * q + i]), r = unpack_pair<T>(yw[2 * q + i]);
+          const float2 z0 = turned(p.x, r.x, i ? c.z : c.x, i ? s.z : s.x);
+          const float2 z1 = turned(p.y, r.y, i ? c.w : c.y, i ? s.w : s.y);
+          xw[2 * q + i] = pack_pair<T>(z0.x, z1.x);
+          yw[2 * q + i] = pack_pair<T>(z0.y, z1.y);
+        }
+      }
+    }
+  }
+}
+
 // The rows of one head: rotated (ROT), copied to dst + (slot, or tt * dst_ts),
 // and their bounds taken (BOUNDS).
 template <typename T, int VEC, bool ROT, bool BOUNDS>
@@ -189,34 +265,8 @@ __device__ __forceinline__ void head_rows(const Tile& t, const T* src, long long
       for (int u = 0; u < U; ++u) {
         const int tk = tt + u * step;
         if (tk >= t.nt) break;
-        if (turn) {
-          const float* cs = t.cosine + tk * t.pairs + it * VEC;
-          const float* sn = t.sine + tk * t.pairs + it * VEC;
-          float c[VEC], w[VEC];
-#pragma unroll
-          for (int e = 0; e < VEC; e += VEC >= 4 ? 4 : 1) {
-            if constexpr (VEC >= 4) {
-              *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(cs + e);
-              *reinterpret_cast<float4*>(w + e) = *reinterpret_cast<const float4*>(sn + e);
-            } else {
-              c[e] = cs[e];
-              w[e] = sn[e];
-            }
-          }
-          auto pair = [&](T& first, T& other, int e) {
-            const float p = to_f32(first), q = to_f32(other);
-            first = from_f32<T>(__fsub_rn(__fmul_rn(p, c[e]), __fmul_rn(q, w[e])));
-            other = from_f32<T>(__fadd_rn(__fmul_rn(q, c[e]), __fmul_rn(p, w[e])));
-          };
-          if (t.interleaved) {
-            auto at = [&](int i) -> T& { return i < VEC ? x[u].e[i] : y[u].e[i - VEC]; };
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) pair(at(2 * e), at(2 * e + 1), e);
-          } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) pair(x[u].e[e], y[u].e[e], e);
-          }
-        }
+        if (turn) turn_pairs<T, VEC>(x[u], y[u], t.cosine + tk * t.pairs + it * VEC, t.sine + tk * t.pairs + it * VEC,
+                                     t.interleaved);
         const long long to = slot ? slot[tk] : tk * dst_ts;
         if (to < 0) continue;
         *reinterpret_cast<Vec<T, VEC>*>(dst + to + o1) = x[u];

@@ -40,18 +40,66 @@ def empty_paged_cache(capacities, hkv, dim, block_size, page_size, *, dtype=torc
                         -lo, block_size, page_size, max(blocks))
 
 
-def _check_ints(t, shape, name, device):
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be contiguous int32 of shape {tuple(shape)} on the cache's device")
+def _ints(x, shape, name, dev):
+    """Address of an int32 tensor of this shape."""
+    if x.dtype != torch.int32 or x.shape != shape or x.device != dev or not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 of shape {shape} on the cache's device")
+    return x.data_ptr()
 
 
-def _check_rows(x, cache, heads, name):
-    if x.ndim != 3 or x.shape[1] != heads or x.shape[2] != cache.k_pages.shape[3]:
-        raise ValueError(f"{name} must be [T, {heads}, D]")
-    if x.dtype != cache.k_pages.dtype or x.device != cache.k_pages.device:
+def _rows(x, shape, name, pool):
+    """Address and token and head strides of rows [T, heads, D]."""
+    if x.shape != shape:
+        raise ValueError(f"{name} must be [T, heads, D] = {shape}, got {tuple(x.shape)}")
+    if x.dtype != pool.dtype or x.device != pool.device:
         raise ValueError(f"{name} must have the cache's dtype and device")
-    if x.stride(2) != 1 and x.shape[2] > 1:
+    token, head, unit = x.stride()
+    if unit != 1 and shape[2] > 1:
         raise ValueError(f"{name} must have unit stride along D")
+    return x.data_ptr(), token, head
+
+
+def _heads(q, hkv, name="q"):
+    """Tokens and heads of q [T, Hq, D]."""
+    if q.ndim != 3 or q.shape[1] == 0 or q.shape[1] % hkv:
+        raise ValueError(f"{name} must be [T, Hq, D] with Hq a multiple of the KV heads")
+    return q.shape[0], q.shape[1]
+
+
+def _tokens(token_offsets, t, requests, dev):
+    """Address of the packed tokens' offsets, or None for one token per request."""
+    if token_offsets is not None:
+        return _ints(token_offsets, (requests + 1,), "token_offsets", dev)
+    if t != requests:
+        raise ValueError("without token_offsets there must be one token per request")
+    return None
+
+
+def _rotary(rotary, positions, t, dev):
+    """The call's stk_rotary and the positions' address."""
+    if rotary is None:
+        if positions is not None:
+            raise ValueError("positions need a rotary table")
+        return None, None
+    cos, sin, axis = rotary.cos, rotary.sin, rotary.axis
+    size = cos.shape
+    if len(size) != 2 or sin.shape != size or cos.dtype != torch.float32 or sin.dtype != torch.float32 or \
+            cos.device != dev or sin.device != dev or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("rotary cos / sin must be contiguous FP32 [positions, pairs] on the cache's device")
+    axes, at = 1, None
+    if positions is not None:
+        axes = positions.shape[0] if positions.ndim == 2 else 1
+        at = _ints(positions, (axes, t) if positions.ndim == 2 else (t,), "positions", dev)
+    if axis is None:
+        if axes > 1:
+            raise ValueError("positions with several axes need a rotary axis for each pair")
+    else:
+        if axis.dtype != torch.uint8 or axis.shape != size[1:] or axis.device != dev or not axis.is_contiguous():
+            raise ValueError("rotary axis must be uint8 [pairs] on the cache's device")
+        if positions is None:
+            raise ValueError("several rotary axes need positions [axes, T]")
+        axis = axis.data_ptr()
+    return L.StkRotary(cos.data_ptr(), sin.data_ptr(), size[1], size[0], rotary.interleaved, axes, axis), at
 
 
 def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=None, rotary: Rotary | None = None,
@@ -65,57 +113,26 @@ def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=N
     strides). Updates the pages and, where the cache keeps them, the blocks'
     lo / hi; returns the rotated q [T, Hq, D] (``q_out``, which may be q
     itself), or None without q."""
-    pool, hkv = cache.k_pages, cache.hkv
-    dev, requests = pool.device, cache.requests
-    _check_rows(k, cache, hkv, "k")
-    _check_rows(v, cache, hkv, "v")
+    pool = cache.k_pages
+    pages, hkv, _, d = pool.shape
+    dev, requests, blocks = pool.device, cache.requests, cache.total_blocks
     t = k.shape[0]
-    if v.shape[0] != t:
-        raise ValueError("k and v must have the same number of tokens")
-    _check_ints(lengths, (requests,), "lengths", dev)
-    if token_offsets is not None:
-        _check_ints(token_offsets, (requests + 1,), "token_offsets", dev)
-    elif t != requests:
-        raise ValueError("without token_offsets there must be one token per request")
-    hq = qt = qh = 0
+    kp, kt, kh = _rows(k, (t, hkv, d), "k", pool)
+    vp, vt, vh = _rows(v, (t, hkv, d), "v", pool)
+    before = _ints(lengths, (requests,), "lengths", dev)
+    offsets = _tokens(token_offsets, t, requests, dev)
+    qp = qt = qh = hq = out = 0
     if q is not None:
-        hq = q.shape[1] if q.ndim == 3 else 0
-        _check_rows(q, cache, hq, "q")
-        if q.shape[0] != t or hq == 0 or hq % hkv:
-            raise ValueError("q must be [T, Hq, D] with Hq a multiple of the KV heads")
+        _, hq = _heads(q, hkv)
+        qp, qt, qh = _rows(q, (t, hq, d), "q", pool)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            q_out = q.new_empty((t, hq, d))
         elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != dev or not q_out.is_contiguous():
             raise ValueError("q_out must be contiguous, of q's shape, dtype and device")
-        qt, qh = q.stride(0), q.stride(1)
-    turn = None
-    if rotary is not None:
-        cos, sin, axis = rotary.cos, rotary.sin, rotary.axis
-        if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or \
-                cos.device != dev or sin.device != dev or not (cos.is_contiguous() and sin.is_contiguous()):
-            raise ValueError("rotary cos / sin must be contiguous FP32 [positions, pairs] on the cache's device")
-        axes = 1
-        if positions is not None:
-            axes = positions.shape[0] if positions.ndim == 2 else 1
-            _check_ints(positions, (axes, t) if positions.ndim == 2 else (t,), "positions", dev)
-        if axis is not None:
-            if axis.dtype != torch.uint8 or axis.shape != cos.shape[1:] or axis.device != dev or \
-                    not axis.is_contiguous():
-                raise ValueError("rotary axis must be uint8 [pairs] on the cache's device")
-            if positions is None:
-                raise ValueError("several rotary axes need positions [axes, T]")
-        elif axes > 1:
-            raise ValueError("positions with several axes need a rotary axis for each pair")
-        turn = L.StkRotary(cos.data_ptr(), sin.data_ptr(), cos.shape[1], cos.shape[0], int(rotary.interleaved), axes,
-                           L.ptr(axis))
-    elif positions is not None:
-        raise ValueError("positions need a rotary table")
-    bounds = cache.total_blocks > 0
-    kv = cache.kv()
-    rc = L.load().stk_append_tokens(
-        kv, pool.shape[0], requests, cache.total_blocks if bounds else 1, t, k.data_ptr(), k.stride(0), k.stride(1),
-        v.data_ptr(), v.stride(0), v.stride(1), L.ptr(q), qt, qh, hq, L.ptr(q_out) if q is not None else None,
-        lengths.data_ptr(), L.ptr(token_offsets), L.ptr(positions), turn, cache.lo.data_ptr() if bounds else None,
-        cache.hi.data_ptr() if bounds else None, L.status_ptr(), L.stream_of(pool))
+        out = q_out.data_ptr()
+    turn, at = _rotary(rotary, positions, t, dev)
+    lo, hi = (cache.lo.data_ptr(), cache.hi.data_ptr()) if blocks else (None, None)
+    rc = L.load().stk_append_tokens(cache.kv(), pages, requests, blocks or 1, t, kp, kt, kh, vp, vt, vh, qp, qt, qh, hq,
+                                    out, before, offsets, at, turn, lo, hi, L.status_ptr(), L.stream_of(pool))
     L.check(rc, "append_tokens")
     return q_out if q is not None else None

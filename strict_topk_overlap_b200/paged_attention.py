@@ -11,68 +11,81 @@ lists of blocks only.
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _lib as L
 from .paged import PagedKVCache
-from .paged_append import _check_ints, _check_rows
+from .paged_append import _heads, _ints, _rows, _tokens
 
 
 def _most(max_tokens, tokens, token_offsets):
     """Bound on a request's new tokens."""
-    if token_offsets is None:
+    if token_offsets is None or tokens == 0:
         return min(1, tokens)
-    return tokens if max_tokens is None else min(int(max_tokens), tokens)
+    if max_tokens is None:
+        return tokens
+    if max_tokens < 1:
+        raise ValueError("max_tokens must be positive")
+    return min(int(max_tokens), tokens)
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(device, dtype, hkv, block, dim, page, requests, tokens, hq, packed, most, longest, prefix):
+    """Workspace of a call, from its sizes alone (a pool address stands for any)."""
+    any_pool = 256
+    kv = L.StkKV(any_pool, any_pool, dtype, hkv, 0, block, dim, any_pool, any_pool, page, 0)
+    with torch.cuda.device(device):
+        return L.load().stk_paged_attention_workspace_bytes(kv, requests, tokens, hq, packed, most, longest, prefix)
 
 
 def attention_workspace(cache: PagedKVCache, tokens, hq, *, token_offsets=None, max_tokens=None, prefix=0):
-    """Workspace for ``attention`` (or, with ``prefix``, ``shared_prefix_attention``) of up to these sizes."""
-    need = L.load().stk_paged_attention_workspace_bytes(cache.kv(), cache.requests, tokens, hq,
-                                                        int(token_offsets is not None),
-                                                        _most(max_tokens, tokens, token_offsets),
-                                                        cache.max_blocks * cache.block_size, prefix)
-    return torch.empty((need,), device=cache.k_pages.device, dtype=torch.uint8)
+    """Workspace for ``attention`` (or, with ``prefix``, ``shared_prefix_attention``) of these sizes."""
+    pool = cache.k_pages
+    need = _workspace_bytes(pool.get_device(), L.dtype_code(pool), cache.hkv, cache.block_size, cache.dim,
+                            cache.page_size, cache.requests, tokens, hq, token_offsets is not None,
+                            _most(max_tokens, tokens, token_offsets), cache.max_blocks * cache.block_size, prefix)
+    return torch.empty((need,), device=pool.device, dtype=torch.uint8)
 
 
 def _attend(q, cache, lengths, token_offsets, max_tokens, kv_lo, kv_hi, softcap, slopes, scale, return_lse, workspace,
             prefix):
-    pool, requests = cache.k_pages, cache.requests
-    dev = pool.device
-    hq = q.shape[1] if q.ndim == 3 else 0
-    _check_rows(q, cache, hq, "q")
-    t = q.shape[0]
-    if hq == 0 or hq % cache.hkv:
-        raise ValueError("query heads must be a multiple of KV heads")
-    _check_ints(lengths, (requests,), "lengths", dev)
-    if token_offsets is not None:
-        _check_ints(token_offsets, (requests + 1,), "token_offsets", dev)
-    elif t != requests:
-        raise ValueError("without token_offsets there must be one token per request")
-    for name, x in (("kv_lo", kv_lo), ("kv_hi", kv_hi)):
-        if x is not None:
-            _check_ints(x, (t,), name, dev)
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (hq,) or slopes.device != dev or
-                               not slopes.is_contiguous()):
-        raise ValueError("slopes must be contiguous FP32 [Hq] on the cache's device")
-    if softcap < 0 or (scale is not None and scale <= 0):
-        raise ValueError("softcap must not be negative and scale must be positive")
-    longest, most = cache.max_blocks * cache.block_size, _most(max_tokens, t, token_offsets)
-    if t and most < 1:
-        raise ValueError("max_tokens must be positive")
-    if prefix < 0 or prefix % cache.page_size or prefix > longest:
-        raise ValueError(f"prefix must be whole pages of {cache.page_size} tokens, at most {longest} tokens")
-    out = torch.empty((t, hq, q.shape[2]), dtype=q.dtype, device=dev)
-    lse = torch.empty((t, hq), dtype=torch.float32, device=dev) if return_lse else None
-    lib, kv = L.load(), cache.kv()
+    pool = cache.k_pages
+    pages, hkv, _, d = pool.shape
+    dev, requests = pool.device, cache.requests
+    t, hq = _heads(q, hkv)
+    qp, qt, qh = _rows(q, (t, hq, d), "q", pool)
+    held = _ints(lengths, (requests,), "lengths", dev)
+    offsets = _tokens(token_offsets, t, requests, dev)
+    most = _most(max_tokens, t, token_offsets)
+    block, page = cache.block_size, cache.page_size
+    longest = cache.max_blocks * block
+    options = None
+    if softcap or slopes is not None or scale is not None or kv_lo is not None or kv_hi is not None:
+        if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (hq,) or slopes.device != dev or
+                                   not slopes.is_contiguous()):
+            raise ValueError("slopes must be contiguous FP32 [Hq] on the cache's device")
+        if softcap < 0 or (scale is not None and scale <= 0):
+            raise ValueError("softcap must not be negative and scale must be positive")
+        options = L.StkAttentionOptions(scale or 0.0, softcap, L.ptr(slopes),
+                                        None if kv_lo is None else _ints(kv_lo, (t,), "kv_lo", dev),
+                                        None if kv_hi is None else _ints(kv_hi, (t,), "kv_hi", dev))
+    if prefix and (prefix < 0 or prefix % page or prefix > longest):
+        raise ValueError(f"prefix must be whole pages of {page} tokens, at most {longest} tokens")
+    kv = cache.kv()
     if workspace is None:
-        need = lib.stk_paged_attention_workspace_bytes(kv, requests, t, hq, int(token_offsets is not None), most, longest,
-                                                       prefix)
-        workspace = torch.empty((need,), device=dev, dtype=torch.uint8)
-    options = L.StkAttentionOptions(scale or 0.0, softcap, L.ptr(slopes), L.ptr(kv_lo), L.ptr(kv_hi))
-    rc = lib.stk_paged_attention(kv, pool.shape[0], q.data_ptr(), q.stride(0), q.stride(1), requests, t, hq,
-                                 lengths.data_ptr(), L.ptr(token_offsets), most, longest, prefix, options,
-                                 out.data_ptr(),
-                                 L.ptr(lse), workspace.data_ptr(), workspace.numel(), L.status_ptr(), L.stream_of(q))
+        need = _workspace_bytes(q.get_device(), kv.kv_dtype, hkv, block, d, page, requests, t, hq, offsets is not None,
+                                most, longest, prefix)
+        if need:
+            workspace = q.new_empty((need,), dtype=torch.uint8)
+    else:
+        need = workspace.numel()
+    out = q.new_empty((t, hq, d))
+    lse = q.new_empty((t, hq), dtype=torch.float32) if return_lse else None
+    rc = L.load().stk_paged_attention(kv, pages, qp, qt, qh, requests, t, hq, held, offsets, most, longest, prefix,
+                                      options, out.data_ptr(), L.ptr(lse), L.ptr(workspace), need, L.status_ptr(),
+                                      L.stream_of(q))
     L.check(rc, "paged attention")
     return (out, lse) if return_lse else out
 
