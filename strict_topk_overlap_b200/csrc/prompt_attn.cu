@@ -39,6 +39,7 @@ constexpr int kRows = 256;    // rows of a CTA
 constexpr int kSoftmaxWarps = 8;
 constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
 constexpr float kLazy = 8.f;  // log2 of the growth of the maximum that is left to P
+constexpr int kPoly = 2;      // of every 8 pairs of weights, those whose exponentials take the FMA units
 
 template <int D>
 struct Plan {
@@ -99,6 +100,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // The registers of a load, after its wait: keeps their uses behind it.
 __device__ __forceinline__ void tmem_loaded(uint32_t* r) {
@@ -129,9 +137,55 @@ constexpr uint32_t mma_desc(int m, int n, bool b_along_n) {
          static_cast<uint32_t>(m >> 4) << 24;
 }
 
+// ---------------------------------------------------------------- pairs of FP32
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 c, a, b, c;\n mov.b64 {%0, %1}, c;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 a, b;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " mul.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 a, b;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+      " add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// 2^x of a pair on the FMA units: x = n + f with |f| <= 1/2 (n by adding and
+// subtracting 1.5 * 2^23), 2^f by a cubic (weighted least-maximum fit on
+// [-1/2, 1/2], relative error 7.5e-5, a fifth of a 16-bit weight's rounding),
+// n added to the exponent. The special function unit yields 16 exponentials
+// per SM and clock, as many as the tensor cores need weights; taking some of
+// them off it shortens a tile's chain of S, P and O.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = add2(x, both(12582912.f));
+  const float2 n = add2(t, both(-12582912.f));
+  const float2 f = fma2(n, both(-1.f), x);
+  float2 p = fma2(f, both(0.05517167f), both(0.24261113f));
+  p = fma2(p, f, both(0.69326099f));
+  p = fma2(p, f, both(0.99992807f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
 struct Shared {
   uint64_t full[10], empty[10];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
   uint32_t tmem;
   int kmin[2], kmax[2], lomax[2], himin[2];
 };
@@ -164,6 +218,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     for (int q = 0; q < 2; ++q) {
       mbar_init(&sh.q_full[q], kTileM);
       mbar_init(&sh.s_full[q], 1);
+      mbar_init(&sh.p_half[q], kTileM);
       mbar_init(&sh.p_full[q], kTileM);
       mbar_init(&sh.o_full[q], 1);
       sh.kmin[q] = sh.himin[q] = 0x7fffffff;
@@ -301,15 +356,20 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         if (ok && i >= qa[q] && i < qb[q]) {
-          ok = ok && warp_wait(&sh.p_full[q], n[q] & 1, a.status);
-          fence_after();
-          if (ok && lane == 0) {
-            const uint32_t v = smem_u32(vt);
+          // O += P V, each half of the keys as soon as its weights are there.
 #pragma unroll
-            for (int s = 0; s < kTileN / 16; ++s)  // O += P V
-              mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + s * 8, smem_desc(v + s * 2048, kHalfBytes), pv,
-                     n[q] > 0 || s > 0);
-            if (i + 1 == qb[q]) mma_commit(&sh.o_full[q]);
+          for (int part = 0; part < 2; ++part) {
+            ok = ok && warp_wait(part ? &sh.p_full[q] : &sh.p_half[q], n[q] & 1, a.status);
+            fence_after();
+            if (ok && lane == 0) {
+              const uint32_t v = smem_u32(vt);
+#pragma unroll
+              for (int s = part * kTileN / 32; s < (part + 1) * kTileN / 32; ++s)
+                mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + s * 8, smem_desc(v + s * 2048, kHalfBytes), pv,
+                       n[q] > 0 || s > 0);
+              if (part && i + 1 == qb[q]) mma_commit(&sh.o_full[q]);
+            }
+            __syncwarp();
           }
           ++n[q];
           __syncwarp();
@@ -322,7 +382,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       }
       __syncwarp();
     }
-  } else {
+  } else if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------ softmax
     const int r = tid & (kTileM - 1);  // row of the MMA tile
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
@@ -350,6 +410,13 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const float slope = (MODE & 2) && a.slopes ? a.slopes[head] : 0.f;
     const float c1 = (MODE & 1) ? a.scale / a.softcap : a.scale * kLog2e;
     const float cap2 = a.softcap * kLog2e, slope2 = slope * kLog2e;
+    // Capped scores cap2 tanh(c1 s) as an odd polynomial in s where |c1 s| <=
+    // 3/4 throughout a tile (fitted there for the least relative error,
+    // 5.2e-7, of the order of FP32's own): no special functions. Scores near
+    // the cap take the exponential form.
+    const float cc = c1 * c1;
+    const float t0 = cap2 * c1 * 0.99999948f, t1 = cap2 * c1 * cc * -0.333285f, t2 = cap2 * c1 * cc * cc * 0.13261181f;
+    const float t3 = cap2 * c1 * cc * cc * cc * -0.05011862f, t4 = cap2 * c1 * cc * cc * cc * cc * 0.012984885f;
     float m = neg_inf(), l = 0.f;  // in log2 units; m is at most kLazy below the true maximum
     bool ok = true;
     for (int i = qa[qt]; i < qb[qt]; ++i) {
@@ -357,33 +424,69 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       ok = ok && warp_wait(&sh.s_full[qt], n & 1, a.status);
       if (!ok) break;
       fence_after();
-      float s[kTileN];
+      float2 s[kTileN / 2];
+      auto load = [&]() {
 #pragma unroll
-      for (int j = 0; j < kTileN; j += 32) tmem_ld32(ts + j, reinterpret_cast<uint32_t*>(s) + j);
-      tmem_wait_ld();
+        for (int j = 0; j < kTileN; j += 32) tmem_ld32(ts + j, reinterpret_cast<uint32_t*>(s) + j);
+        tmem_wait_ld();
 #pragma unroll
-      for (int j = 0; j < kTileN; j += 32) tmem_loaded(reinterpret_cast<uint32_t*>(s) + j);
+        for (int j = 0; j < kTileN; j += 32) tmem_loaded(reinterpret_cast<uint32_t*>(s) + j);
+      };
+      load();
       const int k0 = i * kTileN;
       const bool full = k0 >= sh.lomax[qt] && k0 + kTileN <= sh.himin[qt];
-      if (MODE != 0) {
+      if (MODE & 1) {
+        float zmax = 0.f;
 #pragma unroll
-        for (int j = 0; j < kTileN; ++j) {
-          float x = s[j];
-          if (MODE & 1) x = cap2 * cap_tanh(x * c1); else x *= c1;
-          if (MODE & 2) x = fmaf(-slope2, fabsf(static_cast<float>(rk.pos - k0 - j)), x);
-          s[j] = x;
+        for (int j = 0; j < kTileN / 2; ++j) {
+          const float2 z = mul2(s[j], s[j]);
+          zmax = fmaxf(zmax, fmaxf(z.x, z.y));
+          float2 p = fma2(z, both(t4), both(t3));
+          p = fma2(z, p, both(t2));
+          p = fma2(z, p, both(t1));
+          p = fma2(z, p, both(t0));
+          s[j] = mul2(s[j], p);
+        }
+        if (__any_sync(kFull, !(zmax * cc <= 0.5625f))) {
+          load();
+#pragma unroll
+          for (int j = 0; j < kTileN / 2; ++j)
+            s[j] = make_float2(cap2 * cap_tanh(s[j].x * c1), cap2 * cap_tanh(s[j].y * c1));
+        }
+      }
+      if (MODE & 2) {
+        // - slope |pos - k|: linear in k unless the tile reaches past the row's place.
+        const float c = (MODE & 1) ? 1.f : c1;
+        if (__any_sync(kFull, k0 + kTileN - 1 > rk.pos)) {
+#pragma unroll
+          for (int j = 0; j < kTileN / 2; ++j) {
+            s[j].x = fmaf(-slope2, fabsf(static_cast<float>(rk.pos - k0 - 2 * j)), s[j].x * c);
+            s[j].y = fmaf(-slope2, fabsf(static_cast<float>(rk.pos - k0 - 2 * j - 1)), s[j].y * c);
+          }
+        } else {
+          const float at = static_cast<float>(k0 - rk.pos);
+#pragma unroll
+          for (int j = 0; j < kTileN / 2; ++j) {
+            const float2 away = mul2(make_float2(at + static_cast<float>(2 * j), at + static_cast<float>(2 * j + 1)), both(slope2));
+            s[j] = fma2(s[j], both(c), away);
+          }
         }
       }
       if (!full) {
         const int lo = rk.lo - k0, hi = rk.hi - k0;
 #pragma unroll
-        for (int j = 0; j < kTileN; ++j) s[j] = j >= lo && j < hi ? s[j] : neg_inf();
+        for (int j = 0; j < kTileN / 2; ++j) {
+          s[j].x = 2 * j >= lo && 2 * j < hi ? s[j].x : neg_inf();
+          s[j].y = 2 * j + 1 >= lo && 2 * j + 1 < hi ? s[j].y : neg_inf();
+        }
       }
-      float mx = s[0];
+      float top[4];
 #pragma unroll
-      for (int j = 1; j < kTileN; ++j) mx = fmaxf(mx, s[j]);
+      for (int x = 0; x < 4; ++x) top[x] = fmaxf(s[x].x, s[x].y);
+#pragma unroll
+      for (int j = 4; j < kTileN / 2; ++j) top[j & 3] = fmaxf(fmaxf(top[j & 3], s[j].x), s[j].y);
       const float c = MODE != 0 ? 1.f : c1;
-      mx *= c;
+      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
       const bool grow = mx > m + kLazy || (m == neg_inf() && mx > m);
       if (__any_sync(kFull, grow && m != neg_inf())) {
         // O of the warp's rows by 2^(m - mx); the previous product is complete, S comes after it.
@@ -403,23 +506,26 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       }
       if (grow) m = mx;
       const float nm = m == neg_inf() ? 0.f : -m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int j = 0; j < kTileN; j += 64) {
-        uint32_t p[32];
+      for (int j = 0; j < kTileN / 2; j += 16) {
+        uint32_t p[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float x = ex2(fmaf(s[j + 2 * e], c, nm)), y = ex2(fmaf(s[j + 2 * e + 1], c, nm));
-          sum[(2 * e) & 3] += x;
-          sum[(2 * e + 1) & 3] += y;
-          p[e] = pack2<T>(x, y);
+        for (int e = 0; e < 16; ++e) {
+          float2 x = MODE != 0 ? add2(s[j + e], both(nm)) : fma2(s[j + e], both(c), both(nm));
+          x = (e & 7) < kPoly ? ex2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
+          sum[e & 1] = add2(sum[e & 1], x);
+          p[e] = pack2<T>(x.x, x.y);
         }
-        tmem_st32(ts + j / 2, p);
+        tmem_st16(ts + j, p);
+        if (j & 16) {  // half of the keys
+          tmem_wait_st();
+          fence_before();
+          mbar_arrive(j == 16 ? &sh.p_half[qt] : &sh.p_full[qt]);
+        }
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_wait_st();
-      fence_before();
-      mbar_arrive(&sh.p_full[qt]);
+      sum[0] = add2(sum[0], sum[1]);
+      l += sum[0].x + sum[0].y;
     }
     // ------------------------------------------------------------ output
     const bool any = qa[qt] < qb[qt];
