@@ -39,7 +39,9 @@ constexpr int kRows = 256;    // rows of a CTA
 constexpr int kSoftmaxWarps = 8;
 constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
 constexpr float kLazy = 8.f;  // log2 of the growth of the maximum that is left to P
-constexpr int kPoly = 2;      // of every 8 pairs of weights, those whose exponentials take the FMA units
+
+__device__ constexpr float kTanh3[3] = {0.99999961f, -0.33321959f, 0.1284243f};
+__device__ constexpr float kTanh5[5] = {0.99999948f, -0.333285f, 0.13261181f, -0.05011862f, 0.012984885f};
 
 template <int D>
 struct Plan {
@@ -59,21 +61,27 @@ __device__ __forceinline__ void tmem_free(uint32_t at, int columns) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Issued by one elected lane, as a predicate inside warp-uniform code: with a
+// branch around them, their uniform operands are moved lane by lane and the
+// issue, not the tensor cores, bounds the kernel (100 instead of 64 clocks
+// per 128 x 128 x 16 product).
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p, e;\n setp.ne.u32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "{\n .reg .pred p, e;\n setp.ne.u32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc))
       : "memory");
 }
@@ -115,6 +123,8 @@ __device__ __forceinline__ void tmem_loaded(uint32_t* r) {
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
                       "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
+// The value of lane 0, known to the compiler as the warp's.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(kFull, x, 0); }
 // A bounded wait of a whole warp, converged again on return.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, int* status) {
   return __all_sync(kFull, mbar_wait(bar, parity, status));
@@ -196,13 +206,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap) {
   using P = Plan<D>;
+  constexpr int kFmaPairs = MODE == 0 ? 2 : 1;  // of 8 pairs of weights, those whose exponentials take the FMA units
   constexpr int kHalves = D / 64;
   constexpr int kHalfBytes = kTileN * 128;
   extern __shared__ unsigned char raw[];
   __shared__ Shared sh;
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
   unsigned char* ring = base + 2 * P::kTileBytes;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
   const int h = blockIdx.y;
   // Later row tiles see more keys under a causal mask: they start first.
   const int slots = gridDim.x / a.nsplit;
@@ -268,10 +279,15 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         hi = max(hi, qb[q]);
       }
     }
-    ta = lo;
-    tb = max(lo, hi);
+    ta = uniform(lo);
+    tb = uniform(max(lo, hi));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      qa[q] = uniform(qa[q]);
+      qb[q] = uniform(qb[q]);
+    }
   }
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = uniform(sh.tmem);
   const int rp = t.r;
 
   if (warp == kSoftmaxWarps + 1) {
@@ -308,43 +324,49 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   } else if (warp == kSoftmaxWarps) {
     // ------------------------------------------------------------ MMAs
     constexpr uint32_t qk = mma_desc<T>(kTileM, kTileN, false), pv = mma_desc<T>(kTileM, D, true);
-    const uint32_t sring = smem_u32(ring), sq = smem_u32(base);
-    int n[2] = {0, 0};  // tiles done, per MMA tile
-    bool ok = true;
-    auto wait_full = [&](int item) {
-      ok = ok && warp_wait(&sh.full[item % P::kRing], (item / P::kRing) & 1, a.status);
-    };
-    auto issue_qk = [&](int q, int i) {  // S = Q K^T
-      const uint32_t kt = sring + (2 * (i - ta)) % P::kRing * P::kTileBytes;
-      if (lane == 0) {
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const uint32_t o = (s >> 2) * kHalfBytes + (s & 3) * 32;
-          mma_ss(tmem + q * kTileN, smem_desc(sq + q * P::kTileBytes + o, 16), smem_desc(kt + o, 16), qk, s > 0);
-        }
-        mma_commit(&sh.s_full[q]);
+    const uint64_t q_desc = smem_desc(smem_u32(base), 16), k_desc = smem_desc(smem_u32(ring), 16);
+    const uint64_t v_desc = smem_desc(smem_u32(ring), kHalfBytes);
+    constexpr uint64_t kTile16 = P::kTileBytes >> 4;  // descriptor addresses count 16 bytes
+    const int len = uniform(t.len);
+    int done[2] = {0, 0};  // tiles, per MMA tile
+    // Ring slots and phases of the next K and V tiles (items 0, 2, 4, .. and 1, 3, 5, ..).
+    int slot = 0, phase = 0;
+    auto advance = [&]() {
+      if (++slot == P::kRing) {
+        slot = 0;
+        phase ^= 1;
       }
-      __syncwarp();
     };
+    auto issue_qk = [&](int q, int kslot) {  // S = Q K^T
+      const uint64_t kd = k_desc + kslot * kTile16, qd = q_desc + q * kTile16;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const uint64_t o = ((s >> 2) * kHalfBytes + (s & 3) * 32) >> 4;
+        mma_ss(tmem + q * kTileN, qd + o, kd + o, qk, s > 0);
+      }
+      mma_commit(&sh.s_full[q]);
+    };
+    bool ok = true;
     if (ta < tb) {
-      wait_full(0);
+      ok = warp_wait(&sh.full[0], 0, a.status);
+#pragma unroll
       for (int q = 0; q < 2; ++q) {
         if (qa[q] < qb[q]) ok = ok && warp_wait(&sh.q_full[q], 0, a.status);
         fence_after();
-        if (ok && qa[q] == ta && qa[q] < qb[q]) issue_qk(q, ta);
+        if (ok && qa[q] == ta && qa[q] < qb[q]) issue_qk(q, 0);
       }
-      if (lane == 0) mma_commit(&sh.empty[0]);
-      __syncwarp();
+      mma_commit(&sh.empty[0]);
+      advance();
     }
     for (int i = ta; ok && i < tb; ++i) {
-      const int item = 2 * (i - ta) + 1;
-      wait_full(item);
+      const int vslot = slot;
+      ok = warp_wait(&sh.full[vslot], phase, a.status);
       if (!ok) break;
-      unsigned char* vt = ring + item % P::kRing * P::kTileBytes;
-      const int valid = t.len - i * kTileN;
+      const int valid = len - i * kTileN;
       if (valid < kTileN) {  // slots past the request's tokens: their values must not meet the zero weights
-        const int fill = min(kTileN, (max(valid, 0) + a.L.page_size - 1) / a.L.page_size * a.L.page_size);
+        unsigned char* vt = ring + vslot * P::kTileBytes;
         const int from = max(valid, 0);
+        const int fill = min(kTileN, (from + a.L.page_size - 1) / a.L.page_size * a.L.page_size);
         for (int x = lane; x < (fill - from) * 8 * kHalves; x += 32) {
           const int half = x % kHalves, y = x / kHalves;
           *reinterpret_cast<uint4*>(vt + half * kHalfBytes + (from + y / 8) * 128 + y % 8 * 16) = make_uint4(0, 0, 0, 0);
@@ -352,35 +374,34 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      if (i + 1 < tb) wait_full(item + 1);
+      advance();
+      const int kslot = slot;
+      const bool more = i + 1 < tb;
+      if (more) ok = warp_wait(&sh.full[kslot], phase, a.status);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         if (ok && i >= qa[q] && i < qb[q]) {
           // O += P V, each half of the keys as soon as its weights are there.
+          const uint64_t vd = v_desc + vslot * kTile16;
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
-            ok = ok && warp_wait(part ? &sh.p_full[q] : &sh.p_half[q], n[q] & 1, a.status);
+            ok = ok && warp_wait(part ? &sh.p_full[q] : &sh.p_half[q], done[q] & 1, a.status);
             fence_after();
-            if (ok && lane == 0) {
-              const uint32_t v = smem_u32(vt);
 #pragma unroll
-              for (int s = part * kTileN / 32; s < (part + 1) * kTileN / 32; ++s)
-                mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + s * 8, smem_desc(v + s * 2048, kHalfBytes), pv,
-                       n[q] > 0 || s > 0);
-              if (part && i + 1 == qb[q]) mma_commit(&sh.o_full[q]);
-            }
-            __syncwarp();
+            for (int s = part * kTileN / 32; s < (part + 1) * kTileN / 32; ++s)
+              mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + s * 8, vd + s * (2048 >> 4), pv,
+                     done[q] > 0 || s > 0);
           }
-          ++n[q];
-          __syncwarp();
+          if (i + 1 == qb[q]) mma_commit(&sh.o_full[q]);
+          ++done[q];
         }
-        if (ok && i + 1 >= qa[q] && i + 1 < qb[q]) issue_qk(q, i + 1);
+        if (ok && i + 1 >= qa[q] && i + 1 < qb[q]) issue_qk(q, kslot);
       }
-      if (lane == 0) {
-        mma_commit(&sh.empty[item % P::kRing]);
-        if (i + 1 < tb) mma_commit(&sh.empty[(item + 1) % P::kRing]);
+      mma_commit(&sh.empty[vslot]);
+      if (more) {
+        mma_commit(&sh.empty[kslot]);
+        advance();
       }
-      __syncwarp();
     }
   } else if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------ softmax
@@ -410,13 +431,11 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const float slope = (MODE & 2) && a.slopes ? a.slopes[head] : 0.f;
     const float c1 = (MODE & 1) ? a.scale / a.softcap : a.scale * kLog2e;
     const float cap2 = a.softcap * kLog2e, slope2 = slope * kLog2e;
-    // Capped scores cap2 tanh(c1 s) as an odd polynomial in s where |c1 s| <=
-    // 3/4 throughout a tile (fitted there for the least relative error,
-    // 5.2e-7, of the order of FP32's own): no special functions. Scores near
-    // the cap take the exponential form.
-    const float cc = c1 * c1;
-    const float t0 = cap2 * c1 * 0.99999948f, t1 = cap2 * c1 * cc * -0.333285f, t2 = cap2 * c1 * cc * cc * 0.13261181f;
-    const float t3 = cap2 * c1 * cc * cc * cc * -0.05011862f, t4 = cap2 * c1 * cc * cc * cc * cc * 0.012984885f;
+    // Capped scores cap2 tanh(c1 s) as odd polynomials in s (fitted for the
+    // least relative error), no special functions: three terms where |c1 s|
+    // <= 0.25 throughout a warp's tile (2.3e-7), five up to 0.75 (5.2e-7),
+    // errors of the order of FP32's own; the exponential form beyond.
+    const float cc = c1 * c1, t0 = cap2 * c1, t1 = t0 * cc, t2 = t1 * cc, t3 = t2 * cc, t4 = t3 * cc;
     float m = neg_inf(), l = 0.f;  // in log2 units; m is at most kLazy below the true maximum
     bool ok = true;
     for (int i = qa[qt]; i < qb[qt]; ++i) {
@@ -436,19 +455,26 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       const int k0 = i * kTileN;
       const bool full = k0 >= sh.lomax[qt] && k0 + kTileN <= sh.himin[qt];
       if (MODE & 1) {
-        float zmax = 0.f;
+        float far[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < kTileN / 2; ++j) {
-          const float2 z = mul2(s[j], s[j]);
-          zmax = fmaxf(zmax, fmaxf(z.x, z.y));
-          float2 p = fma2(z, both(t4), both(t3));
-          p = fma2(z, p, both(t2));
-          p = fma2(z, p, both(t1));
-          p = fma2(z, p, both(t0));
-          s[j] = mul2(s[j], p);
-        }
-        if (__any_sync(kFull, !(zmax * cc <= 0.5625f))) {
-          load();
+        for (int j = 0; j < kTileN / 2; ++j) far[j & 3] = fmaxf(fmaxf(far[j & 3], fabsf(s[j].x)), fabsf(s[j].y));
+        const float most = fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) * c1;
+        if (__all_sync(kFull, most <= 0.25f)) {
+          const float2 u0 = both(t0 * kTanh3[0]), u1 = both(t1 * kTanh3[1]), u2 = both(t2 * kTanh3[2]);
+#pragma unroll
+          for (int j = 0; j < kTileN / 2; ++j) {
+            const float2 z = mul2(s[j], s[j]);
+            s[j] = mul2(s[j], fma2(z, fma2(z, u2, u1), u0));
+          }
+        } else if (__all_sync(kFull, most <= 0.75f)) {
+          const float2 u0 = both(t0 * kTanh5[0]), u1 = both(t1 * kTanh5[1]), u2 = both(t2 * kTanh5[2]);
+          const float2 u3 = both(t3 * kTanh5[3]), u4 = both(t4 * kTanh5[4]);
+#pragma unroll
+          for (int j = 0; j < kTileN / 2; ++j) {
+            const float2 z = mul2(s[j], s[j]);
+            s[j] = mul2(s[j], fma2(z, fma2(z, fma2(z, fma2(z, u4, u3), u2), u1), u0));
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < kTileN / 2; ++j)
             s[j] = make_float2(cap2 * cap_tanh(s[j].x * c1), cap2 * cap_tanh(s[j].y * c1));
@@ -465,10 +491,14 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           }
         } else {
           const float at = static_cast<float>(k0 - rk.pos);
+          float2 away[4];  // every fourth pair's bias, eight keys on at a time
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            away[x] = make_float2((at + static_cast<float>(2 * x)) * slope2, (at + static_cast<float>(2 * x + 1)) * slope2);
 #pragma unroll
           for (int j = 0; j < kTileN / 2; ++j) {
-            const float2 away = mul2(make_float2(at + static_cast<float>(2 * j), at + static_cast<float>(2 * j + 1)), both(slope2));
-            s[j] = fma2(s[j], both(c), away);
+            s[j] = fma2(s[j], both(c), away[j & 3]);
+            away[j & 3] = add2(away[j & 3], both(8.f * slope2));
           }
         }
       }
@@ -513,7 +543,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float2 x = MODE != 0 ? add2(s[j + e], both(nm)) : fma2(s[j + e], both(c), both(nm));
-          x = (e & 7) < kPoly ? ex2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
+          x = (e & 7) < kFmaPairs ? ex2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
           sum[e & 1] = add2(sum[e & 1], x);
           p[e] = pack2<T>(x.x, x.y);
         }
