@@ -4,12 +4,13 @@
 // The rows of one KV head (new tokens x query heads of the group, packed) are
 // cut into tiles of 256, two MMA tiles of 128. Per 128 keys:
 //   S = Q K^T          128 x 128, FP32 in tensor memory (TMEM)
-//   P = 2^(c S - m)    one thread per row: cap, bias, mask, running maximum
-//                      and sum in FP32; P rounded to the type, over S in TMEM
+//   P = 2^(c S - m)    two threads per row, 64 keys each: cap, bias, mask,
+//                      running maximum and sum in FP32; P rounded to the type,
+//                      over S in TMEM
 //   O += P V           FP32 in TMEM, P the TMEM operand
-// Warps 0-3 and 4-7 are the softmax of the two MMA tiles, warp 8 issues the
+// Warps 0-7 and 8-15 are the softmax of the two MMA tiles, warp 16 issues the
 // MMAs (one tile's products run while the other tile's weights are formed),
-// warp 9 feeds a ring of K and V tiles by TMA, one box per page and 64 dims,
+// warp 17 feeds a ring of K and V tiles by TMA, one box per page and 64 dims,
 // swizzled as the MMA reads them.
 //
 // Rounding: P has the type's precision (relative 2^-9 or 2^-12 on average of
@@ -36,18 +37,27 @@ namespace {
 constexpr int kTileM = 128;   // rows of an MMA tile
 constexpr int kTileN = 128;   // keys of a tile
 constexpr int kRows = 256;    // rows of a CTA
-constexpr int kSoftmaxWarps = 8;
+constexpr int kSoftmaxWarps = 16;  // two groups of four per MMA tile, 64 keys each
 constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
 constexpr float kLazy = 8.f;  // log2 of the growth of the maximum that is left to P
 
 __device__ constexpr float kTanh3[3] = {0.99999961f, -0.33321959f, 0.1284243f};
 __device__ constexpr float kTanh5[5] = {0.99999948f, -0.333285f, 0.13261181f, -0.05011862f, 0.012984885f};
 
+struct Shared {
+  uint64_t full[10], empty[10];
+  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
+  uint32_t tmem;
+  int kmin[2], kmax[2], lomax[2], himin[2];
+  volatile int failed[2];      // a wait of the MMA tile's softmax ran out
+  float other[2][2][kTileM];  // [MMA tile][half of the keys][row]: maxima, at the end the sums
+};
+
 template <int D>
 struct Plan {
   static constexpr int kTileBytes = kTileN * D * 2;      // one K or V tile, and one Q tile
   static constexpr int kRing = D == 128 ? 5 : 10;        // K and V tiles in flight
-  static constexpr int kBytes = (2 + kRing) * kTileBytes + 1024;  // + alignment of the swizzle atoms
+  static constexpr int kBytes = (2 + kRing) * kTileBytes + static_cast<int>(sizeof(Shared));
 };
 
 // ---------------------------------------------------------------- tcgen05
@@ -123,6 +133,17 @@ __device__ __forceinline__ void tmem_loaded(uint32_t* r) {
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
                       "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
+// Whether x holds for any thread of a group of `count` that meets on named
+// barrier `id`.
+__device__ __forceinline__ bool group_any(int id, int count, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n barrier.cta.red.or.pred p, %2, %3, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(x)), "r"(id), "r"(count)
+      : "memory");
+  return r != 0;
+}
 // The value of lane 0, known to the compiler as the warp's.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(kFull, x, 0); }
 // A bounded wait of a whole warp, converged again on return.
@@ -193,12 +214,6 @@ __device__ __forceinline__ float2 ex2_fma(float2 x) {
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
-struct Shared {
-  uint64_t full[10], empty[10];
-  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
-  uint32_t tmem;
-  int kmin[2], kmax[2], lomax[2], himin[2];
-};
 
 // MODE: 1 capped scores, 2 biased by distance, 3 both.
 template <typename T, int D, int MODE>
@@ -209,10 +224,9 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   constexpr int kFmaPairs = MODE == 0 ? 2 : 1;  // of 8 pairs of weights, those whose exponentials take the FMA units
   constexpr int kHalves = D / 64;
   constexpr int kHalfBytes = kTileN * 128;
-  extern __shared__ unsigned char raw[];
-  __shared__ Shared sh;
-  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
+  extern __shared__ __align__(1024) unsigned char base[];  // swizzle atoms: 1024-byte aligned
   unsigned char* ring = base + 2 * P::kTileBytes;
+  Shared& sh = *reinterpret_cast<Shared*>(ring + P::kRing * P::kTileBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
   const int h = blockIdx.y;
   // Later row tiles see more keys under a causal mask: they start first.
@@ -227,13 +241,14 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       mbar_init(&sh.empty[i], 1);
     }
     for (int q = 0; q < 2; ++q) {
-      mbar_init(&sh.q_full[q], kTileM);
+      mbar_init(&sh.q_full[q], 2 * kTileM);
       mbar_init(&sh.s_full[q], 1);
-      mbar_init(&sh.p_half[q], kTileM);
+      mbar_init(&sh.p_half[q], 2 * kTileM);
       mbar_init(&sh.p_full[q], kTileM);
       mbar_init(&sh.o_full[q], 1);
       sh.kmin[q] = sh.himin[q] = 0x7fffffff;
       sh.kmax[q] = sh.lomax[q] = 0;
+      sh.failed[q] = 0;
     }
     fence_barrier_init();
   }
@@ -242,9 +257,9 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
 
   // ---- the rows' key intervals
   RowKeys rk{0, 0x7fffffff, 0};
-  const int qt = warp >> 2;                       // softmax warps: MMA tile
-  const int row = tid;                            // and row of the CTA
-  const bool have = tid < kRows && row < t.rows;
+  const int qt = warp >> 3, half = (warp >> 2) & 1;        // softmax warps: MMA tile, half of its keys
+  const int row = qt * kTileM + (tid & (kTileM - 1));      // and row of the CTA
+  const bool have = row < t.rows;
   if (warp < kSoftmaxWarps) {
     if (have) rk = row_keys(a, t, (t.row0 + row) / a.G);
     const bool some = have && rk.hi > rk.lo;
@@ -389,7 +404,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
             fence_after();
 #pragma unroll
             for (int s = part * kTileN / 32; s < (part + 1) * kTileN / 32; ++s)
-              mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + s * 8, vd + s * (2048 >> 4), pv,
+              mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + part * (kTileN / 2) + (s & 3) * 8, vd + s * (2048 >> 4), pv,
                      done[q] > 0 || s > 0);
           }
           if (i + 1 == qb[q]) mma_commit(&sh.o_full[q]);
@@ -405,15 +420,17 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     }
   } else if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------ softmax
+    constexpr int kKeys = kTileN / 2;  // of a thread
     const int r = tid & (kTileM - 1);  // row of the MMA tile
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
-    const uint32_t ts = tmem + lanes + qt * kTileN, to = tmem + lanes + 2 * kTileN + qt * D;
+    const uint32_t ts = tmem + lanes + qt * kTileN + half * kKeys;
+    const uint32_t to = tmem + lanes + 2 * kTileN + qt * D + half * (D / 2);
     // Q tile, swizzled: 16-byte chunk c of row x at chunk c ^ (x & 7).
     {
       unsigned char* dst = base + qt * P::kTileBytes;
       const T* q = static_cast<const T*>(a.q);
 #pragma unroll 4
-      for (int x = r; x < kTileM * D / 8; x += kTileM) {
+      for (int x = tid & (2 * kTileM - 1); x < kTileM * D / 8; x += 2 * kTileM) {
         const int rr = x / (D / 8), c = x % (D / 8);
         const int cr = qt * kTileM + rr;
         uint4 w = make_uint4(0, 0, 0, 0);
@@ -433,134 +450,156 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const float cap2 = a.softcap * kLog2e, slope2 = slope * kLog2e;
     // Capped scores cap2 tanh(c1 s) as odd polynomials in s (fitted for the
     // least relative error), no special functions: three terms where |c1 s|
-    // <= 0.25 throughout a warp's tile (2.3e-7), five up to 0.75 (5.2e-7),
+    // <= 0.25 throughout a warp's tile (3.9e-7), five up to 0.75 (5.2e-7),
     // errors of the order of FP32's own; the exponential form beyond.
     const float cc = c1 * c1, t0 = cap2 * c1, t1 = t0 * cc, t2 = t1 * cc, t3 = t2 * cc, t4 = t3 * cc;
     float m = neg_inf(), l = 0.f;  // in log2 units; m is at most kLazy below the true maximum
     bool ok = true;
-    for (int i = qa[qt]; i < qb[qt]; ++i) {
-      const int n = i - qa[qt];
-      ok = ok && warp_wait(&sh.s_full[qt], n & 1, a.status);
-      if (!ok) break;
+    const int begin = qt ? qa[1] : qa[0], end = qt ? qb[1] : qb[0];
+    for (int i = begin; i < end; ++i) {
+      const int n = i - begin;
+      // A wait that runs out is told to the whole group at its next meeting: nobody is left waiting there.
+      ok = warp_wait(&sh.s_full[qt], n & 1, a.status);
+      if (!ok) sh.failed[qt] = 1;
       fence_after();
-      float2 s[kTileN / 2];
-      auto load = [&]() {
-#pragma unroll
-        for (int j = 0; j < kTileN; j += 32) tmem_ld32(ts + j, reinterpret_cast<uint32_t*>(s) + j);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < kTileN; j += 32) tmem_loaded(reinterpret_cast<uint32_t*>(s) + j);
-      };
-      load();
-      const int k0 = i * kTileN;
-      const bool full = k0 >= sh.lomax[qt] && k0 + kTileN <= sh.himin[qt];
-      if (MODE & 1) {
-        float far[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < kTileN / 2; ++j) far[j & 3] = fmaxf(fmaxf(far[j & 3], fabsf(s[j].x)), fabsf(s[j].y));
-        const float most = fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3])) * c1;
-        if (__all_sync(kFull, most <= 0.25f)) {
-          const float2 u0 = both(t0 * kTanh3[0]), u1 = both(t1 * kTanh3[1]), u2 = both(t2 * kTanh3[2]);
-#pragma unroll
-          for (int j = 0; j < kTileN / 2; ++j) {
-            const float2 z = mul2(s[j], s[j]);
-            s[j] = mul2(s[j], fma2(z, fma2(z, u2, u1), u0));
-          }
-        } else if (__all_sync(kFull, most <= 0.75f)) {
-          const float2 u0 = both(t0 * kTanh5[0]), u1 = both(t1 * kTanh5[1]), u2 = both(t2 * kTanh5[2]);
-          const float2 u3 = both(t3 * kTanh5[3]), u4 = both(t4 * kTanh5[4]);
-#pragma unroll
-          for (int j = 0; j < kTileN / 2; ++j) {
-            const float2 z = mul2(s[j], s[j]);
-            s[j] = mul2(s[j], fma2(z, fma2(z, fma2(z, fma2(z, u4, u3), u2), u1), u0));
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kTileN / 2; ++j)
-            s[j] = make_float2(cap2 * cap_tanh(s[j].x * c1), cap2 * cap_tanh(s[j].y * c1));
-        }
-      }
-      if (MODE & 2) {
-        // - slope |pos - k|: linear in k unless the tile reaches past the row's place.
-        const float c = (MODE & 1) ? 1.f : c1;
-        if (__any_sync(kFull, k0 + kTileN - 1 > rk.pos)) {
-#pragma unroll
-          for (int j = 0; j < kTileN / 2; ++j) {
-            s[j].x = fmaf(-slope2, fabsf(static_cast<float>(rk.pos - k0 - 2 * j)), s[j].x * c);
-            s[j].y = fmaf(-slope2, fabsf(static_cast<float>(rk.pos - k0 - 2 * j - 1)), s[j].y * c);
-          }
-        } else {
-          const float at = static_cast<float>(k0 - rk.pos);
-          float2 away[4];  // every fourth pair's bias, eight keys on at a time
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            away[x] = make_float2((at + static_cast<float>(2 * x)) * slope2, (at + static_cast<float>(2 * x + 1)) * slope2);
-#pragma unroll
-          for (int j = 0; j < kTileN / 2; ++j) {
-            s[j] = fma2(s[j], both(c), away[j & 3]);
-            away[j & 3] = add2(away[j & 3], both(8.f * slope2));
-          }
-        }
-      }
-      if (!full) {
-        const int lo = rk.lo - k0, hi = rk.hi - k0;
-#pragma unroll
-        for (int j = 0; j < kTileN / 2; ++j) {
-          s[j].x = 2 * j >= lo && 2 * j < hi ? s[j].x : neg_inf();
-          s[j].y = 2 * j + 1 >= lo && 2 * j + 1 < hi ? s[j].y : neg_inf();
-        }
-      }
-      float top[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) top[x] = fmaxf(s[x].x, s[x].y);
-#pragma unroll
-      for (int j = 4; j < kTileN / 2; ++j) top[j & 3] = fmaxf(fmaxf(top[j & 3], s[j].x), s[j].y);
+      const int k0 = i * kTileN + half * kKeys;
+      const bool full = k0 >= sh.lomax[qt] && k0 + kKeys <= sh.himin[qt];
       const float c = MODE != 0 ? 1.f : c1;
-      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-      const bool grow = mx > m + kLazy || (m == neg_inf() && mx > m);
-      if (__any_sync(kFull, grow && m != neg_inf())) {
-        // O of the warp's rows by 2^(m - mx); the previous product is complete, S comes after it.
-        const float f = grow ? ex2(m - mx) : 1.f;
-        l *= f;
+      float mx = neg_inf();
+      // Scores, 32 at a time: transformed and masked ones go back to TMEM.
 #pragma unroll 1
-        for (int j = 0; j < D; j += 32) {
-          uint32_t o[32];
-          tmem_ld32(to + j, o);
-          tmem_wait_ld();
-          tmem_loaded(o);
+      for (int j0 = 0; j0 < kKeys; j0 += 32) {
+        float2 s[16];
+        tmem_ld32(ts + j0, reinterpret_cast<uint32_t*>(s));
+        tmem_wait_ld();
+        tmem_loaded(reinterpret_cast<uint32_t*>(s));
+        if (MODE & 1) {
+          float far[2] = {0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st32(to + j, o);
+          for (int j = 0; j < 16; ++j) far[j & 1] = fmaxf(fmaxf(far[j & 1], fabsf(s[j].x)), fabsf(s[j].y));
+          const float most = fmaxf(far[0], far[1]) * c1;
+          if (__all_sync(kFull, most <= 0.25f)) {
+            const float2 u0 = both(t0 * kTanh3[0]), u1 = both(t1 * kTanh3[1]), u2 = both(t2 * kTanh3[2]);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 z = mul2(s[j], s[j]);
+              s[j] = mul2(s[j], fma2(z, fma2(z, u2, u1), u0));
+            }
+          } else if (__all_sync(kFull, most <= 0.75f)) {
+            const float2 u0 = both(t0 * kTanh5[0]), u1 = both(t1 * kTanh5[1]), u2 = both(t2 * kTanh5[2]);
+            const float2 u3 = both(t3 * kTanh5[3]), u4 = both(t4 * kTanh5[4]);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 z = mul2(s[j], s[j]);
+              s[j] = mul2(s[j], fma2(z, fma2(z, fma2(z, fma2(z, u4, u3), u2), u1), u0));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              s[j] = make_float2(cap2 * cap_tanh(s[j].x * c1), cap2 * cap_tanh(s[j].y * c1));
+          }
         }
-        tmem_wait_st();
+        if (MODE & 2) {
+          // - slope |pos - k|: linear in k unless the tile reaches past the row's place.
+          const float cb = (MODE & 1) ? 1.f : c1;
+          const float at = static_cast<float>(k0 + j0 - rk.pos);
+          if (__any_sync(kFull, k0 + j0 + 31 > rk.pos)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              s[j].x = fmaf(-slope2, fabsf(at + static_cast<float>(2 * j)), s[j].x * cb);
+              s[j].y = fmaf(-slope2, fabsf(at + static_cast<float>(2 * j + 1)), s[j].y * cb);
+            }
+          } else {
+            float2 away[2];  // every second pair's bias, four keys on at a time
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              away[x] = make_float2((at + static_cast<float>(2 * x)) * slope2, (at + static_cast<float>(2 * x + 1)) * slope2);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              s[j] = fma2(s[j], both(cb), away[j & 1]);
+              away[j & 1] = add2(away[j & 1], both(4.f * slope2));
+            }
+          }
+        }
+        if (!full) {
+          const int lo = rk.lo - k0 - j0, hi = rk.hi - k0 - j0;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            s[j].x = 2 * j >= lo && 2 * j < hi ? s[j].x : neg_inf();
+            s[j].y = 2 * j + 1 >= lo && 2 * j + 1 < hi ? s[j].y : neg_inf();
+          }
+        }
+        if (MODE != 0 || !full) tmem_st32(ts + j0, reinterpret_cast<const uint32_t*>(s));
+        float top[2] = {mx, neg_inf()};
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top[j & 1] = fmaxf(fmaxf(top[j & 1], s[j].x), s[j].y);
+        mx = fmaxf(top[0], top[1]);
       }
-      if (grow) m = mx;
+      if (MODE != 0 || !full) tmem_wait_st();
+      mx *= c;
+      auto grows = [&](float x) { return x > m + kLazy || (m == neg_inf() && x > m); };
+      // Whether any row's maximum has grown, in either half of its keys.
+      // (A row's maximum is read before its P is announced, and written again after the next S, which waits for that.)
+      sh.other[qt][half][r] = mx;
+      if (group_any(1 + qt, 2 * kTileM, grows(mx) || !ok)) {
+        if (sh.failed[qt]) {
+          ok = false;
+          break;
+        }
+        mx = fmaxf(mx, sh.other[qt][half ^ 1][r]);
+        const bool grow = grows(mx);
+        if (__any_sync(kFull, grow && m != neg_inf())) {
+          // O of the warp's rows (this half of its dims) by 2^(m - mx); the previous product is complete, S comes after it.
+          const float f = grow ? ex2(m - mx) : 1.f;
+          l *= f;
+#pragma unroll 1
+          for (int j = 0; j < D / 2; j += 32) {
+            uint32_t o[32];
+            tmem_ld32(to + j, o);
+            tmem_wait_ld();
+            tmem_loaded(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st32(to + j, o);
+          }
+          tmem_wait_st();
+          fence_before();
+        }
+        if (grow) m = mx;
+      }
+      if (half) mbar_arrive(&sh.p_half[qt]);  // O is ready for the product of the other half's keys
       const float nm = m == neg_inf() ? 0.f : -m;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int j = 0; j < kTileN / 2; j += 16) {
+#pragma unroll 1
+      for (int j0 = 0; j0 < kKeys; j0 += 32) {
+        float2 s[16];
+        tmem_ld32(ts + j0, reinterpret_cast<uint32_t*>(s));
+        tmem_wait_ld();
+        tmem_loaded(reinterpret_cast<uint32_t*>(s));
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float2 x = MODE != 0 ? add2(s[j + e], both(nm)) : fma2(s[j + e], both(c), both(nm));
+          float2 x = MODE != 0 ? add2(s[e], both(nm)) : fma2(s[e], both(c), both(nm));
           x = (e & 7) < kFmaPairs ? ex2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
           sum[e & 1] = add2(sum[e & 1], x);
           p[e] = pack2<T>(x.x, x.y);
         }
-        tmem_st16(ts + j, p);
-        if (j & 16) {  // half of the keys
-          tmem_wait_st();
-          fence_before();
-          mbar_arrive(j == 16 ? &sh.p_half[qt] : &sh.p_full[qt]);
-        }
+        tmem_st16(ts + j0 / 2, p);  // over scores that have been read
       }
+      tmem_wait_st();
+      fence_before();
+      mbar_arrive(half ? &sh.p_full[qt] : &sh.p_half[qt]);
       sum[0] = add2(sum[0], sum[1]);
       l += sum[0].x + sum[0].y;
     }
     // ------------------------------------------------------------ output
-    const bool any = qa[qt] < qb[qt];
-    if (any) ok = ok && warp_wait(&sh.o_full[qt], 0, a.status);
+    const bool any = begin < end;
+    if (any) ok = warp_wait(&sh.o_full[qt], 0, a.status) && ok;
     fence_after();
+    // The row's sum over both halves of its keys.
+    sh.other[qt][half][r] = l;
+    group_any(1 + qt, 2 * kTileM, false);
+    l += sh.other[qt][half ^ 1][r];
     const bool empty = m == neg_inf();
     const long long orow = static_cast<long long>(t.t0 + tok) * a.hq + head;
     const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
@@ -568,7 +607,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     bool nan = false;
     if (ok) {
 #pragma unroll 1
-      for (int j = 0; j < D; j += 32) {
+      for (int j = 0; j < D / 2; j += 32) {
         uint32_t o[32];
         __syncwarp();
         if (any) {
@@ -583,24 +622,26 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           f[e] = !any || empty ? 0.f : __uint_as_float(o[e]) * inv;
           nan = nan || f[e] != f[e];
         }
+        const int dd = half * (D / 2) + j;
         if (a.part_ml) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(a.part_o + prow * D + j + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            *reinterpret_cast<float4*>(a.part_o + prow * D + dd + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
         } else {
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) w[e] = pack2<T>(f[2 * e], f[2 * e + 1]);
-          uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + orow * D + j);
+          uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + orow * D + dd);
 #pragma unroll
           for (int e = 0; e < 4; ++e) out[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
         }
       }
-      if (have) {
+      if (have && half == 0) {
         if (a.part_ml) a.part_ml[prow] = make_float2(empty ? neg_inf() : m * kLn2, l);
         else if (a.lse) a.lse[orow] = empty ? neg_inf() : (m + log2f(l)) * kLn2;
       }
-      // Rows that met values which are not finite, of keys that they may not see.
+      // Rows that met values which are not finite, of keys that they may not
+      // see: this half of their dims once more, in the frame (m, l) that stands.
       unsigned redo = __ballot_sync(kFull, nan);
       while (redo) {
         const int src = __ffs(redo) - 1;
@@ -611,25 +652,20 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         const int xlo = max(__shfl_sync(kFull, rk.lo, src), ta * kTileN);
         const int xhi = min(__shfl_sync(kFull, rk.hi, src), tb * kTileN);
         const float xslope = __shfl_sync(kFull, slope, src);
+        const float frame = __shfl_sync(kFull, m, src) * kLn2;
         float xm, xl, xo[D / 32];
         single_row<T, D>(a, rp, h, static_cast<const T*>(a.q) + (t.t0 + xtok) * a.q_ts + xhead * a.q_hs, xlo, xhi,
-                               xpos, xslope, lane, xm, xl, xo);
+                         xpos, xslope, lane, xm, xl, xo);
         const long long xr = static_cast<long long>(t.t0 + xtok) * a.hq + xhead;
         const long long xp = static_cast<long long>(split) * a.T * a.hq + xr;
+        const float factor = a.part_ml ? expf(xm - frame) : 1.f / xl;
+        if ((lane >> 4) == half) {
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const int dd = lane * (D / 32) + j;
-          if (a.part_ml) {
-            a.part_o[xp * D + dd] = xo[j];
-          } else {
-            const float y = xm == neg_inf() ? 0.f : xo[j] / xl;
-            const uint32_t w = pack2<T>(y, 0.f);
-            static_cast<unsigned short*>(a.out)[xr * D + dd] = static_cast<unsigned short>(w & 0xffff);
+          for (int j = 0; j < D / 32; ++j) {
+            const int dd = lane * (D / 32) + j;
+            if (a.part_ml) a.part_o[xp * D + dd] = xo[j] * factor;
+            else static_cast<unsigned short*>(a.out)[xr * D + dd] = static_cast<unsigned short>(pack2<T>(xo[j] * factor, 0.f));
           }
-        }
-        if (lane == 0) {
-          if (a.part_ml) a.part_ml[xp] = make_float2(xm, xl);
-          else if (a.lse) a.lse[xr] = xm == neg_inf() ? neg_inf() : xm + logf(xl);
         }
       }
     }
