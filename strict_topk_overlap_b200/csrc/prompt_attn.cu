@@ -50,7 +50,10 @@ struct Shared {
   uint32_t tmem;
   int kmin[2], kmax[2], lomax[2], himin[2];
   volatile int failed[2];      // a wait of the MMA tile's softmax ran out
-  float other[2][2][kTileM];  // [MMA tile][half of the keys][row]: maxima, at the end the sums
+  union {
+    float other[2][2][kTileM];             // [MMA tile][half of the keys][row]: maxima, at the end the sums
+    unsigned short lag[2][2][2][kTileM];   // [MMA tile][parity of the key tile][half][row]: maxima, upper half of the bits
+  };
 };
 
 template <int D>
@@ -118,6 +121,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
@@ -125,11 +135,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // The registers of a load, after its wait: keeps their uses behind it.
+template <int N = 32>
 __device__ __forceinline__ void tmem_loaded(uint32_t* r) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 8)
+  for (int i = 0; i < N; i += 8)
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
                       "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
@@ -202,8 +218,8 @@ __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // per SM and clock, as many as the tensor cores need weights; taking some of
 // them off it shortens a tile's chain of S, P and O.
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
+  x.x = fminf(fmaxf(x.x, -126.f), 128.f);
+  x.y = fminf(fmaxf(x.y, -126.f), 128.f);
   const float2 t = add2(x, both(12582912.f));
   const float2 n = add2(t, both(-12582912.f));
   const float2 f = fma2(n, both(-1.f), x);
@@ -215,12 +231,107 @@ __device__ __forceinline__ float2 ex2_fma(float2 x) {
 }
 
 
+constexpr int kRun = 16;  // keys taken from TMEM at once
+
+// What turns kRun raw scores S of a row into scores in log2 units: cap, bias
+// and mask. Plain scores (MODE 0) stay raw, their factor joins the exponent.
+struct Score {
+  float c1;                  // scale * log2 e, or scale / cap
+  float cap2;                // cap * log2 e
+  float t0, t1, t2, t3, t4;  // cap2 c1^(2k + 1)
+  float slope2;              // slope * log2 e
+  RowKeys rk;
+};
+
+template <int MODE>
+__device__ __forceinline__ void scores(float2 (&s)[kRun / 2], const Score& z, int k0, bool full) {
+  // Capped scores cap2 tanh(c1 s) as odd polynomials in s (fitted for the
+  // least relative error), no special functions: three terms where |c1 s| <=
+  // 0.25 throughout a warp's run (3.9e-7), five up to 0.75 (5.2e-7), errors
+  // of the order of FP32's own; the exponential form beyond.
+  if (MODE & 1) {
+    float far[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kRun / 2; ++j) far[j & 1] = fmaxf(fmaxf(far[j & 1], fabsf(s[j].x)), fabsf(s[j].y));
+    const float most = fmaxf(far[0], far[1]) * z.c1;
+    if (__all_sync(kFull, most <= 0.25f)) {
+      const float2 u0 = both(z.t0 * kTanh3[0]), u1 = both(z.t1 * kTanh3[1]), u2 = both(z.t2 * kTanh3[2]);
+#pragma unroll
+      for (int j = 0; j < kRun / 2; ++j) {
+        const float2 y = mul2(s[j], s[j]);
+        s[j] = mul2(s[j], fma2(y, fma2(y, u2, u1), u0));
+      }
+    } else if (__all_sync(kFull, most <= 0.75f)) {
+      const float2 u0 = both(z.t0 * kTanh5[0]), u1 = both(z.t1 * kTanh5[1]), u2 = both(z.t2 * kTanh5[2]);
+      const float2 u3 = both(z.t3 * kTanh5[3]), u4 = both(z.t4 * kTanh5[4]);
+#pragma unroll
+      for (int j = 0; j < kRun / 2; ++j) {
+        const float2 y = mul2(s[j], s[j]);
+        s[j] = mul2(s[j], fma2(y, fma2(y, fma2(y, fma2(y, u4, u3), u2), u1), u0));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun / 2; ++j) s[j] = make_float2(z.cap2 * cap_tanh(s[j].x * z.c1), z.cap2 * cap_tanh(s[j].y * z.c1));
+    }
+  }
+  if (MODE & 2) {
+    // - slope |pos - k|: linear in k unless the run reaches past the row's place.
+    const float c = (MODE & 1) ? 1.f : z.c1;
+    const float at = static_cast<float>(k0 - z.rk.pos);
+    if (__any_sync(kFull, k0 + kRun - 1 > z.rk.pos)) {
+#pragma unroll
+      for (int j = 0; j < kRun / 2; ++j) {
+        s[j].x = fmaf(-z.slope2, fabsf(at + static_cast<float>(2 * j)), s[j].x * c);
+        s[j].y = fmaf(-z.slope2, fabsf(at + static_cast<float>(2 * j + 1)), s[j].y * c);
+      }
+    } else {
+      float2 away[2];  // every second pair's bias, four keys on at a time
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        away[x] = make_float2((at + static_cast<float>(2 * x)) * z.slope2, (at + static_cast<float>(2 * x + 1)) * z.slope2);
+#pragma unroll
+      for (int j = 0; j < kRun / 2; ++j) {
+        s[j] = fma2(s[j], both(c), away[j & 1]);
+        away[j & 1] = add2(away[j & 1], both(4.f * z.slope2));
+      }
+    }
+  }
+  if (!full) {
+    const int lo = z.rk.lo - k0, hi = z.rk.hi - k0;
+#pragma unroll
+    for (int j = 0; j < kRun / 2; ++j) {
+      s[j].x = 2 * j >= lo && 2 * j < hi ? s[j].x : neg_inf();
+      s[j].y = 2 * j + 1 >= lo && 2 * j + 1 < hi ? s[j].y : neg_inf();
+    }
+  }
+}
+
+__device__ __forceinline__ float largest(const float2 (&s)[kRun / 2], float mx) {
+  float top[2] = {mx, neg_inf()};
+#pragma unroll
+  for (int j = 0; j < kRun / 2; ++j) top[j & 1] = fmaxf(fmaxf(top[j & 1], s[j].x), s[j].y);
+  return fmaxf(top[0], top[1]);
+}
+
+// Weights 2^(c s - m) of kRun keys, packed, and their sum.
+template <typename T, int MODE, int FMA_PAIRS>
+__device__ __forceinline__ void weights(const float2 (&s)[kRun / 2], float c, float nm, float2 (&sum)[2], uint32_t (&p)[kRun / 2]) {
+#pragma unroll
+  for (int e = 0; e < kRun / 2; ++e) {
+    float2 x = MODE != 0 ? add2(s[e], both(nm)) : fma2(s[e], both(c), both(nm));
+    x = (e & 7) < FMA_PAIRS ? ex2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
+    sum[e & 1] = add2(sum[e & 1], x);
+    p[e] = pack2<T>(x.x, x.y);
+  }
+}
+
 // MODE: 1 capped scores, 2 biased by distance, 3 both.
 template <typename T, int D, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap) {
   using P = Plan<D>;
+  constexpr bool kLag = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kFmaPairs = MODE == 0 ? 2 : 1;  // of 8 pairs of weights, those whose exponentials take the FMA units
   constexpr int kHalves = D / 64;
   constexpr int kHalfBytes = kTileN * 128;
@@ -446,16 +557,42 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const int tok = have ? (t.row0 + row) / a.G : 0;
     const int head = h * a.G + (have ? t.row0 + row - tok * a.G : 0);
     const float slope = (MODE & 2) && a.slopes ? a.slopes[head] : 0.f;
-    const float c1 = (MODE & 1) ? a.scale / a.softcap : a.scale * kLog2e;
-    const float cap2 = a.softcap * kLog2e, slope2 = slope * kLog2e;
-    // Capped scores cap2 tanh(c1 s) as odd polynomials in s (fitted for the
-    // least relative error), no special functions: three terms where |c1 s|
-    // <= 0.25 throughout a warp's tile (3.9e-7), five up to 0.75 (5.2e-7),
-    // errors of the order of FP32's own; the exponential form beyond.
-    const float cc = c1 * c1, t0 = cap2 * c1, t1 = t0 * cc, t2 = t1 * cc, t3 = t2 * cc, t4 = t3 * cc;
-    float m = neg_inf(), l = 0.f;  // in log2 units; m is at most kLazy below the true maximum
-    bool ok = true;
+    Score z;
+    z.c1 = (MODE & 1) ? a.scale / a.softcap : a.scale * kLog2e;
+    z.cap2 = a.softcap * kLog2e;
+    z.slope2 = slope * kLog2e;
+    z.rk = rk;
+    const float cc = z.c1 * z.c1;
+    z.t0 = z.cap2 * z.c1;
+    z.t1 = z.t0 * cc;
+    z.t2 = z.t1 * cc;
+    z.t3 = z.t2 * cc;
+    z.t4 = z.t3 * cc;
+    const float c = MODE != 0 ? 1.f : z.c1;
+    float m = neg_inf(), l = 0.f;  // in log2 units; m is the frame of P, O and l, near the row's maximum
+    bool ok = true, exact = true;
     const int begin = qt ? qa[1] : qa[0], end = qt ? qb[1] : qb[0];
+    // O of the warp's rows (this half of its dims) and l by 2^(m - to): the last product is complete when S is there.
+    auto reframe = [&](bool grow, float frame) {
+      if (__any_sync(kFull, grow && m != neg_inf())) {
+        const float f = grow ? ex2(m - frame) : 1.f;
+        l *= f;
+#pragma unroll 1
+        for (int j = 0; j < D / 2; j += 32) {
+          uint32_t o[32];
+          tmem_ld32(to + j, o);
+          tmem_wait_ld();
+          tmem_loaded(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st32(to + j, o);
+        }
+        tmem_wait_st();
+        fence_before();
+      }
+      if (grow) m = frame;
+    };
+    auto grows = [&](float x) { return x > m + kLazy || (m == neg_inf() && x > m); };
     for (int i = begin; i < end; ++i) {
       const int n = i - begin;
       // A wait that runs out is told to the whole group at its next meeting: nobody is left waiting there.
@@ -464,133 +601,88 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       fence_after();
       const int k0 = i * kTileN + half * kKeys;
       const bool full = k0 >= sh.lomax[qt] && k0 + kKeys <= sh.himin[qt];
-      const float c = MODE != 0 ? 1.f : c1;
-      float mx = neg_inf();
-      // Scores, 32 at a time: transformed and masked ones go back to TMEM.
-#pragma unroll 1
-      for (int j0 = 0; j0 < kKeys; j0 += 32) {
-        float2 s[16];
-        tmem_ld32(ts + j0, reinterpret_cast<uint32_t*>(s));
-        tmem_wait_ld();
-        tmem_loaded(reinterpret_cast<uint32_t*>(s));
-        if (MODE & 1) {
-          float far[2] = {0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 16; ++j) far[j & 1] = fmaxf(fmaxf(far[j & 1], fabsf(s[j].x)), fabsf(s[j].y));
-          const float most = fmaxf(far[0], far[1]) * c1;
-          if (__all_sync(kFull, most <= 0.25f)) {
-            const float2 u0 = both(t0 * kTanh3[0]), u1 = both(t1 * kTanh3[1]), u2 = both(t2 * kTanh3[2]);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float2 z = mul2(s[j], s[j]);
-              s[j] = mul2(s[j], fma2(z, fma2(z, u2, u1), u0));
-            }
-          } else if (__all_sync(kFull, most <= 0.75f)) {
-            const float2 u0 = both(t0 * kTanh5[0]), u1 = both(t1 * kTanh5[1]), u2 = both(t2 * kTanh5[2]);
-            const float2 u3 = both(t3 * kTanh5[3]), u4 = both(t4 * kTanh5[4]);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float2 z = mul2(s[j], s[j]);
-              s[j] = mul2(s[j], fma2(z, fma2(z, fma2(z, fma2(z, u4, u3), u2), u1), u0));
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              s[j] = make_float2(cap2 * cap_tanh(s[j].x * c1), cap2 * cap_tanh(s[j].y * c1));
-          }
-        }
-        if (MODE & 2) {
-          // - slope |pos - k|: linear in k unless the tile reaches past the row's place.
-          const float cb = (MODE & 1) ? 1.f : c1;
-          const float at = static_cast<float>(k0 + j0 - rk.pos);
-          if (__any_sync(kFull, k0 + j0 + 31 > rk.pos)) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              s[j].x = fmaf(-slope2, fabsf(at + static_cast<float>(2 * j)), s[j].x * cb);
-              s[j].y = fmaf(-slope2, fabsf(at + static_cast<float>(2 * j + 1)), s[j].y * cb);
-            }
-          } else {
-            float2 away[2];  // every second pair's bias, four keys on at a time
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-              away[x] = make_float2((at + static_cast<float>(2 * x)) * slope2, (at + static_cast<float>(2 * x + 1)) * slope2);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              s[j] = fma2(s[j], both(cb), away[j & 1]);
-              away[j & 1] = add2(away[j & 1], both(4.f * slope2));
-            }
-          }
-        }
-        if (!full) {
-          const int lo = rk.lo - k0 - j0, hi = rk.hi - k0 - j0;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            s[j].x = 2 * j >= lo && 2 * j < hi ? s[j].x : neg_inf();
-            s[j].y = 2 * j + 1 >= lo && 2 * j + 1 < hi ? s[j].y : neg_inf();
-          }
-        }
-        if (MODE != 0 || !full) tmem_st32(ts + j0, reinterpret_cast<const uint32_t*>(s));
-        float top[2] = {mx, neg_inf()};
-#pragma unroll
-        for (int j = 0; j < 16; ++j) top[j & 1] = fmaxf(fmaxf(top[j & 1], s[j].x), s[j].y);
-        mx = fmaxf(top[0], top[1]);
-      }
-      if (MODE != 0 || !full) tmem_wait_st();
-      mx *= c;
-      auto grows = [&](float x) { return x > m + kLazy || (m == neg_inf() && x > m); };
-      // Whether any row's maximum has grown, in either half of its keys.
-      // (A row's maximum is read before its P is announced, and written again after the next S, which waits for that.)
-      sh.other[qt][half][r] = mx;
-      if (group_any(1 + qt, 2 * kTileM, grows(mx) || !ok)) {
-        if (sh.failed[qt]) {
-          ok = false;
-          break;
-        }
-        mx = fmaxf(mx, sh.other[qt][half ^ 1][r]);
-        const bool grow = grows(mx);
-        if (__any_sync(kFull, grow && m != neg_inf())) {
-          // O of the warp's rows (this half of its dims) by 2^(m - mx); the previous product is complete, S comes after it.
-          const float f = grow ? ex2(m - mx) : 1.f;
-          l *= f;
-#pragma unroll 1
-          for (int j = 0; j < D / 2; j += 32) {
-            uint32_t o[32];
-            tmem_ld32(to + j, o);
-            tmem_wait_ld();
-            tmem_loaded(o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(to + j, o);
-          }
-          tmem_wait_st();
-          fence_before();
-        }
-        if (grow) m = mx;
-      }
-      if (half) mbar_arrive(&sh.p_half[qt]);  // O is ready for the product of the other half's keys
-      const float nm = m == neg_inf() ? 0.f : -m;
+      float bias = 0.f;  // the largest that a key of this tile can have
+      if (MODE & 2) bias = -z.slope2 * static_cast<float>(max(0, rk.pos - (i * kTileN + kTileN - 1)));
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      if (exact) {
+        // The maximum first, over both halves of the row's keys. Transformed and masked scores go back to TMEM.
+        float mx = neg_inf();
 #pragma unroll 1
-      for (int j0 = 0; j0 < kKeys; j0 += 32) {
-        float2 s[16];
-        tmem_ld32(ts + j0, reinterpret_cast<uint32_t*>(s));
-        tmem_wait_ld();
-        tmem_loaded(reinterpret_cast<uint32_t*>(s));
-        uint32_t p[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 x = MODE != 0 ? add2(s[e], both(nm)) : fma2(s[e], both(c), both(nm));
-          x = (e & 7) < kFmaPairs ? ex2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
-          sum[e & 1] = add2(sum[e & 1], x);
-          p[e] = pack2<T>(x.x, x.y);
+        for (int j0 = 0; j0 < kKeys; j0 += kRun) {
+          float2 s[kRun / 2];
+          tmem_ld16(ts + j0, reinterpret_cast<uint32_t*>(s));
+          tmem_wait_ld();
+          tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s));
+          scores<MODE>(s, z, k0 + j0, full);
+          if (MODE != 0 || !full) tmem_st16(ts + j0, reinterpret_cast<const uint32_t*>(s));
+          mx = largest(s, mx);
         }
-        tmem_st16(ts + j0 / 2, p);  // over scores that have been read
+        if (MODE != 0 || !full) tmem_wait_st();
+        mx *= c;
+        // (Read before this thread's P is announced, and written again after the next S, which waits for that.)
+        sh.other[qt][half][r] = mx;
+        if (group_any(1 + qt, 2 * kTileM, grows(mx) || !ok)) {
+          if (sh.failed[qt]) {
+            ok = false;
+            break;
+          }
+          mx = fmaxf(mx, sh.other[qt][half ^ 1][r]);
+          reframe(grows(mx), mx);
+        }
+        if (half) mbar_arrive(&sh.p_half[qt]);  // O is ready for the product of the other half's keys
+        const float nm = m == neg_inf() ? 0.f : -m;
+        float2 s[2][kRun / 2];
+        tmem_ld16(ts, reinterpret_cast<uint32_t*>(s[0]));
+#pragma unroll
+        for (int j = 0; j < kKeys / kRun; ++j) {
+          uint32_t p[kRun / 2];
+          tmem_wait_ld();
+          tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[j & 1]));
+          if (j + 1 < kKeys / kRun) tmem_ld16(ts + (j + 1) * kRun, reinterpret_cast<uint32_t*>(s[(j + 1) & 1]));
+          weights<T, MODE, kFmaPairs>(s[j & 1], c, nm, sum, p);
+          tmem_st8(ts + j * kRun / 2, p);  // over scores that have been read
+        }
+        // Once every row that sees any key has met one, the frames may lag (not f16's: P would leave its range).
+        if (kLag) {
+          exact = group_any(1 + qt, 2 * kTileM, m == neg_inf() && rk.hi > rk.lo);
+          sh.lag[qt][n & 1][half][r] = static_cast<unsigned short>(__float_as_uint(m - bias) >> 16);
+        }
+      } else {
+        // One pass, without a maximum, in a frame taken from the tile before:
+        // P may exceed 1, which bf16's range and relative precision do not
+        // mind. What a half publishes is the logarithm of its weights' sum
+        // (its maximum or a little more) less the largest bias that the tile
+        // allows, so that a bias that grows from tile to tile is followed at
+        // once. (Both halves take the same values, published before the last P
+        // was announced.) A row whose scores grow by more than 2^127 from one
+        // tile to the next overflows and is recomputed like those below.
+        const unsigned short mine = sh.lag[qt][(n & 1) ^ 1][half][r], others = sh.lag[qt][(n & 1) ^ 1][half ^ 1][r];
+        const float last = fmaxf(__uint_as_float(static_cast<uint32_t>(mine) << 16),
+                                 __uint_as_float(static_cast<uint32_t>(others) << 16));
+        reframe(grows(last + bias), last + bias);
+        if (half) mbar_arrive(&sh.p_half[qt]);
+        const float nm = m == neg_inf() ? 0.f : -m;
+        float2 s[2][kRun / 2];
+        tmem_ld16(ts, reinterpret_cast<uint32_t*>(s[0]));
+#pragma unroll
+        for (int j = 0; j < kKeys / kRun; ++j) {
+          uint32_t p[kRun / 2];
+          tmem_wait_ld();
+          tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[j & 1]));
+          if (j + 1 < kKeys / kRun) tmem_ld16(ts + (j + 1) * kRun, reinterpret_cast<uint32_t*>(s[(j + 1) & 1]));
+          scores<MODE>(s[j & 1], z, k0 + j * kRun, full);
+          weights<T, MODE, kFmaPairs>(s[j & 1], c, nm, sum, p);
+          tmem_st8(ts + j * kRun / 2, p);
+        }
+        const float est = log2f((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)) - nm - bias;
+        sh.lag[qt][n & 1][half][r] = static_cast<unsigned short>(__float_as_uint(est) >> 16);
       }
       tmem_wait_st();
       fence_before();
       mbar_arrive(half ? &sh.p_full[qt] : &sh.p_half[qt]);
       sum[0] = add2(sum[0], sum[1]);
       l += sum[0].x + sum[0].y;
+      if (!ok) break;
     }
     // ------------------------------------------------------------ output
     const bool any = begin < end;
@@ -604,7 +696,9 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const long long orow = static_cast<long long>(t.t0 + tok) * a.hq + head;
     const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
     const float inv = empty || a.part_ml ? 1.f : 1.f / l;
-    bool nan = false;
+    // The frame was left behind, or ahead, by more than FP32's range; or scores are NaN.
+    const bool over = !(l <= 3.0e38f) || (l == 0.f && !empty);
+    bool redo_row = have && over;
     if (ok) {
 #pragma unroll 1
       for (int j = 0; j < D / 2; j += 32) {
@@ -620,7 +714,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           f[e] = !any || empty ? 0.f : __uint_as_float(o[e]) * inv;
-          nan = nan || f[e] != f[e];
+          redo_row = redo_row || !(fabsf(f[e]) <= 3.0e38f);
         }
         const int dd = half * (D / 2) + j;
         if (a.part_ml) {
@@ -640,9 +734,10 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         if (a.part_ml) a.part_ml[prow] = make_float2(empty ? neg_inf() : m * kLn2, l);
         else if (a.lse) a.lse[orow] = empty ? neg_inf() : (m + log2f(l)) * kLn2;
       }
-      // Rows that met values which are not finite, of keys that they may not
-      // see: this half of their dims once more, in the frame (m, l) that stands.
-      unsigned redo = __ballot_sync(kFull, nan);
+      // Rows whose sums are not finite, be it for values of keys that they may
+      // not see: this half of their dims once more, in the frame (m, l) that
+      // stands, or in their own where l itself is lost.
+      unsigned redo = __ballot_sync(kFull, redo_row);
       while (redo) {
         const int src = __ffs(redo) - 1;
         redo &= redo - 1;
@@ -653,12 +748,17 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         const int xhi = min(__shfl_sync(kFull, rk.hi, src), tb * kTileN);
         const float xslope = __shfl_sync(kFull, slope, src);
         const float frame = __shfl_sync(kFull, m, src) * kLn2;
+        const bool lost = __shfl_sync(kFull, static_cast<int>(over), src) != 0;
         float xm, xl, xo[D / 32];
         single_row<T, D>(a, rp, h, static_cast<const T*>(a.q) + (t.t0 + xtok) * a.q_ts + xhead * a.q_hs, xlo, xhi,
                          xpos, xslope, lane, xm, xl, xo);
         const long long xr = static_cast<long long>(t.t0 + xtok) * a.hq + xhead;
         const long long xp = static_cast<long long>(split) * a.T * a.hq + xr;
-        const float factor = a.part_ml ? expf(xm - frame) : 1.f / xl;
+        const float factor = !a.part_ml ? 1.f / xl : lost ? 1.f : expf(xm - frame);
+        if (lost && half == 0 && lane == 0) {
+          if (a.part_ml) a.part_ml[xp] = make_float2(xm, xl);
+          else if (a.lse) a.lse[xr] = xm + logf(xl);
+        }
         if ((lane >> 4) == half) {
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
