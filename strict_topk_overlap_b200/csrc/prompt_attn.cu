@@ -46,15 +46,17 @@ __device__ constexpr float kTanh5[5] = {0.99999948f, -0.333285f, 0.13261181f, -0
 
 struct Shared {
   uint64_t full[10], empty[10];
-  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2];  // [MMA tile] or [MMA tile][half of the keys]
+  uint64_t pair[8];            // the two warps that share 32 rows
   uint32_t tmem;
   int kmin[2], kmax[2], lomax[2], himin[2];
   volatile int failed[2];      // a wait of the MMA tile's softmax ran out
   union {
     float other[2][2][kTileM];             // [MMA tile][half of the keys][row]: maxima, at the end the sums
-    unsigned short lag[2][2][2][kTileM];   // [MMA tile][parity of the key tile][half][row]: maxima, upper half of the bits
+    unsigned short frame[2][4][kTileM];    // [MMA tile][key tile mod 4][row]: new frame less the tile's largest bias, upper half of its bits
   };
 };
+constexpr unsigned short kKeep = 0x7fc0;   // (a NaN) the frame stays
 
 template <int D>
 struct Plan {
@@ -353,14 +355,16 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     }
     for (int q = 0; q < 2; ++q) {
       mbar_init(&sh.q_full[q], 2 * kTileM);
-      mbar_init(&sh.s_full[q], 1);
-      mbar_init(&sh.p_half[q], 2 * kTileM);
-      mbar_init(&sh.p_full[q], kTileM);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&sh.s_full[q][x], 1);
+        mbar_init(&sh.p_full[q][x], kTileM);
+      }
       mbar_init(&sh.o_full[q], 1);
       sh.kmin[q] = sh.himin[q] = 0x7fffffff;
       sh.kmax[q] = sh.lomax[q] = 0;
       sh.failed[q] = 0;
     }
+    for (int x = 0; x < 8; ++x) mbar_init(&sh.pair[x], 64);
     fence_barrier_init();
   }
   if (warp == kSoftmaxWarps) tmem_alloc(&sh.tmem, 512);
@@ -449,7 +453,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     }
   } else if (warp == kSoftmaxWarps) {
     // ------------------------------------------------------------ MMAs
-    constexpr uint32_t qk = mma_desc<T>(kTileM, kTileN, false), pv = mma_desc<T>(kTileM, D, true);
+    constexpr uint32_t qk = mma_desc<T>(kTileM, kTileN / 2, false), pv = mma_desc<T>(kTileM, D, true);
     const uint64_t q_desc = smem_desc(smem_u32(base), 16), k_desc = smem_desc(smem_u32(ring), 16);
     const uint64_t v_desc = smem_desc(smem_u32(ring), kHalfBytes);
     constexpr uint64_t kTile16 = P::kTileBytes >> 4;  // descriptor addresses count 16 bytes
@@ -463,14 +467,14 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         phase ^= 1;
       }
     };
-    auto issue_qk = [&](int q, int kslot) {  // S = Q K^T
-      const uint64_t kd = k_desc + kslot * kTile16, qd = q_desc + q * kTile16;
+    auto issue_qk = [&](int q, int x, int kslot) {  // S = Q K^T, half x of the keys
+      const uint64_t kd = k_desc + kslot * kTile16 + x * (kHalfBytes / 2 >> 4), qd = q_desc + q * kTile16;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
         const uint64_t o = ((s >> 2) * kHalfBytes + (s & 3) * 32) >> 4;
-        mma_ss(tmem + q * kTileN, qd + o, kd + o, qk, s > 0);
+        mma_ss(tmem + q * kTileN + x * (kTileN / 2), qd + o, kd + o, qk, s > 0);
       }
-      mma_commit(&sh.s_full[q]);
+      mma_commit(&sh.s_full[q][x]);
     };
     bool ok = true;
     if (ta < tb) {
@@ -479,7 +483,10 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       for (int q = 0; q < 2; ++q) {
         if (qa[q] < qb[q]) ok = ok && warp_wait(&sh.q_full[q], 0, a.status);
         fence_after();
-        if (ok && qa[q] == ta && qa[q] < qb[q]) issue_qk(q, 0);
+        if (ok && qa[q] == ta && qa[q] < qb[q]) {
+          issue_qk(q, 0, 0);
+          issue_qk(q, 1, 0);
+        }
       }
       mma_commit(&sh.empty[0]);
       advance();
@@ -506,22 +513,24 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       if (more) ok = warp_wait(&sh.full[kslot], phase, a.status);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        if (ok && i >= qa[q] && i < qb[q]) {
-          // O += P V, each half of the keys as soon as its weights are there.
-          const uint64_t vd = v_desc + vslot * kTile16;
+        const bool now = i >= qa[q] && i < qb[q], then = i + 1 >= qa[q] && i + 1 < qb[q];
+        const uint64_t vd = v_desc + vslot * kTile16;
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            ok = ok && warp_wait(part ? &sh.p_full[q] : &sh.p_half[q], done[q] & 1, a.status);
+        for (int x = 0; x < 2; ++x) {
+          if (ok && now) {  // O += P V
+            ok = warp_wait(&sh.p_full[q][x], done[q] & 1, a.status);
             fence_after();
 #pragma unroll
-            for (int s = part * kTileN / 32; s < (part + 1) * kTileN / 32; ++s)
-              mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + part * (kTileN / 2) + (s & 3) * 8, vd + s * (2048 >> 4), pv,
-                     done[q] > 0 || s > 0);
+            for (int s = 0; s < kTileN / 32; ++s)
+              mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + x * (kTileN / 2) + s * 8,
+                     vd + (x * (kTileN / 32) + s) * (2048 >> 4), pv, done[q] > 0 || x > 0 || s > 0);
           }
+          if (ok && then) issue_qk(q, x, kslot);
+        }
+        if (now) {
           if (i + 1 == qb[q]) mma_commit(&sh.o_full[q]);
           ++done[q];
         }
-        if (ok && i + 1 >= qa[q] && i + 1 < qb[q]) issue_qk(q, kslot);
       }
       mma_commit(&sh.empty[vslot]);
       if (more) {
@@ -571,51 +580,60 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const float c = MODE != 0 ? 1.f : z.c1;
     float m = neg_inf(), l = 0.f;  // in log2 units; m is the frame of P, O and l, near the row's maximum
     bool ok = true, exact = true;
+    int meetings = 0;
     const int begin = qt ? qa[1] : qa[0], end = qt ? qb[1] : qb[0];
-    // O of the warp's rows (this half of its dims) and l by 2^(m - to): the last product is complete when S is there.
+    // O of the warp's rows (this half of its dims) and l by 2^(m - frame).
     auto reframe = [&](bool grow, float frame) {
-      if (__any_sync(kFull, grow && m != neg_inf())) {
-        const float f = grow ? ex2(m - frame) : 1.f;
-        l *= f;
+      const float f = grow ? ex2(m - frame) : 1.f;
+      l *= f;
 #pragma unroll 1
-        for (int j = 0; j < D / 2; j += 32) {
-          uint32_t o[32];
-          tmem_ld32(to + j, o);
-          tmem_wait_ld();
-          tmem_loaded(o);
+      for (int j = 0; j < D / 2; j += 32) {
+        uint32_t o[32];
+        tmem_ld32(to + j, o);
+        tmem_wait_ld();
+        tmem_loaded(o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st32(to + j, o);
-        }
-        tmem_wait_st();
-        fence_before();
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+        tmem_st32(to + j, o);
       }
+      tmem_wait_st();
+      fence_before();
       if (grow) m = frame;
     };
+    // The two warps of the same rows: neither's next P is announced before both have been here.
+    auto meet = [&]() {
+      uint64_t* bar = &sh.pair[qt * 4 + (warp & 3)];
+      mbar_arrive(bar);
+      ok = warp_wait(bar, meetings & 1, a.status) && ok;
+      ++meetings;
+    };
     auto grows = [&](float x) { return x > m + kLazy || (m == neg_inf() && x > m); };
+    // The largest bias that a key of tile i can have.
+    auto most_bias = [&](int i) {
+      return (MODE & 2) ? -z.slope2 * static_cast<float>(max(0, rk.pos - (i * kTileN + kTileN - 1))) : 0.f;
+    };
     for (int i = begin; i < end; ++i) {
       const int n = i - begin;
       // A wait that runs out is told to the whole group at its next meeting: nobody is left waiting there.
-      ok = warp_wait(&sh.s_full[qt], n & 1, a.status);
+      ok = warp_wait(&sh.s_full[qt][half], n & 1, a.status) && ok;
       if (!ok) sh.failed[qt] = 1;
       fence_after();
       const int k0 = i * kTileN + half * kKeys;
       const bool full = k0 >= sh.lomax[qt] && k0 + kKeys <= sh.himin[qt];
-      float bias = 0.f;  // the largest that a key of this tile can have
-      if (MODE & 2) bias = -z.slope2 * static_cast<float>(max(0, rk.pos - (i * kTileN + kTileN - 1)));
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      float2 s[2][kRun / 2];
+      float est;
       if (exact) {
         // The maximum first, over both halves of the row's keys. Transformed and masked scores go back to TMEM.
         float mx = neg_inf();
 #pragma unroll 1
         for (int j0 = 0; j0 < kKeys; j0 += kRun) {
-          float2 s[kRun / 2];
-          tmem_ld16(ts + j0, reinterpret_cast<uint32_t*>(s));
+          tmem_ld16(ts + j0, reinterpret_cast<uint32_t*>(s[0]));
           tmem_wait_ld();
-          tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s));
-          scores<MODE>(s, z, k0 + j0, full);
-          if (MODE != 0 || !full) tmem_st16(ts + j0, reinterpret_cast<const uint32_t*>(s));
-          mx = largest(s, mx);
+          tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[0]));
+          scores<MODE>(s[0], z, k0 + j0, full);
+          if (MODE != 0 || !full) tmem_st16(ts + j0, reinterpret_cast<const uint32_t*>(s[0]));
+          mx = largest(s[0], mx);
         }
         if (MODE != 0 || !full) tmem_wait_st();
         mx *= c;
@@ -627,11 +645,13 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
             break;
           }
           mx = fmaxf(mx, sh.other[qt][half ^ 1][r]);
-          reframe(grows(mx), mx);
+          // Both halves' products are complete, their S come after them.
+          const bool grow = grows(mx);
+          if (__any_sync(kFull, grow && m != neg_inf())) reframe(grow, mx);
+          else if (grow) m = mx;
+          group_any(1 + qt, 2 * kTileM, false);
         }
-        if (half) mbar_arrive(&sh.p_half[qt]);  // O is ready for the product of the other half's keys
         const float nm = m == neg_inf() ? 0.f : -m;
-        float2 s[2][kRun / 2];
         tmem_ld16(ts, reinterpret_cast<uint32_t*>(s[0]));
 #pragma unroll
         for (int j = 0; j < kKeys / kRun; ++j) {
@@ -643,26 +663,24 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           tmem_st8(ts + j * kRun / 2, p);  // over scores that have been read
         }
         // Once every row that sees any key has met one, the frames may lag (not f16's: P would leave its range).
-        if (kLag) {
-          exact = group_any(1 + qt, 2 * kTileM, m == neg_inf() && rk.hi > rk.lo);
-          sh.lag[qt][n & 1][half][r] = static_cast<unsigned short>(__float_as_uint(m - bias) >> 16);
-        }
+        if (kLag) exact = group_any(1 + qt, 2 * kTileM, m == neg_inf() && rk.hi > rk.lo);
+        est = m;
       } else {
-        // One pass, without a maximum, in a frame taken from the tile before:
-        // P may exceed 1, which bf16's range and relative precision do not
-        // mind. What a half publishes is the logarithm of its weights' sum
-        // (its maximum or a little more) less the largest bias that the tile
-        // allows, so that a bias that grows from tile to tile is followed at
-        // once. (Both halves take the same values, published before the last P
-        // was announced.) A row whose scores grow by more than 2^127 from one
-        // tile to the next overflows and is recomputed like those below.
-        const unsigned short mine = sh.lag[qt][(n & 1) ^ 1][half][r], others = sh.lag[qt][(n & 1) ^ 1][half ^ 1][r];
-        const float last = fmaxf(__uint_as_float(static_cast<uint32_t>(mine) << 16),
-                                 __uint_as_float(static_cast<uint32_t>(others) << 16));
-        reframe(grows(last + bias), last + bias);
-        if (half) mbar_arrive(&sh.p_half[qt]);
+        // One pass, without a maximum, in a frame that the first half of the
+        // keys sets at the end of the tile before: P may exceed 1, which
+        // bf16's range and relative precision do not mind. The two halves of a
+        // row are two independent chains of S, P and O that meet only where
+        // the frame moves. A row whose scores run ahead of its frame by more
+        // than 2^127 overflows and is recomputed like those below.
+        const unsigned short code = sh.frame[qt][n & 3][r];
+        const bool grow = code != kKeep;
+        const float frame = __uint_as_float(static_cast<uint32_t>(code) << 16) + most_bias(i);
+        if (__any_sync(kFull, grow)) {
+          meet();  // both halves' products of the last tile are complete
+          reframe(grow, frame);
+          meet();
+        }
         const float nm = m == neg_inf() ? 0.f : -m;
-        float2 s[2][kRun / 2];
         tmem_ld16(ts, reinterpret_cast<uint32_t*>(s[0]));
 #pragma unroll
         for (int j = 0; j < kKeys / kRun; ++j) {
@@ -674,12 +692,17 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           weights<T, MODE, kFmaPairs>(s[j & 1], c, nm, sum, p);
           tmem_st8(ts + j * kRun / 2, p);
         }
-        const float est = log2f((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)) - nm - bias;
-        sh.lag[qt][n & 1][half][r] = static_cast<unsigned short>(__float_as_uint(est) >> 16);
+        est = log2f((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)) - nm;  // the maximum, or a little more
+      }
+      if (kLag && half == 0 && !exact) {
+        // The next tile's frame. What the largest bias of a tile gains on this one's is known, and followed at once.
+        const uint32_t code = __float_as_uint(est - most_bias(i)) >> 16;
+        const bool grow = m != neg_inf() && grows(__uint_as_float(code << 16) + most_bias(i + 1));
+        sh.frame[qt][(n + 1) & 3][r] = grow ? static_cast<unsigned short>(code) : kKeep;
       }
       tmem_wait_st();
       fence_before();
-      mbar_arrive(half ? &sh.p_full[qt] : &sh.p_half[qt]);
+      mbar_arrive(&sh.p_full[qt][half]);
       sum[0] = add2(sum[0], sum[1]);
       l += sum[0].x + sum[0].y;
       if (!ok) break;
