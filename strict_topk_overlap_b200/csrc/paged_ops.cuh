@@ -84,7 +84,7 @@ struct RowTile {
 // Tokens of request r in the cache, at most as many as its blocks hold.
 __device__ __forceinline__ int cached_tokens(const PagedAttnArgs& a, int r, int n) {
   const int len = a.lengths[r], room = request_blocks(a.L, r) * a.L.b;
-  if (len > room || len < n) report(a.status, kStatusBadLength);
+  if (n > 0 && (len > room || len < n)) report(a.status, kStatusBadLength);
   return min(len, room);
 }
 
@@ -110,10 +110,9 @@ __device__ __forceinline__ RowTile row_tile(const PagedAttnArgs& a, int slot, in
     t.n = a.token_offsets[t.r + 1] - t.t0;
     f = slot - static_cast<int>(static_cast<long long>(t.t0) * a.G / M) - t.r;
   }
+  t.len = a.shared ? request_blocks(a.L, 0) * a.L.b : cached_tokens(a, t.r, t.n);  // loaded beside the offsets
   t.row0 = f * M;
   t.rows = max(0, min(M, t.n * a.G - t.row0));
-  t.len = 0;
-  if (t.rows > 0) t.len = a.shared ? request_blocks(a.L, 0) * a.L.b : cached_tokens(a, t.r, t.n);
   return t;
 }
 

@@ -49,7 +49,7 @@ struct Shared {
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2];  // [MMA tile] or [MMA tile][half of the keys]
   uint64_t pair[8];            // the two warps that share 32 rows
   uint32_t tmem;
-  int kmin[2], kmax[2], lomax[2], himin[2];
+  int4 range[kSoftmaxWarps];   // of a warp's rows: least and largest key, largest lo, least hi
   volatile int failed[2];      // a wait of the MMA tile's softmax ran out
   union {
     float other[2][2][kTileM];             // [MMA tile][half of the keys][row]: maxima, at the end the sums
@@ -61,8 +61,9 @@ constexpr unsigned short kKeep = 0x7fc0;   // (a NaN) the frame stays
 template <int D>
 struct Plan {
   static constexpr int kTileBytes = kTileN * D * 2;      // one K or V tile, and one Q tile
+  static constexpr int kQBytes = 32768;                  // a Q tile's place, at the end 4 KB of output for each warp
   static constexpr int kRing = D == 128 ? 5 : 10;        // K and V tiles in flight
-  static constexpr int kBytes = (2 + kRing) * kTileBytes + static_cast<int>(sizeof(Shared));
+  static constexpr int kBytes = 2 * kQBytes + kRing * kTileBytes + static_cast<int>(sizeof(Shared));
 };
 
 // ---------------------------------------------------------------- tcgen05
@@ -338,7 +339,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   constexpr int kHalves = D / 64;
   constexpr int kHalfBytes = kTileN * 128;
   extern __shared__ __align__(1024) unsigned char base[];  // swizzle atoms: 1024-byte aligned
-  unsigned char* ring = base + 2 * P::kTileBytes;
+  unsigned char* ring = base + 2 * P::kQBytes;
   Shared& sh = *reinterpret_cast<Shared*>(ring + P::kRing * P::kTileBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
   const int h = blockIdx.y;
@@ -348,52 +349,79 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   const RowTile t = row_tile<kRows>(a, slots - 1 - static_cast<int>(blockIdx.x) / a.nsplit, lane);
   if (t.rows == 0) return;
 
-  if (tid == 0) {
-    for (int i = 0; i < P::kRing; ++i) {
-      mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 1);
-    }
-    for (int q = 0; q < 2; ++q) {
-      mbar_init(&sh.q_full[q], 2 * kTileM);
-      for (int x = 0; x < 2; ++x) {
-        mbar_init(&sh.s_full[q][x], 1);
-        mbar_init(&sh.p_full[q][x], kTileM);
-      }
-      mbar_init(&sh.o_full[q], 1);
-      sh.kmin[q] = sh.himin[q] = 0x7fffffff;
-      sh.kmax[q] = sh.lomax[q] = 0;
-      sh.failed[q] = 0;
-    }
-    for (int x = 0; x < 8; ++x) mbar_init(&sh.pair[x], 64);
-    fence_barrier_init();
-  }
-  if (warp == kSoftmaxWarps) tmem_alloc(&sh.tmem, 512);
-  __syncthreads();
-
-  // ---- the rows' key intervals
-  RowKeys rk{0, 0x7fffffff, 0};
   const int qt = warp >> 3, half = (warp >> 2) & 1;        // softmax warps: MMA tile, half of its keys
   const int row = qt * kTileM + (tid & (kTileM - 1));      // and row of the CTA
   const bool have = row < t.rows;
+  RowKeys rk{0, 0x7fffffff, 0};
   if (warp < kSoftmaxWarps) {
+    // Q tiles, swizzled: 16-byte chunk c of row x at chunk c ^ (x & 7). The copies run beside what follows.
+    const T* q = static_cast<const T*>(a.q);
+#pragma unroll
+    for (int it = 0; it < D / 16; ++it) {
+      const int x = it * 2 * kTileM + (tid & (2 * kTileM - 1));
+      const int rr = x / (D / 8), c = x % (D / 8);
+      const int cr = qt * kTileM + rr;
+      unsigned char* dst = base + qt * P::kQBytes + (c >> 3) * kHalfBytes + rr * 128 + ((c ^ rr) & 7) * 16;
+      if (cr < t.rows) {
+        const int tok = (t.row0 + cr) / a.G, g = t.row0 + cr - tok * a.G;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)),
+                     "l"(q + (t.t0 + tok) * a.q_ts + (h * a.G + g) * a.q_hs + c * 8)
+                     : "memory");
+      } else {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    // The rows' key intervals.
     if (have) rk = row_keys(a, t, (t.row0 + row) / a.G);
     const bool some = have && rk.hi > rk.lo;
     const int kmin = __reduce_min_sync(kFull, some ? rk.lo : 0x7fffffff);
     const int kmax = __reduce_max_sync(kFull, some ? rk.hi : 0);
     const int lomax = __reduce_max_sync(kFull, have ? rk.lo : 0);
     const int himin = __reduce_min_sync(kFull, have ? rk.hi : 0x7fffffff);
+    if (lane == 0) sh.range[warp] = make_int4(kmin, kmax, lomax, himin);
+  } else if (warp == kSoftmaxWarps) {
+    tmem_alloc(&sh.tmem, 512);
+  } else {
     if (lane == 0) {
-      atomicMin(&sh.kmin[qt], kmin);
-      atomicMax(&sh.kmax[qt], kmax);
-      atomicMax(&sh.lomax[qt], lomax);
-      atomicMin(&sh.himin[qt], himin);
+      for (int i = 0; i < P::kRing; ++i) {
+        mbar_init(&sh.full[i], 1);
+        mbar_init(&sh.empty[i], 1);
+      }
+      for (int q = 0; q < 2; ++q) {
+        mbar_init(&sh.q_full[q], 2 * kTileM);
+        for (int x = 0; x < 2; ++x) {
+          mbar_init(&sh.s_full[q][x], 1);
+          mbar_init(&sh.p_full[q][x], kTileM);
+        }
+        mbar_init(&sh.o_full[q], 1);
+        sh.failed[q] = 0;
+      }
+      for (int x = 0; x < 8; ++x) mbar_init(&sh.pair[x], 64);
+      fence_barrier_init();
     }
+    __syncwarp();
   }
   __syncthreads();
+  // Each MMA tile's keys [kmin, kmax), and [lomax, himin) that all of its rows see.
+  int4 keys[2];
+  {
+    int4 v = sh.range[lane & 15];
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      v.x = min(v.x, __shfl_xor_sync(kFull, v.x, o));
+      v.y = max(v.y, __shfl_xor_sync(kFull, v.y, o));
+      v.z = max(v.z, __shfl_xor_sync(kFull, v.z, o));
+      v.w = min(v.w, __shfl_xor_sync(kFull, v.w, o));
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      keys[q] = make_int4(__shfl_sync(kFull, v.x, 8 * q), __shfl_sync(kFull, v.y, 8 * q), __shfl_sync(kFull, v.z, 8 * q),
+                          __shfl_sync(kFull, v.w, 8 * q));
+  }
   // Tiles [ta, tb) of this CTA's part, and those of each MMA tile.
   int ta, tb, qa[2], qb[2];
   {
-    const int kmin = min(sh.kmin[0], sh.kmin[1]), kmax = max(sh.kmax[0], sh.kmax[1]);
+    const int kmin = min(keys[0].x, keys[1].x), kmax = max(keys[0].y, keys[1].y);
     const int first = kmax > 0 ? kmin / kTileN : 0, last = (kmax + kTileN - 1) / kTileN;
     const int per = (last - first + a.nsplit - 1) / a.nsplit;
     ta = min(last, first + split * per);
@@ -401,8 +429,8 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     int lo = tb, hi = ta;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      qa[q] = sh.kmax[q] > 0 ? max(ta, sh.kmin[q] / kTileN) : tb;
-      qb[q] = min(tb, (sh.kmax[q] + kTileN - 1) / kTileN);
+      qa[q] = keys[q].y > 0 ? max(ta, keys[q].x / kTileN) : tb;
+      qb[q] = min(tb, (keys[q].y + kTileN - 1) / kTileN);
       if (qb[q] <= qa[q]) qa[q] = qb[q] = ta;
       else {
         lo = min(lo, qa[q]);
@@ -468,7 +496,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       }
     };
     auto issue_qk = [&](int q, int x, int kslot) {  // S = Q K^T, half x of the keys
-      const uint64_t kd = k_desc + kslot * kTile16 + x * (kHalfBytes / 2 >> 4), qd = q_desc + q * kTile16;
+      const uint64_t kd = k_desc + kslot * kTile16 + x * (kHalfBytes / 2 >> 4), qd = q_desc + q * (P::kQBytes >> 4);
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
         const uint64_t o = ((s >> 2) * kHalfBytes + (s & 3) * 32) >> 4;
@@ -545,24 +573,10 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
     const uint32_t ts = tmem + lanes + qt * kTileN + half * kKeys;
     const uint32_t to = tmem + lanes + 2 * kTileN + qt * D + half * (D / 2);
-    // Q tile, swizzled: 16-byte chunk c of row x at chunk c ^ (x & 7).
-    {
-      unsigned char* dst = base + qt * P::kTileBytes;
-      const T* q = static_cast<const T*>(a.q);
-#pragma unroll 4
-      for (int x = tid & (2 * kTileM - 1); x < kTileM * D / 8; x += 2 * kTileM) {
-        const int rr = x / (D / 8), c = x % (D / 8);
-        const int cr = qt * kTileM + rr;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (cr < t.rows) {
-          const int tok = (t.row0 + cr) / a.G, g = t.row0 + cr - tok * a.G;
-          w = *reinterpret_cast<const uint4*>(q + (t.t0 + tok) * a.q_ts + (h * a.G + g) * a.q_hs + c * 8);
-        }
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalfBytes + rr * 128 + ((c ^ rr) & 7) * 16) = w;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(&sh.q_full[qt]);
-    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mbar_arrive(&sh.q_full[qt]);
+    const int lomax = qt ? keys[1].z : keys[0].z, himin = qt ? keys[1].w : keys[0].w;
     const int tok = have ? (t.row0 + row) / a.G : 0;
     const int head = h * a.G + (have ? t.row0 + row - tok * a.G : 0);
     const float slope = (MODE & 2) && a.slopes ? a.slopes[head] : 0.f;
@@ -619,7 +633,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       if (!ok) sh.failed[qt] = 1;
       fence_after();
       const int k0 = i * kTileN + half * kKeys;
-      const bool full = k0 >= sh.lomax[qt] && k0 + kKeys <= sh.himin[qt];
+      const bool full = k0 >= lomax && k0 + kKeys <= himin;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       float2 s[2][kRun / 2];
       float est;
@@ -723,34 +737,52 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const bool over = !(l <= 3.0e38f) || (l == 0.f && !empty);
     bool redo_row = have && over;
     if (ok) {
+      // 128 bytes a row at a time through this warp's share of the Q tile's
+      // place, which is free now, so that a store instruction covers whole rows.
+      unsigned char* stage = base + qt * P::kQBytes + (warp & 7) * 4096;
+      auto put = [&](int c, uint4 w) {  // 16-byte chunk c of the lane's row
+        *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ lane) & 7) * 16) = w;
+      };
+      // The staged rows' first `bytes` to byte `at` of their rows of `stride` bytes.
+      auto flush = [&](unsigned char* to, long long my_row, long long stride, int at, int bytes) {
+        __syncwarp();
+        const int per = bytes / 16, rows = 32 / per;  // lanes a row, rows an instruction
+        const int c = lane % per;
+        for (int r0 = 0; r0 < 32; r0 += rows) {
+          const int rr = r0 + lane / per;
+          const long long dst = __shfl_sync(kFull, my_row, rr);
+          const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((c ^ rr) & 7) * 16);
+          if (__shfl_sync(kFull, static_cast<int>(have), rr))
+            *reinterpret_cast<uint4*>(to + dst * stride + at + c * 16) = w;
+        }
+        __syncwarp();
+      };
 #pragma unroll 1
       for (int j = 0; j < D / 2; j += 32) {
         uint32_t o[32];
-        __syncwarp();
         if (any) {
           tmem_ld32(to + j, o);
           tmem_wait_ld();
           tmem_loaded(o);
         }
-        if (!have) continue;
-        float f[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          f[e] = !any || empty ? 0.f : __uint_as_float(o[e]) * inv;
-          redo_row = redo_row || !(fabsf(f[e]) <= 3.0e38f);
+          const float f = !any || empty ? 0.f : __uint_as_float(o[e]) * inv;
+          redo_row = redo_row || (have && !(fabsf(f) <= 3.0e38f));
+          o[e] = __float_as_uint(f);
         }
-        const int dd = half * (D / 2) + j;
         if (a.part_ml) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(a.part_o + prow * D + dd + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+          for (int e = 0; e < 8; ++e) put(e, make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
+          flush(reinterpret_cast<unsigned char*>(a.part_o), prow, D * 4, (half * (D / 2) + j) * 4, 128);
         } else {
           uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = pack2<T>(f[2 * e], f[2 * e + 1]);
-          uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + orow * D + dd);
+          for (int e = 0; e < 16; ++e) w[e] = pack2<T>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) out[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+          for (int e = 0; e < 4; ++e)
+            put((j & 32) / 8 + e, make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]));
+          if (j + 32 == D / 2) flush(static_cast<unsigned char*>(a.out), orow, D * 2, half * D, D);
         }
       }
       if (have && half == 0) {
