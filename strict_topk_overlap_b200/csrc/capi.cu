@@ -918,7 +918,7 @@ enum AttnKind { kAttnRows, kAttnTokens, kAttnPrompt };
 
 struct AttnPhase {
   AttnKind kind;
-  int nsplit;  // tokens: CTAs
+  int nsplit;  // tokens: warps
   int span_lo, span_hi, shared;
   int requests, most_rows;
   size_t states, bytes;  // partial states; their bytes (and the unit counts'), a multiple of 16
@@ -942,13 +942,13 @@ AttnPhase plan_phase(const stk_kv* kv, int R, int T, int hq, bool offsets, bool 
   p.most_rows = static_cast<int>(rows < 16 ? rows : 16);
   p.kind = rows <= 16 ? (token_ok ? kAttnTokens : kAttnRows) : (prompt_ok ? kAttnPrompt : kAttnRows);
   if (p.kind == kAttnTokens) {
-    p.nsplit = 2 * sms;
+    p.nsplit = 8 * sms;  // two CTAs of four warps per SM
     p.states = (static_cast<size_t>(p.nsplit) + static_cast<size_t>(p.requests) * hkv) * p.most_rows;
     p.bytes = p.states * (kv->d + 2) * sizeof(float) + (p.requests + 1) * sizeof(int);
   } else {
     const bool prompt = p.kind == kAttnPrompt;
     const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared, prompt ? 256 : 16)) * hkv;
-    const long long most = prompt ? (keys + 255) / 256 : (keys + 63) / 64;
+    const long long most = prompt ? (keys + 127) / 128 : (keys + 63) / 64;
     long long n = (prompt ? sms : 2 * sms) / tiles;
     n = n < most ? n : most;
     p.nsplit = static_cast<int>(n < 1 ? 1 : n);

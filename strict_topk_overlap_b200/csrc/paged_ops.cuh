@@ -172,13 +172,13 @@ bool prompt_attn_takes(int kv_dtype, int d, int page_size, const void* k, const 
 int launch_prompt_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream);
 int set_wait_limit_prompt(unsigned long long ns);
 
-// Few rows per KV head (see token_attn.cu): `ctas` CTAs share the batch's
-// units evenly; CTA c's state of KV head h of request r is partial
-// c + r * hkv + h, most_rows rows each. Writes the units before each request
-// to prefix [requests + 1].
+// Few rows per KV head (see token_attn.cu): `streams` warps (a multiple of
+// 4) share the batch's units evenly; warp w's state of KV head h of request r
+// is partial w + r * hkv + h, most_rows rows each. Writes the units before
+// each request to prefix [requests + 1].
 bool token_attn_takes(int kv_dtype, int d, int page_size, int R, const void* k, const void* v, const void* q,
                       long long q_ts, long long q_hs);
-int launch_token_attn(const PagedAttnArgs& a, int kv_dtype, int ctas, int most_rows, int* prefix, cudaStream_t stream);
+int launch_token_attn(const PagedAttnArgs& a, int kv_dtype, int streams, int most_rows, int* prefix, cudaStream_t stream);
 int set_wait_limit_token(unsigned long long ns);
 
 // One set of partial softmax states to be joined. Without prefix, part s of
@@ -189,7 +189,7 @@ struct PartSource {
   const float* o;
   int parts;
   const int* prefix;
-  int ctas, most_rows, requests, shared;
+  int streams, most_rows, requests, shared;
 };
 
 struct JoinArgs {

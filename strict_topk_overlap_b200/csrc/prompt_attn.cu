@@ -710,7 +710,9 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       }
       if (kLag && half == 0 && !exact) {
         // The next tile's frame. What the largest bias of a tile gains on this one's is known, and followed at once.
-        const uint32_t code = __float_as_uint(est - most_bias(i)) >> 16;
+        // Rounded down: a frame above the maximum would lose weights, one below it costs range only.
+        const float level = est - most_bias(i);
+        const uint32_t code = (__float_as_uint(level) + (level < 0.f ? 0xffffu : 0u)) >> 16;
         const bool grow = m != neg_inf() && grows(__uint_as_float(code << 16) + most_bias(i + 1));
         sh.frame[qt][(n + 1) & 3][r] = grow ? static_cast<unsigned short>(code) : kKeep;
       }
@@ -734,7 +736,8 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
     const float inv = empty || a.part_ml ? 1.f : 1.f / l;
     // The frame was left behind, or ahead, by more than FP32's range; or scores are NaN.
-    const bool over = !(l <= 3.0e38f) || (l == 0.f && !empty);
+    // (2^-100: below what a frame that follows leaves, above what clamped exponentials of masked keys add up to.)
+    const bool over = !empty && !(l <= 3.0e38f && l >= 7.9e-31f);
     bool redo_row = have && over;
     if (ok) {
       // 128 bytes a row at a time through this warp's share of the Q tile's

@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(JoinArgs a) {
         }
       }
       const long long total = static_cast<long long>(p.prefix[p.requests]) * hkv;
-      const long long per = (total + p.ctas - 1) / p.ctas;
+      const long long per = (total + p.streams - 1) / p.streams;
       const int units = p.prefix[r + 1] - p.prefix[r];
       const long long u0 = static_cast<long long>(p.prefix[r]) * hkv + static_cast<long long>(h) * units;
       const int c0 = units ? static_cast<int>(u0 / per) : 0;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(JoinArgs a) {
 
 template <typename T, int V>
 static int launch_join_v(const JoinArgs& a, int sms, cudaStream_t stream) {
-  if (a.rows >= 2 * sms * kJoinWarps)
+  if (a.rows >= 2 * sms)
     return launch_pdl(join_kernel<T, V, 1>, dim3(static_cast<unsigned>((a.rows + kJoinWarps - 1) / kJoinWarps)),
                       dim3(kJoinWarps * 32), 0, stream, 0, a);
   return launch_pdl(join_kernel<T, V, kJoinWarps>, dim3(static_cast<unsigned>(a.rows)), dim3(kJoinWarps * 32), 0,

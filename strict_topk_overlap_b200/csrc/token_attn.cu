@@ -1,18 +1,18 @@
 // Dense paged attention of few rows per KV head (at most 16: single tokens,
 // a few drafted ones), HBM-bound: every key and value is read once per KV head.
 //
-// The work of a batch is the list of all (request, KV head, 64 keys) units in
-// order; a persistent grid cuts it into equal runs, so that requests of any
-// lengths load every SM alike. Each CTA finds its run from the requests' key
-// ranges (a prefix sum over the batch, taken by every CTA). A unit's 64 keys
-// are 16 for each of the CTA's four warps; a warp streams its keys through a
-// ring of its own (TMA boxes of 16 keys x 64 dims, swizzled for ldmatrix,
-// page ids looked up one unit ahead) across the borders of requests and heads.
+// The work of a batch is the list of all (request, KV head, 16 keys) units in
+// order; the warps of a persistent grid cut it into equal runs, so that
+// requests of any lengths load every SM alike and no warp waits for another.
+// Each CTA finds its warps' runs from the requests' key ranges (a prefix sum
+// over the batch, taken by every CTA). A warp streams its keys through a ring
+// of its own (TMA boxes of 16 keys x 64 dims, swizzled for ldmatrix, page ids
+// looked up one unit ahead) across the borders of requests and heads.
 // The rows form the 16-row side of mma.sync tiles, which hold up to 16 query
 // heads whatever their number and are far from bounding the kernel; the
 // online softmax is FP32, P rounded to the type. Where a (request, head) ends
-// inside a run, the four warps' states join in shared memory and go to one
-// partial state; the join kernel adds the partials of each row.
+// inside a run, its state goes to one partial; the join kernel adds the
+// partials of each row.
 //
 // Values past the keys that any row sees are zeroed in shared memory. Rows of
 // several tokens that see different keys are recomputed one by one where a
@@ -27,17 +27,15 @@ int set_wait_limit_token(unsigned long long ns) { return set_wait_limit_this_uni
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kChunk = 16;               // keys of a warp
-constexpr int kUnit = kWarps * kChunk;   // keys of a unit
+constexpr int kUnit = 16;  // keys of a unit
 
 template <int D>
 struct TokenPlan {
   static constexpr int kHalves = D / 64;
-  static constexpr int kStage = 2 * kChunk * D * 2;             // K and V of one warp's 16 keys
+  static constexpr int kStage = 2 * kUnit * D * 2;              // K and V of a unit
   static constexpr int kStages = D == 128 ? 3 : 6;              // per warp: 96 KB per CTA, two CTAs per SM
-  static constexpr int kJoin = D * 16 * 4;                      // one warp's O
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kBytes = kRing + kJoin + 1024;           // + alignment of the swizzle atoms
+  static constexpr int kBytes = kRing + 1024;                    // + alignment of the swizzle atoms
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -70,6 +68,7 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
 struct Request {
   RowTile t;
   int kmin, kmax;
+  int pos;  // of the last of them
 };
 
 __device__ __forceinline__ Request request_at(const PagedAttnArgs& a, int r) {
@@ -81,9 +80,10 @@ __device__ __forceinline__ Request request_at(const PagedAttnArgs& a, int r) {
   q.t.rows = q.t.n * a.G;
   q.t.len = a.shared ? request_blocks(a.L, 0) * a.L.b : q.t.n > 0 ? cached_tokens(a, r, q.t.n) : 0;
   q.kmin = 0x7fffffff;
-  q.kmax = 0;
+  q.kmax = q.pos = 0;
   for (int i = 0; i < q.t.n; ++i) {
     const RowKeys k = row_keys(a, q.t, i);
+    q.pos = k.pos;
     if (k.hi > k.lo) {
       q.kmin = min(q.kmin, k.lo);
       q.kmax = max(q.kmax, k.hi);
@@ -135,10 +135,8 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
   constexpr int NT = D / 8;
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t bars[kWarps][P::kStages];
-  __shared__ float2 ml[32 * 2];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
-  float* join = reinterpret_cast<float*>(base + P::kRing);           // [D / 2 values][32 lanes]
-  int* prefix = reinterpret_cast<int*>(base + P::kRing + P::kJoin);  // [requests + 1] units before each request
+  int* prefix = reinterpret_cast<int*>(base + P::kRing);  // [requests + 1] units before each request
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (tid == 0) {
@@ -166,35 +164,27 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
   if (blockIdx.x == 0)
     for (int r = tid; r <= requests; r += blockDim.x) prefix_out[r] = prefix[r];
   const long long total = static_cast<long long>(prefix[requests]) * a.L.hkv;
-  const long long per = (total + gridDim.x - 1) / gridDim.x;
-  const long long first = min(total, blockIdx.x * per), last = min(total, first + per);
+  const int stream = blockIdx.x * kWarps + warp, streams = gridDim.x * kWarps;
+  const long long per = (total + streams - 1) / streams;
+  const long long first = min(total, stream * per), last = min(total, first + per);
   if (first >= last) return;
   const int jobs = static_cast<int>(last - first);
 
-  // ---- this warp's stream of 16-key chunks, issued kStages units ahead
+  // ---- this warp's stream of units, issued kStages ahead
   const int ppb = a.L.b / a.L.page_size;
   unsigned char* ring = base + warp * P::kStages * P::kStage;
   Walk ahead;
   ahead.start(a, prefix, requests, first);
-  int issued = 0, queued = 0;  // chunks asked for; units walked
+  int issued = 0;  // units asked for
   int page = 0, key = 0, head = 0;
-  // Steps `ahead` to the warp's next chunk with keys that a row sees; false at the run's end.
-  auto find = [&]() -> bool {
-    while (queued < jobs) {
-      const int k = (ahead.q.kmin / kUnit + ahead.u) * kUnit + warp * kChunk;
-      const bool take = k < ahead.q.kmax && k + kChunk > ahead.q.kmin;
-      if (take) {
-        const int rp = ahead.q.t.r;
-        const int entry = k / a.L.page_size;  // in the table: kmax is at most the request's room
-        page = a.L.page_table[static_cast<long long>(a.L.block_offsets[rp]) * ppb + entry];
-        key = k % a.L.page_size;
-        head = ahead.h;
-      }
-      ++queued;
-      if (queued < jobs) ahead.next(a, prefix, requests);
-      if (take) return true;
-    }
-    return false;
+  // The place of the next unit to ask for; the page id arrives while others are computed.
+  auto find = [&]() {
+    const int k = (ahead.q.kmin / kUnit + ahead.u) * kUnit;
+    const int rp = ahead.q.t.r;
+    // In the table: kmax is at most the request's room.
+    page = a.L.page_table[static_cast<long long>(a.L.block_offsets[rp]) * ppb + k / a.L.page_size];
+    key = k % a.L.page_size;
+    head = ahead.h;
   };
   auto issue = [&]() {
     if (lane == 0) {
@@ -211,13 +201,13 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
         tma_load(&vmap, dst + P::kStage / 2 + half * 2048, &bars[warp][slot], half * 64, key, head, page);
       }
     }
-    ++issued;
+    if (++issued < jobs) {
+      ahead.next(a, prefix, requests);
+      find();
+    }
   };
-  bool more = find();
-  for (int i = 0; more && i < P::kStages; ++i) {
-    issue();
-    more = find();
-  }
+  find();
+  for (int i = 0; i < P::kStages && issued < jobs; ++i) issue();
 
   const int g = lane >> 2, t4 = lane & 3;
   const uint32_t sring = smem_u32(ring);
@@ -238,7 +228,7 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
       const int row = g + 8 * x;
       const bool have = row < q.t.rows;
       const int tok = have ? row / a.G : 0, hd = h * a.G + (have ? row - tok * a.G : 0);
-      rk[x] = have ? row_keys(a, q.t, tok) : RowKeys{0, 0, 0};
+      rk[x] = !have ? RowKeys{0, 0, 0} : q.t.n == 1 ? RowKeys{q.kmin, q.kmax, q.pos} : row_keys(a, q.t, tok);
       slope[x] = a.slopes && have ? a.slopes[hd] * kLog2e : 0.f;
       const T* src = static_cast<const T*>(a.q) + (q.t.t0 + tok) * a.q_ts + hd * a.q_hs + t4 * 2;
 #pragma unroll
@@ -253,16 +243,15 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
     float m[2] = {neg_inf(), neg_inf()}, l[2] = {0.f, 0.f};
     const float c = a.softcap > 0.f ? a.scale / a.softcap : a.scale * kLog2e, cap2 = a.softcap * kLog2e;
     for (int u = u0; u < u1; ++u) {
-      const int k0 = (q.kmin / kUnit + u) * kUnit + warp * kChunk;
-      if (k0 >= q.kmax || k0 + kChunk <= q.kmin) continue;
+      const int k0 = (q.kmin / kUnit + u) * kUnit;
       const int slot = taken % P::kStages;
       ok = ok && __all_sync(kFull, mbar_wait(&bars[warp][slot], (taken / P::kStages) & 1, a.status));
       ++taken;
       if (!ok) break;
       const uint32_t ks = sring + slot * P::kStage, vs = ks + P::kStage / 2;
-      if (k0 < q.kmin || k0 + kChunk > q.kmax) {  // values that no row sees may be anything
+      if (k0 < q.kmin || k0 + kUnit > q.kmax) {  // values that no row sees may be anything
         unsigned char* v = ring + slot * P::kStage + P::kStage / 2;
-        for (int x = lane; x < kChunk * 8 * P::kHalves; x += 32) {
+        for (int x = lane; x < kUnit * 8 * P::kHalves; x += 32) {
           const int y = x / (8 * P::kHalves);
           if (k0 + y < q.kmin || k0 + y >= q.kmax)
             *reinterpret_cast<uint4*>(v + x % P::kHalves * 2048 + y * 128 + x / P::kHalves % 8 * 16) = make_uint4(0, 0, 0, 0);
@@ -337,51 +326,15 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
         mma<T>(o[2 * np + 1], p, b[2], b[3]);
       }
       __syncwarp();  // every lane has read the stage
-      if (more) {
-        issue();
-        more = find();
-      }
+      if (issued < jobs) issue();
     }
-    // ---- the other warps' states into warp 0's, in order
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       l[x] += __shfl_xor_sync(kFull, l[x], 1);
       l[x] += __shfl_xor_sync(kFull, l[x], 2);
     }
-#pragma unroll 1
-    for (int w = 1; w < kWarps; ++w) {
-      if (warp == w) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) join[(n * 4 + e) * 32 + lane] = o[n][e];
-        }
-        ml[lane] = make_float2(m[0], l[0]);
-        ml[32 + lane] = make_float2(m[1], l[1]);
-      }
-      __syncthreads();
-      if (warp == 0) {
-        float mine[2], other[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float2 y = ml[32 * x + lane];
-          const float mn = fmaxf(m[x], y.x), b = mn == neg_inf() ? 0.f : mn;
-          mine[x] = ex2(m[x] - b);
-          other[x] = ex2(y.x - b);
-          l[x] = l[x] * mine[x] + y.y * other[x];
-          m[x] = mn;
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[n][e] = o[n][e] * mine[e >> 1] + join[(n * 4 + e) * 32 + lane] * other[e >> 1];
-        }
-      }
-      __syncthreads();
-    }
-    if (warp == 0 && ok) {
-      const long long slot = static_cast<long long>(blockIdx.x) + slot_rh;
+    if (ok) {
+      const long long slot = static_cast<long long>(stream) + slot_rh;
       unsigned redo = 0;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -417,7 +370,7 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
       }
     }
     done += u1 - u0;
-    if (!__syncthreads_and(ok)) {  // a wait ran out and was reported: leave after this warp's copies have landed
+    if (!ok) {  // a wait ran out and was reported: leave after this warp's copies have landed
       for (; taken < issued; ++taken)
         mbar_wait(&bars[warp][taken % P::kStages], (taken / P::kStages) & 1, a.status);
       return;
@@ -428,14 +381,14 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
 }
 
 template <typename T, int D>
-int launch_t(const PagedAttnArgs& a, int ctas, int most_rows, int* prefix, const CUtensorMap& km, const CUtensorMap& vm,
+int launch_t(const PagedAttnArgs& a, int streams, int most_rows, int* prefix, const CUtensorMap& km, const CUtensorMap& vm,
              cudaStream_t stream) {
   const int requests = a.shared ? 1 : a.R;
   auto kern = token_attn_kernel<T, D>;
   const int smem = TokenPlan<D>::kBytes + (requests + 1) * 4;
   const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (rc) return rc;
-  kern<<<ctas, kWarps * 32, smem, stream>>>(a, requests, most_rows, prefix, km, vm);
+  kern<<<streams / kWarps, kWarps * 32, smem, stream>>>(a, requests, most_rows, prefix, km, vm);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -445,20 +398,20 @@ bool token_attn_takes(int kv_dtype, int d, int page_size, int R, const void* k, 
                       long long q_ts, long long q_hs) {
   const uintptr_t pool = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
   const uintptr_t rows = reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(q_ts * 2) | static_cast<uintptr_t>(q_hs * 2);
-  return kv_dtype != kF32 && (d == 64 || d == 128) && page_size % kChunk == 0 && R <= 16384 && pool % 16 == 0 &&
+  return kv_dtype != kF32 && (d == 64 || d == 128) && page_size % kUnit == 0 && R <= 16384 && pool % 16 == 0 &&
          rows % 4 == 0;
 }
 
-int launch_token_attn(const PagedAttnArgs& a, int kv_dtype, int ctas, int most_rows, int* prefix, cudaStream_t stream) {
+int launch_token_attn(const PagedAttnArgs& a, int kv_dtype, int streams, int most_rows, int* prefix, cudaStream_t stream) {
   CUtensorMap km, vm;
-  int rc = encode_pool_map(&km, a, a.L.k, kv_dtype, kChunk);
-  if (rc == 0) rc = encode_pool_map(&vm, a, a.L.v, kv_dtype, kChunk);
+  int rc = encode_pool_map(&km, a, a.L.k, kv_dtype, kUnit);
+  if (rc == 0) rc = encode_pool_map(&vm, a, a.L.v, kv_dtype, kUnit);
   if (rc) return rc;
   if (kv_dtype == kBF16)
-    return a.d == 64 ? launch_t<__nv_bfloat16, 64>(a, ctas, most_rows, prefix, km, vm, stream)
-                     : launch_t<__nv_bfloat16, 128>(a, ctas, most_rows, prefix, km, vm, stream);
-  return a.d == 64 ? launch_t<__half, 64>(a, ctas, most_rows, prefix, km, vm, stream)
-                   : launch_t<__half, 128>(a, ctas, most_rows, prefix, km, vm, stream);
+    return a.d == 64 ? launch_t<__nv_bfloat16, 64>(a, streams, most_rows, prefix, km, vm, stream)
+                     : launch_t<__nv_bfloat16, 128>(a, streams, most_rows, prefix, km, vm, stream);
+  return a.d == 64 ? launch_t<__half, 64>(a, streams, most_rows, prefix, km, vm, stream)
+                   : launch_t<__half, 128>(a, streams, most_rows, prefix, km, vm, stream);
 }
 
 }  // namespace stk
