@@ -264,13 +264,14 @@ int launch_rows_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream) 
 }
 
 // ------------------------------------------------------------------ join
-// out = sum_s e^{m_s - M} o_s / sum_s e^{m_s - M} l_s over the parts of a row;
-// parts without keys have m = -inf and are not read. The parts' states are
-// FP32 and read once (L2-resident); the kernel is bound by its few dependent
-// loads. WPR warps share a row: with one, a CTA joins eight rows; where there
-// are too few rows to fill the SMs that way, all eight warps take every eighth
-// part of one row and add up in shared memory, in warp order. Lanes hold V
-// consecutive dims (d = 32 V) or, V = 0, every 32nd.
+// out = sum_s e^{m_s - M} o_s / sum_s e^{m_s - M} l_s over the parts of a row,
+// in one pass with a running maximum; parts without keys have m = -inf. The
+// parts' states are FP32 and read once (L2-resident); the kernel is bound by
+// its few dependent loads, so eight parts' maxima, sums and dims are asked for
+// at once. WPR warps share a row: with one, a CTA joins eight rows; where
+// there are too few rows to fill the SMs that way, all eight warps take every
+// eighth part of one row and meet in shared memory, in warp order. Lanes hold
+// V consecutive dims (d = 32 V) or, V = 0, every 32nd.
 constexpr int kJoinWarps = 8;
 
 template <typename T, int V, int WPR>
@@ -315,67 +316,78 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(JoinArgs a) {
       step[k] = p.most_rows;
     }
   }
-  float M = neg_inf();
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    for (int s = lane; s < parts[k]; s += 32) M = fmaxf(M, a.src[k].ml[base[k] + s * step[k]].x);
-  M = warp_max(M);
-  const bool empty = M == neg_inf();
   constexpr int N = V ? V : 4;
-  __shared__ float sum_o[WPR == 1 ? 1 : kJoinWarps][32 * N + 1];
+  constexpr int kBatch = 8;  // parts in flight
+  __shared__ float part_o[WPR == 1 ? 1 : kJoinWarps][32 * N];
+  __shared__ float2 part_ml[kJoinWarps];
   for (int d0 = 0; d0 < a.d; d0 += 32 * N) {
-    float o[N], Z = 0.f;
+    float o[N], M = neg_inf(), Z = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = 0.f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      // Lane i has the weight of part first_part + WPR (s0 + i).
-      for (int s0 = 0; first_part + WPR * s0 < parts[k]; s0 += 32) {
-        const int s = first_part + WPR * (s0 + lane);
-        float c = 0.f;
-        if (s < parts[k]) {
-          const float2 ml = a.src[k].ml[base[k] + s * step[k]];
-          c = ml.x == neg_inf() ? 0.f : expf(ml.x - M);
-          Z += c == 0.f ? 0.f : c * ml.y;
-        }
-        const int count = min(32, (parts[k] - first_part + WPR - 1) / WPR - s0);
-#pragma unroll 8
-        for (int i = 0; i < count; ++i) {
-          const float w = __shfl_sync(kFull, c, i);
-          if (w == 0.f) continue;  // also a part that was never written
-          const float* p = a.src[k].o + (base[k] + (first_part + WPR * (s0 + i)) * step[k]) * a.d + d0;
-          float x[N];
+      for (int s0 = first_part; s0 < parts[k]; s0 += WPR * kBatch) {
+        float2 ml[kBatch];
+        float x[kBatch][N];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {  // the last part again past the end, with no weight
+          const int s = s0 + WPR * i;
+          const long long at = base[k] + min(s, parts[k] - 1) * step[k];
+          ml[i] = a.src[k].ml[at];
+          if (s >= parts[k]) ml[i].x = neg_inf();
+          const float* p = a.src[k].o + at * a.d + d0;
           if constexpr (V != 0) {
-            load_vec<float, N>(p + lane * N, x);
+            load_vec<float, N>(p + lane * N, x[i]);
           } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = d0 + lane + 32 * j < a.d ? p[lane + 32 * j] : 0.f;
+            for (int j = 0; j < N; ++j) x[i][j] = d0 + lane + 32 * j < a.d ? p[lane + 32 * j] : 0.f;
           }
-#pragma unroll
-          for (int j = 0; j < N; ++j) o[j] = fmaf(w, x[j], o[j]);
         }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[i].x);
+        if (top == neg_inf()) continue;
+        const float f = expf(M - top);
+        Z *= f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] *= f;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (ml[i].x == neg_inf()) continue;  // also a part that was never written
+          const float w = expf(ml[i].x - top);
+          Z = fmaf(w, ml[i].y, Z);
+#pragma unroll
+          for (int j = 0; j < N; ++j) o[j] = fmaf(w, x[i][j], o[j]);
+        }
+        M = top;
       }
     }
-    Z = warp_sum(Z);
     if constexpr (WPR > 1) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) sum_o[warp][lane * N + j] = o[j];
-      if (lane == 0) sum_o[warp][32 * N] = Z;
+      for (int j = 0; j < N; ++j) part_o[warp][lane * N + j] = o[j];
+      if (lane == 0) part_ml[warp] = make_float2(M, Z);
       __syncthreads();
       if (warp == 0) {
+        M = neg_inf();
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) M = fmaxf(M, part_ml[w].x);
         Z = 0.f;
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j] = 0.f;
+        if (M != neg_inf()) {
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) {
-          Z += sum_o[w][32 * N];
+          for (int w = 0; w < kJoinWarps; ++w) {
+            const float f = expf(part_ml[w].x - M);
+            Z = fmaf(f, part_ml[w].y, Z);
 #pragma unroll
-          for (int j = 0; j < N; ++j) o[j] += sum_o[w][lane * N + j];
+            for (int j = 0; j < N; ++j) o[j] = fmaf(f, part_o[w][lane * N + j], o[j]);
+          }
         }
       }
       __syncthreads();
       if (warp != 0) continue;
     }
+    const bool empty = M == neg_inf();
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int dd = d0 + (V ? lane * N + j : lane + 32 * j);
