@@ -61,12 +61,17 @@ class PagedKVCache:
         return self.lo.shape[1]
 
     def kv(self) -> L.StkKV:
+        return L.kv_struct(self.k_pages, self.v_pages, page_table=self.page_table,
+                           block_offsets=self.block_offsets, page_size=self.page_size, hkv=self.hkv, n=0,
+                           b=self.block_size, d=self.dim)
+
+    def packed_kv(self, hkv, dim) -> bytes:
+        """``kv()`` as the packed bytes that the paged token calls take."""
         k, v = self.k_pages, self.v_pages
-        if k.dtype != v.dtype:
+        if k.dtype is not v.dtype:
             raise ValueError("K and V must share a dtype")
-        _, hkv, _, d = k.shape
-        return L.StkKV(k.data_ptr(), v.data_ptr(), L.dtype_code(k), hkv, 0, self.block_size, d,
-                       self.page_table.data_ptr(), self.block_offsets.data_ptr(), self.page_size, 0)
+        return L.PACK_KV(k.data_ptr(), v.data_ptr(), L.dtype_code(k), hkv, 0, self.block_size, dim,
+                         self.page_table.data_ptr(), self.block_offsets.data_ptr(), self.page_size, 0)
 
 
 def build_paged_cache(ks, vs, page_size, *, generator=None, device=None) -> PagedKVCache:

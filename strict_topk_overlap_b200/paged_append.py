@@ -8,8 +8,6 @@ calls read. New: the reference starts from a filled dense cache.
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib as L
@@ -40,18 +38,18 @@ def empty_paged_cache(capacities, hkv, dim, block_size, page_size, *, dtype=torc
                         -lo, block_size, page_size, max(blocks))
 
 
-def _ints(x, shape, name, dev):
-    """Address of an int32 tensor of this shape."""
-    if x.dtype != torch.int32 or x.shape != shape or x.device != dev or not x.is_contiguous():
+def _ints(x, shape, name, index):
+    """Address of an int32 tensor of this shape on device ``index``."""
+    if x.dtype is not torch.int32 or x.shape != shape or x.get_device() != index or not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 of shape {shape} on the cache's device")
     return x.data_ptr()
 
 
-def _rows(x, shape, name, pool):
+def _rows(x, shape, name, dtype, index):
     """Address and token and head strides of rows [T, heads, D]."""
     if x.shape != shape:
         raise ValueError(f"{name} must be [T, heads, D] = {shape}, got {tuple(x.shape)}")
-    if x.dtype != pool.dtype or x.device != pool.device:
+    if x.dtype is not dtype or x.get_device() != index:
         raise ValueError(f"{name} must have the cache's dtype and device")
     token, head, unit = x.stride()
     if unit != 1 and shape[2] > 1:
@@ -59,47 +57,50 @@ def _rows(x, shape, name, pool):
     return x.data_ptr(), token, head
 
 
-def _heads(q, hkv, name="q"):
+def _heads(q, hkv):
     """Tokens and heads of q [T, Hq, D]."""
-    if q.ndim != 3 or q.shape[1] == 0 or q.shape[1] % hkv:
-        raise ValueError(f"{name} must be [T, Hq, D] with Hq a multiple of the KV heads")
-    return q.shape[0], q.shape[1]
+    shape = q.shape
+    if len(shape) != 3 or shape[1] == 0 or shape[1] % hkv:
+        raise ValueError("q must be [T, Hq, D] with Hq a multiple of the KV heads")
+    return shape[0], shape[1]
 
 
-def _tokens(token_offsets, t, requests, dev):
+def _tokens(token_offsets, t, requests, index):
     """Address of the packed tokens' offsets, or None for one token per request."""
     if token_offsets is not None:
-        return _ints(token_offsets, (requests + 1,), "token_offsets", dev)
+        return _ints(token_offsets, (requests + 1,), "token_offsets", index)
     if t != requests:
         raise ValueError("without token_offsets there must be one token per request")
     return None
 
 
-def _rotary(rotary, positions, t, dev):
-    """The call's stk_rotary and the positions' address."""
+def _rotary(rotary, positions, t, index):
+    """The call's packed stk_rotary and the positions' address."""
     if rotary is None:
         if positions is not None:
             raise ValueError("positions need a rotary table")
         return None, None
     cos, sin, axis = rotary.cos, rotary.sin, rotary.axis
     size = cos.shape
-    if len(size) != 2 or sin.shape != size or cos.dtype != torch.float32 or sin.dtype != torch.float32 or \
-            cos.device != dev or sin.device != dev or not (cos.is_contiguous() and sin.is_contiguous()):
+    if len(size) != 2 or sin.shape != size or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or \
+            cos.get_device() != index or sin.get_device() != index or not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("rotary cos / sin must be contiguous FP32 [positions, pairs] on the cache's device")
     axes, at = 1, None
     if positions is not None:
         axes = positions.shape[0] if positions.ndim == 2 else 1
-        at = _ints(positions, (axes, t) if positions.ndim == 2 else (t,), "positions", dev)
+        at = _ints(positions, (axes, t) if positions.ndim == 2 else (t,), "positions", index)
     if axis is None:
         if axes > 1:
             raise ValueError("positions with several axes need a rotary axis for each pair")
+        axis_at = 0
     else:
-        if axis.dtype != torch.uint8 or axis.shape != size[1:] or axis.device != dev or not axis.is_contiguous():
+        if axis.dtype is not torch.uint8 or axis.shape != size[1:] or axis.get_device() != index or \
+                not axis.is_contiguous():
             raise ValueError("rotary axis must be uint8 [pairs] on the cache's device")
         if positions is None:
             raise ValueError("several rotary axes need positions [axes, T]")
-        axis = axis.data_ptr()
-    return L.StkRotary(cos.data_ptr(), sin.data_ptr(), size[1], size[0], rotary.interleaved, axes, axis), at
+        axis_at = axis.data_ptr()
+    return L.PACK_ROTARY(cos.data_ptr(), sin.data_ptr(), size[1], size[0], rotary.interleaved, axes, axis_at), at
 
 
 def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=None, rotary: Rotary | None = None,
@@ -115,24 +116,28 @@ def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=N
     itself), or None without q."""
     pool = cache.k_pages
     pages, hkv, _, d = pool.shape
-    dev, requests, blocks = pool.device, cache.requests, cache.total_blocks
+    dtype, index = pool.dtype, pool.get_device()
+    requests, blocks = cache.block_offsets.shape[0] - 1, cache.lo.shape[1]
     t = k.shape[0]
-    kp, kt, kh = _rows(k, (t, hkv, d), "k", pool)
-    vp, vt, vh = _rows(v, (t, hkv, d), "v", pool)
-    before = _ints(lengths, (requests,), "lengths", dev)
-    offsets = _tokens(token_offsets, t, requests, dev)
+    kp, kt, kh = _rows(k, (t, hkv, d), "k", dtype, index)
+    vp, vt, vh = _rows(v, (t, hkv, d), "v", dtype, index)
+    before = _ints(lengths, (requests,), "lengths", index)
+    offsets = _tokens(token_offsets, t, requests, index)
     qp = qt = qh = hq = out = 0
     if q is not None:
-        _, hq = _heads(q, hkv)
-        qp, qt, qh = _rows(q, (t, hq, d), "q", pool)
+        hq = _heads(q, hkv)[1]
+        qp, qt, qh = _rows(q, (t, hq, d), "q", dtype, index)
         if q_out is None:
             q_out = q.new_empty((t, hq, d))
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != dev or not q_out.is_contiguous():
+        elif q_out.shape != (t, hq, d) or q_out.dtype is not dtype or q_out.get_device() != index or \
+                not q_out.is_contiguous():
             raise ValueError("q_out must be contiguous, of q's shape, dtype and device")
         out = q_out.data_ptr()
-    turn, at = _rotary(rotary, positions, t, dev)
+    turn, at = _rotary(rotary, positions, t, index)
     lo, hi = (cache.lo.data_ptr(), cache.hi.data_ptr()) if blocks else (None, None)
-    rc = L.load().stk_append_tokens(cache.kv(), pages, requests, blocks or 1, t, kp, kt, kh, vp, vt, vh, qp, qt, qh, hq,
-                                    out, before, offsets, at, turn, lo, hi, L.status_ptr(), L.stream_of(pool))
-    L.check(rc, "append_tokens")
+    rc = L.load().stk_append_tokens(cache.packed_kv(hkv, d), pages, requests, blocks or 1, t, kp, kt, kh, vp, vt, vh, qp,
+                                    qt, qh, hq, out, before, offsets, at, turn, lo, hi, L.status_ptr(),
+                                    L.stream_of(pool))
+    if rc:
+        L.check(rc, "append_tokens")
     return q_out if q is not None else None

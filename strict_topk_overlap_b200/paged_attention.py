@@ -35,7 +35,7 @@ def _most(max_tokens, tokens, token_offsets):
 def _workspace_bytes(device, dtype, hkv, block, dim, page, requests, tokens, hq, packed, most, longest, prefix):
     """Workspace of a call, from its sizes alone (a pool address stands for any)."""
     any_pool = 256
-    kv = L.StkKV(any_pool, any_pool, dtype, hkv, 0, block, dim, any_pool, any_pool, page, 0)
+    kv = L.PACK_KV(any_pool, any_pool, dtype, hkv, 0, block, dim, any_pool, any_pool, page, 0)
     with torch.cuda.device(device):
         return L.load().stk_paged_attention_workspace_bytes(kv, requests, tokens, hq, packed, most, longest, prefix)
 
@@ -53,29 +53,29 @@ def _attend(q, cache, lengths, token_offsets, max_tokens, kv_lo, kv_hi, softcap,
             prefix):
     pool = cache.k_pages
     pages, hkv, _, d = pool.shape
-    dev, requests = pool.device, cache.requests
+    dtype, index = pool.dtype, pool.get_device()
+    requests = cache.block_offsets.shape[0] - 1
     t, hq = _heads(q, hkv)
-    qp, qt, qh = _rows(q, (t, hq, d), "q", pool)
-    held = _ints(lengths, (requests,), "lengths", dev)
-    offsets = _tokens(token_offsets, t, requests, dev)
+    qp, qt, qh = _rows(q, (t, hq, d), "q", dtype, index)
+    held = _ints(lengths, (requests,), "lengths", index)
+    offsets = _tokens(token_offsets, t, requests, index)
     most = _most(max_tokens, t, token_offsets)
     block, page = cache.block_size, cache.page_size
     longest = cache.max_blocks * block
     options = None
     if softcap or slopes is not None or scale is not None or kv_lo is not None or kv_hi is not None:
-        if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (hq,) or slopes.device != dev or
-                                   not slopes.is_contiguous()):
+        if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (hq,) or
+                                   slopes.get_device() != index or not slopes.is_contiguous()):
             raise ValueError("slopes must be contiguous FP32 [Hq] on the cache's device")
         if softcap < 0 or (scale is not None and scale <= 0):
             raise ValueError("softcap must not be negative and scale must be positive")
-        options = L.StkAttentionOptions(scale or 0.0, softcap, L.ptr(slopes),
-                                        None if kv_lo is None else _ints(kv_lo, (t,), "kv_lo", dev),
-                                        None if kv_hi is None else _ints(kv_hi, (t,), "kv_hi", dev))
+        options = L.PACK_OPTIONS(scale or 0.0, softcap, 0 if slopes is None else slopes.data_ptr(),
+                                 0 if kv_lo is None else _ints(kv_lo, (t,), "kv_lo", index),
+                                 0 if kv_hi is None else _ints(kv_hi, (t,), "kv_hi", index))
     if prefix and (prefix < 0 or prefix % page or prefix > longest):
         raise ValueError(f"prefix must be whole pages of {page} tokens, at most {longest} tokens")
-    kv = cache.kv()
     if workspace is None:
-        need = _workspace_bytes(q.get_device(), kv.kv_dtype, hkv, block, d, page, requests, t, hq, offsets is not None,
+        need = _workspace_bytes(index, L.dtype_code(pool), hkv, block, d, page, requests, t, hq, offsets is not None,
                                 most, longest, prefix)
         if need:
             workspace = q.new_empty((need,), dtype=torch.uint8)
@@ -83,10 +83,11 @@ def _attend(q, cache, lengths, token_offsets, max_tokens, kv_lo, kv_hi, softcap,
         need = workspace.numel()
     out = q.new_empty((t, hq, d))
     lse = q.new_empty((t, hq), dtype=torch.float32) if return_lse else None
-    rc = L.load().stk_paged_attention(kv, pages, qp, qt, qh, requests, t, hq, held, offsets, most, longest, prefix,
-                                      options, out.data_ptr(), L.ptr(lse), L.ptr(workspace), need, L.status_ptr(),
-                                      L.stream_of(q))
-    L.check(rc, "paged attention")
+    rc = L.load().stk_paged_attention(cache.packed_kv(hkv, d), pages, qp, qt, qh, requests, t, hq, held, offsets, most,
+                                      longest, prefix, options, out.data_ptr(), L.ptr(lse), L.ptr(workspace), need,
+                                      L.status_ptr(), L.stream_of(q))
+    if rc:
+        L.check(rc, "paged attention")
     return (out, lse) if return_lse else out
 
 
