@@ -296,38 +296,12 @@ __device__ __forceinline__ void head_rows(const Tile& t, const T* src, long long
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kAppendWarps * 32, VEC > 1 ? 3 : 2) append_kernel(AppendArgs a, int tile_tokens) {
+__global__ void __launch_bounds__(kAppendWarps * 32, VEC > 1 ? 3 : 2)
+append_kernel(AppendArgs a, int tile_tokens, int chunks, int items) {
   extern __shared__ float tables[];  // cosines, then sines, of tile_tokens tokens
-  __shared__ long long slot[32];
+  __shared__ long long page_slot[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int B = a.L.b, D = a.L.d, hkv = a.L.hkv, ps = a.L.page_size;
-  int r, t0, n, f;
-  if (a.token_offsets == nullptr) {
-    r = blockIdx.x;
-    t0 = r;
-    n = 1;
-    f = 0;
-  } else {
-    r = request_of_slot(a.token_offsets, a.R, 1, B, 2, blockIdx.x, lane);
-    t0 = a.token_offsets[r];
-    n = a.token_offsets[r + 1] - t0;
-    f = blockIdx.x - t0 / B - 2 * r;
-  }
-  if (n <= 0) return;
-  const int len = a.lengths[r];
-  if (len < 0) {
-    if (tid == 0) report(a.status, kStatusBadLength);
-    return;
-  }
-  const int j = len / B + f;  // block of the request
-  const int begin = max(len, j * B);
-  const int end = static_cast<int>(min(static_cast<long long>(len) + n, (j + 1ll) * B));
-  if (begin >= end) return;
-  const bool room = j < request_blocks(a.L, r);
-  if (!room && tid == 0) report(a.status, kStatusBadLength);
-  const int base = a.L.block_offsets ? a.L.block_offsets[r] : 0;
-  const int* table = a.L.page_table + (static_cast<long long>(base) + j) * (B / ps);
-
   Tile t;
   t.pairs = a.cos ? a.pairs : 0;
   t.rot_items = t.pairs / VEC;
@@ -338,36 +312,74 @@ __global__ void __launch_bounds__(kAppendWarps * 32, VEC > 1 ? 3 : 2) append_ker
   float* sine = tables + tile_tokens * t.pairs;
   t.cosine = cosine;
   t.sine = sine;
-  t.slot = slot;
+  t.slot = page_slot;
   const int hq = a.q ? a.hq : 0, heads = hq + 2 * hkv;
-  for (int tile = begin; tile < end; tile += tile_tokens) {
-    t.nt = min(tile_tokens, end - tile);
-    const int token = t0 + (tile - len);  // packed token of the tile's first
-    if (tile != begin) __syncthreads();
-    if (tid < t.nt) {
-      const int in = tile + tid - j * B, pg = in / ps;
-      const int page = room ? table[pg] : -1;
-      if (room && (page < 0 || page >= a.pages)) report(a.status, kStatusBadBlockId);
-      slot[tid] = page < 0 || page >= a.pages ? -1 : (static_cast<long long>(page) * hkv * ps + (in - pg * ps)) * D;
-    }
-    for (int tt = warp; tt < t.nt; tt += kAppendWarps) {
-      for (int p = lane; p < t.pairs; p += 32) {
-        int pos = tile + tt;
-        if (a.positions) {
-          const int ax = a.axis ? a.axis[p] : 0;
-          pos = ax < a.axes ? a.positions[static_cast<long long>(ax) * a.T + token + tt] : -1;
-        }
-        if (pos < 0 || pos >= a.max_position) {
-          report(a.status, kStatusBadPosition);
-          pos = 0;
-        }
-        const long long o = static_cast<long long>(pos) * t.pairs + p;
-        cosine[tt * t.pairs + p] = a.cos[o];
-        sine[tt * t.pairs + p] = a.sin[o];
+  // Items (slot, chunk of heads) in order; a run of chunks of one slot shares its tables.
+  const int per = (items + gridDim.x - 1) / gridDim.x;
+  const int last = min(items, static_cast<int>(blockIdx.x + 1) * per);
+  int at = -1, staged = -1;
+  int r = 0, t0 = 0, n = 0, len = 0, j = 0, begin = 0, end = 0, base = 0;
+  bool room = false;
+  const int* table = nullptr;
+  for (int item = blockIdx.x * per; item < last; ++item) {
+    const int slot = item / chunks, chunk = item - slot * chunks;
+    if (slot != at) {
+      at = slot;
+      int f = 0;
+      if (a.token_offsets == nullptr) {
+        r = t0 = slot;
+        n = 1;
+      } else {
+        r = request_of_slot(a.token_offsets, a.R, 1, B, 2, slot, lane);
+        t0 = a.token_offsets[r];
+        n = a.token_offsets[r + 1] - t0;
+        f = slot - t0 / B - 2 * r;
       }
+      len = a.lengths[r];
+      base = a.L.block_offsets[r];
+      const int blocks = a.L.block_offsets[r + 1] - base;
+      begin = end = 0;
+      if (n > 0 && len >= 0) {
+        j = len / B + f;  // block of the request
+        begin = max(len, j * B);
+        end = static_cast<int>(min(static_cast<long long>(len) + n, (j + 1ll) * B));
+      }
+      room = j < blocks;
+      if (tid == 0 && n > 0 && (len < 0 || (begin < end && !room))) report(a.status, kStatusBadLength);
+      table = a.L.page_table + (static_cast<long long>(base) + j) * (B / ps);
     }
-    __syncthreads();
-    for (int hd = blockIdx.y * kAppendWarps + warp; hd < heads; hd += gridDim.y * kAppendWarps) {
+    for (int tile = begin; tile < end; tile += tile_tokens) {
+      t.nt = min(tile_tokens, end - tile);
+      const int token = t0 + (tile - len);  // packed token of the tile's first
+      if (staged != slot || end - begin > tile_tokens) {
+        staged = slot;
+        __syncthreads();
+        if (tid < t.nt) {
+          const int in = tile + tid - j * B, pg = in / ps;
+          const int page = room ? table[pg] : -1;
+          if (room && (page < 0 || page >= a.pages)) report(a.status, kStatusBadBlockId);
+          page_slot[tid] =
+              page < 0 || page >= a.pages ? -1 : (static_cast<long long>(page) * hkv * ps + (in - pg * ps)) * D;
+        }
+        for (int tt = warp; tt < t.nt; tt += kAppendWarps) {
+          for (int p = lane; p < t.pairs; p += 32) {
+            int pos = tile + tt;
+            if (a.positions) {
+              const int ax = a.axis ? a.axis[p] : 0;
+              pos = ax < a.axes ? a.positions[static_cast<long long>(ax) * a.T + token + tt] : -1;
+            }
+            if (pos < 0 || pos >= a.max_position) {
+              report(a.status, kStatusBadPosition);
+              pos = 0;
+            }
+            const long long o = static_cast<long long>(pos) * t.pairs + p;
+            cosine[tt * t.pairs + p] = a.cos[o];
+            sine[tt * t.pairs + p] = a.sin[o];
+          }
+        }
+        __syncthreads();
+      }
+      const int hd = chunk * kAppendWarps + warp;
       if (hd < hq) {
         const T* src = static_cast<const T*>(a.q) + token * a.q_ts + hd * a.q_hs;
         T* dst = static_cast<T*>(a.q_out) + (static_cast<long long>(token) * a.hq + hd) * D;
@@ -379,21 +391,21 @@ __global__ void __launch_bounds__(kAppendWarps * 32, VEC > 1 ? 3 : 2) append_ker
         T* dst = static_cast<T*>(const_cast<void*>(a.L.k)) + static_cast<long long>(h) * ps * D;
         const long long o = (static_cast<long long>(h) * a.total + base + j) * D;
         if (a.lo != nullptr && room)
-          head_rows<T, VEC, true, true>(t, src, a.k_ts, dst, slot, 0, lane, a.lo + o, a.hi + o, tile > j * B);
+          head_rows<T, VEC, true, true>(t, src, a.k_ts, dst, page_slot, 0, lane, a.lo + o, a.hi + o, tile > j * B);
         else
-          head_rows<T, VEC, true, false>(t, src, a.k_ts, dst, slot, 0, lane, nullptr, nullptr, false);
-      } else {
+          head_rows<T, VEC, true, false>(t, src, a.k_ts, dst, page_slot, 0, lane, nullptr, nullptr, false);
+      } else if (hd < heads) {
         const int h = hd - hq - hkv;
         const T* src = static_cast<const T*>(a.v) + token * a.v_ts + h * a.v_hs;
         T* dst = static_cast<T*>(const_cast<void*>(a.L.v)) + static_cast<long long>(h) * ps * D;
-        head_rows<T, VEC, false, false>(t, src, a.v_ts, dst, slot, 0, lane, nullptr, nullptr, false);
+        head_rows<T, VEC, false, false>(t, src, a.v_ts, dst, page_slot, 0, lane, nullptr, nullptr, false);
       }
     }
   }
 }
 
 template <typename T, int VEC>
-static int launch_append_t(const AppendArgs& a, cudaStream_t stream) {
+static int launch_append_t(const AppendArgs& a, int sms, cudaStream_t stream) {
   const int slots = a.token_offsets ? a.T / a.L.b + 2 * a.R : a.R;
   const int heads = (a.q ? a.hq : 0) + 2 * a.L.hkv;
   // 32 tokens of tables per tile up to 128 pairs, fewer for wider heads.
@@ -403,13 +415,19 @@ static int launch_append_t(const AppendArgs& a, cudaStream_t stream) {
   auto kern = append_kernel<T, VEC>;
   if (smem > 48 * 1024)
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  const int y = (heads + kAppendWarps - 1) / kAppendWarps;
-  kern<<<dim3(static_cast<unsigned>(slots), static_cast<unsigned>(y)), kAppendWarps * 32, smem, stream>>>(a, tile);
+  // One item (a slot's eight heads, one per warp) per CTA while that leaves
+  // SMs free; beyond, equal runs of items for the CTAs that fit.
+  const int chunks = (heads + kAppendWarps - 1) / kAppendWarps;
+  const long long items = static_cast<long long>(slots) * chunks;
+  if (items > 0x3fffffff) return static_cast<int>(cudaErrorInvalidValue);
+  const long long fit = 3ll * sms;
+  kern<<<static_cast<unsigned>(items < fit ? items : fit), kAppendWarps * 32, smem, stream>>>(a, tile, chunks,
+                                                                                              static_cast<int>(items));
   return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T>
-static int launch_append_v(const AppendArgs& a, cudaStream_t stream) {
+static int launch_append_v(const AppendArgs& a, int sms, cudaStream_t stream) {
   // 16-byte vectors where every row of every tensor starts on one and a
   // pair's two vectors stay inside the rotated dims; single elements else.
   constexpr int VEC = 16 / sizeof(T);
@@ -418,14 +436,14 @@ static int launch_append_v(const AppendArgs& a, cudaStream_t stream) {
             aligned(a.k) && aligned(a.v) && aligned(a.L.k) && aligned(a.L.v);
   if (a.q) ok = ok && a.q_ts % VEC == 0 && a.q_hs % VEC == 0 && aligned(a.q) && aligned(a.q_out);
   if (a.cos) ok = ok && a.pairs % VEC == 0;
-  return ok ? launch_append_t<T, VEC>(a, stream) : launch_append_t<T, 1>(a, stream);
+  return ok ? launch_append_t<T, VEC>(a, sms, stream) : launch_append_t<T, 1>(a, sms, stream);
 }
 
-int launch_append_tokens(const AppendArgs& a, int kv_dtype, cudaStream_t stream) {
+int launch_append_tokens(const AppendArgs& a, int kv_dtype, int sms, cudaStream_t stream) {
   switch (kv_dtype) {
-    case kF32: return launch_append_v<float>(a, stream);
-    case kF16: return launch_append_v<__half>(a, stream);
-    default: return launch_append_v<__nv_bfloat16>(a, stream);
+    case kF32: return launch_append_v<float>(a, sms, stream);
+    case kF16: return launch_append_v<__half>(a, sms, stream);
+    default: return launch_append_v<__nv_bfloat16>(a, sms, stream);
   }
 }
 

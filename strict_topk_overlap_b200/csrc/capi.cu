@@ -905,7 +905,7 @@ extern "C" int stk_append_tokens(const stk_kv* kv, int pages, int R, int total_b
     a.interleaved = rotary->interleaved; a.axes = rotary->axes; a.axis = rotary->axis; a.positions = positions;
   }
   a.lo = lo; a.hi = hi; a.total = total_blocks; a.status = status;
-  return cuda_status(launch_append_tokens(a, kv->kv_dtype, static_cast<cudaStream_t>(stream)), "append_tokens");
+  return cuda_status(launch_append_tokens(a, kv->kv_dtype, sm_count_current(), static_cast<cudaStream_t>(stream)), "append_tokens");
 }
 
 namespace {

@@ -164,7 +164,7 @@ __device__ __forceinline__ int page_of(const PagedAttnArgs& a, int rp, int j) {
   return page;
 }
 
-int launch_append_tokens(const AppendArgs& a, int kv_dtype, cudaStream_t stream);
+int launch_append_tokens(const AppendArgs& a, int kv_dtype, int sms, cudaStream_t stream);
 int launch_rows_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream);
 // Whether the tensor-core kernel takes these types, sizes and addresses.
 bool prompt_attn_takes(int kv_dtype, int d, int page_size, const void* k, const void* v, const void* q, long long q_ts,
