@@ -335,6 +335,11 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
                    const __grid_constant__ CUtensorMap vmap) {
   using P = Plan<D>;
   constexpr bool kLag = std::is_same<T, __nv_bfloat16>::value;
+  // Heads of 64 dims leave room in TMEM for an O of its own for each half of
+  // the keys: the halves then share nothing until the end. Heads of 128 dims
+  // share O, each half's warps keeping half of its dims in frame.
+  constexpr bool kOwnO = D == 64;
+  constexpr int kOCols = 64;  // of O, a warp's
   constexpr int kFmaPairs = MODE == 0 ? 2 : 1;  // of 8 pairs of weights, those whose exponentials take the FMA units
   constexpr int kHalves = D / 64;
   constexpr int kHalfBytes = kTileN * 128;
@@ -550,8 +555,8 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
             fence_after();
 #pragma unroll
             for (int s = 0; s < kTileN / 32; ++s)
-              mma_ts(tmem + 2 * kTileN + q * D, tmem + q * kTileN + x * (kTileN / 2) + s * 8,
-                     vd + (x * (kTileN / 32) + s) * (2048 >> 4), pv, done[q] > 0 || x > 0 || s > 0);
+              mma_ts(tmem + 2 * kTileN + (kOwnO ? q * 2 + x : q * 2) * kOCols, tmem + q * kTileN + x * (kTileN / 2) + s * 8,
+                     vd + (x * (kTileN / 32) + s) * (2048 >> 4), pv, done[q] > 0 || (!kOwnO && x > 0) || s > 0);
           }
           if (ok && then) issue_qk(q, x, kslot);
         }
@@ -572,7 +577,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const int r = tid & (kTileM - 1);  // row of the MMA tile
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
     const uint32_t ts = tmem + lanes + qt * kTileN + half * kKeys;
-    const uint32_t to = tmem + lanes + 2 * kTileN + qt * D + half * (D / 2);
+    const uint32_t to = tmem + lanes + 2 * kTileN + (qt * 2 + half) * kOCols;
     asm volatile("cp.async.wait_all;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mbar_arrive(&sh.q_full[qt]);
@@ -595,13 +600,14 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     float m = neg_inf(), l = 0.f;  // in log2 units; m is the frame of P, O and l, near the row's maximum
     bool ok = true, exact = true;
     int meetings = 0;
+    float level = neg_inf();  // the last tile's maximum, or a little more, less its largest bias
     const int begin = qt ? qa[1] : qa[0], end = qt ? qb[1] : qb[0];
     // O of the warp's rows (this half of its dims) and l by 2^(m - frame).
     auto reframe = [&](bool grow, float frame) {
       const float f = grow ? ex2(m - frame) : 1.f;
       l *= f;
 #pragma unroll 1
-      for (int j = 0; j < D / 2; j += 32) {
+      for (int j = 0; j < kOCols; j += 32) {
         uint32_t o[32];
         tmem_ld32(to + j, o);
         tmem_wait_ld();
@@ -631,6 +637,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       // A wait that runs out is told to the whole group at its next meeting: nobody is left waiting there.
       ok = warp_wait(&sh.s_full[qt][half], n & 1, a.status) && ok;
       if (!ok) sh.failed[qt] = 1;
+      if (kOwnO && !ok) break;
       fence_after();
       const int k0 = i * kTileN + half * kKeys;
       const bool full = k0 >= lomax && k0 + kKeys <= himin;
@@ -652,8 +659,12 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         if (MODE != 0 || !full) tmem_wait_st();
         mx *= c;
         // (Read before this thread's P is announced, and written again after the next S, which waits for that.)
-        sh.other[qt][half][r] = mx;
-        if (group_any(1 + qt, 2 * kTileM, grows(mx) || !ok)) {
+        if (!kOwnO) sh.other[qt][half][r] = mx;
+        if (kOwnO) {
+          const bool grow = grows(mx);
+          if (__any_sync(kFull, grow && m != neg_inf())) reframe(grow, mx);
+          else if (grow) m = mx;
+        } else if (group_any(1 + qt, 2 * kTileM, grows(mx) || !ok)) {
           if (sh.failed[qt]) {
             ok = false;
             break;
@@ -677,7 +688,8 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           tmem_st8(ts + j * kRun / 2, p);  // over scores that have been read
         }
         // Once every row that sees any key has met one, the frames may lag (not f16's: P would leave its range).
-        if (kLag) exact = group_any(1 + qt, 2 * kTileM, m == neg_inf() && rk.hi > rk.lo);
+        const bool waiting = m == neg_inf() && rk.hi > rk.lo;
+        if (kLag) exact = kOwnO ? __any_sync(kFull, waiting) : group_any(1 + qt, 2 * kTileM, waiting);
         est = m;
       } else {
         // One pass, without a maximum, in a frame that the first half of the
@@ -686,13 +698,18 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         // row are two independent chains of S, P and O that meet only where
         // the frame moves. A row whose scores run ahead of its frame by more
         // than 2^127 overflows and is recomputed like those below.
-        const unsigned short code = sh.frame[qt][n & 3][r];
-        const bool grow = code != kKeep;
-        const float frame = __uint_as_float(static_cast<uint32_t>(code) << 16) + most_bias(i);
-        if (__any_sync(kFull, grow)) {
-          meet();  // both halves' products of the last tile are complete
-          reframe(grow, frame);
-          meet();
+        if (kOwnO) {
+          const bool grow = grows(level + most_bias(i));
+          if (__any_sync(kFull, grow)) reframe(grow, level + most_bias(i));
+        } else {
+          const unsigned short code = sh.frame[qt][n & 3][r];
+          const bool grow = code != kKeep;
+          const float frame = __uint_as_float(static_cast<uint32_t>(code) << 16) + most_bias(i);
+          if (__any_sync(kFull, grow)) {
+            meet();  // both halves' products of the last tile are complete
+            reframe(grow, frame);
+            meet();
+          }
         }
         const float nm = m == neg_inf() ? 0.f : -m;
         tmem_ld16(ts, reinterpret_cast<uint32_t*>(s[0]));
@@ -708,10 +725,10 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         }
         est = log2f((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)) - nm;  // the maximum, or a little more
       }
-      if (kLag && half == 0 && !exact) {
-        // The next tile's frame. What the largest bias of a tile gains on this one's is known, and followed at once.
+      // The next tile's frame. What the largest bias of a tile gains on this one's is known, and followed at once.
+      level = m == neg_inf() ? neg_inf() : est - most_bias(i);
+      if (kLag && !kOwnO && half == 0 && !exact) {
         // Rounded down: a frame above the maximum would lose weights, one below it costs range only.
-        const float level = est - most_bias(i);
         const uint32_t code = (__float_as_uint(level) + (level < 0.f ? 0xffffu : 0u)) >> 16;
         const bool grow = m != neg_inf() && grows(__uint_as_float(code << 16) + most_bias(i + 1));
         sh.frame[qt][(n + 1) & 3][r] = grow ? static_cast<unsigned short>(code) : kKeep;
@@ -727,10 +744,23 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const bool any = begin < end;
     if (any) ok = warp_wait(&sh.o_full[qt], 0, a.status) && ok;
     fence_after();
-    // The row's sum over both halves of its keys.
-    sh.other[qt][half][r] = l;
-    group_any(1 + qt, 2 * kTileM, false);
-    l += sh.other[qt][half ^ 1][r];
+    auto swap = [&](float x) {  // the value of the row's other thread
+      sh.other[qt][half][r] = x;
+      group_any(1 + qt, 2 * kTileM, false);
+      const float y = sh.other[qt][half ^ 1][r];
+      group_any(1 + qt, 2 * kTileM, false);
+      return y;
+    };
+    // The row's sum over both halves of its keys, with their own O in one frame for both.
+    float mine = 1.f;
+    if (kOwnO) {
+      const float frame = fmaxf(m, swap(m));
+      mine = m == neg_inf() ? 0.f : ex2(m - frame);
+      l *= mine;
+      m = frame;
+    }
+    l += swap(l);
+    ok = !group_any(1 + qt, 2 * kTileM, !ok);
     const bool empty = m == neg_inf();
     const long long orow = static_cast<long long>(t.t0 + tok) * a.hq + head;
     const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
@@ -746,13 +776,12 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       auto put = [&](int c, uint4 w) {  // 16-byte chunk c of the lane's row
         *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ lane) & 7) * 16) = w;
       };
-      // The staged rows' first `bytes` to byte `at` of their rows of `stride` bytes.
-      auto flush = [&](unsigned char* to, long long my_row, long long stride, int at, int bytes) {
+      // The staged rows to byte `at` of their rows of `stride` bytes.
+      auto flush = [&](unsigned char* to, long long my_row, long long stride, int at) {
         __syncwarp();
-        const int per = bytes / 16, rows = 32 / per;  // lanes a row, rows an instruction
-        const int c = lane % per;
-        for (int r0 = 0; r0 < 32; r0 += rows) {
-          const int rr = r0 + lane / per;
+        const int c = lane & 7;
+        for (int r0 = 0; r0 < 32; r0 += 4) {
+          const int rr = r0 + lane / 8;
           const long long dst = __shfl_sync(kFull, my_row, rr);
           const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((c ^ rr) & 7) * 16);
           if (__shfl_sync(kFull, static_cast<int>(have), rr))
@@ -760,13 +789,40 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         }
         __syncwarp();
       };
+      const int first_dim = kOwnO ? 0 : half * kOCols;
 #pragma unroll 1
-      for (int j = 0; j < D / 2; j += 32) {
+      for (int j = 0; j < kOCols; j += 32) {
         uint32_t o[32];
         if (any) {
           tmem_ld32(to + j, o);
           tmem_wait_ld();
           tmem_loaded(o);
+        }
+        if (kOwnO) {  // the second half's dims through shared memory to the first half's thread
+          unsigned char* pass = base + qt * P::kQBytes + P::kQBytes / 2 + r * 128;  // beside the first half's stages
+          if (half) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              auto x = [&](int i) { return mine == 0.f ? 0.f : __uint_as_float(o[4 * e + i]) * mine; };
+              *reinterpret_cast<float4*>(pass + ((e ^ r) & 7) * 16) = make_float4(x(0), x(1), x(2), x(3));
+            }
+          }
+          group_any(1 + qt, 2 * kTileM, false);
+          if (half == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 y = *reinterpret_cast<const float4*>(pass + ((e ^ r) & 7) * 16);
+              auto x = [&](int i, float other) {
+                return __float_as_uint((mine == 0.f ? 0.f : __uint_as_float(o[4 * e + i]) * mine) + other);
+              };
+              o[4 * e] = x(0, y.x);
+              o[4 * e + 1] = x(1, y.y);
+              o[4 * e + 2] = x(2, y.z);
+              o[4 * e + 3] = x(3, y.w);
+            }
+          }
+          group_any(1 + qt, 2 * kTileM, false);
+          if (half) continue;
         }
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
@@ -777,7 +833,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         if (a.part_ml) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) put(e, make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
-          flush(reinterpret_cast<unsigned char*>(a.part_o), prow, D * 4, (half * (D / 2) + j) * 4, 128);
+          flush(reinterpret_cast<unsigned char*>(a.part_o), prow, D * 4, (first_dim + j) * 4);
         } else {
           uint32_t w[16];
 #pragma unroll
@@ -785,7 +841,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             put((j & 32) / 8 + e, make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]));
-          if (j + 32 == D / 2) flush(static_cast<unsigned char*>(a.out), orow, D * 2, half * D, D);
+          if (j) flush(static_cast<unsigned char*>(a.out), orow, D * 2, first_dim * 2);
         }
       }
       if (have && half == 0) {
@@ -795,7 +851,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       // Rows whose sums are not finite, be it for values of keys that they may
       // not see: this half of their dims once more, in the frame (m, l) that
       // stands, or in their own where l itself is lost.
-      unsigned redo = __ballot_sync(kFull, redo_row);
+      unsigned redo = __ballot_sync(kFull, redo_row && !(kOwnO && half));
       while (redo) {
         const int src = __ffs(redo) - 1;
         redo &= redo - 1;
@@ -817,7 +873,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           if (a.part_ml) a.part_ml[xp] = make_float2(xm, xl);
           else if (a.lse) a.lse[xr] = xm + logf(xl);
         }
-        if ((lane >> 4) == half) {
+        if (kOwnO || (lane >> 4) == half) {
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
             const int dd = lane * (D / 32) + j;
