@@ -947,9 +947,10 @@ AttnPhase plan_phase(const stk_kv* kv, int R, int T, int hq, bool offsets, bool 
     p.bytes = p.states * (kv->d + 2) * sizeof(float) + (p.requests + 1) * sizeof(int);
   } else {
     const bool prompt = p.kind == kAttnPrompt;
-    const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared, prompt ? 256 : 16)) * hkv;
+    const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared,
+                                                                prompt ? prompt_tile_rows(kv->d) : 16)) * hkv;
     const long long most = prompt ? (keys + 127) / 128 : (keys + 63) / 64;
-    long long n = (prompt ? sms : 2 * sms) / tiles;
+    long long n = (prompt ? prompt_ctas_per_sm(kv->d) : 2) * sms / tiles;
     n = n < most ? n : most;
     p.nsplit = static_cast<int>(n < 1 ? 1 : n);
     p.states = static_cast<size_t>(p.nsplit) * T * hq;

@@ -169,6 +169,9 @@ int launch_rows_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream);
 // Whether the tensor-core kernel takes these types, sizes and addresses.
 bool prompt_attn_takes(int kv_dtype, int d, int page_size, const void* k, const void* v, const void* q, long long q_ts,
                        long long q_hs);
+// Rows of its CTAs, and how many of them an SM holds.
+inline int prompt_tile_rows(int d) { return d == 64 ? 128 : 256; }
+inline int prompt_ctas_per_sm(int d) { return d == 64 ? 2 : 1; }
 int launch_prompt_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream);
 int set_wait_limit_prompt(unsigned long long ns);
 

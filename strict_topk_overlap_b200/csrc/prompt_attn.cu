@@ -2,7 +2,7 @@
 // pieces of prompts, and all requests' tokens over a shared prefix.
 //
 // The rows of one KV head (new tokens x query heads of the group, packed) are
-// cut into tiles of 256, two MMA tiles of 128. Per 128 keys:
+// cut into MMA tiles of 128, one or two to a CTA. Per 128 keys:
 //   S = Q K^T          128 x 128, FP32 in tensor memory (TMEM)
 //   P = 2^(c S - m)    two threads per row, 64 keys each: cap, bias, mask,
 //                      running maximum and sum in FP32; P rounded to the type,
@@ -36,9 +36,6 @@ namespace {
 
 constexpr int kTileM = 128;   // rows of an MMA tile
 constexpr int kTileN = 128;   // keys of a tile
-constexpr int kRows = 256;    // rows of a CTA
-constexpr int kSoftmaxWarps = 16;  // two groups of four per MMA tile, 64 keys each
-constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
 constexpr float kLazy = 8.f;  // log2 of the growth of the maximum that is left to P
 
 __device__ constexpr float kTanh3[3] = {0.99999961f, -0.33321959f, 0.1284243f};
@@ -49,7 +46,7 @@ struct Shared {
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2];  // [MMA tile] or [MMA tile][half of the keys]
   uint64_t pair[8];            // the two warps that share 32 rows
   uint32_t tmem;
-  int4 range[kSoftmaxWarps];   // of a warp's rows: least and largest key, largest lo, least hi
+  int4 range[16];   // of a warp's rows: least and largest key, largest lo, least hi
   volatile int failed[2];      // a wait of the MMA tile's softmax ran out
   union {
     float other[2][2][kTileM];             // [MMA tile][half of the keys][row]: maxima, at the end the sums
@@ -58,12 +55,22 @@ struct Shared {
 };
 constexpr unsigned short kKeep = 0x7fc0;   // (a NaN) the frame stays
 
+// Heads of 128 dims: two MMA tiles (256 rows) in a CTA that fills the SM, so
+// that a K and V tile from L2 serves both. Heads of 64 dims need half the
+// bytes and TMEM per MMA tile: one MMA tile in a CTA and two CTAs an SM, which
+// start and end beside one another.
 template <int D>
 struct Plan {
+  static constexpr int kMmaTiles = D == 128 ? 2 : 1;
+  static constexpr int kRows = kMmaTiles * kTileM;
+  static constexpr int kSoftmaxWarps = 8 * kMmaTiles;    // two groups of four per MMA tile, 64 keys each
+  static constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
+  static constexpr int kCtas = 3 - kMmaTiles;            // per SM
+  static constexpr int kTmem = 256 * kMmaTiles;          // columns: S, then O
   static constexpr int kTileBytes = kTileN * D * 2;      // one K or V tile, and one Q tile
   static constexpr int kQBytes = 32768;                  // a Q tile's place, at the end 4 KB of output for each warp
-  static constexpr int kRing = D == 128 ? 5 : 10;        // K and V tiles in flight
-  static constexpr int kBytes = 2 * kQBytes + kRing * kTileBytes + static_cast<int>(sizeof(Shared));
+  static constexpr int kRing = D == 128 ? 5 : 4;         // K and V tiles in flight
+  static constexpr int kBytes = kMmaTiles * kQBytes + kRing * kTileBytes + static_cast<int>(sizeof(Shared));
 };
 
 // ---------------------------------------------------------------- tcgen05
@@ -330,10 +337,11 @@ __device__ __forceinline__ void weights(const float2 (&s)[kRun / 2], float c, fl
 
 // MODE: 1 capped scores, 2 biased by distance, 3 both.
 template <typename T, int D, int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Plan<D>::kThreads, Plan<D>::kCtas)
 prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap) {
   using P = Plan<D>;
+  constexpr int QT = P::kMmaTiles, kSoftmaxWarps = P::kSoftmaxWarps;
   constexpr bool kLag = std::is_same<T, __nv_bfloat16>::value;
   // Heads of 64 dims leave room in TMEM for an O of its own for each half of
   // the keys: the halves then share nothing until the end. Heads of 128 dims
@@ -344,14 +352,14 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   constexpr int kHalves = D / 64;
   constexpr int kHalfBytes = kTileN * 128;
   extern __shared__ __align__(1024) unsigned char base[];  // swizzle atoms: 1024-byte aligned
-  unsigned char* ring = base + 2 * P::kQBytes;
+  unsigned char* ring = base + QT * P::kQBytes;
   Shared& sh = *reinterpret_cast<Shared*>(ring + P::kRing * P::kTileBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
   const int h = blockIdx.y;
   // Later row tiles see more keys under a causal mask: they start first.
   const int slots = gridDim.x / a.nsplit;
   const int split = blockIdx.x % a.nsplit;
-  const RowTile t = row_tile<kRows>(a, slots - 1 - static_cast<int>(blockIdx.x) / a.nsplit, lane);
+  const RowTile t = row_tile<P::kRows>(a, slots - 1 - static_cast<int>(blockIdx.x) / a.nsplit, lane);
   if (t.rows == 0) return;
 
   const int qt = warp >> 3, half = (warp >> 2) & 1;        // softmax warps: MMA tile, half of its keys
@@ -385,14 +393,14 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const int himin = __reduce_min_sync(kFull, have ? rk.hi : 0x7fffffff);
     if (lane == 0) sh.range[warp] = make_int4(kmin, kmax, lomax, himin);
   } else if (warp == kSoftmaxWarps) {
-    tmem_alloc(&sh.tmem, 512);
+    tmem_alloc(&sh.tmem, P::kTmem);
   } else {
     if (lane == 0) {
       for (int i = 0; i < P::kRing; ++i) {
         mbar_init(&sh.full[i], 1);
         mbar_init(&sh.empty[i], 1);
       }
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < QT; ++q) {
         mbar_init(&sh.q_full[q], 2 * kTileM);
         for (int x = 0; x < 2; ++x) {
           mbar_init(&sh.s_full[q][x], 1);
@@ -408,9 +416,9 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   }
   __syncthreads();
   // Each MMA tile's keys [kmin, kmax), and [lomax, himin) that all of its rows see.
-  int4 keys[2];
+  int4 keys[2] = {make_int4(0x7fffffff, 0, 0, 0x7fffffff), make_int4(0x7fffffff, 0, 0, 0x7fffffff)};
   {
-    int4 v = sh.range[lane & 15];
+    int4 v = sh.range[lane & (kSoftmaxWarps - 1)];
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
       v.x = min(v.x, __shfl_xor_sync(kFull, v.x, o));
@@ -419,12 +427,12 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       v.w = min(v.w, __shfl_xor_sync(kFull, v.w, o));
     }
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+    for (int q = 0; q < QT; ++q)
       keys[q] = make_int4(__shfl_sync(kFull, v.x, 8 * q), __shfl_sync(kFull, v.y, 8 * q), __shfl_sync(kFull, v.z, 8 * q),
                           __shfl_sync(kFull, v.w, 8 * q));
   }
   // Tiles [ta, tb) of this CTA's part, and those of each MMA tile.
-  int ta, tb, qa[2], qb[2];
+  int ta, tb, qa[2] = {0, 0}, qb[2] = {0, 0};
   {
     const int kmin = min(keys[0].x, keys[1].x), kmax = max(keys[0].y, keys[1].y);
     const int first = kmax > 0 ? kmin / kTileN : 0, last = (kmax + kTileN - 1) / kTileN;
@@ -433,7 +441,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     tb = min(last, ta + per);
     int lo = tb, hi = ta;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int q = 0; q < QT; ++q) {
       qa[q] = keys[q].y > 0 ? max(ta, keys[q].x / kTileN) : tb;
       qb[q] = min(tb, (keys[q].y + kTileN - 1) / kTileN);
       if (qb[q] <= qa[q]) qa[q] = qb[q] = ta;
@@ -445,7 +453,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     ta = uniform(lo);
     tb = uniform(max(lo, hi));
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int q = 0; q < QT; ++q) {
       qa[q] = uniform(qa[q]);
       qb[q] = uniform(qb[q]);
     }
@@ -513,7 +521,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     if (ta < tb) {
       ok = warp_wait(&sh.full[0], 0, a.status);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < QT; ++q) {
         if (qa[q] < qb[q]) ok = ok && warp_wait(&sh.q_full[q], 0, a.status);
         fence_after();
         if (ok && qa[q] == ta && qa[q] < qb[q]) {
@@ -545,7 +553,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       const bool more = i + 1 < tb;
       if (more) ok = warp_wait(&sh.full[kslot], phase, a.status);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < QT; ++q) {
         const bool now = i >= qa[q] && i < qb[q], then = i + 1 >= qa[q] && i + 1 < qb[q];
         const uint64_t vd = v_desc + vslot * kTile16;
 #pragma unroll
@@ -555,7 +563,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
             fence_after();
 #pragma unroll
             for (int s = 0; s < kTileN / 32; ++s)
-              mma_ts(tmem + 2 * kTileN + (kOwnO ? q * 2 + x : q * 2) * kOCols, tmem + q * kTileN + x * (kTileN / 2) + s * 8,
+              mma_ts(tmem + QT * kTileN + (kOwnO ? q * 2 + x : q * 2) * kOCols, tmem + q * kTileN + x * (kTileN / 2) + s * 8,
                      vd + (x * (kTileN / 32) + s) * (2048 >> 4), pv, done[q] > 0 || (!kOwnO && x > 0) || s > 0);
           }
           if (ok && then) issue_qk(q, x, kslot);
@@ -577,7 +585,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const int r = tid & (kTileM - 1);  // row of the MMA tile
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
     const uint32_t ts = tmem + lanes + qt * kTileN + half * kKeys;
-    const uint32_t to = tmem + lanes + 2 * kTileN + (qt * 2 + half) * kOCols;
+    const uint32_t to = tmem + lanes + QT * kTileN + (qt * 2 + half) * kOCols;
     asm volatile("cp.async.wait_all;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mbar_arrive(&sh.q_full[qt]);
@@ -664,7 +672,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           const bool grow = grows(mx);
           if (__any_sync(kFull, grow && m != neg_inf())) reframe(grow, mx);
           else if (grow) m = mx;
-        } else if (group_any(1 + qt, 2 * kTileM, grows(mx) || !ok)) {
+        } else if (group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, grows(mx) || !ok)) {
           if (sh.failed[qt]) {
             ok = false;
             break;
@@ -674,7 +682,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           const bool grow = grows(mx);
           if (__any_sync(kFull, grow && m != neg_inf())) reframe(grow, mx);
           else if (grow) m = mx;
-          group_any(1 + qt, 2 * kTileM, false);
+          group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
         }
         const float nm = m == neg_inf() ? 0.f : -m;
         tmem_ld16(ts, reinterpret_cast<uint32_t*>(s[0]));
@@ -689,7 +697,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         }
         // Once every row that sees any key has met one, the frames may lag (not f16's: P would leave its range).
         const bool waiting = m == neg_inf() && rk.hi > rk.lo;
-        if (kLag) exact = kOwnO ? __any_sync(kFull, waiting) : group_any(1 + qt, 2 * kTileM, waiting);
+        if (kLag) exact = kOwnO ? __any_sync(kFull, waiting) : group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, waiting);
         est = m;
       } else {
         // One pass, without a maximum, in a frame that the first half of the
@@ -746,9 +754,9 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     fence_after();
     auto swap = [&](float x) {  // the value of the row's other thread
       sh.other[qt][half][r] = x;
-      group_any(1 + qt, 2 * kTileM, false);
+      group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
       const float y = sh.other[qt][half ^ 1][r];
-      group_any(1 + qt, 2 * kTileM, false);
+      group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
       return y;
     };
     // The row's sum over both halves of its keys, with their own O in one frame for both.
@@ -760,7 +768,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       m = frame;
     }
     l += swap(l);
-    ok = !group_any(1 + qt, 2 * kTileM, !ok);
+    ok = !group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, !ok);
     const bool empty = m == neg_inf();
     const long long orow = static_cast<long long>(t.t0 + tok) * a.hq + head;
     const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
@@ -807,7 +815,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
               *reinterpret_cast<float4*>(pass + ((e ^ r) & 7) * 16) = make_float4(x(0), x(1), x(2), x(3));
             }
           }
-          group_any(1 + qt, 2 * kTileM, false);
+          group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
           if (half == 0) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -821,7 +829,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
               o[4 * e + 3] = x(3, y.w);
             }
           }
-          group_any(1 + qt, 2 * kTileM, false);
+          group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
           if (half) continue;
         }
 #pragma unroll
@@ -888,7 +896,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   __syncthreads();
   if (warp == kSoftmaxWarps) {
     fence_after();
-    tmem_free(tmem, 512);
+    tmem_free(tmem, P::kTmem);
   }
 }
 
@@ -897,8 +905,8 @@ int launch_mode(const PagedAttnArgs& a, const CUtensorMap& km, const CUtensorMap
   auto kern = prompt_attn_kernel<T, D, MODE>;
   const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Plan<D>::kBytes));
   if (rc) return rc;
-  const int slots = row_tile_slots(a.R, a.T, a.G, a.token_offsets != nullptr, a.shared != 0, kRows);
-  kern<<<dim3(static_cast<unsigned>(slots * a.nsplit), static_cast<unsigned>(a.L.hkv)), kThreads, Plan<D>::kBytes,
+  const int slots = row_tile_slots(a.R, a.T, a.G, a.token_offsets != nullptr, a.shared != 0, Plan<D>::kRows);
+  kern<<<dim3(static_cast<unsigned>(slots * a.nsplit), static_cast<unsigned>(a.L.hkv)), Plan<D>::kThreads, Plan<D>::kBytes,
          stream>>>(a, km, vm);
   return static_cast<int>(cudaGetLastError());
 }
