@@ -127,7 +127,12 @@ struct RowKeys {
   int lo, hi, pos;
 };
 
-__device__ __forceinline__ RowKeys row_keys(const PagedAttnArgs& a, const RowTile& t, int i) {
+__device__ __forceinline__ int2 given_keys(const PagedAttnArgs& a, int token) {
+  return make_int2(a.kv_lo ? a.kv_lo[token] : 0, a.kv_hi ? a.kv_hi[token] : 0);
+}
+
+// `given`: given_keys of the token, loaded ahead of their use.
+__device__ __forceinline__ RowKeys row_keys(const PagedAttnArgs& a, const RowTile& t, int i, int2 given) {
   const int token = t.t0 + i;
   RowKeys k;
   int len = t.len;
@@ -146,10 +151,14 @@ __device__ __forceinline__ RowKeys row_keys(const PagedAttnArgs& a, const RowTil
     len = cached_tokens(a, r, last - a.token_offsets[r]);
     k.pos = len - (last - token);
   }
-  k.lo = max(a.kv_lo ? a.kv_lo[token] : 0, a.span_lo);
-  k.hi = min(min(a.kv_hi ? a.kv_hi[token] : k.pos + 1, min(len, t.len)), a.span_hi);
+  k.lo = max(given.x, a.span_lo);
+  k.hi = min(min(a.kv_hi ? given.y : k.pos + 1, min(len, t.len)), a.span_hi);
   k.hi = max(k.lo, k.hi);
   return k;
+}
+
+__device__ __forceinline__ RowKeys row_keys(const PagedAttnArgs& a, const RowTile& t, int i) {
+  return row_keys(a, t, i, given_keys(a, t.t0 + i));
 }
 
 // Page of key token `j` of request `rp`, or -1 (reported) when its table

@@ -366,7 +366,11 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   const int row = qt * kTileM + (tid & (kTileM - 1));      // and row of the CTA
   const bool have = row < t.rows;
   RowKeys rk{0, 0x7fffffff, 0};
+  const int* table = nullptr;  // loads: the request's page table
+  int pages = 0, ppb = 0;
   if (warp < kSoftmaxWarps) {
+    const int my_tok = have ? (t.row0 + row) / a.G : 0;
+    const int2 given = given_keys(a, t.t0 + my_tok);
     // Q tiles, swizzled: 16-byte chunk c of row x at chunk c ^ (x & 7). The copies run beside what follows.
     const T* q = static_cast<const T*>(a.q);
 #pragma unroll
@@ -385,7 +389,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       }
     }
     // The rows' key intervals.
-    if (have) rk = row_keys(a, t, (t.row0 + row) / a.G);
+    if (have) rk = row_keys(a, t, my_tok, given);
     const bool some = have && rk.hi > rk.lo;
     const int kmin = __reduce_min_sync(kFull, some ? rk.lo : 0x7fffffff);
     const int kmax = __reduce_max_sync(kFull, some ? rk.hi : 0);
@@ -395,6 +399,10 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   } else if (warp == kSoftmaxWarps) {
     tmem_alloc(&sh.tmem, P::kTmem);
   } else {
+    const int first = a.L.block_offsets[t.r];
+    ppb = a.L.b / a.L.page_size;
+    pages = (a.L.block_offsets[t.r + 1] - first) * ppb;
+    table = a.L.page_table + static_cast<long long>(first) * ppb;
     if (lane == 0) {
       for (int i = 0; i < P::kRing; ++i) {
         mbar_init(&sh.full[i], 1);
@@ -465,11 +473,15 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     // ------------------------------------------------------------ K and V tiles
     const int bp = min(a.L.page_size, kTileN);  // rows of a box
     const int boxes = kTileN / bp;
-    const int pages = request_blocks(a.L, rp) * (a.L.b / a.L.page_size);
     auto page_at = [&](int key) {  // keys past the request's pages, or of a bad entry, read as zeros
       const int entry = key / a.L.page_size;
-      int page = entry < pages ? page_of(a, rp, key) : -1;
-      return page < 0 ? a.pages : page;
+      if (entry >= pages) return a.pages;
+      const int page = table[entry];
+      if (page < 0 || page >= a.pages) {
+        report(a.status, kStatusBadBlockId);
+        return a.pages;
+      }
+      return page;
     };
     int page = lane < boxes && ta < tb ? page_at(ta * kTileN + lane * bp) : 0;
     bool ok = true;
@@ -752,23 +764,40 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const bool any = begin < end;
     if (any) ok = warp_wait(&sh.o_full[qt], 0, a.status) && ok;
     fence_after();
-    auto swap = [&](float x) {  // the value of the row's other thread
-      sh.other[qt][half][r] = x;
-      group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
-      const float y = sh.other[qt][half ^ 1][r];
-      group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
-      return y;
-    };
-    // The row's sum over both halves of its keys, with their own O in one frame for both.
-    float mine = 1.f;
-    if (kOwnO) {
-      const float frame = fmaxf(m, swap(m));
-      mine = m == neg_inf() ? 0.f : ex2(m - frame);
-      l *= mine;
-      m = frame;
+    // The row's two threads meet once. A shared O: its sum over both halves of
+    // the keys. An O of its own for each half: the second half's thread hands
+    // its state to the first's, through the ring, which is free now.
+    float* handed = reinterpret_cast<float*>(ring + r * 256);  // 16-byte chunk c of row r at chunk c ^ (r & 7)
+    if (kOwnO && half && ok) {
+#pragma unroll 1
+      for (int j = 0; j < kOCols; j += 32) {
+        uint32_t o[32];
+        if (any) {
+          tmem_ld32(to + j, o);
+          tmem_wait_ld();
+          tmem_loaded(o);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(handed + (((j / 4 + e) ^ (r & 7)) * 4)) =
+              any ? make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_uint4(0, 0, 0, 0);
+      }
+      reinterpret_cast<float*>(ring + kTileM * 256)[r] = m;
     }
-    l += swap(l);
+    sh.other[qt][half][r] = l;
     ok = !group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, !ok);
+    const float l2 = sh.other[qt][half ^ 1][r];
+    float mine = 1.f, others = 0.f;
+    if (kOwnO) {
+      const float m2 = half ? neg_inf() : reinterpret_cast<const float*>(ring + kTileM * 256)[r];
+      const float frame = fmaxf(m, m2);
+      mine = m == neg_inf() ? 0.f : ex2(m - frame);
+      others = m2 == neg_inf() ? 0.f : ex2(m2 - frame);
+      l = (mine == 0.f ? 0.f : l * mine) + (others == 0.f ? 0.f : l2 * others);
+      m = frame;
+    } else {
+      l += l2;
+    }
     const bool empty = m == neg_inf();
     const long long orow = static_cast<long long>(t.t0 + tok) * a.hq + head;
     const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
@@ -777,7 +806,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     // (2^-100: below what a frame that follows leaves, above what clamped exponentials of masked keys add up to.)
     const bool over = !empty && !(l <= 3.0e38f && l >= 7.9e-31f);
     bool redo_row = have && over;
-    if (ok) {
+    if (ok && !(kOwnO && half)) {
       // 128 bytes a row at a time through this warp's share of the Q tile's
       // place, which is free now, so that a store instruction covers whole rows.
       unsigned char* stage = base + qt * P::kQBytes + (warp & 7) * 4096;
@@ -806,31 +835,18 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           tmem_wait_ld();
           tmem_loaded(o);
         }
-        if (kOwnO) {  // the second half's dims through shared memory to the first half's thread
-          unsigned char* pass = base + qt * P::kQBytes + P::kQBytes / 2 + r * 128;  // beside the first half's stages
-          if (half) {
+        if (kOwnO) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              auto x = [&](int i) { return mine == 0.f ? 0.f : __uint_as_float(o[4 * e + i]) * mine; };
-              *reinterpret_cast<float4*>(pass + ((e ^ r) & 7) * 16) = make_float4(x(0), x(1), x(2), x(3));
-            }
+          for (int e = 0; e < 8; ++e) {
+            const float4 y = *reinterpret_cast<const float4*>(handed + (((j / 4 + e) ^ (r & 7)) * 4));
+            auto sum = [&](uint32_t x, float z) {
+              return __float_as_uint((mine == 0.f ? 0.f : __uint_as_float(x) * mine) + (others == 0.f ? 0.f : z * others));
+            };
+            o[4 * e] = sum(o[4 * e], y.x);
+            o[4 * e + 1] = sum(o[4 * e + 1], y.y);
+            o[4 * e + 2] = sum(o[4 * e + 2], y.z);
+            o[4 * e + 3] = sum(o[4 * e + 3], y.w);
           }
-          group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
-          if (half == 0) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 y = *reinterpret_cast<const float4*>(pass + ((e ^ r) & 7) * 16);
-              auto x = [&](int i, float other) {
-                return __float_as_uint((mine == 0.f ? 0.f : __uint_as_float(o[4 * e + i]) * mine) + other);
-              };
-              o[4 * e] = x(0, y.x);
-              o[4 * e + 1] = x(1, y.y);
-              o[4 * e + 2] = x(2, y.z);
-              o[4 * e + 3] = x(3, y.w);
-            }
-          }
-          group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
-          if (half) continue;
         }
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
@@ -859,7 +875,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       // Rows whose sums are not finite, be it for values of keys that they may
       // not see: this half of their dims once more, in the frame (m, l) that
       // stands, or in their own where l itself is lost.
-      unsigned redo = __ballot_sync(kFull, redo_row && !(kOwnO && half));
+      unsigned redo = __ballot_sync(kFull, redo_row);
       while (redo) {
         const int src = __ffs(redo) - 1;
         redo &= redo - 1;
