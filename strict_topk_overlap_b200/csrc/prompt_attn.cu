@@ -46,7 +46,7 @@ struct Shared {
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2];  // [MMA tile] or [MMA tile][half of the keys]
   uint64_t pair[8];            // the two warps that share 32 rows
   uint32_t tmem;
-  int4 range[16];   // of a warp's rows: least and largest key, largest lo, least hi
+  int2 range[16];              // of a warp's rows: least and largest key
   volatile int failed[2];      // a wait of the MMA tile's softmax ran out
   union {
     float other[2][2][kTileM];             // [MMA tile][half of the keys][row]: maxima, at the end the sums
@@ -348,7 +348,8 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   // share O, each half's warps keeping half of its dims in frame.
   constexpr bool kOwnO = D == 64;
   constexpr int kOCols = 64;  // of O, a warp's
-  constexpr int kFmaPairs = MODE == 0 ? 2 : 1;  // of 8 pairs of weights, those whose exponentials take the FMA units
+  // Of 8 pairs of weights, those whose exponentials take the FMA units: none where the cap keeps these busy.
+  constexpr int kFmaPairs = (MODE & 1) ? 0 : 2;
   constexpr int kHalves = D / 64;
   constexpr int kHalfBytes = kTileN * 128;
   extern __shared__ __align__(1024) unsigned char base[];  // swizzle atoms: 1024-byte aligned
@@ -393,9 +394,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const bool some = have && rk.hi > rk.lo;
     const int kmin = __reduce_min_sync(kFull, some ? rk.lo : 0x7fffffff);
     const int kmax = __reduce_max_sync(kFull, some ? rk.hi : 0);
-    const int lomax = __reduce_max_sync(kFull, have ? rk.lo : 0);
-    const int himin = __reduce_min_sync(kFull, have ? rk.hi : 0x7fffffff);
-    if (lane == 0) sh.range[warp] = make_int4(kmin, kmax, lomax, himin);
+    if (lane == 0) sh.range[warp] = make_int2(kmin, kmax);
   } else if (warp == kSoftmaxWarps) {
     tmem_alloc(&sh.tmem, P::kTmem);
   } else {
@@ -423,21 +422,17 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     __syncwarp();
   }
   __syncthreads();
-  // Each MMA tile's keys [kmin, kmax), and [lomax, himin) that all of its rows see.
-  int4 keys[2] = {make_int4(0x7fffffff, 0, 0, 0x7fffffff), make_int4(0x7fffffff, 0, 0, 0x7fffffff)};
+  // Each MMA tile's keys [kmin, kmax).
+  int2 keys[2] = {make_int2(0x7fffffff, 0), make_int2(0x7fffffff, 0)};
   {
-    int4 v = sh.range[lane & (kSoftmaxWarps - 1)];
+    int2 v = sh.range[lane & (kSoftmaxWarps - 1)];
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
       v.x = min(v.x, __shfl_xor_sync(kFull, v.x, o));
       v.y = max(v.y, __shfl_xor_sync(kFull, v.y, o));
-      v.z = max(v.z, __shfl_xor_sync(kFull, v.z, o));
-      v.w = min(v.w, __shfl_xor_sync(kFull, v.w, o));
     }
 #pragma unroll
-    for (int q = 0; q < QT; ++q)
-      keys[q] = make_int4(__shfl_sync(kFull, v.x, 8 * q), __shfl_sync(kFull, v.y, 8 * q), __shfl_sync(kFull, v.z, 8 * q),
-                          __shfl_sync(kFull, v.w, 8 * q));
+    for (int q = 0; q < QT; ++q) keys[q] = make_int2(__shfl_sync(kFull, v.x, 8 * q), __shfl_sync(kFull, v.y, 8 * q));
   }
   // Tiles [ta, tb) of this CTA's part, and those of each MMA tile.
   int ta, tb, qa[2] = {0, 0}, qb[2] = {0, 0};
@@ -601,7 +596,13 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     asm volatile("cp.async.wait_all;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mbar_arrive(&sh.q_full[qt]);
-    const int lomax = qt ? keys[1].z : keys[0].z, himin = qt ? keys[1].w : keys[0].w;
+    // What the warp's 32 rows see of a run of keys: nothing (no weights to form), all of it (no mask), or some.
+    enum { kNone, kSome, kAll };
+    const int lo_min = __reduce_min_sync(kFull, have ? rk.lo : 0x7fffffff), lo_max = __reduce_max_sync(kFull, rk.lo);
+    const int hi_max = __reduce_max_sync(kFull, have ? rk.hi : 0), hi_min = __reduce_min_sync(kFull, rk.hi);
+    auto seen = [&](int k) {
+      return k + kRun <= lo_min || k >= hi_max ? kNone : k >= lo_max && k + kRun <= hi_min ? kAll : kSome;
+    };
     const int tok = have ? (t.row0 + row) / a.G : 0;
     const int head = h * a.G + (have ? t.row0 + row - tok * a.G : 0);
     const float slope = (MODE & 2) && a.slopes ? a.slopes[head] : 0.f;
@@ -647,6 +648,31 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       ok = warp_wait(bar, meetings & 1, a.status) && ok;
       ++meetings;
     };
+    // P of the thread's keys from k0 on, over S, and their sum. WHOLE: every
+    // row of the warp sees all of them, one straight run of code; else run by
+    // run. RAW: S are still raw scores. The next run is on its way from TMEM
+    // while one is computed.
+    auto form_weights = [&](auto whole_t, auto raw_t, int k0, float nm, float2 (&sum)[2]) {
+      constexpr bool WHOLE = decltype(whole_t)::value, RAW = decltype(raw_t)::value;
+      float2 s[2][kRun / 2];
+      tmem_ld16(ts, reinterpret_cast<uint32_t*>(s[0]));
+#pragma unroll
+      for (int j = 0; j < kKeys / kRun; ++j) {
+        uint32_t p[kRun / 2];
+        tmem_wait_ld();
+        tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[j & 1]));
+        if (j + 1 < kKeys / kRun) tmem_ld16(ts + (j + 1) * kRun, reinterpret_cast<uint32_t*>(s[(j + 1) & 1]));
+        const int view = WHOLE ? static_cast<int>(kAll) : seen(k0 + j * kRun);
+        if (!WHOLE && view == kNone) {
+#pragma unroll
+          for (int e = 0; e < kRun / 2; ++e) p[e] = 0u;
+        } else {
+          if (RAW) scores<MODE>(s[j & 1], z, k0 + j * kRun, view == kAll);
+          weights<T, MODE, kFmaPairs>(s[j & 1], c, nm, sum, p);
+        }
+        tmem_st8(ts + j * kRun / 2, p);  // over scores that have been read
+      }
+    };
     auto grows = [&](float x) { return x > m + kLazy || (m == neg_inf() && x > m); };
     // The largest bias that a key of tile i can have.
     auto most_bias = [&](int i) {
@@ -660,23 +686,29 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       if (kOwnO && !ok) break;
       fence_after();
       const int k0 = i * kTileN + half * kKeys;
-      const bool full = k0 >= lomax && k0 + kKeys <= himin;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      float2 s[2][kRun / 2];
+      const bool whole = k0 >= lo_max && k0 + kKeys <= hi_min;
       float est;
       if (exact) {
         // The maximum first, over both halves of the row's keys. Transformed and masked scores go back to TMEM.
         float mx = neg_inf();
+        bool wrote = false;
+        float2 s[kRun / 2];
 #pragma unroll 1
         for (int j0 = 0; j0 < kKeys; j0 += kRun) {
-          tmem_ld16(ts + j0, reinterpret_cast<uint32_t*>(s[0]));
+          const int view = seen(k0 + j0);
+          if (view == kNone) continue;
+          tmem_ld16(ts + j0, reinterpret_cast<uint32_t*>(s));
           tmem_wait_ld();
-          tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[0]));
-          scores<MODE>(s[0], z, k0 + j0, full);
-          if (MODE != 0 || !full) tmem_st16(ts + j0, reinterpret_cast<const uint32_t*>(s[0]));
-          mx = largest(s[0], mx);
+          tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s));
+          scores<MODE>(s, z, k0 + j0, view == kAll);
+          if (MODE != 0 || view != kAll) {
+            tmem_st16(ts + j0, reinterpret_cast<const uint32_t*>(s));
+            wrote = true;
+          }
+          mx = largest(s, mx);
         }
-        if (MODE != 0 || !full) tmem_wait_st();
+        if (wrote) tmem_wait_st();
         mx *= c;
         // (Read before this thread's P is announced, and written again after the next S, which waits for that.)
         if (!kOwnO) sh.other[qt][half][r] = mx;
@@ -697,16 +729,8 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, false);
         }
         const float nm = m == neg_inf() ? 0.f : -m;
-        tmem_ld16(ts, reinterpret_cast<uint32_t*>(s[0]));
-#pragma unroll
-        for (int j = 0; j < kKeys / kRun; ++j) {
-          uint32_t p[kRun / 2];
-          tmem_wait_ld();
-          tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[j & 1]));
-          if (j + 1 < kKeys / kRun) tmem_ld16(ts + (j + 1) * kRun, reinterpret_cast<uint32_t*>(s[(j + 1) & 1]));
-          weights<T, MODE, kFmaPairs>(s[j & 1], c, nm, sum, p);
-          tmem_st8(ts + j * kRun / 2, p);  // over scores that have been read
-        }
+        if (whole) form_weights(std::true_type{}, std::false_type{}, k0, nm, sum);
+        else form_weights(std::false_type{}, std::false_type{}, k0, nm, sum);
         // Once every row that sees any key has met one, the frames may lag (not f16's: P would leave its range).
         const bool waiting = m == neg_inf() && rk.hi > rk.lo;
         if (kLag) exact = kOwnO ? __any_sync(kFull, waiting) : group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, waiting);
@@ -732,17 +756,8 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
           }
         }
         const float nm = m == neg_inf() ? 0.f : -m;
-        tmem_ld16(ts, reinterpret_cast<uint32_t*>(s[0]));
-#pragma unroll
-        for (int j = 0; j < kKeys / kRun; ++j) {
-          uint32_t p[kRun / 2];
-          tmem_wait_ld();
-          tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[j & 1]));
-          if (j + 1 < kKeys / kRun) tmem_ld16(ts + (j + 1) * kRun, reinterpret_cast<uint32_t*>(s[(j + 1) & 1]));
-          scores<MODE>(s[j & 1], z, k0 + j * kRun, full);
-          weights<T, MODE, kFmaPairs>(s[j & 1], c, nm, sum, p);
-          tmem_st8(ts + j * kRun / 2, p);
-        }
+        if (whole) form_weights(std::true_type{}, std::true_type{}, k0, nm, sum);
+        else form_weights(std::false_type{}, std::true_type{}, k0, nm, sum);
         est = log2f((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)) - nm;  // the maximum, or a little more
       }
       // The next tile's frame. What the largest bias of a tile gains on this one's is known, and followed at once.
