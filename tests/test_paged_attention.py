@@ -254,6 +254,68 @@ def test_scores_of_the_types_lowest_value():
             assert bool(lse.isfinite().all())
 
 
+def _scores_along(pattern, n):
+    """Scores of n keys, in nats, that move far from one run of keys to the next."""
+    j = torch.arange(n, device=DEV, dtype=torch.float32)
+    if pattern == "ramp":
+        return 0.7 * (j - n / 2)
+    if pattern == "fall":
+        return -0.7 * j
+    if pattern == "jump":  # one key far above all before it, more than the types' range of weights
+        return torch.where(j == 300, 150.0, torch.where(j > 300, 20.0, 0.0))
+    if pattern == "halves":  # every second run of 64 keys far above the other
+        return torch.where(j % 128 >= 64, 110.0, 0.0) + 0.01 * j
+    return torch.where(j < n - 3, -400.0, 300.0)  # "last": all weight on the last keys
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pattern", ["ramp", "fall", "jump", "halves", "last"])
+@pytest.mark.parametrize("new", [1, 40, 200])
+def test_scores_that_move(dtype, pattern, new):
+    """The running maximum, wherever a kernel keeps it, follows scores that grow by hundreds between runs of keys."""
+    from strict_topk_overlap_b200 import paged_attention
+    for hq, hkv, d, block, page in ((8, 2, 128, 32, 16), (4, 2, 64, 32, 32), (2, 1, 96, 32, 16)):
+        n = 700
+        cache = _cache([n], hkv, d, block, page, dtype, 70)
+        along = _scores_along(pattern, n) * d ** 0.5 / 16
+        j = torch.arange(n, device=DEV)
+        pg = cache.page_table[j // page].long()
+        cache.k_pages[pg, :, j % page] *= 0.25
+        cache.k_pages[pg, :, j % page, 0] = along.to(dtype)[:, None].expand(-1, hkv)
+        q = (0.25 * torch.randn((new, hq, d), generator=torch.Generator(DEV).manual_seed(71), device=DEV)).to(dtype)
+        q[..., 0] = 16.0
+        offsets = None if new == 1 else _ints([0, new])
+        for softcap, slopes in ((0.0, None), (300.0, None), (0.0, torch.full((hq,), 4.0, device=DEV))):
+            out, lse = paged_attention.attention(q, cache, _ints([n]), token_offsets=offsets, max_tokens=new,
+                                                 softcap=softcap, slopes=slopes, return_lse=True)
+            _compare(q, cache, [n], [new], None, None, out, lse, softcap, slopes, d ** -0.5)
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """Pages whose elements lie beyond 2^31 of their pool: the append writes them, every attention form reads them."""
+    from strict_topk_overlap_b200 import paged, paged_append, paged_attention
+    pages, hkv, page, d = 140000, 8, 16, 128  # 2.3e9 elements
+    pool = [torch.empty((pages, hkv, page, d), dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    table = (pages - 1 - torch.arange(20, device=DEV)).to(torch.int32)
+    none = torch.empty((hkv, 0, d), device=DEV)
+    cache = paged.PagedKVCache(pool[0], pool[1], table, _ints([0, 10]), none, none, 32, page, 10)
+    g = torch.Generator(DEV).manual_seed(80)
+    k, v = (torch.randn((300, hkv, d), generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    paged_append.append_tokens(cache, k, v, _ints([0]), token_offsets=_ints([0, 300]))
+    got = pool[0][table.long()].transpose(0, 1).reshape(hkv, -1, d)[:, :300].transpose(0, 1)
+    assert torch.equal(got, k)
+    q = torch.randn((300, 16, d), generator=g, device=DEV).to(torch.bfloat16)
+    for new in (1, 300):
+        x = q[300 - new:]
+        more = dict(token_offsets=None if new == 1 else _ints([0, new]), max_tokens=new, return_lse=True)
+        out, lse = paged_attention.attention(x, cache, _ints([300]), **more)
+        _compare(x, cache, [300], [new], None, None, out, lse, 0.0, None, d ** -0.5)
+    out, lse = paged_attention.shared_prefix_attention(q[:1], cache, _ints([300]), 160, return_lse=True)
+    _compare(q[:1], cache, [300], [1], None, None, out, lse, 0.0, None, d ** -0.5)
+
+
 @gpu
 def test_streams_graphs_and_workspaces():
     from strict_topk_overlap_b200 import paged_attention
