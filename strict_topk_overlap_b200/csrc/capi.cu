@@ -950,7 +950,9 @@ AttnPhase plan_phase(const stk_kv* kv, int R, int T, int hq, bool offsets, bool 
     const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared,
                                                                 prompt ? prompt_tile_rows(kv->d) : 16)) * hkv;
     const long long most = prompt ? (keys + 127) / 128 : (keys + 63) / 64;
-    long long n = (prompt ? prompt_ctas_per_sm(kv->d) : 2) * sms / tiles;
+    // Requests of different lengths are cut into as many parts each: four
+    // CTAs of the FP32-unit kernel for each place let the hardware even them out.
+    long long n = (prompt ? prompt_ctas_per_sm(kv->d) : 8) * sms / tiles;
     n = n < most ? n : most;
     p.nsplit = static_cast<int>(n < 1 ? 1 : n);
     p.states = static_cast<size_t>(p.nsplit) * T * hq;

@@ -96,35 +96,51 @@ __global__ void __launch_bounds__(kRowsWarps * 32) rows_attn_kernel(PagedAttnArg
     const float icap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
     float m = neg_inf(), l = 0.f;
     const int rp = t.r;
+    // Element of key token t0 + lane in its head of the pool, or -1.
+    auto place = [&](int t0) -> long long {
+      if (lane >= TB || t0 + lane >= end) return -1;
+      const int page = page_of(a, rp, t0 + lane);
+      if (page < 0) return -1;
+      return ((static_cast<long long>(page) * a.L.hkv + h) * a.L.page_size + (t0 + lane) % a.L.page_size) * D;
+    };
+    long long next = idle ? -1 : place(begin + slice * TB);
     for (int t0 = begin + slice * TB; !idle && t0 < end; t0 += slices * TB) {
-      const int nt = min(TB, end - t0);
-      long long off = -1;
-      if (lane < nt) {
-        const int page = page_of(a, rp, t0 + lane);
-        if (page >= 0)
-          off = ((static_cast<long long>(page) * a.L.hkv + h) * a.L.page_size + (t0 + lane) % a.L.page_size) * D;
-      }
+      const long long off = next;
       float p[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) p[i] = 0.f;
       float vv[NPL <= 8 ? TB : 1][NPL];  // the run's values, requested before its scores are needed
+      if constexpr (NPL <= 8) {
+        // All of the run's rows at once; a token without a place reads the pool's first row and is not seen.
+        float kk[TB][NPL];
 #pragma unroll
-      for (int k = 0; k < TB; ++k) {
-        const long long o = __shfl_sync(kFull, off, k);
-        if (o < 0) {
-          if constexpr (NPL <= 8) {
+        for (int k = 0; k < TB; ++k)
+          load_lane<T, NPL, VEC>(static_cast<const T*>(a.L.k) + max(__shfl_sync(kFull, off, k), 0ll), D, lane, kk[k]);
 #pragma unroll
-            for (int j = 0; j < NPL; ++j) vv[k][j] = 0.f;
+        for (int k = 0; k < TB; ++k)
+          load_lane<T, NPL, VEC>(static_cast<const T*>(a.L.v) + max(__shfl_sync(kFull, off, k), 0ll), D, lane, vv[k]);
+        next = place(t0 + slices * TB);
+#pragma unroll
+        for (int k = 0; k < TB; ++k) {
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+            float x = 0.f;
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) x = fmaf(q[i][j], kk[k][j], x);
+            p[k * RW + i] = x;
           }
-          continue;
         }
-        float kk[NPL];
-        load_lane<T, NPL, VEC>(static_cast<const T*>(a.L.k) + o, D, lane, kk);
-        if constexpr (NPL <= 8) load_lane<T, NPL, VEC>(static_cast<const T*>(a.L.v) + o, D, lane, vv[k]);
+      } else {
+        next = place(t0 + slices * TB);
 #pragma unroll
-        for (int i = 0; i < RW; ++i) {
+        for (int k = 0; k < TB; ++k) {
+          float kk[NPL];
+          load_lane<T, NPL, VEC>(static_cast<const T*>(a.L.k) + max(__shfl_sync(kFull, off, k), 0ll), D, lane, kk);
 #pragma unroll
-          for (int j = 0; j < NPL; ++j) p[k * RW + i] = fmaf(q[i][j], kk[j], p[k * RW + i]);
+          for (int i = 0; i < RW; ++i) {
+            float x = 0.f;
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) x = fmaf(q[i][j], kk[j], x);
+            p[k * RW + i] = x;
+          }
         }
       }
       float s = finish32(p, lane) * a.scale;
@@ -156,9 +172,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) rows_attn_kernel(PagedAttnArg
       for (int k = 0; k < TB; ++k) {
         float vl[NPL];
         if constexpr (NPL > 8) {
-          const long long o = __shfl_sync(kFull, off, k);
-          if (o < 0) continue;
-          load_lane<T, NPL, VEC>(static_cast<const T*>(a.L.v) + o, D, lane, vl);
+          load_lane<T, NPL, VEC>(static_cast<const T*>(a.L.v) + max(__shfl_sync(kFull, off, k), 0ll), D, lane, vl);
         }
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
