@@ -13,15 +13,26 @@
 //
 // HBM-bound for prompts: every q, k, v element is read and written once, plus
 // 8 bytes of table per (token, pair) and 8 bytes of bounds per (block, KV
-// head, dim). One CTA takes the new tokens of one block (request, block) and
-// eight heads, so a block's bounds have one writer and need no atomics. It
+// head, dim). A CTA takes the new tokens of one block (request, block) and
+// eight heads at a time, so a block's bounds have one writer and need no atomics. It
 // stages the cosines, sines and page slots of its tokens in shared memory
 // once; each warp then takes whole heads: lanes cover a head's 16-byte
 // vectors, two per lane (the two halves of a pair in one lane, no shuffles),
 // and several tokens at once. Bounds of 16-bit keys are kept as packed pairs
 // (the stored values themselves), which halves their registers and leaves
 // three CTAs per SM.
-// Which (request, block) a CTA has follows from token_offsets on the device:
+// CTAs take equal runs of (block, eight heads) items, so that the last wave is
+// as full as the others and a block's tables are staged once; with few items
+// (a decode step) each is a CTA of its own and latency is all that counts.
+//
+// Measured (B200, D 128): 8 tokens, 32 / 8 heads bf16: 7 us, a launch and
+// three dependent loads. 8 K prompt tokens of five requests (167 MB): 37 us,
+// 4.5 TB/s. 32 K tokens, 16 / 8 heads f16, three axes (552 MB): 113 us, 4.9
+// TB/s, 75 % of a copy's rate; one item per CTA took 126 us, and asking L2 for
+// the next heads' rows ahead 125 us (the loads are waited for either way, and
+// the requests compete with the stores).
+//
+// Which (request, block) an item is follows from token_offsets on the device:
 // request r's blocks start at slot offs[r] / B + 2 r, which leaves room for
 // the ceil of its tokens wherever its first block begins.
 

@@ -13,15 +13,36 @@
 // warp 17 feeds a ring of K and V tiles by TMA, one box per page and 64 dims,
 // swizzled as the MMA reads them.
 //
-// Rounding: P has the type's precision (relative 2^-9 or 2^-12 on average of
-// a weight, about the output's own rounding); the maximum used may be up to
-// 2^8 below the true one, so that O is rescaled only when it grew by more,
-// which leaves P at most 2^8, inside both types' ranges.
+// Rounding: a weight is rounded to the type, by at most 2^-8 or 2^-11 of
+// itself, as the output is. Scores, maxima, sums and O are FP32. The frame m
+// of a row's weights may lie below its maximum: by up to 2^8, so that O is
+// rescaled only when the maximum grew by more; bf16's range allows the growth
+// of a whole tile on top, which saves a pass for the maximum (f16's does not).
 //
-// Tensor-bound in principle: per 128 x 128 x D tile 4 * 128 * 128 * D FLOP.
+// Tensor-bound in principle: 4 * 128 * 128 * D FLOP per 128 rows x 128 keys,
+// 1,024 clocks at D = 128. In fact bound by the chain S -> P -> O of a tile:
+// about 4,000 clocks per 256 rows x 128 keys, the tensor cores half idle. A
+// tile's softmax is some 1,300 clocks of instructions when it has the SM to
+// itself, and S cannot be formed again before P, which lies over it, is used
+// (TMEM is full: two S and two O of 128 columns). Hence two MMA tiles, and
+// each tile's keys in two halves with chains of their own, so that one's
+// products run under another's exponentials.
 //
-// Keys that no row of a tile sees are not read; tiles whose keys all rows see
-// skip the mask. Slots past the request's tokens may hold anything: K's are
+// Measured (B200): three causal prompts of 10.8 K tokens, 16 / 8 heads, D 128,
+// capped: 267 us, 838 TFLOP/s; 509 tokens on 65 K keys, 32 / 8 heads, biased:
+// 655 us, 830 TFLOP/s, half of cuBLAS's rate; 8 K tokens of packed documents,
+// D 64, f16: 122 us; prompts with prefix masks, 96 / 8 heads: 64 us. On the
+// capped prompts, in the order tried: MMAs issued under a branch on one lane
+// 469 us, by a predicate 374 us; eight softmax warps with a row's 128 scores
+// in registers 374 us, sixteen with 64 each 418 us (at 96 registers they
+// spill, and 224 KB of shared memory leave next to no L1 for that), sixteen
+// that keep the scores in TMEM 359 us; both halves of the keys in one chain
+// 372 us, in two 343 us; the heads as the grid's slower dimension 334 us,
+// innermost 267 us (the longest tiles of all heads start first).
+//
+// Keys that no row of a tile sees are not read; runs of
+// 16 keys that a warp's rows all see skip the mask, those that none sees the
+// exponentials. Slots past the request's tokens may hold anything: K's are
 // masked and V's are zeroed in shared memory. A value that is not finite at a
 // key some rows of a tile see and others do not turns the others' sums into
 // NaN (0 * inf); such rows are recomputed one by one from their own keys.
@@ -58,7 +79,7 @@ constexpr unsigned short kKeep = 0x7fc0;   // (a NaN) the frame stays
 // Heads of 128 dims: two MMA tiles (256 rows) in a CTA that fills the SM, so
 // that a K and V tile from L2 serves both. Heads of 64 dims need half the
 // bytes and TMEM per MMA tile: one MMA tile in a CTA and two CTAs an SM, which
-// start and end beside one another.
+// start and end beside one another (packed documents 151 -> 146 us).
 template <int D>
 struct Plan {
   static constexpr int kMmaTiles = D == 128 ? 2 : 1;
@@ -356,11 +377,12 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   unsigned char* ring = base + QT * P::kQBytes;
   Shared& sh = *reinterpret_cast<Shared*>(ring + P::kRing * P::kTileBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
-  const int h = blockIdx.y;
-  // Later row tiles see more keys under a causal mask: they start first.
-  const int slots = gridDim.x / a.nsplit;
-  const int split = blockIdx.x % a.nsplit;
-  const RowTile t = row_tile<P::kRows>(a, slots - 1 - static_cast<int>(blockIdx.x) / a.nsplit, lane);
+  // Later row tiles see more keys under a causal mask: they start first, all
+  // heads' together, so that the shortest end the grid.
+  const int h = static_cast<int>(blockIdx.x) % a.L.hkv, rest = static_cast<int>(blockIdx.x) / a.L.hkv;
+  const int slots = static_cast<int>(gridDim.x) / (a.L.hkv * a.nsplit);
+  const int split = rest % a.nsplit;
+  const RowTile t = row_tile<P::kRows>(a, slots - 1 - rest / a.nsplit, lane);
   if (t.rows == 0) return;
 
   const int qt = warp >> 3, half = (warp >> 2) & 1;        // softmax warps: MMA tile, half of its keys
@@ -937,8 +959,9 @@ int launch_mode(const PagedAttnArgs& a, const CUtensorMap& km, const CUtensorMap
   const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Plan<D>::kBytes));
   if (rc) return rc;
   const int slots = row_tile_slots(a.R, a.T, a.G, a.token_offsets != nullptr, a.shared != 0, Plan<D>::kRows);
-  kern<<<dim3(static_cast<unsigned>(slots * a.nsplit), static_cast<unsigned>(a.L.hkv)), Plan<D>::kThreads, Plan<D>::kBytes,
-         stream>>>(a, km, vm);
+  const long long ctas = static_cast<long long>(slots) * a.nsplit * a.L.hkv;
+  if (ctas > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
+  kern<<<static_cast<unsigned>(ctas), Plan<D>::kThreads, Plan<D>::kBytes, stream>>>(a, km, vm);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -14,6 +14,15 @@
 // inside a run, its state goes to one partial; the join kernel adds the
 // partials of each row.
 //
+// Measured (B200, bf16, D 128): 64 requests of 8-32 K tokens, 16 / 8 heads
+// (5.1 GB): 800 us with the join, 6.4 TB/s, 97 % of a copy's rate. One request
+// of 65,536 tokens, 32 / 8 heads, capped: 57 us, 4.7 TB/s; the other 16 us are
+// launches, the first loads and the join. The tcgen05 kernel on the same
+// calls, its 128-row tiles mostly empty: 1,317 and 85 us (and 184 against 92
+// us for 12 heads a group), so it takes over above 16 rows only. Runs of
+// whole CTAs with a join of their four warps took 65 us for the long request
+// and 36 % more for many short ones.
+//
 // Values past the keys that any row sees are zeroed in shared memory. Rows of
 // several tokens that see different keys are recomputed one by one where a
 // value that is not finite made their sum NaN.
