@@ -482,7 +482,8 @@ STK_API size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int 
  * log-sum-exp of the row's scores (-inf there). prefix > 0: the first prefix
  * tokens (whole pages) of every request are the same pages (those of request
  * 0's table are read), attended once for all requests' tokens and joined
- * with each request's own rest. New: the reference attends block lists only. */
+ * with each request's own rest. Offsets past T and requests with more tokens
+ * than max_tokens are cut and reported in status (STK_STATUS_SHAPE_OVERFLOW). New: the reference attends block lists only. */
 STK_API int stk_paged_attention(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
                                 long long q_head_stride, int R, int T, int hq, const int32_t* lengths,
                                 const int32_t* token_offsets, int max_tokens, int max_length, int prefix,

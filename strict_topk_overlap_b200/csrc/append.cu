@@ -342,15 +342,16 @@ append_kernel(AppendArgs a, int tile_tokens, int chunks, int items) {
         n = 1;
       } else {
         r = request_of_slot(a.token_offsets, a.R, 1, B, 2, slot, lane);
-        t0 = a.token_offsets[r];
-        n = a.token_offsets[r + 1] - t0;
+        const int2 tn = new_tokens(a.token_offsets, r, a.T, a.status);
+        t0 = tn.x;
+        n = tn.y;
         f = slot - t0 / B - 2 * r;
       }
       len = a.lengths[r];
       base = a.L.block_offsets[r];
       const int blocks = a.L.block_offsets[r + 1] - base;
       begin = end = 0;
-      if (n > 0 && len >= 0) {
+      if (n > 0 && len >= 0 && f >= 0) {
         j = len / B + f;  // block of the request
         begin = max(len, j * B);
         end = static_cast<int>(min(static_cast<long long>(len) + n, (j + 1ll) * B));
@@ -419,13 +420,11 @@ template <typename T, int VEC>
 static int launch_append_t(const AppendArgs& a, int sms, cudaStream_t stream) {
   const int slots = a.token_offsets ? a.T / a.L.b + 2 * a.R : a.R;
   const int heads = (a.q ? a.hq : 0) + 2 * a.L.hkv;
-  // 32 tokens of tables per tile up to 128 pairs, fewer for wider heads.
+  // 32 tokens of tables per tile up to 128 pairs, 8 for wider heads: at most 32 KB.
   const int pairs = a.cos ? a.pairs : 0;
   const int tile = pairs <= 128 ? 32 : 8;
   const size_t smem = static_cast<size_t>(tile) * pairs * sizeof(float2);
   auto kern = append_kernel<T, VEC>;
-  if (smem > 48 * 1024)
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   // One item (a slot's eight heads, one per warp) per CTA while that leaves
   // SMs free; beyond, equal runs of items for the CTAs that fit.
   const int chunks = (heads + kAppendWarps - 1) / kAppendWarps;

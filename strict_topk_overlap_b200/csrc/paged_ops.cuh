@@ -71,7 +71,28 @@ __device__ __forceinline__ int request_of_slot(const int* offs, int R, int mul, 
     count += c;
     if (c < 32) break;
   }
-  return count - 1;
+  return max(count - 1, 0);
+}
+
+// First packed token and number of new tokens of request r. Offsets that run
+// backwards or past the T tokens are cut to them and reported.
+__device__ __forceinline__ int2 new_tokens(const int* offs, int r, int T, int* status) {
+  if (offs == nullptr) return make_int2(r, 1);
+  const int a = offs[r], b = offs[r + 1];
+  if (a < 0 || b < a || b > T) report(status, kStatusShapeOverflow);
+  const int first = min(max(a, 0), T);
+  return make_int2(first, max(0, min(b, T) - first));
+}
+
+// The last request that starts at or before a packed token.
+__device__ __forceinline__ int request_of_token(const int* offs, int R, int token) {
+  if (offs == nullptr) return token;
+  int r = 0, end = R;
+  while (end - r > 1) {
+    const int mid = (r + end) >> 1;
+    if (offs[mid] <= token) r = mid; else end = mid;
+  }
+  return r;
 }
 
 // Rows [row0, row0 + rows) of request r: n new tokens from packed token t0
@@ -106,13 +127,14 @@ __device__ __forceinline__ RowTile row_tile(const PagedAttnArgs& a, int slot, in
     t.n = 1;
   } else {
     t.r = request_of_slot(a.token_offsets, a.R, a.G, M, 1, slot, lane);
-    t.t0 = a.token_offsets[t.r];
-    t.n = a.token_offsets[t.r + 1] - t.t0;
+    const int2 tn = new_tokens(a.token_offsets, t.r, a.T, a.status);
+    t.t0 = tn.x;
+    t.n = tn.y;
     f = slot - static_cast<int>(static_cast<long long>(t.t0) * a.G / M) - t.r;
   }
   t.len = a.shared ? request_blocks(a.L, 0) * a.L.b : cached_tokens(a, t.r, t.n);  // loaded beside the offsets
-  t.row0 = f * M;
-  t.rows = max(0, min(M, t.n * a.G - t.row0));
+  t.row0 = max(f, 0) * M;
+  t.rows = f < 0 ? 0 : max(0, min(M, t.n * a.G - t.row0));
   return t;
 }
 
@@ -138,18 +160,11 @@ __device__ __forceinline__ RowKeys row_keys(const PagedAttnArgs& a, const RowTil
   int len = t.len;
   if (!a.shared) {
     k.pos = t.len - t.n + i;
-  } else if (a.token_offsets == nullptr) {
-    len = cached_tokens(a, token, 1);
-    k.pos = len - 1;
   } else {
-    int r = 0, end = a.R;  // the last request that starts at or before the token
-    while (end - r > 1) {
-      const int mid = (r + end) >> 1;
-      if (a.token_offsets[mid] <= token) r = mid; else end = mid;
-    }
-    const int last = a.token_offsets[r + 1];
-    len = cached_tokens(a, r, last - a.token_offsets[r]);
-    k.pos = len - (last - token);
+    const int r = request_of_token(a.token_offsets, a.R, token);
+    const int2 tn = new_tokens(a.token_offsets, r, a.T, a.status);
+    len = cached_tokens(a, r, tn.y);
+    k.pos = len - (tn.x + tn.y - token);
   }
   k.lo = max(given.x, a.span_lo);
   k.hi = min(min(a.kv_hi ? given.y : k.pos + 1, min(len, t.len)), a.span_hi);

@@ -247,10 +247,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32) rows_attn_kernel(PagedAttnArg
 
 template <typename T, int NPL, int RW, bool VEC>
 static int launch_rows_t(const PagedAttnArgs& a, cudaStream_t stream) {
-  const size_t smem = static_cast<size_t>(kRowsWarps) * RW * a.d * sizeof(float);
+  const size_t smem = static_cast<size_t>(kRowsWarps) * RW * a.d * sizeof(float);  // at most 32 KB
   auto kern = rows_attn_kernel<T, NPL, RW, VEC>;
-  if (smem > 48 * 1024)
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   const int slots = row_tile_slots(a.R, a.T, a.G, a.token_offsets != nullptr, a.shared != 0, kRowTile);
   kern<<<dim3(static_cast<unsigned>(slots * a.nsplit), static_cast<unsigned>(a.L.hkv)), kRowsWarps * 32, smem,
          stream>>>(a);
@@ -317,26 +315,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(JoinArgs a) {
     parts[k] = p.parts;
     if (p.prefix != nullptr) {
       const int token = row / a.hq, head = row - token * a.hq, h = head / a.G, hkv = a.hq / a.G;
-      int r = 0, first = 0;
-      if (!p.shared) {
-        r = first = token;
-        if (a.token_offsets != nullptr) {
-          int hi = p.requests;
-          r = 0;
-          while (hi - r > 1) {
-            const int mid = (r + hi) >> 1;
-            if (a.token_offsets[mid] <= token) r = mid; else hi = mid;
-          }
-          first = a.token_offsets[r];
-        }
-      }
+      const int r = p.shared ? 0 : request_of_token(a.token_offsets, p.requests, token);
+      const int first = p.shared ? 0 : a.token_offsets != nullptr ? max(a.token_offsets[r], 0) : token;
+      const int local = (token - first) * a.G + head - h * a.G;  // row of the request's tile
       const long long total = static_cast<long long>(p.prefix[p.requests]) * hkv;
       const long long per = (total + p.streams - 1) / p.streams;
       const int units = p.prefix[r + 1] - p.prefix[r];
       const long long u0 = static_cast<long long>(p.prefix[r]) * hkv + static_cast<long long>(h) * units;
       const int c0 = units ? static_cast<int>(u0 / per) : 0;
-      parts[k] = units ? static_cast<int>((u0 + units - 1) / per) - c0 + 1 : 0;
-      base[k] = (static_cast<long long>(c0) + r * hkv + h) * p.most_rows + (token - first) * a.G + head - h * a.G;
+      const bool written = units > 0 && local >= 0 && local < p.most_rows;
+      parts[k] = written ? static_cast<int>((u0 + units - 1) / per) - c0 + 1 : 0;
+      base[k] = (static_cast<long long>(c0) + r * hkv + h) * p.most_rows + local;
       step[k] = p.most_rows;
     }
   }

@@ -80,17 +80,20 @@ struct Request {
   int pos;  // of the last of them
 };
 
-__device__ __forceinline__ Request request_at(const PagedAttnArgs& a, int r) {
+// (A request with more rows than the call's max_tokens allows keeps its first ones and is reported.)
+__device__ __forceinline__ Request request_at(const PagedAttnArgs& a, int r, int most_rows) {
   Request q;
   q.t.r = a.shared ? 0 : r;
   q.t.row0 = 0;
-  q.t.t0 = a.shared ? 0 : a.token_offsets ? a.token_offsets[r] : r;
-  q.t.n = a.shared ? a.T : a.token_offsets ? a.token_offsets[r + 1] - q.t.t0 : 1;
-  q.t.rows = q.t.n * a.G;
+  const int2 tn = a.shared ? make_int2(0, a.T) : new_tokens(a.token_offsets, r, a.T, a.status);
+  q.t.t0 = tn.x;
+  q.t.n = tn.y;
+  q.t.rows = min(q.t.n * a.G, most_rows);
+  if (q.t.n * a.G > most_rows) report(a.status, kStatusShapeOverflow);
   q.t.len = a.shared ? request_blocks(a.L, 0) * a.L.b : q.t.n > 0 ? cached_tokens(a, r, q.t.n) : 0;
   q.kmin = 0x7fffffff;
   q.kmax = q.pos = 0;
-  for (int i = 0; i < q.t.n; ++i) {
+  for (int i = 0; i * a.G < q.t.rows; ++i) {
     const RowKeys k = row_keys(a, q.t, i);
     q.pos = k.pos;
     if (k.hi > k.lo) {
@@ -108,7 +111,8 @@ __device__ __forceinline__ int units_of(const Request& q) { return (q.kmax + kUn
 struct Walk {
   int r, h, u, units;
   Request q;
-  __device__ __forceinline__ void start(const PagedAttnArgs& a, const int* prefix, int requests, long long at) {
+  __device__ __forceinline__ void start(const PagedAttnArgs& a, const int* prefix, int requests, int most_rows,
+                                        long long at) {
     int lo = 0, hi = requests;  // the request with prefix[r] * hkv <= at < prefix[r + 1] * hkv
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -119,9 +123,9 @@ struct Walk {
     const int in = static_cast<int>(at - static_cast<long long>(prefix[r]) * a.L.hkv);
     h = in / units;
     u = in - h * units;
-    q = request_at(a, r);
+    q = request_at(a, r, most_rows);
   }
-  __device__ __forceinline__ void next(const PagedAttnArgs& a, const int* prefix, int requests) {
+  __device__ __forceinline__ void next(const PagedAttnArgs& a, const int* prefix, int requests, int most_rows) {
     if (++u < units) return;
     u = 0;
     if (++h < a.L.hkv) return;
@@ -131,7 +135,7 @@ struct Walk {
     } while (r < requests && prefix[r + 1] == prefix[r]);
     if (r < requests) {
       units = prefix[r + 1] - prefix[r];
-      q = request_at(a, r);
+      q = request_at(a, r, most_rows);
     }
   }
 };
@@ -153,7 +157,7 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
       for (int i = 0; i < P::kStages; ++i) mbar_init(&bars[w][i], 1);
     fence_barrier_init();
   }
-  for (int r = tid; r < requests; r += blockDim.x) prefix[r + 1] = units_of(request_at(a, r));
+  for (int r = tid; r < requests; r += blockDim.x) prefix[r + 1] = units_of(request_at(a, r, most_rows));
   __syncthreads();
   if (warp == 0) {
     int carry = 0;
@@ -183,7 +187,7 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
   const int ppb = a.L.b / a.L.page_size;
   unsigned char* ring = base + warp * P::kStages * P::kStage;
   Walk ahead;
-  ahead.start(a, prefix, requests, first);
+  ahead.start(a, prefix, requests, most_rows, first);
   int issued = 0;  // units asked for
   int page = 0, key = 0, head = 0;
   // The place of the next unit to ask for; the page id arrives while others are computed.
@@ -211,7 +215,7 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
       }
     }
     if (++issued < jobs) {
-      ahead.next(a, prefix, requests);
+      ahead.next(a, prefix, requests, most_rows);
       find();
     }
   };
@@ -221,7 +225,7 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
   const int g = lane >> 2, t4 = lane & 3;
   const uint32_t sring = smem_u32(ring);
   Walk walk;
-  walk.start(a, prefix, requests, first);
+  walk.start(a, prefix, requests, most_rows, first);
   int taken = 0;  // chunks consumed
   bool ok = true;
   for (int done = 0; done < jobs;) {
@@ -385,7 +389,7 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
       return;
     }
     walk.u = u1 - 1;
-    if (done < jobs) walk.next(a, prefix, requests);
+    if (done < jobs) walk.next(a, prefix, requests, most_rows);
   }
 }
 

@@ -366,6 +366,30 @@ def test_bad_data_is_reported():
 
 
 @gpu
+@pytest.mark.parametrize("offsets,new", [([0, 9, 4], 1), ([0, 2, 900], 1), ([-5, 2, 6], 1), ([0, 400, 500], 130),
+                                         ([0, 4, 6], 1)])
+def test_bad_offsets_and_bounds_are_reported(offsets, new):
+    """Offsets that leave the packed tokens, and more tokens than max_tokens: cut, reported, nothing else touched."""
+    from strict_topk_overlap_b200 import _lib, paged_append, paged_attention
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cache = _cache([200, 300], 2, 64, 32, 16, torch.bfloat16, 51)
+    t = 6 if new == 1 else 260
+    q = torch.randn((t, 8, 64), device=DEV).to(torch.bfloat16)
+    try:
+        _lib.set_status_tensor(status)
+        paged_attention.attention(q, cache, _ints([200, 300]), token_offsets=_ints(offsets), max_tokens=new)
+        assert int(status) == 3
+        if offsets != [0, 4, 6]:
+            status.zero_()
+            kv = q[:, :2].contiguous()
+            paged_append.append_tokens(cache, kv, kv, _ints([10, 20]), token_offsets=_ints(offsets))
+            assert int(status) == 3
+    finally:
+        _lib.set_status_tensor(None)
+    torch.cuda.synchronize()
+
+
+@gpu
 def test_refusals():
     from strict_topk_overlap_b200 import paged_attention
     cache = _cache([64, 64], 2, 64, 32, 16, torch.bfloat16, 60)
