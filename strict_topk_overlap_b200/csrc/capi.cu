@@ -1043,6 +1043,7 @@ extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, l
   for (int i = 0; i < p.phases; ++i) {
     const AttnPhase& ph = p.phase[i];
     a.span_lo = ph.span_lo; a.span_hi = ph.span_hi; a.shared = ph.shared; a.nsplit = ph.nsplit;
+    a.chained = i > 0 && ph.kind == kAttnTokens;
     int* prefix_units = nullptr;
     if (p.join) {
       a.part_o = reinterpret_cast<float*>(at);

@@ -54,6 +54,7 @@ struct PagedAttnArgs {
   int span_lo, span_hi;  // only keys in [span_lo, span_hi)
   int shared;            // 1: every token reads the pages of request 0
   int nsplit;            // parts of a tile's key range
+  int chained;           // launched while the call's first phase still runs: ends after it
   float2* part_ml;       // [nsplit, T * hq] (m, l) of each part; null: the output is written
   float* part_o;         // [nsplit, T * hq, d] unnormalised
   int* status;

@@ -798,6 +798,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       if (!ok) break;
     }
     // ------------------------------------------------------------ output
+    pdl_release();  // what follows in the call may be launched: a join waits for the states, a second phase for nothing
     const bool any = begin < end;
     if (any) ok = warp_wait(&sh.o_full[qt], 0, a.status) && ok;
     fence_after();

@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) rows_attn_kernel(PagedAttnArg
         }
       }
     }
+    if (g0 + kRowsWarps >= groups) pdl_release();  // the join may be launched: it waits for the states
     // Join the slices of each row group in shared memory, in slice order.
     __syncthreads();
     float* mine = rsm + static_cast<size_t>(warp) * RW * D;

@@ -180,7 +180,10 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
   const int stream = blockIdx.x * kWarps + warp, streams = gridDim.x * kWarps;
   const long long per = (total + streams - 1) / streams;
   const long long first = min(total, stream * per), last = min(total, first + per);
-  if (first >= last) return;
+  if (first >= last) {
+    if (a.chained) pdl_wait();
+    return;
+  }
   const int jobs = static_cast<int>(last - first);
 
   // ---- this warp's stream of units, issued kStages ahead
@@ -232,6 +235,7 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
     const Request q = walk.q;
     const int h = walk.h, u0 = walk.u, slot_rh = walk.r * a.L.hkv + walk.h;
     const int u1 = min(walk.units, u0 + (jobs - done));
+    if (done + (u1 - u0) >= jobs) pdl_release();  // the join may be launched: it waits for the states
     // ---- rows g and g + 8 of the tile: their queries, keys and slopes
     uint32_t qf[D / 16][4];
     RowKeys rk[2];
@@ -386,11 +390,15 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
     if (!ok) {  // a wait ran out and was reported: leave after this warp's copies have landed
       for (; taken < issued; ++taken)
         mbar_wait(&bars[warp][taken % P::kStages], (taken / P::kStages) & 1, a.status);
-      return;
+      break;
     }
     walk.u = u1 - 1;
     if (done < jobs) walk.next(a, prefix, requests, most_rows);
   }
+  // Behind a first phase: this grid's completion has to imply that one's. The
+  // phases read the same inputs and write different states, so that nothing
+  // before this point waits for the first.
+  if (a.chained) pdl_wait();
 }
 
 template <typename T, int D>
@@ -401,6 +409,9 @@ int launch_t(const PagedAttnArgs& a, int streams, int most_rows, int* prefix, co
   const int smem = TokenPlan<D>::kBytes + (requests + 1) * 4;
   const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (rc) return rc;
+  if (a.chained)
+    return launch_pdl(kern, dim3(streams / kWarps), dim3(kWarps * 32), smem, stream, 0, a, requests, most_rows, prefix, km,
+                      vm);
   kern<<<streams / kWarps, kWarps * 32, smem, stream>>>(a, requests, most_rows, prefix, km, vm);
   return static_cast<int>(cudaGetLastError());
 }
