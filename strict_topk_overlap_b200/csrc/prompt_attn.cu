@@ -643,7 +643,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     float m = neg_inf(), l = 0.f;  // in log2 units; m is the frame of P, O and l, near the row's maximum
     bool ok = true, exact = true;
     int meetings = 0;
-    float level = neg_inf();  // the last tile's maximum, or a little more, less its largest bias
+    float level = neg_inf();  // the scores' maximum so far, or a little more, less the bias
     const int begin = qt ? qa[1] : qa[0], end = qt ? qb[1] : qb[0];
     // O of the warp's rows (this half of its dims) and l by 2^(m - frame).
     auto reframe = [&](bool grow, float frame) {
@@ -696,10 +696,12 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       }
     };
     auto grows = [&](float x) { return x > m + kLazy || (m == neg_inf() && x > m); };
-    // The largest bias that a key of tile i can have.
-    auto most_bias = [&](int i) {
-      return (MODE & 2) ? -z.slope2 * static_cast<float>(max(0, rk.pos - (i * kTileN + kTileN - 1))) : 0.f;
+    // The bias of key `last`, or of the row's last key before it: the largest of a run that ends there.
+    auto bias_at = [&](int last) {
+      return (MODE & 2) ? -z.slope2 * static_cast<float>(max(0, rk.pos - min(last, rk.hi - 1))) : 0.f;
     };
+    auto half_bias = [&](int i) { return bias_at(i * kTileN + half * kKeys + kKeys - 1); };  // of this thread's keys
+    auto tile_bias = [&](int i) { return bias_at(i * kTileN + kTileN - 1); };
     for (int i = begin; i < end; ++i) {
       const int n = i - begin;
       // A wait that runs out is told to the whole group at its next meeting: nobody is left waiting there.
@@ -709,8 +711,8 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       fence_after();
       const int k0 = i * kTileN + half * kKeys;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      const bool whole = k0 >= lo_max && k0 + kKeys <= hi_min;
-      float est;
+      const bool whole = k0 >= lo_max && k0 + kKeys <= hi_min, was_exact = exact;
+      float est = 0.f;
       if (exact) {
         // The maximum first, over both halves of the row's keys. Transformed and masked scores go back to TMEM.
         float mx = neg_inf();
@@ -753,10 +755,9 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         const float nm = m == neg_inf() ? 0.f : -m;
         if (whole) form_weights(std::true_type{}, std::false_type{}, k0, nm, sum);
         else form_weights(std::false_type{}, std::false_type{}, k0, nm, sum);
-        // Once every row that sees any key has met one, the frames may lag (not f16's: P would leave its range).
-        const bool waiting = m == neg_inf() && rk.hi > rk.lo;
+        // Once every row that sees a key in this part has met one, the frames may lag (not f16's: P would leave its range).
+        const bool waiting = m == neg_inf() && rk.hi > (i + 1) * kTileN && rk.lo < end * kTileN;
         if (kLag) exact = kOwnO ? __any_sync(kFull, waiting) : group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, waiting);
-        est = m;
       } else {
         // One pass, without a maximum, in a frame that the first half of the
         // keys sets at the end of the tile before: P may exceed 1, which
@@ -765,12 +766,13 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         // the frame moves. A row whose scores run ahead of its frame by more
         // than 2^127 overflows and is recomputed like those below.
         if (kOwnO) {
-          const bool grow = grows(level + most_bias(i));
-          if (__any_sync(kFull, grow)) reframe(grow, level + most_bias(i));
+          const float frame = level + half_bias(i);
+          const bool grow = grows(frame);
+          if (__any_sync(kFull, grow)) reframe(grow, frame);
         } else {
           const unsigned short code = sh.frame[qt][n & 3][r];
           const bool grow = code != kKeep;
-          const float frame = __uint_as_float(static_cast<uint32_t>(code) << 16) + most_bias(i);
+          const float frame = __uint_as_float(static_cast<uint32_t>(code) << 16) + tile_bias(i);
           if (__any_sync(kFull, grow)) {
             meet();  // both halves' products of the last tile are complete
             reframe(grow, frame);
@@ -782,12 +784,17 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         else form_weights(std::false_type{}, std::true_type{}, k0, nm, sum);
         est = log2f((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)) - nm;  // the maximum, or a little more
       }
-      // The next tile's frame. What the largest bias of a tile gains on this one's is known, and followed at once.
-      level = m == neg_inf() ? neg_inf() : est - most_bias(i);
+      // The next tile's frame: the level of the scores without their bias, and
+      // the largest bias that the row meets there, so that a bias which grows
+      // from tile to tile is followed at once. Keys too far below the frame to
+      // weigh anything say nothing of the level.
+      if (m == neg_inf()) level = neg_inf();
+      else if (was_exact) level = m - (kOwnO ? half_bias(i) : tile_bias(i));
+      else if (est - m > -100.f) level = est - half_bias(i);
       if (kLag && !kOwnO && half == 0 && !exact) {
         // Rounded down: a frame above the maximum would lose weights, one below it costs range only.
         const uint32_t code = (__float_as_uint(level) + (level < 0.f ? 0xffffu : 0u)) >> 16;
-        const bool grow = m != neg_inf() && grows(__uint_as_float(code << 16) + most_bias(i + 1));
+        const bool grow = m != neg_inf() && grows(__uint_as_float(code << 16) + tile_bias(i + 1));
         sh.frame[qt][(n + 1) & 3][r] = grow ? static_cast<unsigned short>(code) : kKeep;
       }
       tmem_wait_st();

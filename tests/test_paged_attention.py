@@ -293,6 +293,23 @@ def test_scores_that_move(dtype, pattern, new):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_steep_biases(dtype):
+    """Biases that grow by hundreds from tile to tile, ranges that end inside a tile, tokens far behind the keys they see."""
+    from strict_topk_overlap_b200 import paged_attention
+    for hq, hkv, d, block, page in ((8, 2, 128, 32, 16), (4, 2, 64, 32, 32)):
+        for n, new, seen in ((1000, 70, 1000), (1000, 70, 545), (1000, 40, 640 + 1), (1500, 300, 900)):
+            cache = _cache([n], hkv, d, block, page, dtype, 90)
+            q = torch.randn((new, hq, d), generator=torch.Generator(DEV).manual_seed(91), device=DEV).to(dtype)
+            pos = list(range(n - new, n))
+            hi = [min(p + 1, seen) for p in pos]
+            slopes = torch.tensor([(0.84, 3.0, 0.1, 0.5)[h % 4] for h in range(hq)], device=DEV)
+            out, lse = paged_attention.attention(q, cache, _ints([n]), token_offsets=_ints([0, new]), max_tokens=new,
+                                                 kv_hi=_ints(hi), slopes=slopes, return_lse=True)
+            _compare(q, cache, [n], [new], None, hi, out, lse, 0.0, slopes, d ** -0.5)
+
+
+@gpu
 def test_offsets_past_32_bits():
     """Pages whose elements lie beyond 2^31 of their pool: the append writes them, every attention form reads them."""
     from strict_topk_overlap_b200 import paged, paged_append, paged_attention
