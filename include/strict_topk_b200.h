@@ -469,7 +469,8 @@ typedef struct stk_attention_options {
   const int32_t* kv_hi; /* [T] */
 } stk_attention_options;
 
-/* Workspace (bytes) for stk_paged_attention of the same sizes. */
+/* Workspace (bytes, from a 16-byte boundary on) for stk_paged_attention of the
+ * same sizes. */
 STK_API size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int T, int hq, int has_offsets,
                                                    int max_tokens, int max_length, int prefix);
 

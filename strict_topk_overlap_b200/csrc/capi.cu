@@ -1020,9 +1020,11 @@ extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, l
     return fail(STK_EINVAL, "scale and softcap must not be negative");
   const AttnPlan p = plan_attention(
       kv, R, T, hq, token_offsets != nullptr, max_tokens, max_length, prefix,
-      prompt_attn_takes(kv->kv_dtype, kv->d, kv->page_size, kv->k, kv->v, q, q_token_stride, q_head_stride),
+      prompt_attn_takes(kv->kv_dtype, kv->d, kv->page_size, kv->k, kv->v, q, q_token_stride, q_head_stride, out),
       token_attn_takes(kv->kv_dtype, kv->d, kv->page_size, R, kv->k, kv->v, q, q_token_stride, q_head_stride));
   if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return fail(STK_EWS, "attention workspace too small");
+  if (p.bytes && reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(STK_EINVAL, "the attention workspace must start on a 16-byte boundary");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   PagedAttnArgs a{};
   a.L = make_layout(kv);

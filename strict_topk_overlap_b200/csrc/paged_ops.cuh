@@ -193,7 +193,7 @@ int launch_append_tokens(const AppendArgs& a, int kv_dtype, int sms, cudaStream_
 int launch_rows_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream);
 // Whether the tensor-core kernel takes these types, sizes and addresses.
 bool prompt_attn_takes(int kv_dtype, int d, int page_size, const void* k, const void* v, const void* q, long long q_ts,
-                       long long q_hs);
+                       long long q_hs, const void* out);
 // Rows of its CTAs, and how many of them an SM holds.
 inline int prompt_tile_rows(int d) { return d == 64 ? 128 : 256; }
 inline int prompt_ctas_per_sm(int d) { return d == 64 ? 2 : 1; }

@@ -988,10 +988,10 @@ int launch_d(const PagedAttnArgs& a, const CUtensorMap& km, const CUtensorMap& v
 // 16-bit types, heads of 64 or 128 dims, pages that tile 128 keys (or are
 // tiled by them), 16-byte rows.
 bool prompt_attn_takes(int kv_dtype, int d, int page_size, const void* k, const void* v, const void* q, long long q_ts,
-                       long long q_hs) {
+                       long long q_hs, const void* out) {
   const bool pages = page_size >= 8 && (page_size <= kTileN ? kTileN % page_size == 0 : page_size % kTileN == 0);
   const uintptr_t any = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q) |
-                        static_cast<uintptr_t>(q_ts * 2) | static_cast<uintptr_t>(q_hs * 2);
+                        reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(q_ts * 2) | static_cast<uintptr_t>(q_hs * 2);
   return kv_dtype != kF32 && (d == 64 || d == 128) && pages && any % 16 == 0;
 }
 

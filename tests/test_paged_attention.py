@@ -359,6 +359,43 @@ def test_streams_graphs_and_workspaces():
     assert torch.equal(held, paged_attention.attention(q, cache, shorter))  # the same bits every time
     with pytest.raises(RuntimeError, match="workspace"):
         paged_attention.attention(q, cache, at, workspace=ws[:16])
+    with pytest.raises(RuntimeError, match="16-byte"):
+        paged_attention.attention(q, cache, at, workspace=torch.cat((ws, ws))[8:])
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 130])
+def test_unaligned_tensors(new):
+    """Queries, pools and outputs that start off a 16-byte boundary take another kernel, not another result."""
+    import ctypes
+
+    from strict_topk_overlap_b200 import _lib as L
+    from strict_topk_overlap_b200 import paged, paged_attention
+    cache = _cache([200], 2, 64, 32, 16, torch.bfloat16, 52)
+
+    def shifted(x):
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)[1:].view(x.shape)
+        return y.copy_(x)
+
+    q = torch.randn((new, 4, 64), device=DEV).to(torch.bfloat16)
+    off = paged.PagedKVCache(shifted(cache.k_pages), shifted(cache.v_pages), cache.page_table, cache.block_offsets,
+                             cache.lo, cache.hi, 32, 16, cache.max_blocks)
+    more = dict(max_tokens=new, token_offsets=None if new == 1 else _ints([0, new]), return_lse=True)
+    for x, c in ((shifted(q), cache), (q, off)):
+        out, lse = paged_attention.attention(x, c, _ints([200]), **more)
+        _compare(q, cache, [200], [new], None, None, out, lse, 0.0, None, 64 ** -0.5)
+    # An output off its boundary, through the C entry point.
+    out = shifted(torch.zeros_like(q))
+    longest = cache.max_blocks * 32
+    kv, offsets = cache.packed_kv(2, 64), None if new == 1 else _ints([0, new])
+    need = L.load().stk_paged_attention_workspace_bytes(kv, 1, new, 4, int(new > 1), new, longest, 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    length = _ints([200])
+    rc = L.load().stk_paged_attention(kv, cache.k_pages.shape[0], q.data_ptr(), q.stride(0), q.stride(1), 1, new, 4,
+                                      length.data_ptr(), L.ptr(offsets), new, longest, 0, None, out.data_ptr(), None,
+                                      ws.data_ptr(), need, None, ctypes.c_void_p(L.stream_of(q)))
+    assert rc == 0
+    _compare(q, cache, [200], [new], None, None, out, None, 0.0, None, 64 ** -0.5)
 
 
 @gpu
