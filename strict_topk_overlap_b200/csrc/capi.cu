@@ -930,6 +930,29 @@ struct AttnPlan {
   size_t bytes;
 };
 
+// Parts that the prompt kernel cuts its tiles' key ranges into: the fewest
+// thousand clocks of waves x (key tiles of a part + start and end of a CTA) +
+// partial states written and read, by the kernel's measured costs (4 a key
+// tile of 256 rows at 128 dims, 2 of 128 rows at 64, 13 a CTA). 509 tokens on
+// 65 K keys, 64 row tiles: 643 us in 9 parts (3.9 waves), 674 in 2 (0.9 of
+// one), 772 in 7 (3.03). Four waves of tiles and more stay whole.
+int prompt_splits(long long tiles, int keys, int d, double rows, int places) {
+  const int key_tiles = (keys + 127) / 128;
+  if (tiles >= 4ll * places) return 1;
+  int best = 1;
+  double least = 0;
+  for (int n = 1; n <= key_tiles && n <= 64; ++n) {
+    const double waves = static_cast<double>((tiles * n + places - 1) / places);
+    const double part = (key_tiles + n - 1) / n * (d == 64 ? 2.0 : 4.0) + 13.0;
+    const double cost = waves * part + (n > 1 ? n * rows * (d + 2) * 8 / 3.4e6 : 0);
+    if (n == 1 || cost < least) {
+      best = n;
+      least = cost;
+    }
+  }
+  return best;
+}
+
 AttnPhase plan_phase(const stk_kv* kv, int R, int T, int hq, bool offsets, bool shared, int max_tokens, int keys,
                      bool prompt_ok, bool token_ok) {
   AttnPhase p{};
@@ -949,11 +972,16 @@ AttnPhase plan_phase(const stk_kv* kv, int R, int T, int hq, bool offsets, bool 
     const bool prompt = p.kind == kAttnPrompt;
     const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared,
                                                                 prompt ? prompt_tile_rows(kv->d) : 16)) * hkv;
-    const long long most = prompt ? (keys + 127) / 128 : (keys + 63) / 64;
-    // Requests of different lengths are cut into as many parts each: four
-    // CTAs of the FP32-unit kernel for each place let the hardware even them out.
-    long long n = (prompt ? prompt_ctas_per_sm(kv->d) : 8) * sms / tiles;
-    n = n < most ? n : most;
+    long long n;
+    if (prompt) {
+      n = prompt_splits(tiles, keys, kv->d, static_cast<double>(T) * hq, prompt_ctas_per_sm(kv->d) * sms);
+    } else {
+      // Requests of different lengths are cut into as many parts each: four
+      // CTAs of the FP32-unit kernel for each place let the hardware even them out.
+      const long long most = (keys + 63) / 64;
+      n = 8ll * sms / tiles;
+      n = n < most ? n : most;
+    }
     p.nsplit = static_cast<int>(n < 1 ? 1 : n);
     p.states = static_cast<size_t>(p.nsplit) * T * hq;
     p.bytes = p.states * (kv->d + 2) * sizeof(float);

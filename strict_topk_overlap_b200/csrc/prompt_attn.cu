@@ -30,7 +30,7 @@
 //
 // Measured (B200): three causal prompts of 10.8 K tokens, 16 / 8 heads, D 128,
 // capped: 267 us, 838 TFLOP/s; 509 tokens on 65 K keys, 32 / 8 heads, biased:
-// 655 us, 830 TFLOP/s, half of cuBLAS's rate; 8 K tokens of packed documents,
+// 650 us, 837 TFLOP/s, half of cuBLAS's rate; 8 K tokens of packed documents,
 // D 64, f16: 122 us; prompts with prefix masks, 96 / 8 heads: 64 us. On the
 // capped prompts, in the order tried: MMAs issued under a branch on one lane
 // 469 us, by a predicate 374 us; eight softmax warps with a row's 128 scores
