@@ -243,24 +243,29 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // 2^x of a pair on the FMA units: x = n + f with |f| <= 1/2 (n by adding and
-// subtracting 1.5 * 2^23), 2^f by a cubic (weighted least-maximum fit on
-// [-1/2, 1/2], relative error 7.5e-5, a fifth of a 16-bit weight's rounding),
-// n added to the exponent. The special function unit yields 16 exponentials
-// per SM and clock, as many as the tensor cores need weights; taking some of
-// them off it shortens a tile's chain of S, P and O.
+// subtracting 1.5 * 2^23), 2^f by a quartic that is 1 at 0 (weighted
+// least-maximum fit on [-1/2, 1/2], relative error 2.9e-6, far below a 16-bit
+// weight's rounding), n added to the exponent. x is clamped to [-127, 128],
+// where 1 becomes an exact 0 and infinity: a masked key's -inf has no weight at
+// all, whatever its value holds. NaN comes out as NaN (the clamp passes it on;
+// the last addition undoes what the exponent did to it). The special function
+// unit yields 16 exponentials per SM and clock, as many as the tensor cores
+// need weights.
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
-  x.x = fminf(fmaxf(x.x, -126.f), 128.f);
-  x.y = fminf(fmaxf(x.y, -126.f), 128.f);
+  asm("{\n .reg .f32 t;\n max.NaN.f32 t, %2, %4;\n min.NaN.f32 %0, t, %5;\n max.NaN.f32 t, %3, %4;\n min.NaN.f32 %1, t, %5;\n}\n"
+      : "=f"(x.x), "=f"(x.y)
+      : "f"(x.x), "f"(x.y), "f"(-127.f), "f"(128.f));
   const float2 t = add2(x, both(12582912.f));
   const float2 n = add2(t, both(-12582912.f));
   const float2 f = fma2(n, both(-1.f), x);
-  float2 p = fma2(f, both(0.05517167f), both(0.24261113f));
-  p = fma2(p, f, both(0.69326099f));
-  p = fma2(p, f, both(0.99992807f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+  float2 p = fma2(f, both(0.009582853f), both(0.055906426f));
+  p = fma2(p, f, both(0.24024099f));
+  p = fma2(p, f, both(0.6931242f));
+  p = fma2(p, f, both(1.f));
+  p = make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                  __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+  return fma2(x, both(0.f), p);
 }
-
 
 constexpr int kRun = 16;  // keys taken from TMEM at once
 
@@ -369,8 +374,11 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   // share O, each half's warps keeping half of its dims in frame.
   constexpr bool kOwnO = D == 64;
   constexpr int kOCols = 64;  // of O, a warp's
-  // Of 8 pairs of weights, those whose exponentials take the FMA units: none where the cap keeps these busy.
-  constexpr int kFmaPairs = (MODE & 1) ? 0 : 2;
+  // Of 8 pairs of weights, those whose exponentials take the FMA units: two for
+  // biased scores, whose frames move most (509 tokens on 65 K keys: 660 us, 672
+  // with none); none for others (plain causal prompts of 10.8 K tokens 238 us,
+  // 249 with two; 512 tokens on 16 K keys 149 against 159).
+  constexpr int kFmaPairs = MODE == 2 ? 2 : 0;
   constexpr int kHalves = D / 64;
   constexpr int kHalfBytes = kTileN * 128;
   extern __shared__ __align__(1024) unsigned char base[];  // swizzle atoms: 1024-byte aligned
@@ -848,7 +856,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
     const float inv = empty || a.part_ml ? 1.f : 1.f / l;
     // The frame was left behind, or ahead, by more than FP32's range; or scores are NaN.
-    // (2^-100: below what a frame that follows leaves, above what clamped exponentials of masked keys add up to.)
+    // (2^-100: below what a frame that follows leaves.)
     const bool over = !empty && !(l <= 3.0e38f && l >= 7.9e-31f);
     bool redo_row = have && over;
     if (ok && !(kOwnO && half)) {

@@ -1,0 +1,90 @@
+"""Dense paged attention where values, lengths and tables are at their edges:
+huge values and NaN at seen and unseen keys, unfilled pages, tokens of no
+request. Outputs that an edge must not touch are compared bit for bit with
+those of the same call without it; others with the 64-bit definition and the
+tolerances of test_paged_attention.py."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_paged_attention import DEV, TYPES, _cache, _compare_equal, _ints
+
+gpu = pytest.mark.gpu
+TILED = [(8, 2, 128, 32, 16), (4, 4, 64, 32, 16)]  # hq, hkv, d, block, page that the tensor-core kernels take
+
+
+def _queries(new, hq, d, dtype, seed):
+    return torch.randn((new, hq, d), generator=torch.Generator(DEV).manual_seed(seed), device=DEV).to(dtype)
+
+
+def _at(cache, r, j):
+    """Pages and slots of key tokens j (an int tensor) of request r."""
+    ppb = cache.block_size // cache.page_size
+    first = int(cache.block_offsets[r]) * ppb
+    return cache.page_table[first + j // cache.page_size].long(), j % cache.page_size
+
+
+def _span(a, b):
+    return torch.arange(a, b, device=DEV)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", TILED)
+@pytest.mark.parametrize("new", [1, 4, 200])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_unseen_values_near_the_types_limit(dtype, shape, new, sign):
+    """A key outside a row's interval weighs exactly nothing: its value may be as large as the type holds."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    cache = _cache([300], hkv, d, block, page, dtype, 100)
+    q = _queries(new, hq, d, dtype, 101)
+    pos = list(range(300 - new, 300))
+    split = [(p - 80) // 7 * 7 for p in pos]  # a first document of 14 to 217 keys
+    for scores in (dict(), dict(softcap=20.0), dict(slopes=torch.full((hq,), 0.05, device=DEV))):
+        args = dict(token_offsets=None if new == 1 else _ints([0, new]), max_tokens=new, return_lse=True, **scores)
+        for lo, hi, keys in ((split, None, _span(0, min(split))), (None, [240] * new, _span(240, 300)),
+                             (None, None, _span(300 - new + 1, 300))):
+            if keys.numel() == 0:
+                continue
+            more = dict(args, kv_lo=None if lo is None else _ints(lo), kv_hi=None if hi is None else _ints(hi))
+            clean, clean_lse = paged_attention.attention(q, cache, _ints([300]), **more)
+            at = _at(cache, 0, keys)
+            held = cache.v_pages[at[0], :, at[1]].clone()
+            cache.v_pages[at[0], :, at[1]] = sign * {torch.float16: 65504.0}.get(dtype, 3e38)
+            out, lse = paged_attention.attention(q, cache, _ints([300]), **more)
+            cache.v_pages[at[0], :, at[1]] = held
+            first = int(keys[0])
+            blind = torch.tensor([(hi is not None) or (lo is not None) or p < first for p in pos], device=DEV)
+            assert bool(blind.any())
+            assert torch.equal(out[blind], clean[blind])
+            assert torch.equal(lse, clean_lse)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", TILED)
+@pytest.mark.parametrize("new", [1, 200])
+@pytest.mark.parametrize("biased", [False, True])
+def test_seen_nan_keys_are_not_lost(dtype, shape, new, biased):
+    """A NaN in one key (its value is a number) makes every row that sees it NaN, wherever in a run of keys it lies,
+    and no other row."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    cache = _cache([300], hkv, d, block, page, dtype, 102)
+    q = _queries(new, hq, d, dtype, 103)
+    args = dict(token_offsets=None if new == 1 else _ints([0, new]), max_tokens=new, return_lse=True,
+                slopes=torch.full((hq,), 0.05, device=DEV) if biased else None)
+    clean, _ = paged_attention.attention(q, cache, _ints([300]), **args)
+    pos = _span(300 - new, 300)
+    for j in list(range(32, 48)) + [150, 215, 290, 299]:
+        pg, slot = _at(cache, 0, _span(j, j + 1))
+        held = cache.k_pages[pg, :, slot, 5].clone()
+        cache.k_pages[pg, :, slot, 5] = float("nan")
+        out, lse = paged_attention.attention(q, cache, _ints([300]), **args)
+        cache.k_pages[pg, :, slot, 5] = held
+        sees = pos >= j
+        assert bool(out[sees].isnan().all()) and bool(lse[sees].isnan().all()), j
+        if bool((~sees).any()):
+            _compare_equal(out[~sees], clean[~sees], dtype)
