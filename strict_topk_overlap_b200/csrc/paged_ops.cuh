@@ -189,6 +189,11 @@ __device__ __forceinline__ int page_of(const PagedAttnArgs& a, int rp, int j) {
   return page;
 }
 
+// The maximum of a softmax state as it is handed on: -inf says that the row
+// saw no key. Scores that are all NaN leave the running maximum there too
+// (fmaxf drops them) with a sum of NaN; such a state must reach the output.
+__device__ __forceinline__ float state_max(float m, float l) { return m == neg_inf() && l != l ? 0.f : m; }
+
 int launch_append_tokens(const AppendArgs& a, int kv_dtype, int sms, cudaStream_t stream);
 int launch_rows_attn(const PagedAttnArgs& a, int kv_dtype, cudaStream_t stream);
 // Whether the tensor-core kernel takes these types, sizes and addresses.

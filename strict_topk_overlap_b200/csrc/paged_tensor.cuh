@@ -83,6 +83,7 @@ __device__ void single_row(const PagedAttnArgs& a, int rp, int h, const T* q, in
     for (int j = 0; j < N; ++j) o[j] = o[j] * alpha + (w == 0.f ? 0.f : w * to_f32(vr[j]));
     m = mn;
   }
+  m = state_max(m, l);
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

@@ -841,6 +841,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     ok = !group_any(QT == 1 ? 1 : 1 + qt, 2 * kTileM, !ok);
     const float l2 = sh.other[qt][half ^ 1][r];
     float mine = 1.f, others = 0.f;
+    const bool nan = l != l || l2 != l2;
     if (kOwnO) {
       const float m2 = half ? neg_inf() : reinterpret_cast<const float*>(ring + kTileM * 256)[r];
       const float frame = fmaxf(m, m2);
@@ -855,10 +856,12 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const long long orow = static_cast<long long>(t.t0 + tok) * a.hq + head;
     const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
     const float inv = empty || a.part_ml ? 1.f : 1.f / l;
-    // The frame was left behind, or ahead, by more than FP32's range; or scores are NaN.
+    // The frame was left behind, or ahead, by more than FP32's range; or scores
+    // are NaN, perhaps all that the row sees here (which leaves no maximum).
     // (2^-100: below what a frame that follows leaves.)
-    const bool over = !empty && !(l <= 3.0e38f && l >= 7.9e-31f);
-    bool redo_row = have && over;
+    const bool sees = have && max(rk.lo, ta * kTileN) < min(rk.hi, tb * kTileN);
+    const bool over = sees && (empty || nan || !(l <= 3.0e38f && l >= 7.9e-31f));
+    bool redo_row = over;
     if (ok && !(kOwnO && half)) {
       // 128 bytes a row at a time through this warp's share of the Q tile's
       // place, which is free now, so that a store instruction covers whole rows.
@@ -945,7 +948,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
                          xpos, xslope, lane, xm, xl, xo);
         const long long xr = static_cast<long long>(t.t0 + xtok) * a.hq + xhead;
         const long long xp = static_cast<long long>(split) * a.T * a.hq + xr;
-        const float factor = !a.part_ml ? 1.f / xl : lost ? 1.f : expf(xm - frame);
+        const float factor = !a.part_ml ? (xl == 0.f ? 0.f : 1.f / xl) : lost ? 1.f : expf(xm - frame);
         if (lost && half == 0 && lane == 0) {
           if (a.part_ml) a.part_ml[xp] = make_float2(xm, xl);
           else if (a.lse) a.lse[xr] = xm + logf(xl);

@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) rows_attn_kernel(PagedAttnArg
     float* mine = rsm + static_cast<size_t>(warp) * RW * D;
     if (!idle) {
       if (lane < RW) {
-        wm[warp][lane] = m;
+        wm[warp][lane] = state_max(m, l);
         wl[warp][lane] = l;
       }
 #pragma unroll

@@ -88,3 +88,80 @@ def test_seen_nan_keys_are_not_lost(dtype, shape, new, biased):
         assert bool(out[sees].isnan().all()) and bool(lse[sees].isnan().all()), j
         if bool((~sees).any()):
             _compare_equal(out[~sees], clean[~sees], dtype)
+
+
+FORMS = TILED + [(6, 2, 96, 24, 8)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", FORMS)
+@pytest.mark.parametrize("new,prefix", [(1, 0), (4, 0), (200, 0), (1, 240), (40, 240)])
+def test_nan_query(dtype, shape, new, prefix):
+    """A query row that is NaN comes out as NaN, not as one that sees no keys; the others do not change."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    prefix = prefix // block * block
+    cache = _cache([300, 400], hkv, d, block, page, dtype, 104, shared=prefix)
+    q = _queries(2 * new, hq, d, dtype, 105)
+    args = dict(token_offsets=None if new == 1 else _ints([0, new, 2 * new]), max_tokens=new, return_lse=True)
+
+    def call(q):
+        if prefix:
+            return paged_attention.shared_prefix_attention(q, cache, _ints([300, 400]), prefix, **args)
+        return paged_attention.attention(q, cache, _ints([300, 400]), **args)
+
+    clean, clean_lse = call(q)
+    broken = torch.zeros((2 * new, hq), dtype=torch.bool, device=DEV)
+    broken[0, 0] = broken[-1, hq - 1] = broken[new // 2, hq // 2] = True
+    q[broken] = float("nan")
+    out, lse = call(q)
+    assert bool(out[broken].isnan().all()) and bool(lse[broken].isnan().all())
+    _compare_equal(out[~broken], clean[~broken], dtype)
+    assert float((lse - clean_lse)[~broken].abs().max()) <= 1e-3
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", FORMS)
+@pytest.mark.parametrize("new", [1, 4, 200])
+def test_only_nan_keys(dtype, shape, new):
+    """Rows whose only visible keys score NaN are NaN; rows that see no key at all are zero."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    cache = _cache([300], hkv, d, block, page, dtype, 106)
+    q = _queries(new, hq, d, dtype, 107)
+    pos = list(range(300 - new, 300))
+    for width in (0, 1, 30):
+        keys = _span(299 - new - 30, 300)
+        at = _at(cache, 0, keys)
+        held = cache.k_pages[at[0], :, at[1]].clone()
+        cache.k_pages[at[0], :, at[1], 3] = float("nan")
+        out, lse = paged_attention.attention(q, cache, _ints([300]), max_tokens=new, return_lse=True,
+                                             token_offsets=None if new == 1 else _ints([0, new]),
+                                             kv_lo=_ints([p + 1 - width for p in pos]))
+        cache.k_pages[at[0], :, at[1]] = held
+        if width:
+            assert bool(out.isnan().all()) and bool(lse.isnan().all())
+        else:
+            assert not bool(out.any()) and bool((lse == float("-inf")).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", FORMS)
+@pytest.mark.parametrize("new", [1, 130])
+def test_a_part_of_nan_keys_does_not_vanish(dtype, shape, new):
+    """Long ranges are cut into parts and tiles into halves: one whose keys are all NaN still makes the row NaN."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    cache = _cache([6000], hkv, d, block, page, dtype, 108)
+    q = _queries(new, hq, d, dtype, 109)
+    for a, b in ((0, 64), (64, 128), (3000, 3700), (5760, 5824)):
+        at = _at(cache, 0, _span(a, b))
+        held = cache.k_pages[at[0], :, at[1]].clone()
+        cache.k_pages[at[0], :, at[1], 1] = float("nan")
+        out, lse = paged_attention.attention(q, cache, _ints([6000]), max_tokens=new, return_lse=True,
+                                             token_offsets=None if new == 1 else _ints([0, new]))
+        cache.k_pages[at[0], :, at[1]] = held
+        assert bool(out.isnan().all()) and bool(lse.isnan().all())
