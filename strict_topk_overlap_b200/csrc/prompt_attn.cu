@@ -40,12 +40,14 @@
 // 372 us, in two 343 us; the heads as the grid's slower dimension 334 us,
 // innermost 267 us (the longest tiles of all heads start first).
 //
-// Keys that no row of a tile sees are not read; runs of
-// 16 keys that a warp's rows all see skip the mask, those that none sees the
-// exponentials. Slots past the request's tokens may hold anything: K's are
-// masked and V's are zeroed in shared memory. A value that is not finite at a
-// key some rows of a tile see and others do not turns the others' sums into
-// NaN (0 * inf); such rows are recomputed one by one from their own keys.
+// Tiles of keys that no row sees are not read; runs of 16 keys that a warp's
+// rows all see skip the mask, those that none sees the exponentials. Places
+// that no row of a CTA sees may hold anything, unwritten memory or unassigned
+// table entries: pages of such keys alone read as zeros, and in pages that
+// seen keys share K is masked and V zeroed in shared memory. A value that is
+// not finite at a key some rows of a tile see and others do not turns the
+// others' sums into NaN (0 * inf); such rows are recomputed one by one from
+// their own keys.
 
 #include "paged_tensor.cuh"
 
@@ -398,7 +400,6 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   const bool have = row < t.rows;
   RowKeys rk{0, 0x7fffffff, 0};
   const int* table = nullptr;  // loads: the request's page table
-  int pages = 0, ppb = 0;
   if (warp < kSoftmaxWarps) {
     const int my_tok = have ? (t.row0 + row) / a.G : 0;
     const int2 given = given_keys(a, t.t0 + my_tok);
@@ -428,10 +429,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   } else if (warp == kSoftmaxWarps) {
     tmem_alloc(&sh.tmem, P::kTmem);
   } else {
-    const int first = a.L.block_offsets[t.r];
-    ppb = a.L.b / a.L.page_size;
-    pages = (a.L.block_offsets[t.r + 1] - first) * ppb;
-    table = a.L.page_table + static_cast<long long>(first) * ppb;
+    table = a.L.page_table + static_cast<long long>(a.L.block_offsets[t.r]) * (a.L.b / a.L.page_size);
     if (lane == 0) {
       for (int i = 0; i < P::kRing; ++i) {
         mbar_init(&sh.full[i], 1);
@@ -491,6 +489,12 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       qb[q] = uniform(qb[q]);
     }
   }
+  // The keys that any row here sees lie in [.x, .y). (From shared memory once
+  // more: the softmax warps have no registers to keep it in.)
+  auto seen_keys = [&]() {
+    const int2 v = sh.range[lane & (kSoftmaxWarps - 1)];
+    return make_int2(__reduce_min_sync(kFull, v.x), __reduce_max_sync(kFull, v.y));
+  };
   const uint32_t tmem = uniform(sh.tmem);
   const int rp = t.r;
 
@@ -498,10 +502,13 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     // ------------------------------------------------------------ K and V tiles
     const int bp = min(a.L.page_size, kTileN);  // rows of a box
     const int boxes = kTileN / bp;
-    auto page_at = [&](int key) {  // keys past the request's pages, or of a bad entry, read as zeros
-      const int entry = key / a.L.page_size;
-      if (entry >= pages) return a.pages;
-      const int page = table[entry];
+    const int2 any = seen_keys();
+    // Page of the box of keys from `key` on. Boxes of keys that no row here
+    // sees read as zeros, whatever the table or the pool holds there; a bad
+    // entry reads as zeros and is reported.
+    auto page_at = [&](int key) {
+      if (key >= any.y || key + bp <= any.x) return a.pages;
+      const int page = table[key / a.L.page_size];
       if (page < 0 || page >= a.pages) {
         report(a.status, kStatusBadBlockId);
         return a.pages;
@@ -535,7 +542,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const uint64_t q_desc = smem_desc(smem_u32(base), 16), k_desc = smem_desc(smem_u32(ring), 16);
     const uint64_t v_desc = smem_desc(smem_u32(ring), kHalfBytes);
     constexpr uint64_t kTile16 = P::kTileBytes >> 4;  // descriptor addresses count 16 bytes
-    const int len = uniform(t.len);
+    const int2 any = seen_keys();
     int done[2] = {0, 0};  // tiles, per MMA tile
     // Ring slots and phases of the next K and V tiles (items 0, 2, 4, .. and 1, 3, 5, ..).
     int slot = 0, phase = 0;
@@ -573,14 +580,19 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       const int vslot = slot;
       ok = warp_wait(&sh.full[vslot], phase, a.status);
       if (!ok) break;
-      const int valid = len - i * kTileN;
-      if (valid < kTileN) {  // slots past the request's tokens: their values must not meet the zero weights
+      // Keys that no row here sees, in pages that others of theirs share:
+      // their values must not meet the zero weights.
+      const int from = any.x - i * kTileN, to = any.y - i * kTileN;
+      if (from > 0 || to < kTileN) {
+        // Below `from` and from `to` on, each to the end of its box.
         unsigned char* vt = ring + vslot * P::kTileBytes;
-        const int from = max(valid, 0);
-        const int fill = min(kTileN, (from + a.L.page_size - 1) / a.L.page_size * a.L.page_size);
-        for (int x = lane; x < (fill - from) * 8 * kHalves; x += 32) {
-          const int half = x % kHalves, y = x / kHalves;
-          *reinterpret_cast<uint4*>(vt + half * kHalfBytes + (from + y / 8) * 128 + y % 8 * 16) = make_uint4(0, 0, 0, 0);
+        const int bp = min(a.L.page_size, kTileN);
+        const int below = max(from, 0) % bp, above = to < kTileN ? (bp - to % bp) % bp : 0;
+#pragma unroll 1
+        for (int x = lane; x < (below + above) * 8 * kHalves; x += 32) {
+          const int half = x % kHalves, c = x / kHalves % 8, y = x / (8 * kHalves);
+          const int at = y < below ? from - below + y : to + y - below;
+          *reinterpret_cast<uint4*>(vt + half * kHalfBytes + at * 128 + c * 16) = make_uint4(0, 0, 0, 0);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();

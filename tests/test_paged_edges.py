@@ -165,3 +165,74 @@ def test_a_part_of_nan_keys_does_not_vanish(dtype, shape, new):
                                              token_offsets=None if new == 1 else _ints([0, new]))
         cache.k_pages[at[0], :, at[1]] = held
         assert bool(out.isnan().all()) and bool(lse.isnan().all())
+
+
+ROOMY = TILED + [(8, 2, 128, 128, 16), (4, 1, 64, 256, 32), (24, 2, 128, 256, 256)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", ROOMY)
+@pytest.mark.parametrize("new", [[1] * 4, [130, 90, 1, 44]])
+def test_unfilled_pages_change_nothing(dtype, shape, new):
+    """NaN in every slot past the tokens, whole pages of it, gives the bits that zeros there give: no row leaves its
+    fast path for what it does not see."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    lengths = [130, 200, 1, 300]
+    cache = _cache(lengths, hkv, d, block, page, dtype, 110)
+    q = _queries(sum(new), hq, d, dtype, 111)
+    at = torch.tensor([0] + new).cumsum(0).tolist()
+    args = dict(token_offsets=None if max(new) == 1 else _ints(at), max_tokens=max(new), return_lse=True)
+    for scores in (dict(), dict(softcap=20.0, slopes=torch.full((hq,), 0.1, device=DEV))):
+        got = paged_attention.attention(q, cache, _ints(lengths), **args, **scores)
+        held = cache.k_pages, cache.v_pages
+        cache.k_pages, cache.v_pages = held[0].nan_to_num(0.0), held[1].nan_to_num(0.0)
+        want = paged_attention.attention(q, cache, _ints(lengths), **args, **scores)
+        cache.k_pages, cache.v_pages = held
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", ROOMY[:3])
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_unfilled_pages_behind_a_prefix(dtype, shape, new):
+    """The pages behind a shared prefix that ends inside a tile of keys belong to request 0 alone, filled or not."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    prefix = 9 * block
+    lengths = [prefix + new, prefix + new + 3]
+    cache = _cache(lengths, hkv, d, block, page, dtype, 112, shared=prefix, room=2 * block)
+    q = _queries(2 * new, hq, d, dtype, 113)
+    args = dict(token_offsets=None if new == 1 else _ints([0, new, 2 * new]), max_tokens=new, return_lse=True)
+    got = paged_attention.shared_prefix_attention(q, cache, _ints(lengths), prefix, **args)
+    cache.k_pages, cache.v_pages = cache.k_pages.nan_to_num(0.0), cache.v_pages.nan_to_num(0.0)
+    want = paged_attention.shared_prefix_attention(q, cache, _ints(lengths), prefix, **args)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", ROOMY[:3])
+@pytest.mark.parametrize("new", [1, 4, 150])
+def test_unassigned_table_entries(dtype, shape, new):
+    """Table entries behind the last token or below every window are not looked at: no status, the same bits."""
+    from strict_topk_overlap_b200 import _lib, paged_attention
+    hq, hkv, d, block, page = shape
+    length, window = 420, 200
+    cache = _cache([length], hkv, d, block, page, dtype, 114, room=2 * block)
+    q = _queries(new, hq, d, dtype, 115)
+    lo = [p + 1 - window for p in range(length - new, length)]
+    args = dict(token_offsets=None if new == 1 else _ints([0, new]), max_tokens=new, return_lse=True, kv_lo=_ints(lo))
+    want = paged_attention.attention(q, cache, _ints([length]), **args)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cache.page_table[-(-length // page):] = -1
+    cache.page_table[:lo[0] // page] = -1
+    try:
+        _lib.set_status_tensor(status)
+        got = paged_attention.attention(q, cache, _ints([length]), **args)
+    finally:
+        _lib.set_status_tensor(None)
+    assert int(status) == 0
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
