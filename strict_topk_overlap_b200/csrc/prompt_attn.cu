@@ -183,14 +183,17 @@ __device__ __forceinline__ void tmem_loaded(uint32_t* r) {
                       "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 // Whether x holds for any thread of a group of `count` that meets on named
-// barrier `id`.
+// barrier `id`. What one half's threads know of finished products, and their
+// own accesses to tensor memory, are ordered before the other's after it.
 __device__ __forceinline__ bool group_any(int id, int count, bool x) {
   uint32_t r;
+  fence_before();
   asm volatile(
       "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n barrier.cta.red.or.pred p, %2, %3, q;\n selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(r)
       : "r"(static_cast<uint32_t>(x)), "r"(id), "r"(count)
       : "memory");
+  fence_after();
   return r != 0;
 }
 // The value of lane 0, known to the compiler as the warp's.
@@ -686,8 +689,10 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     // The two warps of the same rows: neither's next P is announced before both have been here.
     auto meet = [&]() {
       uint64_t* bar = &sh.pair[qt * 4 + (warp & 3)];
+      fence_before();
       mbar_arrive(bar);
       ok = warp_wait(bar, meetings & 1, a.status) && ok;
+      fence_after();  // the other's products and its accesses to O come before ours from here on
       ++meetings;
     };
     // P of the thread's keys from k0 on, over S, and their sum. WHOLE: every
