@@ -273,6 +273,7 @@ token_attn_kernel(const PagedAttnArgs a, int requests, int most_rows, int* prefi
           if (k0 + y < q.kmin || k0 + y >= q.kmax)
             *reinterpret_cast<uint4*>(v + x % P::kHalves * 2048 + y * 128 + x / P::kHalves % 8 * 16) = make_uint4(0, 0, 0, 0);
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next copy
         __syncwarp();
       }
       // ---- S = Q K^T: two tiles of 8 keys
