@@ -923,6 +923,12 @@ struct AttnPhase {
   int requests, most_rows;
   size_t states, bytes;  // partial states; their bytes (and the unit counts'), a multiple of 16
 };
+
+// Bytes of the states' sums of values; the (m, l) pairs behind them need their
+// own alignment whatever the head size and the number of states.
+size_t state_sum_bytes(size_t states, int d) {
+  return (states * d * sizeof(float) + 15) & ~static_cast<size_t>(15);
+}
 struct AttnPlan {
   AttnPhase phase[2];
   int phases;
@@ -967,7 +973,7 @@ AttnPhase plan_phase(const stk_kv* kv, int R, int T, int hq, bool offsets, bool 
   if (p.kind == kAttnTokens) {
     p.nsplit = 8 * sms;  // two CTAs of four warps per SM
     p.states = (static_cast<size_t>(p.nsplit) + static_cast<size_t>(p.requests) * hkv) * p.most_rows;
-    p.bytes = p.states * (kv->d + 2) * sizeof(float) + (p.requests + 1) * sizeof(int);
+    p.bytes = state_sum_bytes(p.states, kv->d) + p.states * sizeof(float2) + (p.requests + 1) * sizeof(int);
   } else {
     const bool prompt = p.kind == kAttnPrompt;
     const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared,
@@ -984,7 +990,7 @@ AttnPhase plan_phase(const stk_kv* kv, int R, int T, int hq, bool offsets, bool 
     }
     p.nsplit = static_cast<int>(n < 1 ? 1 : n);
     p.states = static_cast<size_t>(p.nsplit) * T * hq;
-    p.bytes = p.states * (kv->d + 2) * sizeof(float);
+    p.bytes = state_sum_bytes(p.states, kv->d) + p.states * sizeof(float2);
   }
   p.bytes = (p.bytes + 15) & ~static_cast<size_t>(15);
   return p;
@@ -1077,7 +1083,7 @@ extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, l
     int* prefix_units = nullptr;
     if (p.join) {
       a.part_o = reinterpret_cast<float*>(at);
-      a.part_ml = reinterpret_cast<float2*>(a.part_o + ph.states * kv->d);
+      a.part_ml = reinterpret_cast<float2*>(at + state_sum_bytes(ph.states, kv->d));
       if (ph.kind == kAttnTokens) prefix_units = reinterpret_cast<int*>(a.part_ml + ph.states);
       at += ph.bytes;
       j.src[i] = {a.part_ml, a.part_o, ph.nsplit, prefix_units, ph.nsplit, ph.most_rows, ph.requests, ph.shared};

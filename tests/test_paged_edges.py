@@ -8,7 +8,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_paged_attention import DEV, TYPES, _cache, _compare_equal, _ints
+from test_paged_attention import DEV, TYPES, _cache, _compare, _compare_equal, _ints
 
 gpu = pytest.mark.gpu
 TILED = [(8, 2, 128, 32, 16), (4, 4, 64, 32, 16)]  # hq, hkv, d, block, page that the tensor-core kernels take
@@ -236,3 +236,22 @@ def test_unassigned_table_entries(dtype, shape, new):
         _lib.set_status_tensor(None)
     assert int(status) == 0
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1, 33, 16, 16), (3, 1, 5, 16, 8), (3, 3, 81, 32, 16), (1, 1, 1, 16, 16)])
+@pytest.mark.parametrize("new,prefix", [(1, 0), (3, 0), (1, 64)])
+def test_odd_heads_in_an_odd_number_of_parts(dtype, shape, new, prefix):
+    """Partial states of an odd number of odd rows: what lies behind them in the workspace keeps its alignment."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    for length in (64 + 70, 190, 300):  # 3 and 5 parts of 64 keys
+        cache = _cache([length], hkv, d, block, page, dtype, 116, shared=prefix)
+        q = _queries(new, hq, d, dtype, 117)
+        args = dict(token_offsets=None if new == 1 else _ints([0, new]), max_tokens=new, return_lse=True)
+        if prefix:
+            out, lse = paged_attention.shared_prefix_attention(q, cache, _ints([length]), prefix, **args)
+        else:
+            out, lse = paged_attention.attention(q, cache, _ints([length]), **args)
+        _compare(q, cache, [length], [new], None, None, out, lse, 0.0, None, d ** -0.5)
