@@ -789,7 +789,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         // bf16's range and relative precision do not mind. The two halves of a
         // row are two independent chains of S, P and O that meet only where
         // the frame moves. A row whose scores run ahead of its frame by more
-        // than 2^127 overflows and is recomputed like those below.
+        // than 2^100 at the end is recomputed like those below.
         if (kOwnO) {
           const float frame = level + half_bias(i);
           const bool grow = grows(frame);
@@ -873,11 +873,12 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     const long long orow = static_cast<long long>(t.t0 + tok) * a.hq + head;
     const long long prow = static_cast<long long>(split) * a.T * a.hq + orow;
     const float inv = empty || a.part_ml ? 1.f : 1.f / l;
-    // The frame was left behind, or ahead, by more than FP32's range; or scores
-    // are NaN, perhaps all that the row sees here (which leaves no maximum).
-    // (2^-100: below what a frame that follows leaves.)
+    // The frame was left behind, or ahead, by so much that sums of large values
+    // may have left FP32's range (2^100; a frame that follows stays far inside);
+    // or scores are NaN, perhaps all that the row sees here (which leaves no
+    // maximum). The row's state is then taken anew in a frame of its own.
     const bool sees = have && max(rk.lo, ta * kTileN) < min(rk.hi, tb * kTileN);
-    const bool over = sees && (empty || nan || !(l <= 3.0e38f && l >= 7.9e-31f));
+    const bool over = sees && (empty || nan || !(l <= 1.3e30f && l >= 7.9e-31f));
     bool redo_row = over;
     if (ok && !(kOwnO && half)) {
       // 128 bytes a row at a time through this warp's share of the Q tile's

@@ -255,3 +255,25 @@ def test_odd_heads_in_an_odd_number_of_parts(dtype, shape, new, prefix):
         else:
             out, lse = paged_attention.attention(q, cache, _ints([length]), **args)
         _compare(q, cache, [length], [new], None, None, out, lse, 0.0, None, d ** -0.5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", TILED)
+@pytest.mark.parametrize("length,new", [(700, 40), (20000, 40), (20000, 300)])
+@pytest.mark.parametrize("jump", [60.0, 80.0])
+def test_scores_that_jump_under_large_values(dtype, shape, length, new, jump):
+    """Scores that leave their frame far behind at the end of a part, times values that take the sum beyond FP32 there."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    cache = _cache([length], hkv, d, block, page, dtype, 118)
+    at = _at(cache, 0, _span(0, length))
+    cache.k_pages[at[0], :, at[1]] *= 0.25
+    along = torch.where(_span(0, length) >= length - new - 60, jump, 0.0) * d ** 0.5 / 16
+    cache.k_pages[at[0], :, at[1], 0] = along.to(dtype)[:, None].expand(-1, hkv)
+    cache.v_pages *= 3e4 if dtype == torch.float16 else 1e7
+    q = 0.25 * _queries(new, hq, d, dtype, 119)
+    q[..., 0] = 16.0
+    out, lse = paged_attention.attention(q, cache, _ints([length]), token_offsets=_ints([0, new]), max_tokens=new,
+                                         return_lse=True)
+    _compare(q, cache, [length], [new], None, None, out, lse, 0.0, None, d ** -0.5)
