@@ -191,7 +191,10 @@ def id_is64(t: torch.Tensor) -> int:
 
 def stream_of(t: torch.Tensor) -> int:
     """Raw handle of the current stream of t's device (without a Stream object: a tenth of the host time)."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+    index = t.get_device()
+    if index < 0:
+        raise ValueError("expected tensors on a CUDA device; there is no CPU fallback")
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -66,12 +66,20 @@ class PagedKVCache:
                            b=self.block_size, d=self.dim)
 
     def packed_kv(self, hkv, dim) -> bytes:
-        """``kv()`` as the packed bytes that the paged token calls take."""
-        k, v = self.k_pages, self.v_pages
-        if k.dtype is not v.dtype:
+        """``kv()`` as the packed bytes that the paged token calls take, its tensors checked."""
+        k, v, table, offsets = self.k_pages, self.v_pages, self.page_table, self.block_offsets
+        index = k.get_device()
+        if index < 0:
+            raise ValueError("the cache must be on a CUDA device; there is no CPU fallback")
+        if v.dtype is not k.dtype:
             raise ValueError("K and V must share a dtype")
-        return L.PACK_KV(k.data_ptr(), v.data_ptr(), L.dtype_code(k), hkv, 0, self.block_size, dim,
-                         self.page_table.data_ptr(), self.block_offsets.data_ptr(), self.page_size, 0)
+        if v.shape != k.shape or v.get_device() != index or not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("K and V pages must be contiguous, of one shape and on one device")
+        for x in (table, offsets):
+            if x.dtype is not torch.int32 or x.get_device() != index or not x.is_contiguous():
+                raise ValueError("page_table and block_offsets must be contiguous int32 on the pages' device")
+        return L.PACK_KV(k.data_ptr(), v.data_ptr(), L.dtype_code(k), hkv, 0, self.block_size, dim, table.data_ptr(),
+                         offsets.data_ptr(), self.page_size, 0)
 
 
 def build_paged_cache(ks, vs, page_size, *, generator=None, device=None) -> PagedKVCache:

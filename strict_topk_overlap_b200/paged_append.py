@@ -117,6 +117,7 @@ def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=N
     pool = cache.k_pages
     pages, hkv, _, d = pool.shape
     dtype, index = pool.dtype, pool.get_device()
+    kv = cache.packed_kv(hkv, d)
     requests, blocks = cache.block_offsets.shape[0] - 1, cache.lo.shape[1]
     t = k.shape[0]
     kp, kt, kh = _rows(k, (t, hkv, d), "k", dtype, index)
@@ -134,8 +135,14 @@ def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=N
             raise ValueError("q_out must be contiguous, of q's shape, dtype and device")
         out = q_out.data_ptr()
     turn, at = _rotary(rotary, positions, t, index)
-    lo, hi = (cache.lo.data_ptr(), cache.hi.data_ptr()) if blocks else (None, None)
-    rc = L.load().stk_append_tokens(cache.packed_kv(hkv, d), pages, requests, blocks or 1, t, kp, kt, kh, vp, vt, vh, qp,
+    lo = hi = None
+    if blocks:
+        for x in (cache.lo, cache.hi):
+            if x.dtype is not torch.float32 or x.shape != (hkv, blocks, d) or x.get_device() != index or \
+                    not x.is_contiguous():
+                raise ValueError("lo and hi must be contiguous FP32 [Hkv, blocks, D] on the cache's device")
+        lo, hi = cache.lo.data_ptr(), cache.hi.data_ptr()
+    rc = L.load().stk_append_tokens(kv, pages, requests, blocks or 1, t, kp, kt, kh, vp, vt, vh, qp,
                                     qt, qh, hq, out, before, offsets, at, turn, lo, hi, L.status_ptr(),
                                     L.stream_of(pool))
     if rc:

@@ -54,6 +54,7 @@ def _attend(q, cache, lengths, token_offsets, max_tokens, kv_lo, kv_hi, softcap,
     pool = cache.k_pages
     pages, hkv, _, d = pool.shape
     dtype, index = pool.dtype, pool.get_device()
+    kv = cache.packed_kv(hkv, d)
     requests = cache.block_offsets.shape[0] - 1
     t, hq = _heads(q, hkv)
     qp, qt, qh = _rows(q, (t, hq, d), "q", dtype, index)
@@ -80,10 +81,12 @@ def _attend(q, cache, lengths, token_offsets, max_tokens, kv_lo, kv_hi, softcap,
         if need:
             workspace = q.new_empty((need,), dtype=torch.uint8)
     else:
+        if workspace.get_device() != index:
+            raise ValueError("workspace must be on the cache's device")
         need = workspace.numel()
     out = q.new_empty((t, hq, d))
     lse = q.new_empty((t, hq), dtype=torch.float32) if return_lse else None
-    rc = L.load().stk_paged_attention(cache.packed_kv(hkv, d), pages, qp, qt, qh, requests, t, hq, held, offsets, most,
+    rc = L.load().stk_paged_attention(kv, pages, qp, qt, qh, requests, t, hq, held, offsets, most,
                                       longest, prefix, options, out.data_ptr(), L.ptr(lse), L.ptr(workspace), need,
                                       L.status_ptr(), L.stream_of(q))
     if rc:
