@@ -446,8 +446,9 @@ typedef struct stk_rotary {
  * and values [T, hkv, d] are written to their page slots and the bounds lo /
  * hi of their blocks (NULL: none kept) are folded over the stored keys; a
  * block's first token resets its bounds. rotary NULL: no rotation. Inputs
- * have the cache's type and unit stride along d; strides are in elements. A
- * token beyond its request's blocks is not written and a position outside
+ * have the cache's type and unit stride along d; strides are in elements.
+ * Tokens from token_offsets[R] on (padding) are stored nowhere, their queries
+ * turned by position 0. A token beyond its request's blocks is not written and a position outside
  * the table is taken as 0; both are reported in status. New: the reference
  * starts from a filled cache. */
 STK_API int stk_append_tokens(const stk_kv* kv, int pages, int R, int total_blocks, int T, const void* k_new,
@@ -483,8 +484,10 @@ STK_API size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int 
  * log-sum-exp of the row's scores (-inf there). prefix > 0: the first prefix
  * tokens (whole pages) of every request are the same pages (those of request
  * 0's table are read), attended once for all requests' tokens and joined
- * with each request's own rest. Offsets past T and requests with more tokens
- * than max_tokens are cut and reported in status (STK_STATUS_SHAPE_OVERFLOW). New: the reference attends block lists only. */
+ * with each request's own rest. Tokens from token_offsets[R] on (padding) see
+ * no key. Offsets that do not begin at 0 or go past T and requests with more
+ * tokens than max_tokens are cut and reported in status
+ * (STK_STATUS_SHAPE_OVERFLOW). New: the reference attends block lists only. */
 STK_API int stk_paged_attention(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
                                 long long q_head_stride, int R, int T, int hq, const int32_t* lengths,
                                 const int32_t* token_offsets, int max_tokens, int max_length, int prefix,

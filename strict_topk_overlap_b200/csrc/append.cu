@@ -34,7 +34,8 @@
 //
 // Which (request, block) an item is follows from token_offsets on the device:
 // request r's blocks start at slot offs[r] / B + 2 r, which leaves room for
-// the ceil of its tokens wherever its first block begins.
+// the ceil of its tokens wherever its first block begins; padding's "blocks"
+// come last.
 
 #include <type_traits>
 
@@ -330,7 +331,7 @@ append_kernel(AppendArgs a, int tile_tokens, int chunks, int items) {
   const int last = min(items, static_cast<int>(blockIdx.x + 1) * per);
   int at = -1, staged = -1;
   int r = 0, t0 = 0, n = 0, len = 0, j = 0, begin = 0, end = 0, base = 0;
-  bool room = false;
+  bool room = false, padding = false;
   const int* table = nullptr;
   for (int item = blockIdx.x * per; item < last; ++item) {
     const int slot = item / chunks, chunk = item - slot * chunks;
@@ -341,15 +342,16 @@ append_kernel(AppendArgs a, int tile_tokens, int chunks, int items) {
         r = t0 = slot;
         n = 1;
       } else {
-        r = request_of_slot(a.token_offsets, a.R, 1, B, 2, slot, lane);
-        const int2 tn = new_tokens(a.token_offsets, r, a.T, a.status);
+        r = request_of_slot(a.token_offsets, a.R + 1, 1, B, 2, slot, lane);
+        const int2 tn = new_tokens(a.token_offsets, r, a.R, a.T, a.status);
         t0 = tn.x;
         n = tn.y;
         f = slot - t0 / B - 2 * r;
       }
-      len = a.lengths[r];
+      padding = r >= a.R;  // tokens of no request: stored nowhere, their q turned by position 0
+      len = padding ? 0 : a.lengths[r];
       base = a.L.block_offsets[r];
-      const int blocks = a.L.block_offsets[r + 1] - base;
+      const int blocks = padding ? 0 : a.L.block_offsets[r + 1] - base;
       begin = end = 0;
       if (n > 0 && len >= 0 && f >= 0) {
         j = len / B + f;  // block of the request
@@ -357,7 +359,7 @@ append_kernel(AppendArgs a, int tile_tokens, int chunks, int items) {
         end = static_cast<int>(min(static_cast<long long>(len) + n, (j + 1ll) * B));
       }
       room = j < blocks;
-      if (tid == 0 && n > 0 && (len < 0 || (begin < end && !room))) report(a.status, kStatusBadLength);
+      if (tid == 0 && n > 0 && !padding && (len < 0 || (begin < end && !room))) report(a.status, kStatusBadLength);
       table = a.L.page_table + (static_cast<long long>(base) + j) * (B / ps);
     }
     for (int tile = begin; tile < end; tile += tile_tokens) {
@@ -375,8 +377,8 @@ append_kernel(AppendArgs a, int tile_tokens, int chunks, int items) {
         }
         for (int tt = warp; tt < t.nt; tt += kAppendWarps) {
           for (int p = lane; p < t.pairs; p += 32) {
-            int pos = tile + tt;
-            if (a.positions) {
+            int pos = padding ? 0 : tile + tt;
+            if (a.positions && !padding) {
               const int ax = a.axis ? a.axis[p] : 0;
               pos = ax < a.axes ? a.positions[static_cast<long long>(ax) * a.T + token + tt] : -1;
             }
@@ -418,7 +420,7 @@ append_kernel(AppendArgs a, int tile_tokens, int chunks, int items) {
 
 template <typename T, int VEC>
 static int launch_append_t(const AppendArgs& a, int sms, cudaStream_t stream) {
-  const int slots = a.token_offsets ? a.T / a.L.b + 2 * a.R : a.R;
+  const int slots = a.token_offsets ? a.T / a.L.b + 2 * a.R + 1 : a.R;
   const int heads = (a.q ? a.hq : 0) + 2 * a.L.hkv;
   // 32 tokens of tables per tile up to 128 pairs, 8 for wider heads: at most 32 KB.
   const int pairs = a.cos ? a.pairs : 0;

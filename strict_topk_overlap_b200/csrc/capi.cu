@@ -976,8 +976,8 @@ AttnPhase plan_phase(const stk_kv* kv, int R, int T, int hq, bool offsets, bool 
     p.bytes = state_sum_bytes(p.states, kv->d) + p.states * sizeof(float2) + (p.requests + 1) * sizeof(int);
   } else {
     const bool prompt = p.kind == kAttnPrompt;
-    const long long tiles = static_cast<long long>(row_tile_slots(R, T, G, offsets, shared,
-                                                                prompt ? prompt_tile_rows(kv->d) : 16)) * hkv;
+    const int slots = row_tile_slots(R, T, G, offsets, shared, prompt ? prompt_tile_rows(kv->d) : 16);
+    const long long tiles = static_cast<long long>(offsets && !shared ? slots - 1 : slots) * hkv;  // without padding's slot
     long long n;
     if (prompt) {
       n = prompt_splits(tiles, keys, kv->d, static_cast<double>(T) * hq, prompt_ctas_per_sm(kv->d) * sms);

@@ -5,6 +5,8 @@
 // tokens token_offsets[r] .. token_offsets[r + 1] (without token_offsets,
 // one token each). A token's query heads of one KV head are G consecutive
 // "rows"; request r has n_r * G rows per KV head, row = token * G + head.
+// Tokens from token_offsets[R] on (padding, as a captured graph has) belong to
+// no request: they are the tokens of a request R that holds nothing.
 #pragma once
 
 #include "internal.cuh"
@@ -75,20 +77,21 @@ __device__ __forceinline__ int request_of_slot(const int* offs, int R, int mul, 
   return max(count - 1, 0);
 }
 
-// First packed token and number of new tokens of request r. Offsets that run
-// backwards or past the T tokens are cut to them and reported.
-__device__ __forceinline__ int2 new_tokens(const int* offs, int r, int T, int* status) {
+// First packed token and number of new tokens of request r < R, or of the
+// padding, r = R. Offsets that do not start at 0, run backwards or go past the
+// T tokens are cut to them and reported.
+__device__ __forceinline__ int2 new_tokens(const int* offs, int r, int R, int T, int* status) {
   if (offs == nullptr) return make_int2(r, 1);
-  const int a = offs[r], b = offs[r + 1];
-  if (a < 0 || b < a || b > T) report(status, kStatusShapeOverflow);
+  const int a = offs[r], b = r < R ? offs[r + 1] : max(a, T);
+  if (r < R && (a < 0 || b < a || b > T || (r == 0 && a > 0))) report(status, kStatusShapeOverflow);
   const int first = min(max(a, 0), T);
   return make_int2(first, max(0, min(b, T) - first));
 }
 
-// The last request that starts at or before a packed token.
+// The last request that starts at or before a packed token, R for padding.
 __device__ __forceinline__ int request_of_token(const int* offs, int R, int token) {
   if (offs == nullptr) return token;
-  int r = 0, end = R;
+  int r = 0, end = R + 1;
   while (end - r > 1) {
     const int mid = (r + end) >> 1;
     if (offs[mid] <= token) r = mid; else end = mid;
@@ -105,6 +108,7 @@ struct RowTile {
 
 // Tokens of request r in the cache, at most as many as its blocks hold.
 __device__ __forceinline__ int cached_tokens(const PagedAttnArgs& a, int r, int n) {
+  if (r >= a.R) return 0;  // padding
   const int len = a.lengths[r], room = request_blocks(a.L, r) * a.L.b;
   if (n > 0 && (len > room || len < n)) report(a.status, kStatusBadLength);
   return min(len, room);
@@ -127,8 +131,8 @@ __device__ __forceinline__ RowTile row_tile(const PagedAttnArgs& a, int slot, in
     t.t0 = t.r;
     t.n = 1;
   } else {
-    t.r = request_of_slot(a.token_offsets, a.R, a.G, M, 1, slot, lane);
-    const int2 tn = new_tokens(a.token_offsets, t.r, a.T, a.status);
+    t.r = request_of_slot(a.token_offsets, a.R + 1, a.G, M, 1, slot, lane);
+    const int2 tn = new_tokens(a.token_offsets, t.r, a.R, a.T, a.status);
     t.t0 = tn.x;
     t.n = tn.y;
     f = slot - static_cast<int>(static_cast<long long>(t.t0) * a.G / M) - t.r;
@@ -141,7 +145,7 @@ __device__ __forceinline__ RowTile row_tile(const PagedAttnArgs& a, int slot, in
 
 inline int row_tile_slots(int R, int T, int G, bool offsets, bool shared, int M) {
   if (shared) return static_cast<int>((static_cast<long long>(T) * G + M - 1) / M);
-  return offsets ? static_cast<int>(static_cast<long long>(T) * G / M) + R : R * ((G + M - 1) / M);
+  return offsets ? static_cast<int>(static_cast<long long>(T) * G / M) + R + 1 : R * ((G + M - 1) / M);
 }
 
 // Keys lo <= j < hi that token i of a tile's request sees inside the call's
@@ -163,7 +167,7 @@ __device__ __forceinline__ RowKeys row_keys(const PagedAttnArgs& a, const RowTil
     k.pos = t.len - t.n + i;
   } else {
     const int r = request_of_token(a.token_offsets, a.R, token);
-    const int2 tn = new_tokens(a.token_offsets, r, a.T, a.status);
+    const int2 tn = new_tokens(a.token_offsets, r, a.R, a.T, a.status);
     len = cached_tokens(a, r, tn.y);
     k.pos = len - (tn.x + tn.y - token);
   }

@@ -321,8 +321,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(JoinArgs a) {
       const int local = (token - first) * a.G + head - h * a.G;  // row of the request's tile
       const long long total = static_cast<long long>(p.prefix[p.requests]) * hkv;
       const long long per = (total + p.streams - 1) / p.streams;
-      const int units = p.prefix[r + 1] - p.prefix[r];
-      const long long u0 = static_cast<long long>(p.prefix[r]) * hkv + static_cast<long long>(h) * units;
+      const int before = p.prefix[r], units = r < p.requests ? p.prefix[r + 1] - before : 0;  // padding has none
+      const long long u0 = static_cast<long long>(before) * hkv + static_cast<long long>(h) * units;
       const int c0 = units ? static_cast<int>(u0 / per) : 0;
       const bool written = units > 0 && local >= 0 && local < p.most_rows;
       parts[k] = written ? static_cast<int>((u0 + units - 1) / per) - c0 + 1 : 0;

@@ -85,7 +85,7 @@ __device__ __forceinline__ Request request_at(const PagedAttnArgs& a, int r, int
   Request q;
   q.t.r = a.shared ? 0 : r;
   q.t.row0 = 0;
-  const int2 tn = a.shared ? make_int2(0, a.T) : new_tokens(a.token_offsets, r, a.T, a.status);
+  const int2 tn = a.shared ? make_int2(0, a.T) : new_tokens(a.token_offsets, r, a.R, a.T, a.status);
   q.t.t0 = tn.x;
   q.t.n = tn.y;
   q.t.rows = min(q.t.n * a.G, most_rows);

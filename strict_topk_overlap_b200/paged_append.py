@@ -112,7 +112,8 @@ def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=N
     by ``positions`` (int32 [T], or [axes, T]; None: the token's place). k, v
     and q may be slices of one projection's output (any token and head
     strides). Updates the pages and, where the cache keeps them, the blocks'
-    lo / hi; returns the rotated q [T, Hq, D] (``q_out``, which may be q
+    lo / hi (tokens from token_offsets[R] on are padding and stored nowhere);
+    returns the rotated q [T, Hq, D] (``q_out``, which may be q
     itself), or None without q."""
     pool = cache.k_pages
     pages, hkv, _, d = pool.shape

@@ -99,8 +99,8 @@ def attention(q, cache: PagedKVCache, lengths, *, token_offsets=None, max_tokens
     """Attention of packed tokens q [T, Hq, D], the last ones of their requests,
     over the ``lengths[r]`` (int32 [R]) tokens that the cache holds of each:
     request r's tokens are token_offsets[r] .. token_offsets[r + 1] (int32
-    [R + 1]; None: one token per request), at most ``max_tokens`` of them
-    (None: T). ``kv_lo`` / ``kv_hi`` int32 [T] bound each token's keys (None:
+    [R + 1]; None: one token per request; tokens from token_offsets[R] on are
+    padding and get zeros), at most ``max_tokens`` of them (None: T). ``kv_lo`` / ``kv_hi`` int32 [T] bound each token's keys (None:
     causal), ``slopes`` FP32 [Hq]. Returns [T, Hq, D] in q's dtype and, with
     ``return_lse``, the log-sum-exp of each row's scores, FP32 [T, Hq]."""
     return _attend(q, cache, lengths, token_offsets, max_tokens, kv_lo, kv_hi, softcap, slopes, scale, return_lse,

@@ -277,3 +277,90 @@ def test_scores_that_jump_under_large_values(dtype, shape, length, new, jump):
     out, lse = paged_attention.attention(q, cache, _ints([length]), token_offsets=_ints([0, new]), max_tokens=new,
                                          return_lse=True)
     _compare(q, cache, [length], [new], None, None, out, lse, 0.0, None, d ** -0.5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", FORMS + [(24, 2, 128, 32, 16)])
+@pytest.mark.parametrize("new,most", [([1, 1, 1], 1), ([2, 0, 1], 2), ([40, 3, 1], 40), ([150, 130, 0], 150)])
+@pytest.mark.parametrize("pad", [1, 5, 300])
+@pytest.mark.parametrize("prefix", [0, 96])
+def test_padding_gets_zeros(dtype, shape, new, most, pad, prefix):
+    """Tokens behind the last request's, as a padded graph has: zeros in the output, -inf in the log-sum-exp, no status;
+    nothing else changes."""
+    from strict_topk_overlap_b200 import _lib, paged_attention
+    hq, hkv, d, block, page = shape
+    prefix = prefix // block * block
+    lengths = [prefix + max(1, n) + e for n, e in zip(new, (150, 20, 3))]
+    t = sum(new)
+    cache = _cache(lengths, hkv, d, block, page, dtype, 120, shared=prefix)
+    q = _queries(t + pad, hq, d, dtype, 121)
+    at = _ints(torch.tensor([0] + new).cumsum(0).tolist())
+    args = dict(token_offsets=at, max_tokens=most, return_lse=True)
+    ws = paged_attention.attention_workspace(cache, t + pad, hq, token_offsets=at, max_tokens=most, prefix=prefix)
+    ws.fill_(255)
+    stale = torch.full((t + pad, hq, d), float("nan"), dtype=dtype, device=DEV)  # what the output's memory held
+    del stale
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    try:
+        _lib.set_status_tensor(status)
+        if prefix:
+            out, lse = paged_attention.shared_prefix_attention(q, cache, _ints(lengths), prefix, workspace=ws, **args)
+        else:
+            out, lse = paged_attention.attention(q, cache, _ints(lengths), workspace=ws, **args)
+    finally:
+        _lib.set_status_tensor(None)
+    assert int(status) == 0
+    assert not bool(out[t:].any()) and bool((lse[t:] == float("-inf")).all())
+    _compare(q[:t], cache, lengths, new, None, None, out[:t], lse[:t], 0.0, None, d ** -0.5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pad", [1, 70])
+def test_padding_is_not_appended(dtype, pad):
+    """Padding's keys and values go nowhere, whatever its positions hold; its queries are turned by position 0."""
+    from strict_topk_overlap_b200 import _lib, paged_append, rotary
+    past, new, hq, hkv, d = [5, 40], [30, 2], 4, 2, 64
+    g = torch.Generator(DEV).manual_seed(122)
+    t = sum(new) + pad
+    qkv = torch.randn((t, hq + 2 * hkv, d), generator=g, device=DEV).to(dtype)
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+    turn = rotary.build_rotary(100, d)
+    positions = torch.cat([_span(5, 35), _span(40, 42), torch.full((pad,), -9, device=DEV)]).to(torch.int32)
+    caches = [paged_append.empty_paged_cache([64, 64], hkv, d, 32, 16, dtype=dtype,
+                                             generator=torch.Generator().manual_seed(1)) for _ in range(2)]
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = torch.full((t, hq, d), float("nan"), dtype=dtype, device=DEV)
+    more = dict(token_offsets=_ints([0, 30, 32]), rotary=turn)
+    try:
+        _lib.set_status_tensor(status)
+        paged_append.append_tokens(caches[0], k, v, _ints(past), q=q, q_out=out, positions=positions, **more)
+    finally:
+        _lib.set_status_tensor(None)
+    n = sum(new)
+    want = paged_append.append_tokens(caches[1], k[:n], v[:n], _ints(past), q=q[:n], positions=positions[:n].contiguous(), **more)
+    assert int(status) == 0
+    assert torch.equal(out[:n], want) and torch.equal(out[n:], q[n:])
+    for name in ("k_pages", "v_pages", "lo", "hi"):
+        assert torch.equal(getattr(caches[0], name), getattr(caches[1], name))
+
+
+@gpu
+def test_offsets_that_do_not_begin_at_zero_are_reported():
+    from strict_topk_overlap_b200 import _lib, paged_append, paged_attention
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cache = _cache([200, 300], 2, 64, 32, 16, torch.bfloat16, 123)
+    try:
+        _lib.set_status_tensor(status)
+        for new in (3, 130):
+            q = _queries(2 * new, 8, 64, torch.bfloat16, 124)
+            paged_attention.attention(q, cache, _ints([200, 300]), token_offsets=_ints([1, new, 2 * new]), max_tokens=new)
+            assert int(status) == 3
+            status.zero_()
+            kv = q[:, :2].contiguous()
+            paged_append.append_tokens(cache, kv, kv, _ints([10, 20]), token_offsets=_ints([1, new, 2 * new]))
+            assert int(status) == 3
+            status.zero_()
+    finally:
+        _lib.set_status_tensor(None)
