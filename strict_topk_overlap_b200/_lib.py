@@ -197,6 +197,14 @@ def stream_of(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def on_device(index: int, call, *args) -> int:
+    """``call(*args)`` with device ``index`` current: the library launches on the current one."""
+    if torch._C._cuda_getDevice() == index:
+        return call(*args)
+    with torch.cuda.device(index):
+        return call(*args)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

@@ -143,9 +143,8 @@ def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=N
                     not x.is_contiguous():
                 raise ValueError("lo and hi must be contiguous FP32 [Hkv, blocks, D] on the cache's device")
         lo, hi = cache.lo.data_ptr(), cache.hi.data_ptr()
-    rc = L.load().stk_append_tokens(kv, pages, requests, blocks or 1, t, kp, kt, kh, vp, vt, vh, qp,
-                                    qt, qh, hq, out, before, offsets, at, turn, lo, hi, L.status_ptr(),
-                                    L.stream_of(pool))
+    rc = L.on_device(index, L.load().stk_append_tokens, kv, pages, requests, blocks or 1, t, kp, kt, kh, vp, vt, vh, qp,
+                     qt, qh, hq, out, before, offsets, at, turn, lo, hi, L.status_ptr(), L.stream_of(pool))
     if rc:
         L.check(rc, "append_tokens")
     return q_out if q is not None else None

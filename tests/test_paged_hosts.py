@@ -96,3 +96,34 @@ def test_streams_of_host_tensors_are_refused():
     k, lo = torch.zeros((2, 3, 8, 16)), torch.zeros((2, 3, 16))
     with pytest.raises(ValueError, match="CUDA"):
         metadata.append_token(k, k.clone(), lo, lo.clone(), k[:, 0, 0], k[:, 0, 0], 4)
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_launches_happen_on_the_tensors_device(monkeypatch, current):
+    """Two devices in one process: the library launches on the current one, which has to be the tensors'."""
+    state, seen = {"device": current}, []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, state["device"] = state["device"], self.index
+
+        def __exit__(self, *error):
+            state["device"] = self.before
+
+    class Launches(Untouched):
+        def __getattr__(self, name):
+            def call(*args):
+                seen.append(state["device"])
+                return 0
+            return call
+
+    monkeypatch.setattr(_lib, "load", lambda path=None: Launches())
+    monkeypatch.setattr(_lib, "stream_of", lambda t: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state["device"], raising=False)
+    for call in _calls(_cache(_on_device), _on_device):
+        call()
+    assert seen == [0, 0, 0] and state["device"] == current
