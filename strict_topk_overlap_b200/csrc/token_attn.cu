@@ -37,6 +37,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kUnit = 16;  // keys of a unit
+constexpr int kMostRequests = 16384;
 
 template <int D>
 struct TokenPlan {
@@ -408,7 +409,10 @@ int launch_t(const PagedAttnArgs& a, int streams, int most_rows, int* prefix, co
   const int requests = a.shared ? 1 : a.R;
   auto kern = token_attn_kernel<T, D>;
   const int smem = TokenPlan<D>::kBytes + (requests + 1) * 4;
-  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // The limit belongs to the kernel, not to this call: always that of the
+  // largest batch, so that no other thread's call lowers it before the launch.
+  constexpr int kMost = TokenPlan<D>::kBytes + (kMostRequests + 1) * 4;
+  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
   if (rc) return rc;
   if (a.chained)
     return launch_pdl(kern, dim3(streams / kWarps), dim3(kWarps * 32), smem, stream, 0, a, requests, most_rows, prefix, km,
@@ -423,7 +427,7 @@ bool token_attn_takes(int kv_dtype, int d, int page_size, int R, const void* k, 
                       long long q_ts, long long q_hs) {
   const uintptr_t pool = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
   const uintptr_t rows = reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(q_ts * 2) | static_cast<uintptr_t>(q_hs * 2);
-  return kv_dtype != kF32 && (d == 64 || d == 128) && page_size % kUnit == 0 && R <= 16384 && pool % 16 == 0 &&
+  return kv_dtype != kF32 && (d == 64 || d == 128) && page_size % kUnit == 0 && R <= kMostRequests && pool % 16 == 0 &&
          rows % 4 == 0;
 }
 

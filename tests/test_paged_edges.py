@@ -364,3 +364,36 @@ def test_offsets_that_do_not_begin_at_zero_are_reported():
             status.zero_()
     finally:
         _lib.set_status_tensor(None)
+
+
+@gpu
+def test_batches_of_different_sizes_from_several_threads():
+    """Calls of one request and of thousands, from two threads at a time, do not disturb one another's launches."""
+    import threading
+
+    from strict_topk_overlap_b200 import paged_attention
+    sizes, caches, wrong = (1, 15000), [], []
+    for n in sizes:
+        cache = _cache([16] * n, 1, 64, 16, 16, torch.bfloat16, 125)
+        caches.append((cache, _queries(n, 2, 64, torch.bfloat16, 126), _ints([16] * n)))
+    want = [paged_attention.attention(q, cache, at) for cache, q, at in caches]
+    torch.cuda.synchronize()
+
+    def work(i):
+        cache, q, at = caches[i]
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(1500 if i == 0 else 300):
+                    out = paged_attention.attention(q, cache, at)
+                torch.cuda.current_stream().synchronize()
+            if not torch.equal(out, want[i]):
+                wrong.append("another result")
+        except RuntimeError as e:
+            wrong.append(str(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1, 0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:2]
