@@ -68,6 +68,9 @@ struct Shared {
   uint64_t full[10], empty[10];
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_full[2];  // [MMA tile] or [MMA tile][half of the keys]
   uint64_t pair[8];            // the two warps that share 32 rows
+  uint64_t drained;            // the products issued before a wait ran out
+  volatile int abandoned;      // one of the MMA warp ran out
+  volatile int asked;          // copies asked for when one of the load warp ran out, -1: all
   uint32_t tmem;
   int2 range[16];              // of a warp's rows: least and largest key
   volatile int failed[2];      // a wait of the MMA tile's softmax ran out
@@ -448,6 +451,9 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         sh.failed[q] = 0;
       }
       for (int x = 0; x < 8; ++x) mbar_init(&sh.pair[x], 64);
+      mbar_init(&sh.drained, 1);
+      sh.abandoned = 0;
+      sh.asked = -1;
       fence_barrier_init();
     }
     __syncwarp();
@@ -526,7 +532,10 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
       for (int kv = 0; kv < 2; ++kv) {
         const int item = 2 * (i - ta) + kv, slot = item % P::kRing;
         if (item >= P::kRing) ok = ok && warp_wait(&sh.empty[slot], (item / P::kRing - 1) & 1, a.status);
-        if (!ok) break;
+        if (!ok) {
+          sh.asked = item;
+          break;
+        }
         if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], P::kTileBytes);
         __syncwarp();
         if (lane < boxes) {
@@ -630,6 +639,11 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         mma_commit(&sh.empty[kslot]);
         advance();
       }
+    }
+    if (!ok) {  // a wait ran out and was reported: tensor memory is freed after the products under way
+      sh.abandoned = 1;
+      mma_commit(&sh.drained);
+      warp_wait(&sh.drained, 0, a.status);
     }
   } else if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------ softmax
@@ -987,6 +1001,11 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   if (warp == kSoftmaxWarps) {
     fence_after();
     tmem_free(tmem, P::kTmem);
+  }
+  if (warp == kSoftmaxWarps + 1 && sh.abandoned) {  // the CTA does not end under copies that nobody waited for
+    const int asked = sh.asked >= 0 ? sh.asked : 2 * (tb - ta);
+    for (int item = max(0, asked - P::kRing); item < asked; ++item)
+      if (!warp_wait(&sh.full[item % P::kRing], (item / P::kRing) & 1, a.status)) break;
   }
 }
 
