@@ -15,12 +15,17 @@ from .paged import PagedKVCache
 from .rotary import Rotary
 
 
+_NOTHING = 1e30  # lo, and minus hi, of a block without tokens
+
+
 def empty_paged_cache(capacities, hkv, dim, block_size, page_size, *, dtype=torch.bfloat16, bounds=True,
                       generator=None, device="cuda") -> PagedKVCache:
     """A pool for requests of up to ``capacities`` tokens, its pages handed out
     in a seeded random order. ``bounds=False`` keeps no per-block key bounds
     (a cache that no block selection reads). The pool is zeroed; a block
-    without tokens has bounds that no query scores high: lo = 3e38, hi = -3e38."""
+    without tokens has bounds that no query scores high, lo = 1e30 and
+    hi = -1e30: far below every block of tokens, yet with sums over a head that
+    FP32 holds, so that selection need not rescore them."""
     if not capacities or min(capacities) <= 0:
         raise ValueError("every request needs room for at least one token")
     if block_size % page_size:
@@ -33,7 +38,7 @@ def empty_paged_cache(capacities, hkv, dim, block_size, page_size, *, dtype=torc
         offsets.append(offsets[-1] + n)
     table = torch.randperm(pages, generator=generator).to(torch.int32).to(device)
     k = torch.zeros((pages, hkv, page_size, dim), dtype=dtype, device=device)
-    lo = torch.full((hkv, total if bounds else 0, dim), 3e38, device=device)
+    lo = torch.full((hkv, total if bounds else 0, dim), _NOTHING, device=device)
     return PagedKVCache(k, torch.zeros_like(k), table, torch.tensor(offsets, dtype=torch.int32, device=device), lo,
                         -lo, block_size, page_size, max(blocks))
 

@@ -397,3 +397,27 @@ def test_batches_of_different_sizes_from_several_threads():
     for t in threads:
         t.join()
     assert not wrong, wrong[:2]
+
+
+@gpu
+@pytest.mark.parametrize("room", [0, 40])
+def test_selection_over_a_cache_with_spare_room(room):
+    """Blocks without tokens are never selected before blocks with some, and change nothing about those."""
+    from strict_topk_overlap_b200 import paged, paged_append
+    hq, hkv, d, block, page, filled = 8, 2, 128, 32, 16, [12, 30]
+    g = torch.Generator(DEV).manual_seed(127)
+    cache = paged_append.empty_paged_cache([(n + room) * block for n in filled], hkv, d, block, page,
+                                           generator=torch.Generator().manual_seed(2))
+    t = sum(filled) * block
+    k, v = (torch.randn((t, hkv, d), generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    paged_append.append_tokens(cache, k, v, _ints([0, 0]), token_offsets=_ints([0, filled[0] * block, t]))
+    q = torch.randn((2 * hq, d), generator=g, device=DEV).to(torch.bfloat16)
+    ids = paged.select_blocks(q, cache, 10).view(2, hq, 10)
+    for r, n in enumerate(filled):
+        first = sum(filled[:r]) * block
+        keys = k[first:first + n * block].view(n, block, hkv, d).float()
+        lo, hi = keys.amin(1), keys.amax(1)  # [n, hkv, d]
+        x = q.view(2, hkv, hq // hkv, d)[r].double()
+        score = torch.einsum("hgd,nhd->hgn", x.clamp(min=0), hi.double()) + torch.einsum("hgd,nhd->hgn", x.clamp(max=0), lo.double())
+        want = score.reshape(hq, n).topk(10).indices
+        assert torch.equal(ids[r].long().sort(-1).values, want.sort(-1).values)

@@ -127,3 +127,14 @@ def test_launches_happen_on_the_tensors_device(monkeypatch, current):
     for call in _calls(_cache(_on_device), _on_device):
         call()
     assert seen == [0, 0, 0] and state["device"] == current
+
+
+@pytest.mark.parametrize("d,scale", [(64, 1.0), (128, 60.0), (1024, 65504.0)])
+def test_bounds_of_empty_blocks_score_in_fp32(d, scale):
+    """A block without tokens scores far below all others, in sums that stay finite (infinite ones would have every
+    such block rescored exactly)."""
+    cache = paged_append.empty_paged_cache([64], 2, d, 32, 16, device="cpu")
+    q = scale * torch.randn((16, d), generator=torch.Generator().manual_seed(1))
+    for h in range(2):
+        top = (q.clamp(min=0) @ cache.hi[h].T + q.clamp(max=0) @ cache.lo[h].T)
+        assert bool(top.isfinite().all()) and bool((top < -1e28).all())
