@@ -936,21 +936,22 @@ struct AttnPlan {
   size_t bytes;
 };
 
-// Parts that the prompt kernel cuts its tiles' key ranges into: the fewest
-// thousand clocks of waves x (key tiles of a part + start and end of a CTA) +
-// partial states written and read, by the kernel's measured costs (4 a key
-// tile of 256 rows at 128 dims, 2 of 128 rows at 64, 13 a CTA). 509 tokens on
-// 65 K keys, 64 row tiles: 643 us in 9 parts (3.9 waves), 674 in 2 (0.9 of
-// one), 772 in 7 (3.03). Four waves of tiles and more stay whole.
+// Parts that the prompt kernel cuts its tiles' key ranges into, as many as one
+// wave of CTAs takes at most: by roughly the thousand clocks of the key tiles
+// of a part (4 each at 128 dims, 2 at 64) and of the partial states written and
+// read, so that short ranges stay whole (300 tokens, 40 row tiles, 3 key
+// tiles: 18 us whole, 22 in 3 parts). More waves of smaller parts even the SMs
+// out and win in short bursts (509 tokens on 65 K keys, 72 row tiles: 683 us in
+// 9 parts, 721 in 2) but lose where the power limit holds the clocks down
+// (784 against 757 us of calls in a row for seconds; 2,048 tokens on 65 K keys
+// at 64 dims 1,550 in parts, 1,520 whole).
 int prompt_splits(long long tiles, int keys, int d, double rows, int places) {
   const int key_tiles = (keys + 127) / 128;
-  if (tiles >= 4ll * places) return 1;
   int best = 1;
   double least = 0;
-  for (int n = 1; n <= key_tiles && n <= 64; ++n) {
-    const double waves = static_cast<double>((tiles * n + places - 1) / places);
-    const double part = (key_tiles + n - 1) / n * (d == 64 ? 2.0 : 4.0) + 13.0;
-    const double cost = waves * part + (n > 1 ? n * rows * (d + 2) * 8 / 3.4e6 : 0);
+  for (int n = 1; n <= key_tiles && (n == 1 || tiles * n <= places); ++n) {
+    const double part = (key_tiles + n - 1) / n * (d == 64 ? 2.0 : 4.0);
+    const double cost = part + (n > 1 ? n * rows * (d + 2) * 8 / 3.4e6 : 0);
     if (n == 1 || cost < least) {
       best = n;
       least = cost;
