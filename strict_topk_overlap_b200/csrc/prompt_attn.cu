@@ -891,7 +891,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
     // may have left FP32's range (2^100; a frame that follows stays far inside);
     // or scores are NaN, perhaps all that the row sees here (which leaves no
     // maximum). The row's state is then taken anew in a frame of its own.
-    const bool sees = have && max(rk.lo, ta * kTileN) < min(rk.hi, tb * kTileN);
+    const bool sees = have && max(rk.lo, begin * kTileN) < min(rk.hi, end * kTileN);
     const bool over = sees && (empty || nan || !(l <= 1.3e30f && l >= 7.9e-31f));
     bool redo_row = over;
     if (ok && !(kOwnO && half)) {
@@ -970,8 +970,8 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
         __syncwarp();
         const int xtok = __shfl_sync(kFull, tok, src);
         const int xhead = __shfl_sync(kFull, head, src), xpos = __shfl_sync(kFull, rk.pos, src);
-        const int xlo = max(__shfl_sync(kFull, rk.lo, src), ta * kTileN);
-        const int xhi = min(__shfl_sync(kFull, rk.hi, src), tb * kTileN);
+        const int xlo = max(__shfl_sync(kFull, rk.lo, src), begin * kTileN);
+        const int xhi = min(__shfl_sync(kFull, rk.hi, src), end * kTileN);
         const float xslope = __shfl_sync(kFull, slope, src);
         const float frame = __shfl_sync(kFull, m, src) * kLn2;
         const bool lost = __shfl_sync(kFull, static_cast<int>(over), src) != 0;
@@ -1000,7 +1000,7 @@ prompt_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap km
   __syncthreads();
   if (warp == kSoftmaxWarps) {
     fence_after();
-    tmem_free(tmem, P::kTmem);
+    tmem_free(sh.tmem, P::kTmem);
   }
   if (warp == kSoftmaxWarps + 1 && sh.abandoned) {  // the CTA does not end under copies that nobody waited for
     const int asked = sh.asked >= 0 ? sh.asked : 2 * (tb - ta);
