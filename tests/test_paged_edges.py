@@ -8,7 +8,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_paged_attention import DEV, TYPES, _cache, _compare, _compare_equal, _ints
+from oracle import paged_dense as O
+from test_paged_attention import DEV, TYPES, UNIT, _cache, _compare, _compare_equal, _ints
 
 gpu = pytest.mark.gpu
 TILED = [(8, 2, 128, 32, 16), (4, 4, 64, 32, 16)]  # hq, hkv, d, block, page that the tensor-core kernels take
@@ -421,3 +422,63 @@ def test_selection_over_a_cache_with_spare_room(room):
         score = torch.einsum("hgd,nhd->hgn", x.clamp(min=0), hi.double()) + torch.einsum("hgd,nhd->hgn", x.clamp(max=0), lo.double())
         want = score.reshape(hq, n).topk(10).indices
         assert torch.equal(ids[r].long().sort(-1).values, want.sort(-1).values)
+
+
+def _strict(q, cache, lengths, new, lo, got, lse, softcap, slopes):
+    """Against the definition in 64 bits, infinite and NaN outputs and log-sum-exps included: where the reference is
+    not finite, the same value; elsewhere the tolerances of test_paged_attention.py."""
+    dtype, d = q.dtype, q.shape[2]
+    off, start = cache.block_offsets.tolist(), 0
+    for r, (n, length) in enumerate(zip(new, lengths)):
+        rows = slice(start, start + n)
+        k, v = (O.gather(x, cache.page_table, off, cache.block_size, cache.page_size, r, length)
+                for x in (cache.k_pages, cache.v_pages))
+        pos = list(range(length - n, length))
+        want, wlse, size, vmax = O.attention(q[rows], k, v, lo[rows] if lo else [0] * n, [p + 1 for p in pos], pos,
+                                             scale=d ** -0.5, softcap=softcap, slopes=slopes)
+        size = size.nan_to_num(0.0, 0.0)  # rows without a finite score are compared below
+        ds = (d + 16) * 2.0 ** -24 * size + (1e-4 if dtype != torch.float32 else 0.0)
+        u = UNIT[dtype]
+        tol = u * want.abs() + ((0.0 if dtype == torch.float32 else u) + 2 * ds + 64 * 2.0 ** -24)[..., None] * vmax[..., None]
+        out, ends = got[rows].double(), lse[rows].double()
+        assert torch.equal(out.isnan(), want.isnan()) and torch.equal(ends.isnan(), wlse.isnan())
+        odd = want.isinf()
+        assert torch.equal(out[odd], want[odd]) and not bool(out[~odd].isinf().any())
+        ok = want.isfinite()
+        assert bool(((out - want).abs() <= tol)[ok].all())
+        live = wlse.isfinite()
+        assert bool(((ends - wlse).abs() <= ds + 64 * 2.0 ** -24 + 2.0 ** -22 * wlse.abs())[live].all())
+        start += n
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", FORMS)
+@pytest.mark.parametrize("new", [1, 4, 200])
+@pytest.mark.parametrize("scores", [dict(), dict(softcap=20.0), dict(biased=True)])
+def test_seen_infinities(dtype, shape, new, scores):
+    """Infinite values and infinite key elements at keys that some rows see: exactly the definition's infinities and
+    NaN there, everything else as if nothing had happened."""
+    from strict_topk_overlap_b200 import paged_attention
+    hq, hkv, d, block, page = shape
+    cache = _cache([300, 260], hkv, d, block, page, dtype, 128)
+    q = _queries(2 * new, hq, d, dtype, 129)
+    softcap = scores.get("softcap", 0.0)
+    slopes = torch.full((hq,), 0.05, device=DEV) if scores.get("biased") else None
+    pos = [p for length in (300, 260) for p in range(length - new, length)]
+    lo = [p // 64 * 64 for p in pos]
+    args = dict(token_offsets=None if new == 1 else _ints([0, new, 2 * new]), max_tokens=new, return_lse=True,
+                softcap=softcap, slopes=slopes)
+    for name, j, e, value in (("v_pages", 293, 5, float("inf")), ("v_pages", 259, 40, float("-inf")),
+                              ("k_pages", 290, 3, float("inf")), ("k_pages", 257, d - 1, float("-inf"))):
+        for low in (None, lo):
+            pool = getattr(cache, name)
+            held = pool.clone()
+            for r in (0, 1):
+                if j < (300, 260)[r]:
+                    pg, slot = _at(cache, r, _span(j, j + 1))
+                    pool[pg, :, slot, e] = value
+            out, lse = paged_attention.attention(q, cache, _ints([300, 260]), kv_lo=None if low is None else _ints(low),
+                                                 **args)
+            _strict(q, cache, [300, 260], [new, new], low, out, lse, softcap, slopes)
+            pool.copy_(held)
