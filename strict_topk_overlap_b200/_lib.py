@@ -194,12 +194,17 @@ def stream_of(t: torch.Tensor) -> int:
     index = t.get_device()
     if index < 0:
         raise ValueError("expected tensors on a CUDA device; there is no CPU fallback")
-    return torch._C._cuda_getCurrentRawStream(index)
+    return raw_stream(index)
+
+
+# Raw handle of a device's current stream, and the current device, by number.
+raw_stream = torch._C._cuda_getCurrentRawStream
+current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def on_device(index: int, call, *args) -> int:
     """``call(*args)`` with device ``index`` current: the library launches on the current one."""
-    if torch._C._cuda_getDevice() == index:
+    if current_device() == index:
         return call(*args)
     with torch.cuda.device(index):
         return call(*args)

@@ -31,6 +31,9 @@ from .kernels import (PartialState, Prediction, RepairResult, _allocate_state, _
                       compact_capacity)
 
 
+_INT = torch.int32
+
+
 @dataclass
 class PagedKVCache:
     """A batch's KV page pool, page table, block offsets and block metadata."""
@@ -68,16 +71,16 @@ class PagedKVCache:
     def packed_kv(self, hkv, dim) -> bytes:
         """``kv()`` as the packed bytes that the paged token calls take, its tensors checked."""
         k, v, table, offsets = self.k_pages, self.v_pages, self.page_table, self.block_offsets
-        index = k.get_device()
+        dtype, index = k.dtype, k.get_device()
         if index < 0:
             raise ValueError("the cache must be on a CUDA device; there is no CPU fallback")
-        if v.dtype is not k.dtype:
+        if v.dtype is not dtype:
             raise ValueError("K and V must share a dtype")
-        if v.shape != k.shape or v.get_device() != index or not (k.is_contiguous() and v.is_contiguous()):
+        if v.get_device() != index or v.shape != k.shape or not k.is_contiguous() or not v.is_contiguous():
             raise ValueError("K and V pages must be contiguous, of one shape and on one device")
-        for x in (table, offsets):
-            if x.dtype is not torch.int32 or x.get_device() != index or not x.is_contiguous():
-                raise ValueError("page_table and block_offsets must be contiguous int32 on the pages' device")
+        if table.dtype is not _INT or offsets.dtype is not _INT or table.get_device() != index or \
+                offsets.get_device() != index or not table.is_contiguous() or not offsets.is_contiguous():
+            raise ValueError("page_table and block_offsets must be contiguous int32 on the pages' device")
         return L.PACK_KV(k.data_ptr(), v.data_ptr(), L.dtype_code(k), hkv, 0, self.block_size, dim, table.data_ptr(),
                          offsets.data_ptr(), self.page_size, 0)
 

@@ -15,6 +15,7 @@ from .paged import PagedKVCache
 from .rotary import Rotary
 
 
+_FLOAT = torch.float32
 _NOTHING = 1e30  # lo, and minus hi, of a block without tokens
 
 
@@ -124,7 +125,8 @@ def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=N
     pages, hkv, _, d = pool.shape
     dtype, index = pool.dtype, pool.get_device()
     kv = cache.packed_kv(hkv, d)
-    requests, blocks = cache.block_offsets.shape[0] - 1, cache.lo.shape[1]
+    bounds = cache.lo.shape
+    requests, blocks = cache.block_offsets.shape[0] - 1, bounds[1]
     t = k.shape[0]
     kp, kt, kh = _rows(k, (t, hkv, d), "k", dtype, index)
     vp, vt, vh = _rows(v, (t, hkv, d), "v", dtype, index)
@@ -143,13 +145,14 @@ def append_tokens(cache: PagedKVCache, k, v, lengths, *, token_offsets=None, q=N
     turn, at = _rotary(rotary, positions, t, index)
     lo = hi = None
     if blocks:
-        for x in (cache.lo, cache.hi):
-            if x.dtype is not torch.float32 or x.shape != (hkv, blocks, d) or x.get_device() != index or \
-                    not x.is_contiguous():
-                raise ValueError("lo and hi must be contiguous FP32 [Hkv, blocks, D] on the cache's device")
-        lo, hi = cache.lo.data_ptr(), cache.hi.data_ptr()
+        low, high = cache.lo, cache.hi
+        if bounds != (hkv, blocks, d) or high.shape != bounds or low.dtype is not _FLOAT or high.dtype is not _FLOAT or \
+                low.get_device() != index or high.get_device() != index or not low.is_contiguous() or \
+                not high.is_contiguous():
+            raise ValueError("lo and hi must be contiguous FP32 [Hkv, blocks, D] on the cache's device")
+        lo, hi = low.data_ptr(), high.data_ptr()
     rc = L.on_device(index, L.load().stk_append_tokens, kv, pages, requests, blocks or 1, t, kp, kt, kh, vp, vt, vh, qp,
-                     qt, qh, hq, out, before, offsets, at, turn, lo, hi, L.status_ptr(), L.stream_of(pool))
+                     qt, qh, hq, out, before, offsets, at, turn, lo, hi, L.status_ptr(), L.raw_stream(index))
     if rc:
         L.check(rc, "append_tokens")
     return q_out if q is not None else None

@@ -88,7 +88,7 @@ def _attend(q, cache, lengths, token_offsets, max_tokens, kv_lo, kv_hi, softcap,
     lse = q.new_empty((t, hq), dtype=torch.float32) if return_lse else None
     rc = L.on_device(index, L.load().stk_paged_attention, kv, pages, qp, qt, qh, requests, t, hq, held, offsets, most,
                      longest, prefix, options, out.data_ptr(), L.ptr(lse), L.ptr(workspace), need, L.status_ptr(),
-                     L.stream_of(q))
+                     L.raw_stream(index))
     if rc:
         L.check(rc, "paged attention")
     return (out, lse) if return_lse else out

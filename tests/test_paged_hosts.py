@@ -121,9 +121,9 @@ def test_launches_happen_on_the_tensors_device(monkeypatch, current):
             return call
 
     monkeypatch.setattr(_lib, "load", lambda path=None: Launches())
-    monkeypatch.setattr(_lib, "stream_of", lambda t: 0)
+    monkeypatch.setattr(_lib, "raw_stream", lambda index: 0)
     monkeypatch.setattr(torch.cuda, "device", Device)
-    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state["device"], raising=False)
+    monkeypatch.setattr(_lib, "current_device", lambda: state["device"])
     for call in _calls(_cache(_on_device), _on_device):
         call()
     assert seen == [0, 0, 0] and state["device"] == current
