@@ -471,7 +471,8 @@ typedef struct stk_attention_options {
 } stk_attention_options;
 
 /* Workspace (bytes, from a 16-byte boundary on) for stk_paged_attention of the
- * same sizes. */
+ * same sizes. These calls plan for and launch on the current device: it has to
+ * be the one that the pointers belong to. */
 STK_API size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int T, int hq, int has_offsets,
                                                    int max_tokens, int max_length, int prefix);
 

@@ -26,11 +26,11 @@
 // (a decode step) each is a CTA of its own and latency is all that counts.
 //
 // Measured (B200, D 128): 8 tokens, 32 / 8 heads bf16: 7 us, a launch and
-// three dependent loads. 8 K prompt tokens of five requests (167 MB): 37 us,
-// 4.5 TB/s. 32 K tokens, 16 / 8 heads f16, three axes (552 MB): 113 us, 4.9
-// TB/s, 75 % of a copy's rate; one item per CTA took 126 us, and asking L2 for
-// the next heads' rows ahead 125 us (the loads are waited for either way, and
-// the requests compete with the stores).
+// three dependent loads. 8 K prompt tokens of five requests (167 MB): 38 us,
+// 4.4 TB/s; the same in FP32: 71 us, 4.7 TB/s. 32 K tokens, 16 / 8 heads f16,
+// three axes (552 MB): 113 us, 4.9 TB/s, 75 % of a copy's rate; one item per
+// CTA took 126 us, and asking L2 for the next heads' rows ahead 125 us (the
+// loads are waited for either way, and the requests compete with the stores).
 //
 // Which (request, block) an item is follows from token_offsets on the device:
 // request r's blocks start at slot offs[r] / B + 2 r, which leaves room for

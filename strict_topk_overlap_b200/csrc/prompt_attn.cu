@@ -28,17 +28,20 @@
 // each tile's keys in two halves with chains of their own, so that one's
 // products run under another's exponentials.
 //
-// Measured (B200): three causal prompts of 10.8 K tokens, 16 / 8 heads, D 128,
-// capped: 267 us, 838 TFLOP/s; 509 tokens on 65 K keys, 32 / 8 heads, biased:
-// 650 us, 837 TFLOP/s, half of cuBLAS's rate; 8 K tokens of packed documents,
-// D 64, f16: 122 us; prompts with prefix masks, 96 / 8 heads: 64 us. On the
-// capped prompts, in the order tried: MMAs issued under a branch on one lane
-// 469 us, by a predicate 374 us; eight softmax warps with a row's 128 scores
-// in registers 374 us, sixteen with 64 each 418 us (at 96 registers they
-// spill, and 224 KB of shared memory leave next to no L1 for that), sixteen
-// that keep the scores in TMEM 359 us; both halves of the keys in one chain
-// 372 us, in two 343 us; the heads as the grid's slower dimension 334 us,
-// innermost 267 us (the longest tiles of all heads start first).
+// Measured (B200; calls in a row for seconds, where the power limit holds the
+// clocks down, and in brackets short bursts): three causal prompts of 10.8 K
+// tokens, 16 / 8 heads, D 128, capped: 300 (271) us, 746 TFLOP/s, plain (241);
+// 509 tokens on 65 K keys, 32 / 8 heads, biased: 741 (690) us, 734 TFLOP/s,
+// under half of cuBLAS's rate; 8 K tokens of packed documents, D 64, f16: 123
+// us; prompts with prefix masks, 96 / 8 heads: 66 us. On the capped prompts, in
+// bursts and in the order tried: MMAs issued under a branch on one lane 469 us,
+// by a predicate 374 us; eight softmax warps with a row's 128 scores in
+// registers 374 us, sixteen with 64 each 418 us (at 96 registers they spill,
+// and 224 KB of shared memory leave next to no L1 for that), sixteen that keep
+// the scores in TMEM 359 us; both halves of the keys in one chain 372 us, in
+// two 343 us; the heads as the grid's slower dimension 334 us, innermost 267 us
+// (the longest tiles of all heads start first). Even so 20 to 90 bytes a thread
+// of what is used once per CTA spill.
 //
 // Tiles of keys that no row sees are not read; runs of 16 keys that a warp's
 // rows all see skip the mask, those that none sees the exponentials. Places
@@ -291,7 +294,7 @@ template <int MODE>
 __device__ __forceinline__ void scores(float2 (&s)[kRun / 2], const Score& z, int k0, bool full) {
   // Capped scores cap2 tanh(c1 s) as odd polynomials in s (fitted for the
   // least relative error), no special functions: three terms where |c1 s| <=
-  // 0.25 throughout a warp's run (3.9e-7), five up to 0.75 (5.2e-7), errors
+  // 0.25 throughout a warp's run (4.3e-7), five up to 0.75 (6.3e-7), errors
   // of the order of FP32's own; the exponential form beyond.
   if (MODE & 1) {
     float far[2] = {0.f, 0.f};

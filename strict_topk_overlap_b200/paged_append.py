@@ -4,7 +4,11 @@
 (stk_append_tokens) rotates new keys and queries by their positions, writes
 keys and values into their pages and keeps the blocks' key bounds current, in
 one launch. What it leaves is what ``paged.select_blocks`` and the attention
-calls read. New: the reference starts from a filled dense cache.
+calls read. The block-sparse calls (``paged.select_blocks``, ``paged.exact``
+and the speculative ones) know blocks, not token counts: they attend a
+request's last block as a full one, so what they read has to end on a block's
+border. ``paged_attention`` knows the lengths and reads any. New: the reference
+starts from a filled dense cache.
 """
 from __future__ import annotations
 
