@@ -488,7 +488,8 @@ STK_API size_t stk_paged_attention_workspace_bytes(const stk_kv* kv, int R, int 
  * with each request's own rest. Tokens from token_offsets[R] on (padding) see
  * no key. Offsets that do not begin at 0 or go past T and requests with more
  * tokens than max_tokens are cut and reported in status
- * (STK_STATUS_SHAPE_OVERFLOW). New: the reference attends block lists only. */
+ * (STK_STATUS_SHAPE_OVERFLOW), as is a prefix that request 0's blocks do not
+ * hold (STK_STATUS_BAD_LENGTH). New: the reference attends block lists only. */
 STK_API int stk_paged_attention(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
                                 long long q_head_stride, int R, int T, int hq, const int32_t* lengths,
                                 const int32_t* token_offsets, int max_tokens, int max_length, int prefix,

@@ -1076,6 +1076,8 @@ extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, l
   JoinArgs j{};
   j.rows = T * hq; j.d = kv->d; j.dtype = kv->kv_dtype; j.out = out; j.lse = lse; j.nsrc = p.phases;
   j.hq = hq; j.G = a.G; j.token_offsets = token_offsets;
+  if (prefix > 0) j.block_offsets = kv->block_offsets;
+  j.block = kv->b; j.prefix = prefix; j.status = status;
   unsigned char* at = static_cast<unsigned char*>(workspace);
   for (int i = 0; i < p.phases; ++i) {
     const AttnPhase& ph = p.phase[i];

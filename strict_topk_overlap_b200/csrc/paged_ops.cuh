@@ -236,6 +236,10 @@ struct JoinArgs {
   const int* token_offsets;
   void* out;
   float* lse;
+  // Behind a shared prefix: request 0's blocks have to hold it.
+  const int* block_offsets;  // null without one
+  int block, prefix;
+  int* status;
 };
 
 int launch_join(const JoinArgs& a, int sms, cudaStream_t stream);

@@ -306,6 +306,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(JoinArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = WPR == 1 ? blockIdx.x * kJoinWarps + warp : blockIdx.x;
   const int first_part = WPR == 1 ? 0 : warp;
+  if (a.block_offsets != nullptr && blockIdx.x == 0 && threadIdx.x == 0 &&
+      static_cast<long long>(a.block_offsets[1] - a.block_offsets[0]) * a.block < a.prefix)
+    report(a.status, kStatusBadLength);
   if (row >= a.rows) return;
   // Part s of source k is state base[k] + s * step[k].
   long long base[2], step[2];

@@ -482,3 +482,22 @@ def test_seen_infinities(dtype, shape, new, scores):
                                                  **args)
             _strict(q, cache, [300, 260], [new, new], low, out, lse, softcap, slopes)
             pool.copy_(held)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 40])
+def test_prefix_that_request_0_does_not_hold_is_reported(dtype, new):
+    from strict_topk_overlap_b200 import _lib, paged_attention
+    cache = _cache([50, 400], 2, 64, 32, 16, dtype, 130)
+    q = _queries(2 * new, 8, 64, dtype, 131)
+    args = dict(token_offsets=None if new == 1 else _ints([0, new, 2 * new]), max_tokens=new)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    try:
+        _lib.set_status_tensor(status)
+        paged_attention.shared_prefix_attention(q, cache, _ints([50, 400]), 64, **args)
+        assert int(status) == 0
+        paged_attention.shared_prefix_attention(q, cache, _ints([50, 400]), 96, **args)
+        assert int(status) == 5
+    finally:
+        _lib.set_status_tensor(None)
