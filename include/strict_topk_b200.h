@@ -496,6 +496,24 @@ STK_API int stk_paged_attention(const stk_kv* kv, int pages, const void* q, long
                                 const stk_attention_options* options, void* out, float* lse, void* workspace,
                                 size_t workspace_bytes, int32_t* status, void* stream);
 
+/* Workspace (bytes, from a 16-byte boundary on) for stk_accumulate_weights of
+ * the same sizes, on the current device. */
+STK_API size_t stk_accumulate_weights_workspace_bytes(const stk_kv* kv, int R, int T, int hq, int total_blocks,
+                                                      int has_offsets, int max_tokens, int max_length, int has_masks);
+
+/* The attention weight that each cached key receives from T packed tokens (as
+ * in stk_paged_attention, with the same options): weights [hkv, total_blocks,
+ * b] FP32 += sum over the tokens t that see the key and the query heads of the
+ * KV head's group of exp(s - lse[t]), lse [T, hq] the rows' log-sum-exps as
+ * stk_paged_attention returned them. A row whose lse is -inf gives nothing.
+ * Key j of request r is slot block_offsets[r] * b + j of a head. New: the
+ * reference keeps every token. */
+STK_API int stk_accumulate_weights(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
+                                   long long q_head_stride, int R, int T, int hq, int total_blocks,
+                                   const int32_t* lengths, const int32_t* token_offsets, int max_tokens, int max_length,
+                                   const stk_attention_options* options, const float* lse, float* weights,
+                                   void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,7 @@
 
 #include "internal.cuh"
 #include "paged_ops.cuh"
+#include "weigh.cuh"
 #include "../../include/strict_topk_b200.h"
 
 
@@ -139,7 +140,7 @@ int stk_set_wait_limit_ns(unsigned long long ns) {
   if (ns == 0) return fail(STK_EINVAL, "the wait limit must be positive");
   int (*const setters[])(unsigned long long) = {set_wait_limit_select, set_wait_limit_states, set_wait_limit_repair,
                                                 set_wait_limit_attend, set_wait_limit_group_mma, set_wait_limit_step,
-                                                set_wait_limit_prompt, set_wait_limit_token};
+                                                set_wait_limit_prompt, set_wait_limit_token, set_wait_limit_weigh};
   for (auto set : setters) {
     const int rc = set(ns);
     if (rc) return cuda_status(rc, "set wait limit");
@@ -1097,4 +1098,74 @@ extern "C" int stk_paged_attention(const stk_kv* kv, int pages, const void* q, l
     if (r2) return cuda_status(r2, "paged attention");
   }
   return p.join ? cuda_status(launch_join(j, sm_count_current(), st), "attention join") : 0;
+}
+
+// ----------------------------------------------------------------------------- key weights
+
+namespace {
+// The sizes of a call as the kernels take them, and the bytes of its workspace:
+// masks' ranges, then the parts' sums.
+size_t plan_weigh(WeighArgs& w, const stk_kv* kv, int R, int T, int hq, int total_blocks, int max_tokens, int max_length,
+                  bool masks) {
+  w.a.L = make_layout(kv);
+  w.a.R = R; w.a.T = T; w.a.hq = hq; w.a.G = hq / kv->hkv; w.a.d = kv->d;
+  w.slots = static_cast<long long>(total_blocks) * kv->b;
+  w.most = max_tokens;
+  w.longest = max_length;
+  weigh_plan(w, (w.slots + kWeighKeys - 1) / kWeighKeys, sm_count_current());
+  const size_t ranges = masks ? (static_cast<size_t>(T) / w.tokens + R + 2) * sizeof(int4) : 0;
+  return ranges + (w.parts > 1 ? static_cast<size_t>(w.parts) * kv->hkv * w.slots * sizeof(float) : 0);
+}
+}  // namespace
+
+extern "C" size_t stk_accumulate_weights_workspace_bytes(const stk_kv* kv, int R, int T, int hq, int total_blocks,
+                                                         int has_offsets, int max_tokens, int max_length, int has_masks) {
+  if (check_attention(kv, R, T, hq, has_offsets != 0, max_tokens, max_length, 0) || T == 0 || total_blocks <= 0) return 0;
+  WeighArgs w{};
+  return plan_weigh(w, kv, R, T, hq, total_blocks, max_tokens, max_length, has_masks != 0);
+}
+
+extern "C" int stk_accumulate_weights(const stk_kv* kv, int pages, const void* q, long long q_token_stride,
+                                      long long q_head_stride, int R, int T, int hq, int total_blocks,
+                                      const int32_t* lengths, const int32_t* token_offsets, int max_tokens, int max_length,
+                                      const stk_attention_options* options, const float* lse, float* weights,
+                                      void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  const int rc = check_attention(kv, R, T, hq, token_offsets != nullptr, max_tokens, max_length, 0);
+  if (rc) return rc;
+  if (total_blocks <= 0) return fail(STK_EINVAL, "a cache of %d blocks", total_blocks);
+  if (T == 0) return 0;
+  if (!q || !lengths || !lse || !weights || pages <= 0) return fail(STK_EINVAL, "null pointer or empty pool");
+  if (options && (!(options->softcap >= 0.f) || !(options->scale >= 0.f)))
+    return fail(STK_EINVAL, "scale and softcap must not be negative");
+  WeighArgs w{};
+  const bool masks = options && (options->kv_lo || options->kv_hi);
+  const size_t need = plan_weigh(w, kv, R, T, hq, total_blocks, max_tokens, max_length, masks);
+  if (workspace_bytes < need || (need && !workspace)) return fail(STK_EWS, "key weights workspace too small");
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(STK_EINVAL, "the key weights workspace must start on a 16-byte boundary");
+  w.a.pages = pages;
+  w.a.q = q; w.a.q_ts = q_token_stride; w.a.q_hs = q_head_stride;
+  w.a.lengths = lengths; w.a.token_offsets = token_offsets;
+  w.a.scale = attn_scale(kv->d);
+  if (options) {
+    if (options->scale > 0.f) w.a.scale = options->scale;
+    w.a.softcap = options->softcap; w.a.slopes = options->slopes;
+    w.a.kv_lo = options->kv_lo; w.a.kv_hi = options->kv_hi;
+  }
+  w.a.span_hi = 0x7fffffff;
+  w.a.status = status;
+  w.lse = lse;
+  w.weights = weights;
+  unsigned char* at = static_cast<unsigned char*>(workspace);
+  if (masks) {
+    w.ranges = reinterpret_cast<int4*>(at);
+    at += (static_cast<size_t>(T) / w.tokens + R + 2) * sizeof(int4);
+  }
+  if (w.parts > 1) w.partial = reinterpret_cast<float*>(at);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int r2 = 1;
+  if (weigh_tensor_takes(kv->kv_dtype, kv->d, kv->page_size, kv->k, q, q_token_stride, q_head_stride))
+    r2 = launch_weigh_tensor(w, kv->kv_dtype, sm_count_current(), st);
+  if (r2 == 1) r2 = launch_weigh_rows(w, kv->kv_dtype, st);
+  return cuda_status(r2, "accumulate_weights");
 }

@@ -1,0 +1,166 @@
+// Attention weight received by each cached key, on the FP32 units: FP32, head
+// sizes and layouts that the tensor-core kernel does not take.
+//
+// A CTA takes 32 keys of one request's KV head, in shared memory as FP32, one
+// to a lane. Its four warps take every fourth group of four rows (new tokens x
+// query heads), their queries broadcast from shared memory, so that a key's
+// four values are read once for four rows. The four warps' sums are added in
+// order at the end: the result does not depend on timing.
+//
+// HBM-bound for single tokens (K is read once per KV head), bound by shared
+// memory reads (two per four FMAs) for many rows.
+
+#include "weigh.cuh"
+
+namespace stk {
+
+namespace {
+
+constexpr int kKeys = 32, kWarps = 4, kRows = 4;
+
+// Row pitch in floats: whole 16-byte chunks, an odd number of them.
+__host__ __device__ inline int pitch(int d) { return (((d + 3) / 4) | 1) * 4; }
+
+inline size_t shared_bytes(int d) { return sizeof(float) * static_cast<size_t>(pitch(d)) * (kKeys + kWarps * kRows); }
+
+template <typename T>
+__global__ void __launch_bounds__(kWarps * 32)
+weigh_rows_kernel(const WeighArgs w, int tiles, int vector) {
+  const PagedAttnArgs& a = w.a;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ long long place[kKeys];
+  __shared__ int2 seen[kWarps];
+  __shared__ float sums[kWarps][kKeys];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tile = static_cast<int>(blockIdx.x % tiles);
+  const int h = static_cast<int>(blockIdx.x / tiles) % a.L.hkv, r = static_cast<int>(blockIdx.x / tiles) / a.L.hkv;
+  const int2 tn = new_tokens(a.token_offsets, r, a.R, a.T, a.status);
+  const int k0 = tile * kKeys, n = min(tn.y, w.most);
+  RowTile t;
+  t.r = r;
+  t.t0 = tn.x;
+  t.n = tn.y;
+  t.len = cached_tokens(a, r, tn.y);
+  if (tn.y > w.most) report(a.status, kStatusShapeOverflow);
+  if (n == 0 || k0 >= t.len) return;
+
+  // ---- keys that any row sees
+  int lo = 0, hi = t.len - t.n + n;
+  if (a.kv_lo || a.kv_hi) {
+    lo = 0x7fffffff;
+    hi = 0;
+    for (int i = tid; i < n; i += blockDim.x) {
+      const RowKeys k = row_keys(a, t, i);
+      if (k.hi > k.lo) {
+        lo = min(lo, k.lo);
+        hi = max(hi, k.hi);
+      }
+    }
+    lo = __reduce_min_sync(kFull, lo);
+    hi = __reduce_max_sync(kFull, hi);
+    if (lane == 0) seen[warp] = make_int2(lo, hi);
+    __syncthreads();
+    for (int x = 0; x < kWarps; ++x) {
+      lo = min(lo, seen[x].x);
+      hi = max(hi, seen[x].y);
+    }
+  }
+  lo = max(lo, k0);
+  hi = min(hi, k0 + kKeys);
+  if (lo >= hi) return;
+
+  // ---- their K, widened
+  const int d = a.d, p = pitch(d);
+  float* ks = smem;
+  float* qs = smem + (kKeys + warp * kRows) * p;
+  if (tid < kKeys) {
+    const int key = k0 + tid;
+    const int page = key >= lo && key < hi ? page_of(a, r, key) : -1;
+    place[tid] = page < 0 ? -1 : ((static_cast<long long>(page) * a.L.hkv + h) * a.L.page_size + key % a.L.page_size) * d;
+  }
+  __syncthreads();
+  const T* k = static_cast<const T*>(a.L.k);
+  if (vector) {
+    constexpr int N = 16 / sizeof(T);
+    const int chunks = d / N;
+#pragma unroll 4
+    for (int x = tid; x < kKeys * chunks; x += kWarps * 32) {
+      const int row = x / chunks, c = x - row * chunks;
+      float v[N] = {};
+      if (place[row] >= 0) load_vec<T, N>(k + place[row] + c * N, v);
+      store_vec<N>(ks + row * p + c * N, v);
+    }
+  } else {
+    for (int row = warp; row < kKeys; row += kWarps)
+      for (int c = lane; c < p; c += 32) ks[row * p + c] = c < d && place[row] >= 0 ? to_f32(k[place[row] + c]) : 0.f;
+  }
+  __syncthreads();
+
+  // ---- rows
+  const int key = k0 + lane, rows = n * a.G, d4 = (d + 3) / 4;
+  const T* q = static_cast<const T*>(a.q);
+  float sum = 0.f;
+  for (int r0 = warp * kRows; r0 < rows; r0 += kWarps * kRows) {
+    __syncwarp();
+    for (int x = 0; x < kRows; ++x) {
+      const int row = min(r0 + x, rows - 1), tok = row / a.G;
+      const T* src = q + static_cast<long long>(t.t0 + tok) * a.q_ts + static_cast<long long>(h * a.G + row - tok * a.G) * a.q_hs;
+      for (int c = lane; c < 4 * d4; c += 32) qs[x * p + c] = c < d ? to_f32(src[c]) : 0.f;
+    }
+    __syncwarp();
+    float4 dot[kRows] = {};
+    for (int c = 0; c < d4; ++c) {
+      const float4 y = *reinterpret_cast<const float4*>(ks + lane * p + c * 4);
+#pragma unroll
+      for (int x = 0; x < kRows; ++x) {
+        const float4 z = *reinterpret_cast<const float4*>(qs + x * p + c * 4);
+        dot[x].x = fmaf(y.x, z.x, dot[x].x);
+        dot[x].y = fmaf(y.y, z.y, dot[x].y);
+        dot[x].z = fmaf(y.z, z.z, dot[x].z);
+        dot[x].w = fmaf(y.w, z.w, dot[x].w);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kRows; ++x) {
+      const int row = r0 + x;
+      if (row >= rows) break;
+      const int tok = row / a.G, head = h * a.G + row - tok * a.G;
+      const RowKeys rk = row_keys(a, t, tok);
+      const float lse = w.lse[static_cast<long long>(t.t0 + tok) * a.hq + head];
+      float s = ((dot[x].x + dot[x].y) + (dot[x].z + dot[x].w)) * a.scale;
+      if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
+      if (a.slopes) s -= a.slopes[head] * fabsf(static_cast<float>(rk.pos - key));
+      // A row that saw no key (log-sum-exp -inf) gives nothing; unseen keys may hold anything.
+      if (key >= rk.lo && key < rk.hi && lse != neg_inf()) sum += expf(s - lse);
+    }
+  }
+  sums[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && key >= lo && key < hi) {
+    float* to = w.weights + h * w.slots + static_cast<long long>(a.L.block_offsets[r]) * a.L.b + key;
+    *to += (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+  }
+}
+
+template <typename T>
+int launch(const WeighArgs& w, cudaStream_t stream) {
+  const size_t bytes = shared_bytes(w.a.d);
+  auto kern = weigh_rows_kernel<T>;
+  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared_bytes(1024))));
+  if (rc) return rc;
+  const int tiles = (w.longest + kKeys - 1) / kKeys;
+  const long long ctas = static_cast<long long>(tiles) * w.a.L.hkv * w.a.R;
+  if (ctas > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
+  const int vector = w.a.d * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(w.a.L.k) % 16 == 0;
+  kern<<<static_cast<unsigned>(ctas), kWarps * 32, bytes, stream>>>(w, tiles, vector);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace
+
+int launch_weigh_rows(const WeighArgs& w, int kv_dtype, cudaStream_t stream) {
+  if (kv_dtype == kF32) return launch<float>(w, stream);
+  return kv_dtype == kBF16 ? launch<__nv_bfloat16>(w, stream) : launch<__half>(w, stream);
+}
+
+}  // namespace stk
