@@ -1112,8 +1112,8 @@ size_t plan_weigh(WeighArgs& w, const stk_kv* kv, int R, int T, int hq, int tota
   w.slots = static_cast<long long>(total_blocks) * kv->b;
   w.most = max_tokens;
   w.longest = max_length;
-  weigh_plan(w, (w.slots + kWeighKeys - 1) / kWeighKeys, sm_count_current());
-  const size_t ranges = masks ? (static_cast<size_t>(T) / w.tokens + R + 2) * sizeof(int4) : 0;
+  weigh_plan(w, sm_count_current());
+  const size_t ranges = masks ? weigh_range_bytes(w) : 0;
   return ranges + (w.parts > 1 ? static_cast<size_t>(w.parts) * kv->hkv * w.slots * sizeof(float) : 0);
 }
 }  // namespace
@@ -1159,7 +1159,8 @@ extern "C" int stk_accumulate_weights(const stk_kv* kv, int pages, const void* q
   unsigned char* at = static_cast<unsigned char*>(workspace);
   if (masks) {
     w.ranges = reinterpret_cast<int4*>(at);
-    at += (static_cast<size_t>(T) / w.tokens + R + 2) * sizeof(int4);
+    w.part_keys = reinterpret_cast<int2*>(w.ranges + static_cast<size_t>(T) / w.tokens + R + 2);
+    at += weigh_range_bytes(w);
   }
   if (w.parts > 1) w.partial = reinterpret_cast<float*>(at);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

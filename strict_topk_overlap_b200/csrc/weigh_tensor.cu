@@ -8,16 +8,21 @@
 // No running maximum, no reduction across threads, no atomics: a key's sum is
 // taken in the order of its rows.
 //
-// A job is 256 keys of one request's KV head and a part of its rows. The CTAs of a
-// persistent grid (one per SM) take every gridDim'th job; copies run ahead of
-// the products across the borders of jobs, the next job's K under the current
-// one's rows. With single tokens K streams through, with prompts the row tiles
-// do, one in shared memory for both halves of the keys (a tile from L2 serves
-// 256 x 112 scores: half of what 128 keys would ask of L2).
+// A job is 256 keys (128 where the rows are few) of one request's KV head and a
+// part of its rows. The CTAs of a persistent grid (one per SM) take the jobs in
+// turn; copies run ahead of the products across the borders of jobs, the next
+// job's K under the current one's rows. With single tokens K streams through a
+// ring of six tiles, with prompts the row tiles do, one in shared memory for
+// both halves of the keys (a tile from L2 serves 256 x 112 scores: half of
+// what 128 keys would ask of L2). Parts of the rows have sums of their own,
+// which a second kernel adds in order.
 //
-// Warps 0-7: exponentials and sums, one M tile of 128 keys each four. Warp 8:
-// MMAs. Warps 9-12: the walk over jobs and row tiles, log-sum-exps and key
-// intervals of the tiles' rows, K (warp 10) and Q (warp 9) by TMA.
+// Warps 0-15 (0-3 for few rows): exponentials and sums. Four take an MMA tile's
+// 128 keys, and where the rows are many two such groups half of the rows each,
+// in turn, and add up at a job's end. Then one warp for the MMAs, two for the copies (TMA; K and Q, or with few rows every
+// second job), and four for
+// the log-sum-exps and key intervals of the row tiles' rows, in turn. Those
+// five walk over jobs and row tiles alike; the others follow what they hand on.
 //
 // Rows that see none of a warp's keys are skipped tile by tile, tiles whose
 // rows all see all of a warp's keys need no mask. Unseen keys may hold
@@ -34,12 +39,10 @@ int set_wait_limit_weigh(unsigned long long ns) { return set_wait_limit_this_uni
 
 namespace {
 
-constexpr int kSumWarps = 8, kLoadWarps = 4, kThreads = (kSumWarps + 1 + kLoadWarps) * 32;
-constexpr int kBuffers = 2;  // S tiles in tensor memory, each 2 x 128 columns
-constexpr int kInfos = 4;    // row tiles whose rows' data are held
-constexpr int kRun = 16;     // rows taken from tensor memory at once
+constexpr int kInfoWarps = 4, kCopyWarps = 2;
+constexpr int kRun = 16;  // rows taken from tensor memory at once
 
-// Keys that a row tile's rows see: least and largest of any, and of all.
+// Keys that a row tile's rows see: least and end of any row's, of all rows'.
 struct Range {
   int any_lo, any_hi, all_lo, all_hi;
 };
@@ -49,40 +52,71 @@ struct Item {
   int first, last;     // of the job
   int empty;           // a job without rows: only its zeros are to be written
   int stop;
-  int cols;
   Range range;
   long long slot;      // of the request's first key, among the head's
-  int room;            // keys from k0 on that have slots
+  int room;            // keys from k0 on that are there
 };
 
+template <int ROWS, int KEYS>
 struct Info {
   Item item;
-  int odd[kLoadWarps];                      // a warp's rows are not all there, or have no weight
-  alignas(16) float neg_lse[kWeighRows];    // - log-sum-exp * log2 e
-  alignas(16) float2 bias[kWeighRows];      // slope * log2 e, place
-  alignas(16) int2 keys[kWeighRows];        // lo, hi
+  int odd;                           // its rows are not all there, or some have no weight
+  alignas(16) float neg_lse[ROWS];   // - log-sum-exp * log2 e
+  alignas(16) float2 bias[ROWS];     // slope * log2 e, place
+  alignas(16) int2 keys[ROWS];       // lo, hi
+  float other[KEYS > 128 ? KEYS : 1];  // sums of the second group's rows, at a job's end
 };
 
-template <int D>
+template <int D, bool FEW>
 struct Plan {
-  static constexpr int kKBytes = kWeighKeys * D * 2, kKHalf = kWeighKeys * 128;
-  static constexpr int kQBytes = kWeighRows * D * 2, kQHalf = kWeighRows * 128;
-  static constexpr int kKRing = 2, kQRing = D == 128 ? 3 : 6;
+  static constexpr int kTiles = FEW ? 1 : 2;        // MMA tiles of a job
+  static constexpr int kKeys = 128 * kTiles, kRows = FEW ? kWeighFew : kWeighRows;
+  static constexpr int kKBytes = kKeys * D * 2;  // 8 keys of 64 dims after 8 keys of 64 dims, 1,024 bytes each
+  static constexpr int kQBytes = kRows * D * 2, kQHalf = kRows * 128;
+  static constexpr int kKRing = FEW ? (D == 128 ? 6 : 10) : 2;
+  static constexpr int kQRing = FEW ? 4 : D == 128 ? 3 : 6;
+  static constexpr int kInfos = FEW ? 8 : 4;        // row tiles whose rows' data are held
+  static constexpr int kBuffers = FEW ? 4 : 2;      // S in tensor memory
+  static constexpr int kBufferCols = FEW ? 16 : 256, kTmem = kBuffers * kBufferCols;
+  static constexpr int kGroups = FEW ? 1 : 2;
+  static constexpr int kSumWarps = 4 * kTiles * kGroups, kThreads = (kSumWarps + 1 + kCopyWarps + kInfoWarps) * 32;
+  static_assert(kInfos % kInfoWarps == 0 && (!FEW || (kKRing % kCopyWarps == 0 && kQRing % kCopyWarps == 0)),
+                "each slot is filled by one warp");
 };
 
-template <int D>
+template <int D, bool FEW>
 struct Shared {
-  alignas(1024) unsigned char k[Plan<D>::kKRing][Plan<D>::kKBytes];
-  alignas(1024) unsigned char q[Plan<D>::kQRing][Plan<D>::kQBytes];
-  Info info[kInfos];
-  uint64_t k_full[Plan<D>::kKRing], k_empty[Plan<D>::kKRing];
-  uint64_t q_full[Plan<D>::kQRing], q_empty[Plan<D>::kQRing];
-  uint64_t i_full[kInfos], i_empty[kInfos];
-  uint64_t s_full[kBuffers][2], s_empty[kBuffers];
+  using P = Plan<D, FEW>;
+  alignas(1024) unsigned char k[P::kKRing][P::kKBytes];
+  alignas(1024) unsigned char q[P::kQRing][P::kQBytes];
+  Info<P::kRows, P::kKeys> info[P::kInfos];
+  uint64_t k_full[P::kKRing], k_empty[P::kKRing];
+  uint64_t q_full[P::kQRing], q_empty[P::kQRing];
+  uint64_t i_full[P::kInfos], i_empty[P::kInfos], i_other[P::kInfos];
+  uint64_t s_full[P::kBuffers][2], s_empty[P::kBuffers];
   uint64_t drained;
-  volatile int k_asked, q_asked;  // copies asked for
+  volatile int k_asked[kCopyWarps], q_asked[kCopyWarps];  // copies asked for, by each of the warps that ask
   uint32_t tmem;
 };
+
+// Copies by one elected lane, as predicates inside warp-uniform code (under a
+// branch, or with operands by lane, one takes over a hundred clocks).
+__device__ __forceinline__ void tma_keys(const CUtensorMap* map, uint32_t dst, uint32_t bar, int y, int page_head) {
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %3, %3, %4, %5}], "
+      "[%2];\n}\n" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(0), "r"(y), "r"(page_head)
+      : "memory");
+}
+__device__ __forceinline__ void tma_rows(const CUtensorMap* map, uint32_t dst, uint32_t bar, int x, int head, int token) {
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];\n}\n" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(head), "r"(token), "r"(0)
+      : "memory");
+}
 
 // The request r as it is weighed: its new tokens and its row tiles.
 struct Rows {
@@ -105,6 +139,24 @@ __device__ __forceinline__ Rows rows_of(const WeighArgs& w, int r) {
   return x;
 }
 
+__device__ __forceinline__ int parts_of(const WeighArgs& w, const Rows& x) { return (x.tiles + w.per_part - 1) / w.per_part; }
+
+// The keys [.x, .y) that any row of part p of a request sees.
+__device__ __forceinline__ int2 part_keys(const WeighArgs& w, const Rows& x, int p) {
+  if (w.part_keys) return w.part_keys[static_cast<long long>(x.t.r) * w.parts + p];
+  const int tiles = min(x.tiles, (p + 1) * w.per_part);
+  const int tokens = min(x.n, ((tiles - 1) / w.head_parts + 1) * w.tokens);
+  return make_int2(0, max(0, min(x.t.len - x.t.n + tokens, x.t.len)));
+}
+
+// Key tiles of a part: first and number.
+template <int KEYS>
+__device__ __forceinline__ int2 part_tiles(const WeighArgs& w, const Rows& x, int p) {
+  const int2 k = part_keys(w, x, p);
+  if (k.x >= k.y) return make_int2(0, 0);
+  return make_int2(k.x / KEYS, (k.y + KEYS - 1) / KEYS - k.x / KEYS);
+}
+
 // Keys that tokens [i, i + w.tokens) of a request see under the causal mask.
 __device__ __forceinline__ Range causal_range(const WeighArgs& w, const Rows& x, int i) {
   const int pos = x.t.len - x.t.n + i, last = min(w.tokens, x.n - i) - 1;
@@ -115,18 +167,28 @@ __device__ __forceinline__ Range causal_range(const WeighArgs& w, const Rows& x,
   return g;
 }
 
-// A warp's walk over the CTA's jobs and their row tiles. Four warps walk alike.
+// Keys that a chunk of a request's tokens sees.
+__device__ __forceinline__ Range range_of(const WeighArgs& w, const Rows& x, int chunk) {
+  if (w.ranges == nullptr) return causal_range(w, x, chunk * w.tokens);
+  const int4 g = w.ranges[weigh_range_at(x.t.t0, x.t.r, w.tokens) + chunk];
+  return Range{g.x, g.y, g.z, g.w};
+}
+
+// A warp's walk over the CTA's jobs and their row tiles; several warps walk
+// alike. FEW: every request is one row tile, one part.
+template <int KEYS, bool FEW>
 struct Walk {
   // a window of 32 requests, one per lane
-  int r0;
+  int r0, base;          // base: first block of the lane's request
   Rows mine;
-  int key_tiles;
+  int2 whole;            // key tiles of its only part (w.parts = 1)
+  Range only;            // keys of its only row tile (FEW)
   long long end, total, before;  // jobs up to the lane's request, of the window, before the window
-  long long job;
+  long long job;         // of all
+  int in_run;
   // the current job
   Rows x;
-  int h, k0, part, first_row;
-  long long slot;
+  int h, k0, part, first_row, block0;
   int room;
   int q, qb;             // next row tile, end of the job's
   // a window of 32 row tiles from `w0` on
@@ -138,15 +200,19 @@ struct Walk {
   __device__ __forceinline__ void window(const WeighArgs& w, int lane) {
     const int r = r0 + lane;
     mine = Rows{};
-    key_tiles = 0;
-    long long jobs = 0;
+    base = 0;
+    end = 0;
     if (r < w.a.R) {
       mine = rows_of(w, r);
-      key_tiles = mine.n > 0 ? (mine.t.len + kWeighKeys - 1) / kWeighKeys : 0;
-      const int parts = (mine.tiles + w.per_part - 1) / w.per_part;
-      jobs = static_cast<long long>(key_tiles) * parts * w.a.L.hkv;
+      base = w.a.L.block_offsets[r];
+      const int parts = parts_of(w, mine);
+      for (int p = 0; p < parts; ++p) {
+        whole = part_tiles<KEYS>(w, mine, p);
+        end += whole.y;
+      }
+      end *= w.a.L.hkv;
+      if (FEW && mine.n > 0) only = range_of(w, mine, 0);
     }
-    end = jobs;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long y = __shfl_up_sync(kFull, end, o);
@@ -158,8 +224,8 @@ struct Walk {
   __device__ __forceinline__ void start(const WeighArgs& w, int lane) {
     r0 = 0;
     before = 0;
-    job = static_cast<long long>(blockIdx.x) - gridDim.x;
     started = false;
+    whole = make_int2(0, 0);
     window(w, lane);
   }
 
@@ -167,16 +233,8 @@ struct Walk {
   __device__ __forceinline__ void look(const WeighArgs& w, int lane) {
     const int tile = w0 + lane;
     range = Range{0x7fffffff, 0, 0x7fffffff, 0};
-    if (tile < qb) {
-      const int c = tile / w.head_parts;
-      if (w.ranges) {
-        const int4 g = w.ranges[weigh_range_at(x.t.t0, x.t.r, w.tokens) + c];
-        range = Range{g.x, g.y, g.z, g.w};
-      } else {
-        range = causal_range(w, x, c * w.tokens);
-      }
-    }
-    seen = __ballot_sync(kFull, tile < qb && range.any_lo < k0 + kWeighKeys && range.any_hi > k0 && range.any_lo < range.any_hi);
+    if (tile < qb) range = range_of(w, x, w.head_parts == 1 ? tile : tile / w.head_parts);
+    seen = __ballot_sync(kFull, tile < qb && range.any_lo < k0 + KEYS && range.any_hi > k0 && range.any_lo < range.any_hi);
   }
 
   // The first row tile from q on that sees a key of the job: q, or qb if there is none.
@@ -198,7 +256,28 @@ struct Walk {
 
   // Moves to the next job; false when there is none.
   __device__ __forceinline__ bool next_job(const WeighArgs& w, int lane) {
-    job += gridDim.x;
+    if (!started) {
+      started = true;
+      in_run = 0;
+      job = static_cast<long long>(blockIdx.x) * w.run;
+    } else if (++in_run < w.run) {  // the next head of the same keys
+      ++job;
+      ++h;
+      if (FEW) {
+        q = 0;
+        return true;
+      }
+      q = part * w.per_part;
+      if (w0 != q) {
+        w0 = q;
+        look(w, lane);
+      }
+      find(w, lane);
+      return true;
+    } else {
+      in_run = 0;
+      job += 1 + static_cast<long long>(gridDim.x - 1) * w.run;
+    }
     while (job - before >= total) {
       before += total;
       r0 += 32;
@@ -214,14 +293,35 @@ struct Walk {
     x.t.len = __shfl_sync(kFull, mine.t.len, src);
     x.n = __shfl_sync(kFull, mine.n, src);
     x.tiles = __shfl_sync(kFull, mine.tiles, src);
-    const int tiles = __shfl_sync(kFull, key_tiles, src);
-    int at = static_cast<int>(job - before - begin);  // (part, key tile, head)
-    h = at % w.a.L.hkv;
-    at /= w.a.L.hkv;
-    k0 = at % tiles * kWeighKeys;
-    part = at / tiles;
-    slot = static_cast<long long>(w.a.L.block_offsets[x.t.r]) * w.a.L.b;
-    room = min(kWeighKeys, x.t.len - k0);
+    block0 = __shfl_sync(kFull, base, src);
+    const unsigned within = static_cast<unsigned>(job - before - begin), hkv = w.a.L.hkv;  // (part, key tile, head)
+    const int at = static_cast<int>(within / hkv);
+    h = static_cast<int>(within - at * hkv);
+    if (FEW || w.parts == 1) {
+      part = 0;
+      k0 = (__shfl_sync(kFull, whole.x, src) + at) * KEYS;
+    } else {  // the part: one per lane
+      int2 tiles = make_int2(0, 0);
+      if (lane < parts_of(w, x)) tiles = part_tiles<KEYS>(w, x, lane);
+      int sum = tiles.y;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(kFull, sum, o);
+        if (lane >= o) sum += y;
+      }
+      part = __popc(__ballot_sync(kFull, sum <= at));
+      k0 = (__shfl_sync(kFull, tiles.x, part) + at - (part ? __shfl_sync(kFull, sum, part - 1) : 0)) * KEYS;
+    }
+    room = min(KEYS, x.t.len - k0);
+    if (FEW) {
+      q = w0 = 0;
+      qb = 1;
+      range.any_lo = __shfl_sync(kFull, only.any_lo, src);
+      range.any_hi = __shfl_sync(kFull, only.any_hi, src);
+      range.all_lo = __shfl_sync(kFull, only.all_lo, src);
+      range.all_hi = __shfl_sync(kFull, only.all_hi, src);
+      return true;
+    }
     q = part * w.per_part;
     qb = min(x.tiles, q + w.per_part);
     w0 = q;
@@ -235,7 +335,6 @@ struct Walk {
     it.stop = it.empty = it.first = 0;
     if (!started || q >= qb) {
       do {
-        started = true;
         if (!next_job(w, lane)) {
           it.stop = 1;
           return;
@@ -248,12 +347,16 @@ struct Walk {
     it.h = h;
     it.k0 = k0;
     it.part = part;
-    it.slot = slot;
+    it.slot = static_cast<long long>(block0) * w.a.L.b;
     it.room = room;
-    it.cols = w.cols;
     it.last = 1;
     first_row = q;
     if (it.empty) return;
+    if (FEW) {
+      it.range = range;
+      q = 1;
+      return;
+    }
     const int src = q - w0;
     it.range.any_lo = __shfl_sync(kFull, range.any_lo, src);
     it.range.any_hi = __shfl_sync(kFull, range.any_hi, src);
@@ -263,27 +366,23 @@ struct Walk {
     find(w, lane);
     it.last = q >= qb;
   }
-
-  // The keys [.x, .y) that any of the job's rows sees; the row tiles' window is the first one's.
-  __device__ __forceinline__ int2 job_keys(const WeighArgs& w, int lane) {
-    if (w.ranges == nullptr) return make_int2(0, x.t.len);
-    int lo = 0x7fffffff, hi = 0;
-    for (int c = part * w.per_part / w.head_parts + lane; c * w.head_parts < qb; c += 32) {
-      const int4 g = w.ranges[weigh_range_at(x.t.t0, x.t.r, w.tokens) + c];
-      if (g.x < g.y) {
-        lo = min(lo, g.x);
-        hi = max(hi, g.y);
-      }
-    }
-    return make_int2(__reduce_min_sync(kFull, lo), __reduce_max_sync(kFull, hi));
-  }
 };
 
-// tanh for capped scores: odd polynomials in the raw score (least relative
-// error, fitted: 2.5e-9 up to 0.25, 4.2e-9 up to 1), the function beyond.
+// tanh for capped scores: odd polynomials (fitted for the least relative
+// error: 2.5e-9 up to 0.25, 4.2e-9 up to 1), 1 - 2 / (1 + e^2x) beyond, whose
+// absolute error of about 2^-23 is a rounding of the result there.
 __device__ constexpr float kTanh4[4] = {0.999999998f, -0.333332066f, 0.133231367f, -0.0513280764f};
 __device__ constexpr float kTanh8[8] = {0.999999996f,  -0.333332787f,  0.133321604f,  -0.0538709451f,
                                         0.0214648987f, -0.00791754669f, 0.00228229726f, -0.000353363486f};
+
+template <int N>
+__device__ __forceinline__ float2 cap_poly(float2 x, float cap2, const float (&c)[N]) {
+  const float2 y = mul2(x, x);
+  float2 p = both(cap2 * c[N - 1]);
+#pragma unroll
+  for (int i = N - 2; i >= 0; --i) p = fma2(p, y, both(cap2 * c[i]));
+  return mul2(x, p);
+}
 
 __device__ __forceinline__ void cap_scores(float2 (&s)[kRun / 2], float c1, float cap2) {
   float far[2] = {0.f, 0.f};
@@ -295,40 +394,34 @@ __device__ __forceinline__ void cap_scores(float2 (&s)[kRun / 2], float c1, floa
   const float most = fmaxf(far[0], far[1]);
   if (__all_sync(kFull, most <= 0.25f)) {
 #pragma unroll
-    for (int j = 0; j < kRun / 2; ++j) {
-      const float2 y = mul2(s[j], s[j]);
-      float2 p = both(cap2 * kTanh4[3]);
-#pragma unroll
-      for (int i = 2; i >= 0; --i) p = fma2(p, y, both(cap2 * kTanh4[i]));
-      s[j] = mul2(s[j], p);
-    }
-  } else if (__all_sync(kFull, most <= 1.f)) {
-#pragma unroll
-    for (int j = 0; j < kRun / 2; ++j) {
-      const float2 y = mul2(s[j], s[j]);
-      float2 p = both(cap2 * kTanh8[7]);
-#pragma unroll
-      for (int i = 6; i >= 0; --i) p = fma2(p, y, both(cap2 * kTanh8[i]));
-      s[j] = mul2(s[j], p);
-    }
+    for (int j = 0; j < kRun / 2; ++j) s[j] = cap_poly(s[j], cap2, kTanh4);
   } else {
-#pragma unroll 1
-    for (int j = 0; j < kRun / 2; ++j) s[j] = make_float2(cap2 * tanhf(s[j].x), cap2 * tanhf(s[j].y));
+    const bool near = __all_sync(kFull, most <= 1.f);
+#pragma unroll
+    for (int j = 0; j < kRun / 2; ++j) {
+      const float2 x = s[j];
+      s[j] = cap_poly(x, cap2, kTanh8);
+      if (!near) {
+        s[j].x = fabsf(x.x) <= 1.f ? s[j].x : cap2 * cap_tanh(x.x);
+        s[j].y = fabsf(x.y) <= 1.f ? s[j].y : cap2 * cap_tanh(x.y);
+      }
+    }
   }
 }
 
 // MODE: 1 capped scores, 2 biased by distance, 3 both.
-template <typename T, int D, int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int D, int MODE, bool FEW>
+__global__ void __launch_bounds__(Plan<D, FEW>::kThreads, 1)
 weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap qmap) {
-  using P = Plan<D>;
+  using P = Plan<D, FEW>;
+  constexpr int kSumWarps = P::kSumWarps, kThreads = P::kThreads, kInfos = P::kInfos, kBuffers = P::kBuffers;
   const PagedAttnArgs& a = w.a;
   constexpr int kHalves = D / 64;
   extern __shared__ __align__(1024) unsigned char base[];
-  Shared<D>& sh = *reinterpret_cast<Shared<D>*>(base);
+  Shared<D, FEW>& sh = *reinterpret_cast<Shared<D, FEW>*>(base);
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform(tid >> 5);
   if (warp == kSumWarps) {
-    tmem_alloc(&sh.tmem, 512);
+    tmem_alloc(&sh.tmem, P::kTmem);
   } else if (warp == 0 && lane == 0) {
     for (int i = 0; i < P::kKRing; ++i) {
       mbar_init(&sh.k_full[i], 1);
@@ -339,8 +432,9 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
       mbar_init(&sh.q_empty[i], 1);
     }
     for (int i = 0; i < kInfos; ++i) {
-      mbar_init(&sh.i_full[i], kLoadWarps);
+      mbar_init(&sh.i_full[i], 1);
       mbar_init(&sh.i_empty[i], kSumWarps + 1);
+      mbar_init(&sh.i_other[i], 4 * P::kTiles);
     }
     for (int i = 0; i < kBuffers; ++i) {
       mbar_init(&sh.s_full[i][0], 1);
@@ -348,7 +442,7 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
       mbar_init(&sh.s_empty[i], kSumWarps);
     }
     mbar_init(&sh.drained, 1);
-    sh.k_asked = sh.q_asked = 0;
+    for (int i = 0; i < kCopyWarps; ++i) sh.k_asked[i] = sh.q_asked[i] = 0;
     fence_barrier_init();
   }
   {
@@ -365,125 +459,159 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
   const uint32_t tmem = uniform(sh.tmem);
   bool ok = true;
 
-  if (warp > kSumWarps) {
-    // ------------------------------------------------------------ jobs, rows, copies
-    const int lw = warp - kSumWarps - 1, row = lw * 32 + lane;
-    const int row_tok = row / w.heads, row_head = row - row_tok * w.heads;
-    const int bp = min(a.L.page_size, 128), boxes = kWeighKeys / bp;
-    const uint32_t q_bytes = static_cast<uint32_t>(w.tokens) * w.heads * D * 2;
-    Walk walk;
+  if (warp > kSumWarps + kCopyWarps) {
+    // ------------------------------------------------------------ rows
+    const int turn = warp - kSumWarps - 1 - kCopyWarps;
+    constexpr int kPasses = (P::kRows + 31) / 32;
+    const int used = w.tokens * w.heads;
+    int row_tok[kPasses], row_head[kPasses];
+#pragma unroll
+    for (int j = 0; j < kPasses; ++j) {
+      row_tok[j] = (j * 32 + lane) / w.heads;
+      row_head[j] = j * 32 + lane - row_tok[j] * w.heads;
+    }
+    Walk<P::kKeys, FEW> walk;
     walk.start(w, lane);
-    Item now, then;
-    struct Mine {
-      float lse, slope;
-      RowKeys rk;
-      bool have;
-      int page, kq;  // K boxes of a job's first tile; row tile
-    };
-    // Loads of the lane's row (and, warp 1, its box of K) of an item: under way while the item before is handed on.
-    auto fetch = [&](const Item& it) {
-      Mine m{};
-      if (it.stop || it.empty) return m;
-      m.kq = walk.first_row;
-      const int c = m.kq / w.head_parts, tok = c * w.tokens + row_tok;
-      const int g = (m.kq - c * w.head_parts) * w.heads + row_head;
-      m.have = row < w.tokens * w.heads && tok < walk.x.n && g < a.G;
-      if (m.have) {
-        m.lse = w.lse[static_cast<long long>(walk.x.t.t0 + tok) * a.hq + it.h * a.G + g];
-        m.slope = (MODE & 2) ? a.slopes[it.h * a.G + g] : 0.f;
-        m.rk = row_keys(a, walk.x.t, tok);
-      }
-      if (lw == 1 && it.first) {
-        const int2 keys = walk.job_keys(w, lane);
-        const int key = it.k0 + lane * bp;
-        m.page = a.pages;
-        if (lane < boxes && key < keys.y && key + bp > keys.x) {
-          const int page = page_of(a, it.r, key);
-          m.page = page < 0 ? a.pages : page;
-        }
-      }
-      return m;
-    };
-    int n_info = 0, n_q = 0, n_k = 0;
-    walk.next(w, lane, now);
-    int t0 = walk.x.t.t0;
-    Mine m = fetch(now);
-    while (true) {
-      then.stop = 1;
-      int t0_then = 0;
-      Mine mt{};
-      if (!now.stop) {
-        walk.next(w, lane, then);
-        t0_then = walk.x.t.t0;
-        mt = fetch(then);
-      }
-      const int slot = n_info % kInfos;
-      if (n_info >= kInfos) ok = warp_wait(&sh.i_empty[slot], (n_info / kInfos - 1) & 1, a.status);
-      if (!ok) break;
-      Info& info = sh.info[slot];
-      if (lw == 0 && lane == 0) info.item = now;
-      if (!now.stop && !now.empty) {
-        // A row without weight (its log-sum-exp is -inf) sees no key. Rows that only fill up the MMA's are zeros
-        // with a log-sum-exp of infinity.
-        const bool live = m.have && m.lse != neg_inf(), fill = row >= w.tokens * w.heads;
-        if (row < kWeighRows) {
-          info.neg_lse[row] = live ? -m.lse * kLog2e : fill ? neg_inf() : 0.f;
-          info.keys[row] = live ? make_int2(m.rk.lo, m.rk.hi) : make_int2(0, 0);
-          if (MODE & 2) info.bias[row] = make_float2(m.slope * kLog2e, static_cast<float>(m.rk.pos));
-        }
-        const bool odd = __any_sync(kFull, !fill && !live);
-        if (lane == 0) info.odd[lw] = odd;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.i_full[slot]);
-      ++n_info;
-      if (now.stop) break;
-      if (!now.empty) {
-        if (lw == 1 && now.first) {
-          const int ks = n_k % P::kKRing;
-          if (n_k >= P::kKRing) ok = warp_wait(&sh.k_empty[ks], (n_k / P::kKRing - 1) & 1, a.status);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&sh.k_full[ks], P::kKBytes);
-          __syncwarp();
-          if (lane < boxes) {
-            const int y = (now.k0 + lane * bp) % a.L.page_size;
+    Item it;
+    for (int n = 0;; ++n) {
+      walk.next(w, lane, it);
+      if (n % kInfoWarps == turn) {
+        const int slot = n % kInfos;
+        auto& info = sh.info[slot];
+        float lse[kPasses], slope[kPasses];
+        RowKeys rk[kPasses];
+        bool have[kPasses];
+        if (!it.stop && !it.empty) {
+          const int c = w.head_parts == 1 ? walk.first_row : walk.first_row / w.head_parts;
+          const int t0 = c * w.tokens, g0 = (walk.first_row - c * w.head_parts) * w.heads;
 #pragma unroll
-            for (int half = 0; half < kHalves; ++half)
-              tma_load(&kmap, sh.k[ks] + half * P::kKHalf + lane * bp * 128, &sh.k_full[ks], half * 64, y, now.h, m.page);
+          for (int j = 0; j < kPasses; ++j) {
+            const int tok = t0 + row_tok[j], g = g0 + row_head[j];
+            have[j] = j * 32 + lane < used && tok < walk.x.n && g < a.G;
+            lse[j] = slope[j] = 0.f;
+            rk[j] = RowKeys{0, 0, 0};
+            if (have[j]) {
+              lse[j] = w.lse[static_cast<long long>(walk.x.t.t0 + tok) * a.hq + it.h * a.G + g];
+              if (MODE & 2) slope[j] = a.slopes[it.h * a.G + g];
+              rk[j] = row_keys(a, walk.x.t, tok);
+            }
           }
-          __syncwarp();
-          sh.k_asked = ++n_k;
         }
-        if (lw == 0) {
-          const int qs = n_q % P::kQRing;
-          if (n_q >= P::kQRing) ok = warp_wait(&sh.q_empty[qs], (n_q / P::kQRing - 1) & 1, a.status);
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&sh.q_full[qs], q_bytes);
-            const int c = m.kq / w.head_parts;
+        if (n >= kInfos) ok = warp_wait(&sh.i_empty[slot], (n / kInfos - 1) & 1, a.status);
+        if (!ok) break;
+        if (lane == 0) info.item = it;
+        if (!it.stop && !it.empty) {
+          // A row without weight (its log-sum-exp is -inf) sees no key. Rows that only fill up the MMA's are zeros
+          // with a log-sum-exp of infinity.
+          bool odd = false;
 #pragma unroll
-            for (int half = 0; half < kHalves; ++half)
-              tma_load(&qmap, sh.q[qs] + half * P::kQHalf, &sh.q_full[qs], half * 64,
-                       now.h * a.G + (m.kq - c * w.head_parts) * w.heads, t0 + c * w.tokens, 0);
+          for (int j = 0; j < kPasses; ++j) {
+            const int row = j * 32 + lane;
+            const bool live = have[j] && lse[j] != neg_inf(), fill = row >= used;
+            odd = odd || (!fill && !live);
+            if (row < P::kRows) {
+              info.neg_lse[row] = live ? -lse[j] * kLog2e : fill ? neg_inf() : 0.f;
+              info.keys[row] = live ? make_int2(rk[j].lo, rk[j].hi) : make_int2(0, 0);
+              if (MODE & 2) info.bias[row] = make_float2(slope[j] * kLog2e, static_cast<float>(rk[j].pos));
+            }
           }
-          __syncwarp();
-          sh.q_asked = ++n_q;
+          odd = __any_sync(kFull, odd);
+          if (lane == 0) info.odd = odd;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.i_full[slot]);
       }
-      now = then;
-      m = mt;
-      t0 = t0_then;
+      if (it.stop) break;
+    }
+  } else if (warp > kSumWarps) {
+    // ------------------------------------------------------------ copies
+    const int turn = warp - kSumWarps - 1;
+    const bool copies_k = FEW || turn == 0, copies_q = FEW || turn == 1;
+    const unsigned ps = a.L.page_size;
+    const int bp = min(a.L.page_size, 128), boxes = P::kKeys / bp, ppb = a.L.b / a.L.page_size;
+    const uint32_t q_bytes = static_cast<uint32_t>(w.tokens) * w.heads * D * 2;
+    Walk<P::kKeys, FEW> walk;
+    walk.start(w, lane);
+    int n = 0, n_q = 0, n_k = 0;  // items; row tiles and K tiles before the next one
+    struct Place {
+      int page, y;      // the lane's box of K: page, 8 keys of it
+      int token, head;  // of the row tile
+      int q, k;         // copies before it
+    };
+    // The warp's next item, and the page of the lane's box: its load is under way while the item before is copied.
+    auto next = [&](Item& it, Place& at) {
+      while (true) {
+        walk.next(w, lane, it);
+        if (it.stop) return;
+        if (it.empty) continue;
+        at.q = n_q++;
+        at.k = n_k;
+        if (it.first) ++n_k;
+        if (FEW ? n++ % kCopyWarps == turn : copies_q || it.first) break;
+      }
+      const int c = w.head_parts == 1 ? walk.first_row : walk.first_row / w.head_parts;
+      at.token = walk.x.t.t0 + c * w.tokens;
+      at.head = it.h * a.G + (walk.first_row - c * w.head_parts) * w.heads;
+      if (copies_k) {
+        const unsigned key = it.k0 + lane * bp;
+        const int2 keys = FEW ? make_int2(it.range.any_lo, it.range.any_hi) : part_keys(w, walk.x, it.part);
+        at.page = a.pages;
+        at.y = static_cast<int>(key % ps / 8);
+        if (lane < boxes && static_cast<int>(key) < keys.y && static_cast<int>(key) + bp > keys.x)
+          at.page = a.L.page_table[static_cast<long long>(walk.block0) * ppb + key / ps];
+      }
+    };
+    auto copy = [&](const Item& it, Place& at) {
+      if (copies_k) {
+        const int ks = at.k % P::kKRing;
+        if (at.k >= P::kKRing && !warp_wait(&sh.k_empty[ks], (at.k / P::kKRing - 1) & 1, a.status)) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&sh.k_full[ks], P::kKBytes);
+        __syncwarp();
+        if (at.page < 0 || at.page > a.pages) {  // reads as zeros
+          report(a.status, kStatusBadBlockId);
+          at.page = a.pages;
+        }
+        const uint32_t dst = uniform(smem_u32(sh.k[ks])), bar = uniform(smem_u32(&sh.k_full[ks]));
+        for (int x = 0; x < boxes; ++x) {
+          const int page = __shfl_sync(kFull, at.page, x), y = __shfl_sync(kFull, at.y, x);
+          tma_keys(&kmap, dst + x * bp * (D * 2), bar, y, page * a.L.hkv + it.h);
+        }
+        sh.k_asked[FEW ? turn : 0] = at.k + 1;
+      }
+      if (copies_q) {
+        const int qs = at.q % P::kQRing;
+        if (at.q >= P::kQRing && !warp_wait(&sh.q_empty[qs], (at.q / P::kQRing - 1) & 1, a.status)) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[qs], q_bytes);
+        __syncwarp();
+        const uint32_t dst = uniform(smem_u32(sh.q[qs])), bar = uniform(smem_u32(&sh.q_full[qs]));
+#pragma unroll
+        for (int half = 0; half < kHalves; ++half) tma_rows(&qmap, dst + half * P::kQHalf, bar, half * 64, at.head, at.token);
+        sh.q_asked[FEW ? turn : 0] = at.q + 1;
+      }
+      return true;
+    };
+    Item it[2];
+    Place at[2] = {};
+    next(it[0], at[0]);
+    while (true) {  // (two states by turns: no copy of one waits for its loads)
+      if (it[0].stop) break;
+      next(it[1], at[1]);
+      if (!copy(it[0], at[0]) || it[1].stop) break;
+      next(it[0], at[0]);
+      if (!copy(it[1], at[1])) break;
     }
   } else if (warp == kSumWarps) {
     // ------------------------------------------------------------ MMAs
     const uint32_t idesc = mma_desc<T>(128, w.cols, false);
-    const uint64_t k_desc = smem_desc(smem_u32(sh.k[0]), 16), q_desc = smem_desc(smem_u32(sh.q[0]), 16);
+    // K: groups of 8 keys lie D * 16 bytes apart, their 64-dim halves 1,024.
+    const uint64_t k_desc = (smem_desc(smem_u32(sh.k[0]), 16) & ~(0x3fffull << 32)) | static_cast<uint64_t>(D) << 32;
+    const uint64_t q_desc = smem_desc(smem_u32(sh.q[0]), 16);
     int n_info = 0, n_q = 0, n_k = 0;
     while (true) {
       const int slot = n_info % kInfos;
       ok = warp_wait(&sh.i_full[slot], (n_info / kInfos) & 1, a.status);
       if (!ok) break;
-      const Info& info = sh.info[slot];
+      const auto& info = sh.info[slot];
       const int stop = uniform(info.item.stop), empty = uniform(info.item.empty);
       const int first = uniform(info.item.first), last = uniform(info.item.last);
       __syncwarp();
@@ -498,11 +626,11 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
       if (!ok) break;
       fence_after();
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint64_t kd = k_desc + ((ks * P::kKBytes + half * 128 * 128) >> 4), qd = q_desc + (qs * P::kQBytes >> 4);
+      for (int half = 0; half < P::kTiles; ++half) {
+        const uint64_t kd = k_desc + ((ks * P::kKBytes + half * 128 * D * 2) >> 4), qd = q_desc + (qs * P::kQBytes >> 4);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          mma_ss(tmem + (buf * 2 + half) * 128, kd + (((s >> 2) * P::kKHalf + (s & 3) * 32) >> 4),
+          mma_ss(tmem + buf * P::kBufferCols + half * 128, kd + (((s >> 2) * 1024 + (s & 3) * 32) >> 4),
                  qd + (((s >> 2) * P::kQHalf + (s & 3) * 32) >> 4), idesc, s > 0);
         mma_commit(&sh.s_full[buf][half]);
       }
@@ -517,33 +645,42 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
     warp_wait(&sh.drained, 0, a.status);
   } else {
     // ------------------------------------------------------------ weights
-    const int half = warp >> 2, mine = half * 128 + (warp & 3) * 32;  // first of the warp's keys in the job
+    const int half = (warp >> 2) % P::kTiles, group = warp / (4 * P::kTiles);
+    const int mine = half * 128 + (warp & 3) * 32;  // first of the warp's keys in the job
     const uint32_t ts = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * 128;
     const float c = (MODE & 1) ? a.scale / a.softcap : a.scale * kLog2e, cap2 = a.softcap * kLog2e;
+    const int cols = w.cols, first_half = P::kGroups == 1 ? cols : (cols / kRun + 1) / 2 * kRun;
     float2 sum = make_float2(0.f, 0.f);
     int n_info = 0, n_s = 0;
     while (true) {
       const int slot = n_info % kInfos;
       ok = warp_wait(&sh.i_full[slot], (n_info / kInfos) & 1, a.status);
       if (!ok) break;
-      const Info& info = sh.info[slot];
+      auto& info = sh.info[slot];
       if (uniform(info.item.stop)) break;
       if (uniform(info.item.first)) sum = make_float2(0.f, 0.f);
       const int first_key = uniform(info.item.k0) + mine, key = first_key + lane;
       if (!uniform(info.item.empty)) {
-        const int buf = n_s % kBuffers, cols = uniform(info.item.cols);
+        const int buf = n_s % kBuffers;
         ok = warp_wait(&sh.s_full[buf][half], (n_s / kBuffers) & 1, a.status);
         if (!ok) break;
         fence_after();
         const Range g = info.item.range;
         const bool none = g.any_lo >= first_key + 32 || g.any_hi <= first_key;
-        const bool odd = (info.odd[0] | info.odd[1] | info.odd[2] | info.odd[3]) != 0;
-        const bool whole = !odd && g.all_lo <= first_key && g.all_hi >= first_key + 32;
+        const bool whole = !info.odd && g.all_lo <= first_key && g.all_hi >= first_key + 32;
+        // The group's rows [c0, c1): the first and larger half in turn.
+        const bool low = P::kGroups == 1 || ((n_s ^ group) & 1) == 0;
+        const int c0 = low ? 0 : first_half, c1 = low ? first_half : cols;
+        auto release = [&]() {  // the warp has read its S
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.s_empty[buf]);
+        };
         float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         auto tile = [&](auto whole_t) {
           constexpr bool WHOLE = decltype(whole_t)::value;
           float2 s[2][kRun / 2];
-          tmem_ld16(ts + buf * 256, reinterpret_cast<uint32_t*>(s[0]));
+          tmem_ld16(ts + buf * P::kBufferCols + c0, reinterpret_cast<uint32_t*>(s[0]));
           auto run = [&](float2 (&x)[kRun / 2], int j) {
             if (MODE & 1) cap_scores(x, c, cap2);
 #pragma unroll
@@ -570,36 +707,48 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
             }
           };
 #pragma unroll 1
-          for (int j = 0; j < cols; j += 2 * kRun) {
+          for (int j = c0; j < c1; j += 2 * kRun) {
             tmem_wait_ld();
             tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[0]));
-            const bool more = j + kRun < cols;
-            if (more) tmem_ld16(ts + buf * 256 + j + kRun, reinterpret_cast<uint32_t*>(s[1]));
+            const bool more = j + kRun < c1;
+            if (more) tmem_ld16(ts + buf * P::kBufferCols + j + kRun, reinterpret_cast<uint32_t*>(s[1]));
+            else release();
             run(s[0], j);
             if (more) {
               tmem_wait_ld();
               tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[1]));
-              if (j + 2 * kRun < cols) tmem_ld16(ts + buf * 256 + j + 2 * kRun, reinterpret_cast<uint32_t*>(s[0]));
+              if (j + 2 * kRun < c1) tmem_ld16(ts + buf * P::kBufferCols + j + 2 * kRun, reinterpret_cast<uint32_t*>(s[0]));
+              else release();
               run(s[1], j + kRun);
             }
           }
         };
-        if (!none) {
+        if (!none && c0 < c1) {
           if (whole) tile(std::true_type{});
           else tile(std::false_type{});
+        } else {
+          release();
         }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.s_empty[buf]);
         ++n_s;
         part[0] = add2(part[0], part[1]);
         sum = add2(sum, part[0]);
       }
-      if (uniform(info.item.last) && mine + lane < info.item.room) {
-        const long long at = info.item.h * w.slots + info.item.slot + key;
-        const float x = sum.x + sum.y;
-        if (w.partial) w.partial[info.item.part * w.slots * a.L.hkv + at] = x;
-        else if (x != 0.f) w.weights[at] += x;
+      if (P::kGroups == 2 && group == 1) {
+        if (uniform(info.item.last)) info.other[mine + lane] = sum.x + sum.y;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.i_other[slot]);
+      } else if (uniform(info.item.last)) {
+        float x = sum.x + sum.y;
+        if (P::kGroups == 2) {
+          ok = warp_wait(&sh.i_other[slot], (n_info / kInfos) & 1, a.status);
+          if (!ok) break;
+          x += info.other[mine + lane];
+        }
+        if (mine + lane < info.item.room) {
+          const long long at = info.item.h * w.slots + info.item.slot + key;
+          if (w.partial) w.partial[info.item.part * w.slots * a.L.hkv + at] = x;
+          else if (x != 0.f) atomicAdd(w.weights + at, x);  // the key's only one of the call: nothing waits for it
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.i_empty[slot]);
@@ -610,23 +759,30 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
   __syncthreads();
   if (warp == kSumWarps) {
     fence_after();
-    tmem_free(tmem, 512);
+    tmem_free(tmem, P::kTmem);
   } else if (warp == 0) {
     // After a wait that ran out the CTA does not end under copies that nobody waited for.
-    for (int i = max(0, sh.k_asked - P::kKRing); i < sh.k_asked; ++i)
-      if (!warp_wait(&sh.k_full[i % P::kKRing], (i / P::kKRing) & 1, a.status)) break;
-    for (int i = max(0, sh.q_asked - P::kQRing); i < sh.q_asked; ++i)
-      if (!warp_wait(&sh.q_full[i % P::kQRing], (i / P::kQRing) & 1, a.status)) break;
+    for (int c = 0; c < kCopyWarps; ++c) {
+      const int step = FEW ? kCopyWarps : 1;
+      for (int i = sh.k_asked[c] - 1; i >= 0 && i > sh.k_asked[c] - 1 - P::kKRing; i -= step)
+        if (!warp_wait(&sh.k_full[i % P::kKRing], (i / P::kKRing) & 1, a.status)) break;
+      for (int i = sh.q_asked[c] - 1; i >= 0 && i > sh.q_asked[c] - 1 - P::kQRing; i -= step)
+        if (!warp_wait(&sh.q_full[i % P::kQRing], (i / P::kQRing) & 1, a.status)) break;
+    }
   }
 }
 
-// What each chunk of w.tokens tokens sees, for masks that are given.
+// What each chunk of w.tokens tokens, and each part, sees, for masks that are
+// given. A CTA per part.
 __global__ void __launch_bounds__(256) weigh_ranges_kernel(const WeighArgs w) {
+  __shared__ int2 of_warp[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r = blockIdx.x;
+  const int r = blockIdx.x / w.parts, p = blockIdx.x % w.parts;
   const Rows x = rows_of(w, r);
   const long long at = weigh_range_at(x.t.t0, r, w.tokens);
-  for (int c = blockIdx.y * 8 + warp; c * w.tokens < x.n; c += gridDim.y * 8) {
+  int lo = 0x7fffffff, hi = 0;
+  for (int q = p * w.per_part + warp * w.head_parts; q < min(x.tiles, (p + 1) * w.per_part); q += 8 * w.head_parts) {
+    const int c = q / w.head_parts;  // (a chunk that two parts share is written twice, alike)
     Range g{0x7fffffff, 0, 0, 0x7fffffff};
     for (int i = c * w.tokens + lane; i < min(x.n, (c + 1) * w.tokens); i += 32) {
       const RowKeys k = row_keys(w.a, x.t, i);
@@ -642,21 +798,54 @@ __global__ void __launch_bounds__(256) weigh_ranges_kernel(const WeighArgs w) {
     g.all_lo = __reduce_max_sync(kFull, g.all_lo);
     g.all_hi = __reduce_min_sync(kFull, g.all_hi);
     if (lane == 0) w.ranges[at + c] = make_int4(g.any_lo, g.any_hi, g.all_lo, g.all_hi);
+    lo = min(lo, g.any_lo);
+    hi = max(hi, g.any_hi);
+  }
+  if (lane == 0) of_warp[warp] = make_int2(lo, hi);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 8; ++i) {
+      lo = min(lo, of_warp[i].x);
+      hi = max(hi, of_warp[i].y);
+    }
+    w.part_keys[blockIdx.x] = make_int2(lo, hi);
   }
 }
 
 // weights += the parts' sums, in the order of the parts.
+template <int KEYS>
 __global__ void __launch_bounds__(256) weigh_join_kernel(const WeighArgs w, int tiles) {
   const int tile = static_cast<int>(blockIdx.x % tiles);
   const int h = static_cast<int>(blockIdx.x / tiles) % w.a.L.hkv, r = static_cast<int>(blockIdx.x / tiles) / w.a.L.hkv;
   const Rows x = rows_of(w, r);
   const int key = tile * 256 + threadIdx.x;
   if (x.n == 0 || key >= x.t.len) return;
-  const int parts = (x.tiles + w.per_part - 1) / w.per_part;
+  const int parts = parts_of(w, x);
   const long long at = h * w.slots + static_cast<long long>(w.a.L.block_offsets[r]) * w.a.L.b + key;
   float sum = 0.f;
-  for (int p = 0; p < parts; ++p) sum += w.partial[p * w.slots * w.a.L.hkv + at];
-  w.weights[at] += sum;
+  for (int p = 0; p < parts; ++p) {
+    const int2 t = part_tiles<KEYS>(w, x, p);
+    if (key / KEYS >= t.x && key / KEYS < t.x + t.y) sum += w.partial[p * w.slots * w.a.L.hkv + at];
+  }
+  if (sum != 0.f) w.weights[at] += sum;
+}
+
+// A tensor map over K of the page pool: (64 dims, 8 keys, halves of a head,
+// groups of 8 keys, page and head); a box is a page of one head, or 128 keys of
+// it, in one copy.
+int encode_key_map(CUtensorMap* map, const PagedAttnArgs& a, int kv_dtype) {
+  const EncodeTiled fn = encode_tiled();
+  if (fn == nullptr) return static_cast<int>(cudaErrorNotSupported);
+  const cuuint64_t d = a.d, ps = a.L.page_size, halves = d / 64;
+  const cuuint64_t dims[5] = {64, 8, halves, ps / 8, static_cast<cuuint64_t>(a.pages) * a.L.hkv};
+  const cuuint64_t strides[4] = {d * 2, 128, d * 16, ps * d * 2};
+  const cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(halves), static_cast<cuuint32_t>((ps < 128 ? ps : 128) / 8), 1};
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(map, kv_dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                        const_cast<void*>(a.L.k), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : static_cast<int>(cudaErrorInvalidValue);
 }
 
 // A tensor map over the queries: boxes of 64 dims x w.heads heads x w.tokens tokens, 128-byte swizzle.
@@ -676,24 +865,31 @@ int encode_query_map(CUtensorMap* map, const WeighArgs& w, int kv_dtype) {
   return r == CUDA_SUCCESS ? 0 : 1;
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, bool FEW>
 int launch_mode(const WeighArgs& w, int sms, const CUtensorMap& km, const CUtensorMap& qm, cudaStream_t stream) {
-  auto kern = weigh_tensor_kernel<T, D, MODE>;
-  static_assert(sizeof(Shared<D>) <= 227 * 1024, "shared memory of a CTA");
-  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared<D>)));
+  constexpr int bytes = sizeof(Shared<D, FEW>);
+  static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
+  auto kern = weigh_tensor_kernel<T, D, MODE, FEW>;
+  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   if (rc) return rc;
-  kern<<<sms, kThreads, sizeof(Shared<D>), stream>>>(w, km, qm);
+  kern<<<sms, Plan<D, FEW>::kThreads, bytes, stream>>>(w, km, qm);
   return static_cast<int>(cudaGetLastError());
 }
 
-template <typename T, int D>
+template <typename T, int D, bool FEW>
 int launch_d(const WeighArgs& w, int sms, const CUtensorMap& km, const CUtensorMap& qm, cudaStream_t stream) {
   switch ((w.a.softcap > 0.f ? 1 : 0) | (w.a.slopes ? 2 : 0)) {
-    case 0: return launch_mode<T, D, 0>(w, sms, km, qm, stream);
-    case 1: return launch_mode<T, D, 1>(w, sms, km, qm, stream);
-    case 2: return launch_mode<T, D, 2>(w, sms, km, qm, stream);
-    default: return launch_mode<T, D, 3>(w, sms, km, qm, stream);
+    case 0: return launch_mode<T, D, 0, FEW>(w, sms, km, qm, stream);
+    case 1: return launch_mode<T, D, 1, FEW>(w, sms, km, qm, stream);
+    case 2: return launch_mode<T, D, 2, FEW>(w, sms, km, qm, stream);
+    default: return launch_mode<T, D, 3, FEW>(w, sms, km, qm, stream);
   }
+}
+
+template <typename T>
+int launch_t(const WeighArgs& w, int sms, const CUtensorMap& km, const CUtensorMap& qm, cudaStream_t stream) {
+  if (w.few) return w.a.d == 64 ? launch_d<T, 64, true>(w, sms, km, qm, stream) : launch_d<T, 128, true>(w, sms, km, qm, stream);
+  return w.a.d == 64 ? launch_d<T, 64, false>(w, sms, km, qm, stream) : launch_d<T, 128, false>(w, sms, km, qm, stream);
 }
 
 }  // namespace
@@ -709,24 +905,24 @@ bool weigh_tensor_takes(int kv_dtype, int d, int page_size, const void* k, const
 
 int launch_weigh_tensor(const WeighArgs& w, int kv_dtype, int sms, cudaStream_t stream) {
   CUtensorMap km, qm;
-  int rc = encode_pool_map(&km, w.a, w.a.L.k, kv_dtype, w.a.L.page_size < 128 ? w.a.L.page_size : 128);
+  int rc = encode_key_map(&km, w.a, kv_dtype);
   if (rc) return rc;
   rc = encode_query_map(&qm, w, kv_dtype);
   if (rc) return rc;
   if (w.ranges) {
-    weigh_ranges_kernel<<<dim3(w.a.R, 16), 256, 0, stream>>>(w);
+    const long long ctas = static_cast<long long>(w.a.R) * w.parts;
+    if (ctas > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
+    weigh_ranges_kernel<<<static_cast<unsigned>(ctas), 256, 0, stream>>>(w);
     rc = static_cast<int>(cudaGetLastError());
     if (rc) return rc;
   }
-  if (kv_dtype == kBF16)
-    rc = w.a.d == 64 ? launch_d<__nv_bfloat16, 64>(w, sms, km, qm, stream) : launch_d<__nv_bfloat16, 128>(w, sms, km, qm, stream);
-  else
-    rc = w.a.d == 64 ? launch_d<__half, 64>(w, sms, km, qm, stream) : launch_d<__half, 128>(w, sms, km, qm, stream);
+  rc = kv_dtype == kBF16 ? launch_t<__nv_bfloat16>(w, sms, km, qm, stream) : launch_t<__half>(w, sms, km, qm, stream);
   if (rc || !w.partial) return rc;
   const int tiles = (w.longest + 255) / 256;
   const long long ctas = static_cast<long long>(tiles) * w.a.L.hkv * w.a.R;
   if (ctas > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
-  weigh_join_kernel<<<static_cast<unsigned>(ctas), 256, 0, stream>>>(w, tiles);
+  const auto join = w.few ? weigh_join_kernel<128> : weigh_join_kernel<256>;
+  join<<<static_cast<unsigned>(ctas), 256, 0, stream>>>(w, tiles);
   return static_cast<int>(cudaGetLastError());
 }
 
