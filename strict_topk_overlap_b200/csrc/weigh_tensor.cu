@@ -19,10 +19,10 @@
 //
 // Warps 0-15 (0-3 for few rows): exponentials and sums. Four take an MMA tile's
 // 128 keys, and where the rows are many two such groups half of the rows each,
-// in turn, and add up at a job's end. Then one warp for the MMAs, two for the copies (TMA; K and Q, or with few rows every
-// second job), and four for
-// the log-sum-exps and key intervals of the row tiles' rows, in turn. Those
-// five walk over jobs and row tiles alike; the others follow what they hand on.
+// in turn, and add up at a job's end. Then one warp for the MMAs, two for the
+// copies (TMA; K and Q, or with few rows every second job), one that walks over
+// jobs and row tiles ahead of all others, and four for the log-sum-exps and key
+// intervals of the row tiles' rows, in turn.
 //
 // Rows that see none of a warp's keys are skipped tile by tile, tiles whose
 // rows all see all of a warp's keys need no mask. Unseen keys may hold
@@ -47,15 +47,21 @@ struct Range {
   int any_lo, any_hi, all_lo, all_hi;
 };
 
-struct Item {
-  int r, h, k0, part;  // job: request, KV head, first key, part
+// A row tile of a job.
+struct alignas(16) Item {
+  int h, k0, part;     // job: KV head, first key, part of the request's rows
+  int room;            // keys from k0 on that are there
   int first, last;     // of the job
   int empty;           // a job without rows: only its zeros are to be written
   int stop;
   Range range;
-  long long slot;      // of the request's first key, among the head's
-  int room;            // keys from k0 on that are there
+  int block0;          // the request: first block, new tokens, tokens in the cache, tokens weighed
+  int t0, n_all, len;
+  int n, tile;         // row tile
+  int keys_lo, keys_hi;  // that the part's rows see
+  int q, k;            // row tiles and K tiles copied before it
 };
+static_assert(sizeof(Item) % 16 == 0, "moved in 16 bytes");
 
 template <int ROWS, int KEYS>
 struct Info {
@@ -76,10 +82,11 @@ struct Plan {
   static constexpr int kKRing = FEW ? (D == 128 ? 6 : 10) : 2;
   static constexpr int kQRing = FEW ? 4 : D == 128 ? 3 : 6;
   static constexpr int kInfos = FEW ? 8 : 4;        // row tiles whose rows' data are held
+  static constexpr int kAhead = 8;                  // row tiles that the walk is ahead
   static constexpr int kBuffers = FEW ? 4 : 2;      // S in tensor memory
   static constexpr int kBufferCols = FEW ? 16 : 256, kTmem = kBuffers * kBufferCols;
   static constexpr int kGroups = FEW ? 1 : 2;
-  static constexpr int kSumWarps = 4 * kTiles * kGroups, kThreads = (kSumWarps + 1 + kCopyWarps + kInfoWarps) * 32;
+  static constexpr int kSumWarps = 4 * kTiles * kGroups, kThreads = (kSumWarps + 2 + kCopyWarps + kInfoWarps) * 32;
   static_assert(kInfos % kInfoWarps == 0 && (!FEW || (kKRing % kCopyWarps == 0 && kQRing % kCopyWarps == 0)),
                 "each slot is filled by one warp");
 };
@@ -90,9 +97,11 @@ struct Shared {
   alignas(1024) unsigned char k[P::kKRing][P::kKBytes];
   alignas(1024) unsigned char q[P::kQRing][P::kQBytes];
   Info<P::kRows, P::kKeys> info[P::kInfos];
+  Item ahead[P::kAhead];
   uint64_t k_full[P::kKRing], k_empty[P::kKRing];
   uint64_t q_full[P::kQRing], q_empty[P::kQRing];
   uint64_t i_full[P::kInfos], i_empty[P::kInfos], i_other[P::kInfos];
+  uint64_t w_full[P::kAhead], w_empty[P::kAhead];
   uint64_t s_full[P::kBuffers][2], s_empty[P::kBuffers];
   uint64_t drained;
   volatile int k_asked[kCopyWarps], q_asked[kCopyWarps];  // copies asked for, by each of the warps that ask
@@ -174,8 +183,8 @@ __device__ __forceinline__ Range range_of(const WeighArgs& w, const Rows& x, int
   return Range{g.x, g.y, g.z, g.w};
 }
 
-// A warp's walk over the CTA's jobs and their row tiles; several warps walk
-// alike. FEW: every request is one row tile, one part.
+// The walk over the CTA's jobs and their row tiles, by one warp. FEW: every
+// request is one row tile, one part.
 template <int KEYS, bool FEW>
 struct Walk {
   // a window of 32 requests, one per lane
@@ -186,16 +195,20 @@ struct Walk {
   long long end, total, before;  // jobs up to the lane's request, of the window, before the window
   long long job;         // of all
   int in_run;
-  // the current job
+  // the current request and its parts, one per lane: first key tile, key tiles up to it
   Rows x;
-  int h, k0, part, first_row, block0;
-  int room;
+  int block0, part_first, part_end;
+  long long x_begin, x_end;  // its jobs, within the window
+  // the current job
+  int h, k0, part;
+  int2 keys;             // that the part's rows see
   int q, qb;             // next row tile, end of the job's
   // a window of 32 row tiles from `w0` on
   int w0;
   Range range;
   unsigned seen;
   bool started;
+  int n_q, n_k;
 
   __device__ __forceinline__ void window(const WeighArgs& w, int lane) {
     const int r = r0 + lane;
@@ -226,6 +239,8 @@ struct Walk {
     before = 0;
     started = false;
     whole = make_int2(0, 0);
+    x_begin = x_end = 0;
+    n_q = n_k = 0;
     window(w, lane);
   }
 
@@ -283,48 +298,59 @@ struct Walk {
       r0 += 32;
       if (r0 >= w.a.R) return false;
       window(w, lane);
+      x_end = 0;
     }
-    const int src = __popc(__ballot_sync(kFull, end <= job - before));
-    const long long begin = src ? __shfl_sync(kFull, end, src - 1) : 0;
-    x.t.r = r0 + src;
-    x.t.row0 = x.t.rows = 0;
-    x.t.t0 = __shfl_sync(kFull, mine.t.t0, src);
-    x.t.n = __shfl_sync(kFull, mine.t.n, src);
-    x.t.len = __shfl_sync(kFull, mine.t.len, src);
-    x.n = __shfl_sync(kFull, mine.n, src);
-    x.tiles = __shfl_sync(kFull, mine.tiles, src);
-    block0 = __shfl_sync(kFull, base, src);
-    const unsigned within = static_cast<unsigned>(job - before - begin), hkv = w.a.L.hkv;  // (part, key tile, head)
+    const long long here = job - before;
+    if (here >= x_end || here < x_begin) {  // another request
+      const int src = __popc(__ballot_sync(kFull, end <= here));
+      x_end = __shfl_sync(kFull, end, src);
+      x_begin = src ? __shfl_sync(kFull, end, src - 1) : 0;
+      x.t.r = r0 + src;
+      x.t.row0 = x.t.rows = 0;
+      x.t.t0 = __shfl_sync(kFull, mine.t.t0, src);
+      x.t.n = __shfl_sync(kFull, mine.t.n, src);
+      x.t.len = __shfl_sync(kFull, mine.t.len, src);
+      x.n = __shfl_sync(kFull, mine.n, src);
+      x.tiles = __shfl_sync(kFull, mine.tiles, src);
+      block0 = __shfl_sync(kFull, base, src);
+      if (FEW || w.parts == 1) {
+        part_first = __shfl_sync(kFull, whole.x, src);
+      } else {
+        int2 tiles = make_int2(0, 0);
+        if (lane < parts_of(w, x)) tiles = part_tiles<KEYS>(w, x, lane);
+        part_first = tiles.x;
+        part_end = tiles.y;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(kFull, part_end, o);
+          if (lane >= o) part_end += y;
+        }
+      }
+      if (FEW) {
+        range.any_lo = __shfl_sync(kFull, only.any_lo, src);
+        range.any_hi = __shfl_sync(kFull, only.any_hi, src);
+        range.all_lo = __shfl_sync(kFull, only.all_lo, src);
+        range.all_hi = __shfl_sync(kFull, only.all_hi, src);
+      }
+    }
+    const unsigned within = static_cast<unsigned>(here - x_begin), hkv = w.a.L.hkv;  // (part, key tile, head)
     const int at = static_cast<int>(within / hkv);
     h = static_cast<int>(within - at * hkv);
     if (FEW || w.parts == 1) {
       part = 0;
-      k0 = (__shfl_sync(kFull, whole.x, src) + at) * KEYS;
-    } else {  // the part: one per lane
-      int2 tiles = make_int2(0, 0);
-      if (lane < parts_of(w, x)) tiles = part_tiles<KEYS>(w, x, lane);
-      int sum = tiles.y;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(kFull, sum, o);
-        if (lane >= o) sum += y;
-      }
-      part = __popc(__ballot_sync(kFull, sum <= at));
-      k0 = (__shfl_sync(kFull, tiles.x, part) + at - (part ? __shfl_sync(kFull, sum, part - 1) : 0)) * KEYS;
-    }
-    room = min(KEYS, x.t.len - k0);
-    if (FEW) {
-      q = w0 = 0;
-      qb = 1;
-      range.any_lo = __shfl_sync(kFull, only.any_lo, src);
-      range.any_hi = __shfl_sync(kFull, only.any_hi, src);
-      range.all_lo = __shfl_sync(kFull, only.all_lo, src);
-      range.all_hi = __shfl_sync(kFull, only.all_hi, src);
-      return true;
+      k0 = (part_first + at) * KEYS;
+    } else {
+      part = __popc(__ballot_sync(kFull, part_end <= at));
+      k0 = (__shfl_sync(kFull, part_first, part) + at - (part ? __shfl_sync(kFull, part_end, part - 1) : 0)) * KEYS;
     }
     q = part * w.per_part;
     qb = min(x.tiles, q + w.per_part);
     w0 = q;
+    if (FEW) {
+      keys = make_int2(range.any_lo, range.any_hi);
+      return true;
+    }
+    keys = part_keys(w, x, part);
     look(w, lane);
     find(w, lane);
     return true;
@@ -343,18 +369,26 @@ struct Walk {
       it.first = 1;
       it.empty = q >= qb;
     }
-    it.r = x.t.r;
     it.h = h;
     it.k0 = k0;
     it.part = part;
-    it.slot = static_cast<long long>(block0) * w.a.L.b;
-    it.room = room;
+    it.room = min(KEYS, x.t.len - k0);
     it.last = 1;
-    first_row = q;
+    it.block0 = block0;
+    it.t0 = x.t.t0;
+    it.n_all = x.t.n;
+    it.len = x.t.len;
+    it.n = x.n;
+    it.tile = q;
+    it.keys_lo = keys.x;
+    it.keys_hi = keys.y;
     if (it.empty) return;
+    it.q = n_q++;
+    if (it.first) ++n_k;
+    it.k = n_k - 1;
+    it.range = range;
     if (FEW) {
-      it.range = range;
-      q = 1;
+      q = qb;
       return;
     }
     const int src = q - w0;
@@ -436,6 +470,10 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
       mbar_init(&sh.i_empty[i], kSumWarps + 1);
       mbar_init(&sh.i_other[i], 4 * P::kTiles);
     }
+    for (int i = 0; i < P::kAhead; ++i) {
+      mbar_init(&sh.w_full[i], 1);
+      mbar_init(&sh.w_empty[i], 1 + kCopyWarps);
+    }
     for (int i = 0; i < kBuffers; ++i) {
       mbar_init(&sh.s_full[i][0], 1);
       mbar_init(&sh.s_full[i][1], 1);
@@ -459,9 +497,20 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
   const uint32_t tmem = uniform(sh.tmem);
   bool ok = true;
 
-  if (warp > kSumWarps + kCopyWarps) {
+  // The item at place n of the walk, for a warp that reads it ahead of the products.
+  auto read = [&](int n, Item& it) {
+    const int slot = n % P::kAhead;
+    if (!warp_wait(&sh.w_full[slot], (n / P::kAhead) & 1, a.status)) return false;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(Item) / 16); ++i)
+      reinterpret_cast<int4*>(&it)[i] = reinterpret_cast<const int4*>(&sh.ahead[slot])[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.w_empty[slot]);
+    return true;
+  };
+  if (warp > kSumWarps + 1 + kCopyWarps) {
     // ------------------------------------------------------------ rows
-    const int turn = warp - kSumWarps - 1 - kCopyWarps;
+    const int turn = warp - kSumWarps - 2 - kCopyWarps;
     constexpr int kPasses = (P::kRows + 31) / 32;
     const int used = w.tokens * w.heads;
     int row_tok[kPasses], row_head[kPasses];
@@ -470,58 +519,80 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
       row_tok[j] = (j * 32 + lane) / w.heads;
       row_head[j] = j * 32 + lane - row_tok[j] * w.heads;
     }
+    for (int n = turn;; n += kInfoWarps) {
+      Item it;
+      ok = read(n, it);
+      if (!ok) break;
+      const int slot = n % kInfos;
+      auto& info = sh.info[slot];
+      float lse[kPasses], slope[kPasses];
+      RowKeys rk[kPasses];
+      bool have[kPasses];
+      const bool rows = !it.stop && !it.empty;
+      if (rows) {
+        const int c = w.head_parts == 1 ? it.tile : it.tile / w.head_parts;
+        const int first = c * w.tokens, g0 = (it.tile - c * w.head_parts) * w.heads;
+        RowTile t;
+        t.r = t.row0 = t.rows = 0;
+        t.t0 = it.t0;
+        t.n = it.n_all;
+        t.len = it.len;
+#pragma unroll
+        for (int j = 0; j < kPasses; ++j) {
+          const int tok = first + row_tok[j], g = g0 + row_head[j];
+          have[j] = j * 32 + lane < used && tok < it.n && g < a.G;
+          lse[j] = slope[j] = 0.f;
+          rk[j] = RowKeys{0, 0, 0};
+          if (have[j]) {
+            lse[j] = w.lse[static_cast<long long>(it.t0 + tok) * a.hq + it.h * a.G + g];
+            if (MODE & 2) slope[j] = a.slopes[it.h * a.G + g];
+            rk[j] = row_keys(a, t, tok);
+          }
+        }
+      }
+      if (n >= kInfos) ok = warp_wait(&sh.i_empty[slot], (n / kInfos - 1) & 1, a.status);
+      if (!ok) break;
+      if (lane == 0) info.item = it;
+      if (rows) {
+        // A row without weight (its log-sum-exp is -inf) sees no key. Rows that only fill up the MMA's are zeros
+        // with a log-sum-exp of infinity.
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < kPasses; ++j) {
+          const int row = j * 32 + lane;
+          const bool live = have[j] && lse[j] != neg_inf(), fill = row >= used;
+          odd = odd || (!fill && !live);
+          if (row < P::kRows) {
+            info.neg_lse[row] = live ? -lse[j] * kLog2e : fill ? neg_inf() : 0.f;
+            info.keys[row] = live ? make_int2(rk[j].lo, rk[j].hi) : make_int2(0, 0);
+            if (MODE & 2) info.bias[row] = make_float2(slope[j] * kLog2e, static_cast<float>(rk[j].pos));
+          }
+        }
+        odd = __any_sync(kFull, odd);
+        if (lane == 0) info.odd = odd;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.i_full[slot]);
+      if (it.stop) break;
+    }
+  } else if (warp == kSumWarps + 1 + kCopyWarps) {
+    // ------------------------------------------------------------ the walk
     Walk<P::kKeys, FEW> walk;
     walk.start(w, lane);
     Item it;
     for (int n = 0;; ++n) {
       walk.next(w, lane, it);
-      if (n % kInfoWarps == turn) {
-        const int slot = n % kInfos;
-        auto& info = sh.info[slot];
-        float lse[kPasses], slope[kPasses];
-        RowKeys rk[kPasses];
-        bool have[kPasses];
-        if (!it.stop && !it.empty) {
-          const int c = w.head_parts == 1 ? walk.first_row : walk.first_row / w.head_parts;
-          const int t0 = c * w.tokens, g0 = (walk.first_row - c * w.head_parts) * w.heads;
-#pragma unroll
-          for (int j = 0; j < kPasses; ++j) {
-            const int tok = t0 + row_tok[j], g = g0 + row_head[j];
-            have[j] = j * 32 + lane < used && tok < walk.x.n && g < a.G;
-            lse[j] = slope[j] = 0.f;
-            rk[j] = RowKeys{0, 0, 0};
-            if (have[j]) {
-              lse[j] = w.lse[static_cast<long long>(walk.x.t.t0 + tok) * a.hq + it.h * a.G + g];
-              if (MODE & 2) slope[j] = a.slopes[it.h * a.G + g];
-              rk[j] = row_keys(a, walk.x.t, tok);
-            }
-          }
-        }
-        if (n >= kInfos) ok = warp_wait(&sh.i_empty[slot], (n / kInfos - 1) & 1, a.status);
+      // Its end is told to each of the warps that take turns.
+      const int times = it.stop ? kInfoWarps : 1;
+      for (int i = 0; ok && i < times; ++i, n += i < times) {
+        const int slot = n % P::kAhead;
+        if (n >= P::kAhead) ok = warp_wait(&sh.w_empty[slot], (n / P::kAhead - 1) & 1, a.status);
         if (!ok) break;
-        if (lane == 0) info.item = it;
-        if (!it.stop && !it.empty) {
-          // A row without weight (its log-sum-exp is -inf) sees no key. Rows that only fill up the MMA's are zeros
-          // with a log-sum-exp of infinity.
-          bool odd = false;
-#pragma unroll
-          for (int j = 0; j < kPasses; ++j) {
-            const int row = j * 32 + lane;
-            const bool live = have[j] && lse[j] != neg_inf(), fill = row >= used;
-            odd = odd || (!fill && !live);
-            if (row < P::kRows) {
-              info.neg_lse[row] = live ? -lse[j] * kLog2e : fill ? neg_inf() : 0.f;
-              info.keys[row] = live ? make_int2(rk[j].lo, rk[j].hi) : make_int2(0, 0);
-              if (MODE & 2) info.bias[row] = make_float2(slope[j] * kLog2e, static_cast<float>(rk[j].pos));
-            }
-          }
-          odd = __any_sync(kFull, odd);
-          if (lane == 0) info.odd = odd;
-        }
+        if (lane == 0) sh.ahead[slot] = it;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.i_full[slot]);
+        if (lane == 0) mbar_arrive(&sh.w_full[slot]);
       }
-      if (it.stop) break;
+      if (!ok || it.stop) break;
     }
   } else if (warp > kSumWarps) {
     // ------------------------------------------------------------ copies
@@ -530,75 +601,43 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
     const unsigned ps = a.L.page_size;
     const int bp = min(a.L.page_size, 128), boxes = P::kKeys / bp, ppb = a.L.b / a.L.page_size;
     const uint32_t q_bytes = static_cast<uint32_t>(w.tokens) * w.heads * D * 2;
-    Walk<P::kKeys, FEW> walk;
-    walk.start(w, lane);
-    int n = 0, n_q = 0, n_k = 0;  // items; row tiles and K tiles before the next one
-    struct Place {
-      int page, y;      // the lane's box of K: page, 8 keys of it
-      int token, head;  // of the row tile
-      int q, k;         // copies before it
-    };
-    // The warp's next item, and the page of the lane's box: its load is under way while the item before is copied.
-    auto next = [&](Item& it, Place& at) {
-      while (true) {
-        walk.next(w, lane, it);
-        if (it.stop) return;
-        if (it.empty) continue;
-        at.q = n_q++;
-        at.k = n_k;
-        if (it.first) ++n_k;
-        if (FEW ? n++ % kCopyWarps == turn : copies_q || it.first) break;
-      }
-      const int c = w.head_parts == 1 ? walk.first_row : walk.first_row / w.head_parts;
-      at.token = walk.x.t.t0 + c * w.tokens;
-      at.head = it.h * a.G + (walk.first_row - c * w.head_parts) * w.heads;
-      if (copies_k) {
+    for (int n = 0;; ++n) {
+      Item it;
+      ok = read(n, it);
+      if (!ok || it.stop) break;
+      if (it.empty || (FEW && it.q % kCopyWarps != turn)) continue;
+      if (copies_k && it.first) {
         const unsigned key = it.k0 + lane * bp;
-        const int2 keys = FEW ? make_int2(it.range.any_lo, it.range.any_hi) : part_keys(w, walk.x, it.part);
-        at.page = a.pages;
-        at.y = static_cast<int>(key % ps / 8);
-        if (lane < boxes && static_cast<int>(key) < keys.y && static_cast<int>(key) + bp > keys.x)
-          at.page = a.L.page_table[static_cast<long long>(walk.block0) * ppb + key / ps];
-      }
-    };
-    auto copy = [&](const Item& it, Place& at) {
-      if (copies_k) {
-        const int ks = at.k % P::kKRing;
-        if (at.k >= P::kKRing && !warp_wait(&sh.k_empty[ks], (at.k / P::kKRing - 1) & 1, a.status)) return false;
+        int page = a.pages, y = static_cast<int>(key % ps / 8);
+        if (lane < boxes && static_cast<int>(key) < it.keys_hi && static_cast<int>(key) + bp > it.keys_lo)
+          page = a.L.page_table[static_cast<long long>(it.block0) * ppb + key / ps];
+        const int ks = it.k % P::kKRing;
+        if (it.k >= P::kKRing) ok = warp_wait(&sh.k_empty[ks], (it.k / P::kKRing - 1) & 1, a.status);
+        if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&sh.k_full[ks], P::kKBytes);
         __syncwarp();
-        if (at.page < 0 || at.page > a.pages) {  // reads as zeros
+        if (page < 0 || page > a.pages) {  // reads as zeros
           report(a.status, kStatusBadBlockId);
-          at.page = a.pages;
+          page = a.pages;
         }
         const uint32_t dst = uniform(smem_u32(sh.k[ks])), bar = uniform(smem_u32(&sh.k_full[ks]));
-        for (int x = 0; x < boxes; ++x) {
-          const int page = __shfl_sync(kFull, at.page, x), y = __shfl_sync(kFull, at.y, x);
-          tma_keys(&kmap, dst + x * bp * (D * 2), bar, y, page * a.L.hkv + it.h);
-        }
-        sh.k_asked[FEW ? turn : 0] = at.k + 1;
+        for (int x = 0; x < boxes; ++x)
+          tma_keys(&kmap, dst + x * bp * (D * 2), bar, __shfl_sync(kFull, y, x), __shfl_sync(kFull, page, x) * a.L.hkv + uniform(it.h));
+        sh.k_asked[FEW ? turn : 0] = it.k + 1;
       }
       if (copies_q) {
-        const int qs = at.q % P::kQRing;
-        if (at.q >= P::kQRing && !warp_wait(&sh.q_empty[qs], (at.q / P::kQRing - 1) & 1, a.status)) return false;
+        const int qs = it.q % P::kQRing;
+        if (it.q >= P::kQRing) ok = warp_wait(&sh.q_empty[qs], (it.q / P::kQRing - 1) & 1, a.status);
+        if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[qs], q_bytes);
         __syncwarp();
         const uint32_t dst = uniform(smem_u32(sh.q[qs])), bar = uniform(smem_u32(&sh.q_full[qs]));
+        const int c = w.head_parts == 1 ? it.tile : it.tile / w.head_parts;
+        const int head = uniform(it.h * a.G + (it.tile - c * w.head_parts) * w.heads), token = uniform(it.t0 + c * w.tokens);
 #pragma unroll
-        for (int half = 0; half < kHalves; ++half) tma_rows(&qmap, dst + half * P::kQHalf, bar, half * 64, at.head, at.token);
-        sh.q_asked[FEW ? turn : 0] = at.q + 1;
+        for (int half = 0; half < kHalves; ++half) tma_rows(&qmap, dst + half * P::kQHalf, bar, half * 64, head, token);
+        sh.q_asked[FEW ? turn : 0] = it.q + 1;
       }
-      return true;
-    };
-    Item it[2];
-    Place at[2] = {};
-    next(it[0], at[0]);
-    while (true) {  // (two states by turns: no copy of one waits for its loads)
-      if (it[0].stop) break;
-      next(it[1], at[1]);
-      if (!copy(it[0], at[0]) || it[1].stop) break;
-      next(it[0], at[0]);
-      if (!copy(it[1], at[1])) break;
     }
   } else if (warp == kSumWarps) {
     // ------------------------------------------------------------ MMAs
@@ -745,7 +784,7 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
           x += info.other[mine + lane];
         }
         if (mine + lane < info.item.room) {
-          const long long at = info.item.h * w.slots + info.item.slot + key;
+          const long long at = info.item.h * w.slots + static_cast<long long>(info.item.block0) * a.L.b + key;
           if (w.partial) w.partial[info.item.part * w.slots * a.L.hkv + at] = x;
           else if (x != 0.f) atomicAdd(w.weights + at, x);  // the key's only one of the call: nothing waits for it
         }
