@@ -514,6 +514,29 @@ STK_API int stk_accumulate_weights(const stk_kv* kv, int pages, const void* q, l
                                    const stk_attention_options* options, const float* lse, float* weights,
                                    void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
+/* Most tokens of a request that stk_evict_tokens takes. */
+#define STK_EVICT_MAX_TOKENS 393216
+
+/* Workspace (bytes, from a 16-byte boundary on) for stk_evict_tokens. */
+STK_API size_t stk_evict_tokens_workspace_bytes(const stk_kv* kv, int R, int total_blocks, int keep, int max_length);
+
+/* Cut every request of a paged cache that holds more than `keep` tokens (of
+ * lengths[r], at most max_length) back to `keep`: per KV head the first `first`
+ * and the last `last` ones stay, and of the others those of the largest weights
+ * [hkv, total_blocks, b] (ties to the lower place, NaN above all). What stays
+ * moves to the front of the request's own pages, in its order: K, V and the
+ * weights (to weights_out, which may be weights; zeros behind the last token),
+ * and the bounds lo / hi (NULL: none kept) of the blocks that changed, 1e30 and
+ * -1e30 where a block is left without tokens. kept [R, hkv, keep] names the
+ * tokens (ascending; -1 behind the last one of a shorter request), lengths_out
+ * [R] (not lengths) their number. Pages that several requests share are written
+ * where their tokens move: keep a shared prefix by `first`. New: the reference
+ * keeps every token. */
+STK_API int stk_evict_tokens(const stk_kv* kv, int pages, int R, int total_blocks, const int32_t* lengths, int keep,
+                             int first, int last, int max_length, const float* weights, float* weights_out, float* lo,
+                             float* hi, int32_t* kept, int32_t* lengths_out, void* workspace, size_t workspace_bytes,
+                             int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

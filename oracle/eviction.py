@@ -29,3 +29,45 @@ def key_weights(q, k, lse, lo, hi, pos, *, scale, softcap=0.0, slopes=None):
     some = w != 0
     per = lambda y: torch.where(some, w * y, 0.0).view(n, hkv, g, keys).sum((0, 2))  # noqa: E731
     return w.view(n, hkv, g, keys).sum((0, 2)), per(size), per(s.abs() + lse.abs())
+
+
+def kept_tokens(weights, keep, first, last):
+    """Places of the tokens that stay of one row of weights [n], ascending."""
+    n = weights.shape[0]
+    places = list(range(n))
+    if n <= keep:
+        return places
+    rank = [(float("inf") if w != w else 0.0 + w, w != w) for w in weights.tolist()]
+    middle = sorted(places[first:n - last], key=lambda j: (not rank[j][1], -rank[j][0], j))
+    return sorted(places[:first] + middle[:keep - first - last] + places[n - last:])
+
+
+def evict(cache, weights, lengths, keep, first, last):
+    """The cache's tensors, the weights, the lengths and the kept places after an eviction, one row at a time."""
+    k, v, out = cache.k_pages.clone(), cache.v_pages.clone(), torch.zeros_like(weights)
+    lo, hi = cache.lo.clone(), cache.hi.clone()
+    hkv, block, page = cache.hkv, cache.block_size, cache.page_size
+    flat, flat_out = weights.view(hkv, -1), out.view(hkv, -1)
+    off, ppb, d = cache.block_offsets.tolist(), block // page, cache.dim
+    kept = torch.full((len(lengths), hkv, keep), -1, dtype=torch.int32, device=k.device)
+    for r, n in enumerate(lengths):
+        pages = cache.page_table[off[r] * ppb:off[r + 1] * ppb].long()
+        for h in range(hkv):
+            row = flat[h, off[r] * block:off[r] * block + n]
+            stay = torch.tensor(kept_tokens(row, keep, first, last), device=k.device, dtype=torch.long)
+            m = stay.numel()
+            kept[r, h, :m] = stay.int()
+            flat_out[h, off[r] * block:off[r] * block + m] = row[stay]
+            if n <= keep:
+                continue
+            to = torch.arange(m, device=k.device)
+            for pool, old in ((k, cache.k_pages), (v, cache.v_pages)):
+                pool[pages[to // page], h, to % page] = old[pages[stay // page], h, stay % page]
+            for j in range(-(-n // block)):
+                at = torch.arange(j * block, max(j * block, min((j + 1) * block, m)), device=k.device)
+                if lo.shape[1] == 0 or (at.numel() == block and bool((stay[at] == at).all())):
+                    continue
+                keys = k[pages[at // page], h, at % page].float() if at.numel() else None
+                lo[h, off[r] + j] = torch.full((d,), 1e30, device=k.device) if keys is None else keys.amin(0)
+                hi[h, off[r] + j] = torch.full((d,), -1e30, device=k.device) if keys is None else keys.amax(0)
+    return k, v, lo, hi, out, [min(n, keep) for n in lengths], kept

@@ -13,6 +13,7 @@
 
 #include "internal.cuh"
 #include "paged_ops.cuh"
+#include "evict.cuh"
 #include "weigh.cuh"
 #include "../../include/strict_topk_b200.h"
 
@@ -140,7 +141,8 @@ int stk_set_wait_limit_ns(unsigned long long ns) {
   if (ns == 0) return fail(STK_EINVAL, "the wait limit must be positive");
   int (*const setters[])(unsigned long long) = {set_wait_limit_select, set_wait_limit_states, set_wait_limit_repair,
                                                 set_wait_limit_attend, set_wait_limit_group_mma, set_wait_limit_step,
-                                                set_wait_limit_prompt, set_wait_limit_token, set_wait_limit_weigh};
+                                                set_wait_limit_prompt, set_wait_limit_token, set_wait_limit_weigh,
+                                                set_wait_limit_evict};
   for (auto set : setters) {
     const int rc = set(ns);
     if (rc) return cuda_status(rc, "set wait limit");
@@ -1169,4 +1171,75 @@ extern "C" int stk_accumulate_weights(const stk_kv* kv, int pages, const void* q
     r2 = launch_weigh_tensor(w, kv->kv_dtype, sm_count_current(), st);
   if (r2 == 1) r2 = launch_weigh_rows(w, kv->kv_dtype, st);
   return cuda_status(r2, "accumulate_weights");
+}
+
+// ----------------------------------------------------------------------------- eviction
+
+namespace {
+// The plan of a call and the bytes of its workspace: ranks, then flags.
+size_t plan_evict(EvictArgs& a, const stk_kv* kv, int R, int total_blocks, int keep, int max_length, int piece) {
+  a.L = make_layout(kv);
+  a.R = R;
+  a.keep = keep;
+  a.longest = max_length;
+  a.slots = static_cast<long long>(total_blocks) * kv->b;
+  evict_plan(a, kv->kv_dtype, piece);
+  const size_t rows = static_cast<size_t>(R) * kv->hkv;
+  return rows * (static_cast<size_t>(a.chunks) + 1 + static_cast<size_t>(a.chunks) * 2 * a.segments) * sizeof(int);
+}
+
+int check_evict(const stk_kv* kv, int R, int total_blocks, int keep, int first, int last, int max_length) {
+  const int rc = check_kv(kv, kv ? kv->hkv : 1);
+  if (rc) return rc;
+  if (!kv->page_table || !kv->block_offsets) return fail(STK_EINVAL, "a paged cache is expected");
+  if (R <= 0 || total_blocks <= 0 || max_length <= 0)
+    return fail(STK_EINVAL, "bad eviction shape R=%d blocks=%d max_length=%d", R, total_blocks, max_length);
+  if (keep <= 0 || first < 0 || last < 0 || first > keep - last)
+    return fail(STK_EINVAL, "%d kept tokens cannot hold the first %d and the last %d", keep, first, last);
+  if (max_length > kEvictMost)
+    return fail(STK_ESMEM, "requests of up to %d tokens can be cut, not of %d", kEvictMost, max_length);
+  return 0;
+}
+}  // namespace
+
+extern "C" size_t stk_evict_tokens_workspace_bytes(const stk_kv* kv, int R, int total_blocks, int keep, int max_length) {
+  if (check_evict(kv, R, total_blocks, keep, 0, 0, max_length)) return 0;
+  size_t need = 0;  // enough whatever the pools' addresses allow
+  const int size = kv->kv_dtype == STK_F32 ? 4 : 2;
+  for (int piece = size; piece <= 16; piece *= piece == 4 ? 4 : 2) {
+    if (kv->d * size % piece) continue;
+    EvictArgs a{};
+    const size_t n = plan_evict(a, kv, R, total_blocks, keep, max_length, piece);
+    need = n > need ? n : need;
+  }
+  return need;
+}
+
+extern "C" int stk_evict_tokens(const stk_kv* kv, int pages, int R, int total_blocks, const int32_t* lengths, int keep,
+                                int first, int last, int max_length, const float* weights, float* weights_out, float* lo,
+                                float* hi, int32_t* kept, int32_t* lengths_out, void* workspace, size_t workspace_bytes,
+                                int32_t* status, void* stream) {
+  const int rc = check_evict(kv, R, total_blocks, keep, first, last, max_length);
+  if (rc) return rc;
+  if (!lengths || !weights || !weights_out || !kept || !lengths_out || pages <= 0)
+    return fail(STK_EINVAL, "null pointer or empty pool");
+  if ((lo == nullptr) != (hi == nullptr)) return fail(STK_EINVAL, "lo and hi go together");
+  if (lengths == lengths_out) return fail(STK_EINVAL, "lengths_out must not be lengths: both are read and written");
+  EvictArgs a{};
+  const int piece = evict_piece(kv->kv_dtype, kv->d, kv->k, kv->v);
+  const size_t need = plan_evict(a, kv, R, total_blocks, keep, max_length, piece);
+  if (workspace_bytes < need || !workspace) return fail(STK_EWS, "eviction workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(STK_EINVAL, "the eviction workspace must start on a 16-byte boundary");
+  a.pages = pages;
+  a.lengths = lengths; a.first = first; a.last = last;
+  a.weights = weights; a.weights_out = weights_out; a.lo = lo; a.hi = hi;
+  a.kept = kept; a.lengths_out = lengths_out;
+  a.rank = static_cast<int*>(workspace);
+  a.read = a.rank + static_cast<size_t>(R) * kv->hkv * (a.chunks + 1);
+  a.status = status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int r2 = launch_evict_select(a, sm_count_current(), st);
+  if (r2 == 0 && keep < max_length) r2 = launch_evict_move(a, kv->kv_dtype, piece, sm_count_current(), st);
+  return cuda_status(r2, "evict_tokens");
 }

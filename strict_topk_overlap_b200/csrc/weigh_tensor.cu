@@ -18,11 +18,12 @@
 // which a second kernel adds in order.
 //
 // Warps 0-15 (0-3 for few rows): exponentials and sums. Four take an MMA tile's
-// 128 keys, and where the rows are many two such groups half of the rows each,
-// in turn, and add up at a job's end. Then one warp for the MMAs, two for the
-// copies (TMA; K and Q, or with few rows every second job), one that walks over
-// jobs and row tiles ahead of all others, and four for the log-sum-exps and key
-// intervals of the row tiles' rows, in turn.
+// 128 keys; where the rows are many two such groups take every second row tile,
+// so that one's waits run under the other's exponentials, and add up at a job's
+// end. Then one warp for the MMAs, two for the copies (TMA; K and Q, or with few
+// rows every second job), one that walks over jobs and row tiles ahead of all
+// others, and four for the log-sum-exps and key intervals of the row tiles'
+// rows, in turn.
 //
 // Rows that see none of a warp's keys are skipped tile by tile, tiles whose
 // rows all see all of a warp's keys need no mask. Unseen keys may hold
@@ -47,26 +48,31 @@ struct Range {
   int any_lo, any_hi, all_lo, all_hi;
 };
 
-// A row tile of a job.
-struct alignas(16) Item {
-  int h, k0, part;     // job: KV head, first key, part of the request's rows
-  int room;            // keys from k0 on that are there
-  int first, last;     // of the job
-  int empty;           // a job without rows: only its zeros are to be written
+// Up to 32 row tiles of a job, as the walk hands them on.
+struct alignas(16) Batch {
+  int h, k0, part;       // job: KV head, first key, part of the request's rows
+  int room;              // keys from k0 on that are there
+  int first, last;       // batch of the job
   int stop;
-  Range range;
-  int block0;          // the request: first block, new tokens, tokens in the cache, tokens weighed
+  unsigned mask;         // row tiles tile + i; none: a job of which only the zeros are to be written
+  int block0;            // the request: first block, new tokens, tokens in the cache, tokens weighed
   int t0, n_all, len;
-  int n, tile;         // row tile
+  int n, tile;
   int keys_lo, keys_hi;  // that the part's rows see
-  int q, k;            // row tiles and K tiles copied before it
+  int q, k;              // row tiles and K tiles copied before it
 };
-static_assert(sizeof(Item) % 16 == 0, "moved in 16 bytes");
+
+// A row tile of a job, as the products and sums take it.
+struct alignas(16) Item {
+  int h, k0, part, room;
+  int first, last, empty, stop;
+  Range range;
+  int block0;
+};
 
 template <int ROWS, int KEYS>
 struct Info {
   Item item;
-  int odd;                           // its rows are not all there, or some have no weight
   alignas(16) float neg_lse[ROWS];   // - log-sum-exp * log2 e
   alignas(16) float2 bias[ROWS];     // slope * log2 e, place
   alignas(16) int2 keys[ROWS];       // lo, hi
@@ -82,7 +88,7 @@ struct Plan {
   static constexpr int kKRing = FEW ? (D == 128 ? 6 : 10) : 2;
   static constexpr int kQRing = FEW ? 4 : D == 128 ? 3 : 6;
   static constexpr int kInfos = FEW ? 8 : 4;        // row tiles whose rows' data are held
-  static constexpr int kAhead = 8;                  // row tiles that the walk is ahead
+  static constexpr int kAhead = FEW ? 8 : 4;        // batches that the walk is ahead
   static constexpr int kBuffers = FEW ? 4 : 2;      // S in tensor memory
   static constexpr int kBufferCols = FEW ? 16 : 256, kTmem = kBuffers * kBufferCols;
   static constexpr int kGroups = FEW ? 1 : 2;
@@ -97,16 +103,27 @@ struct Shared {
   alignas(1024) unsigned char k[P::kKRing][P::kKBytes];
   alignas(1024) unsigned char q[P::kQRing][P::kQBytes];
   Info<P::kRows, P::kKeys> info[P::kInfos];
-  Item ahead[P::kAhead];
+  Batch ahead[P::kAhead];
   uint64_t k_full[P::kKRing], k_empty[P::kKRing];
   uint64_t q_full[P::kQRing], q_empty[P::kQRing];
   uint64_t i_full[P::kInfos], i_empty[P::kInfos], i_other[P::kInfos];
   uint64_t w_full[P::kAhead], w_empty[P::kAhead];
-  uint64_t s_full[P::kBuffers][2], s_empty[P::kBuffers];
+  uint64_t s_full[P::kBuffers][2], s_empty[P::kBuffers][2];
   uint64_t drained;
   volatile int k_asked[kCopyWarps], q_asked[kCopyWarps];  // copies asked for, by each of the warps that ask
   uint32_t tmem;
 };
+
+// D = A B by one elected lane, from the descriptors' halves: the lower ones
+// differ, the upper ones are the call's.
+__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint32_t a_hi, uint32_t b, uint32_t b_hi, uint32_t idesc,
+                                           bool acc) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n .reg .b64 x, y;\n mov.b64 x, {%1, %2};\n mov.b64 y, {%3, %4};\n setp.ne.u32 p, %6, 0;\n"
+      " elect.sync _|e, 0xffffffff;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(a_hi), "r"(b), "r"(b_hi), "r"(idesc), "r"(static_cast<uint32_t>(acc))
+      : "memory");
+}
 
 // Copies by one elected lane, as predicates inside warp-uniform code (under a
 // branch, or with operands by lane, one takes over a hundred clocks).
@@ -191,7 +208,7 @@ struct Walk {
   int r0, base;          // base: first block of the lane's request
   Rows mine;
   int2 whole;            // key tiles of its only part (w.parts = 1)
-  Range only;            // keys of its only row tile (FEW)
+  int2 seen_keys;        // keys of its only part (FEW)
   long long end, total, before;  // jobs up to the lane's request, of the window, before the window
   long long job;         // of all
   int in_run;
@@ -202,11 +219,8 @@ struct Walk {
   // the current job
   int h, k0, part;
   int2 keys;             // that the part's rows see
-  int q, qb;             // next row tile, end of the job's
-  // a window of 32 row tiles from `w0` on
-  int w0;
-  Range range;
-  unsigned seen;
+  int w0, qb;            // its next 32 row tiles, end of its row tiles
+  unsigned seen;         // those that see a key of the job
   bool started;
   int n_q, n_k;
 
@@ -224,7 +238,7 @@ struct Walk {
         end += whole.y;
       }
       end *= w.a.L.hkv;
-      if (FEW && mine.n > 0) only = range_of(w, mine, 0);
+      if (FEW && mine.n > 0) seen_keys = part_keys(w, mine, 0);
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -244,29 +258,23 @@ struct Walk {
     window(w, lane);
   }
 
-  // The row tiles from `w0` on: what they see, and which see any key of the job.
+  // Which of the row tiles from `w0` on see any key of the job.
   __device__ __forceinline__ void look(const WeighArgs& w, int lane) {
     const int tile = w0 + lane;
-    range = Range{0x7fffffff, 0, 0x7fffffff, 0};
-    if (tile < qb) range = range_of(w, x, w.head_parts == 1 ? tile : tile / w.head_parts);
-    seen = __ballot_sync(kFull, tile < qb && range.any_lo < k0 + KEYS && range.any_hi > k0 && range.any_lo < range.any_hi);
+    Range g{0, 0, 0, 0};
+    if (tile < qb) g = range_of(w, x, w.head_parts == 1 ? tile : tile / w.head_parts);
+    seen = __ballot_sync(kFull, g.any_lo < k0 + KEYS && g.any_hi > k0 && g.any_lo < g.any_hi);
   }
 
-  // The first row tile from q on that sees a key of the job: q, or qb if there is none.
+  // Moves `w0` to the first window from there on with a row tile that sees a key of the job, or to qb.
   __device__ __forceinline__ void find(const WeighArgs& w, int lane) {
-    while (q < qb) {
-      if (q >= w0 + 32) {
-        w0 = q;
-        look(w, lane);
-      }
-      const unsigned m = seen >> (q - w0) << (q - w0);
-      if (m) {
-        q = w0 + __ffs(m) - 1;
-        return;
-      }
-      q = w0 + 32;
+    while (w0 < qb) {
+      look(w, lane);
+      if (seen) return;
+      w0 += 32;
     }
-    q = qb;
+    w0 = qb;
+    seen = 0;
   }
 
   // Moves to the next job; false when there is none.
@@ -278,16 +286,9 @@ struct Walk {
     } else if (++in_run < w.run) {  // the next head of the same keys
       ++job;
       ++h;
-      if (FEW) {
-        q = 0;
-        return true;
-      }
-      q = part * w.per_part;
-      if (w0 != q) {
-        w0 = q;
-        look(w, lane);
-      }
-      find(w, lane);
+      w0 = part * w.per_part;
+      seen = 1;
+      if (!FEW) find(w, lane);
       return true;
     } else {
       in_run = 0;
@@ -313,6 +314,7 @@ struct Walk {
       x.n = __shfl_sync(kFull, mine.n, src);
       x.tiles = __shfl_sync(kFull, mine.tiles, src);
       block0 = __shfl_sync(kFull, base, src);
+      if (FEW) keys = make_int2(__shfl_sync(kFull, seen_keys.x, src), __shfl_sync(kFull, seen_keys.y, src));
       if (FEW || w.parts == 1) {
         part_first = __shfl_sync(kFull, whole.x, src);
       } else {
@@ -326,12 +328,6 @@ struct Walk {
           if (lane >= o) part_end += y;
         }
       }
-      if (FEW) {
-        range.any_lo = __shfl_sync(kFull, only.any_lo, src);
-        range.any_hi = __shfl_sync(kFull, only.any_hi, src);
-        range.all_lo = __shfl_sync(kFull, only.all_lo, src);
-        range.all_hi = __shfl_sync(kFull, only.all_hi, src);
-      }
     }
     const unsigned within = static_cast<unsigned>(here - x_begin), hkv = w.a.L.hkv;  // (part, key tile, head)
     const int at = static_cast<int>(within / hkv);
@@ -343,62 +339,51 @@ struct Walk {
       part = __popc(__ballot_sync(kFull, part_end <= at));
       k0 = (__shfl_sync(kFull, part_first, part) + at - (part ? __shfl_sync(kFull, part_end, part - 1) : 0)) * KEYS;
     }
-    q = part * w.per_part;
-    qb = min(x.tiles, q + w.per_part);
-    w0 = q;
-    if (FEW) {
-      keys = make_int2(range.any_lo, range.any_hi);
-      return true;
-    }
+    w0 = part * w.per_part;
+    qb = min(x.tiles, w0 + w.per_part);
+    seen = 1;
+    if (FEW) return true;
     keys = part_keys(w, x, part);
-    look(w, lane);
     find(w, lane);
     return true;
   }
 
-  // The next item: a row tile of the current job, or the first of a next one.
-  __device__ __forceinline__ void next(const WeighArgs& w, int lane, Item& it) {
-    it.stop = it.empty = it.first = 0;
-    if (!started || q >= qb) {
+  // The next batch: of the current job, or the first of a next one.
+  __device__ __forceinline__ void next(const WeighArgs& w, int lane, Batch& it) {
+    it.stop = it.first = 0;
+    if (!started || w0 >= qb) {
       do {
         if (!next_job(w, lane)) {
           it.stop = 1;
           return;
         }
-      } while (q >= qb && w.partial == nullptr);
+      } while (seen == 0 && w.partial == nullptr);
       it.first = 1;
-      it.empty = q >= qb;
+      if (seen) ++n_k;
     }
     it.h = h;
     it.k0 = k0;
     it.part = part;
     it.room = min(KEYS, x.t.len - k0);
-    it.last = 1;
+    it.mask = seen;
     it.block0 = block0;
     it.t0 = x.t.t0;
     it.n_all = x.t.n;
     it.len = x.t.len;
     it.n = x.n;
-    it.tile = q;
+    it.tile = w0;
     it.keys_lo = keys.x;
     it.keys_hi = keys.y;
-    if (it.empty) return;
-    it.q = n_q++;
-    if (it.first) ++n_k;
+    it.q = n_q;
     it.k = n_k - 1;
-    it.range = range;
+    n_q += __popc(seen);
     if (FEW) {
-      q = qb;
-      return;
+      w0 = qb;
+    } else {
+      w0 += 32;
+      find(w, lane);
     }
-    const int src = q - w0;
-    it.range.any_lo = __shfl_sync(kFull, range.any_lo, src);
-    it.range.any_hi = __shfl_sync(kFull, range.any_hi, src);
-    it.range.all_lo = __shfl_sync(kFull, range.all_lo, src);
-    it.range.all_hi = __shfl_sync(kFull, range.all_hi, src);
-    ++q;
-    find(w, lane);
-    it.last = q >= qb;
+    it.last = w0 >= qb;
   }
 };
 
@@ -472,12 +457,13 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
     }
     for (int i = 0; i < P::kAhead; ++i) {
       mbar_init(&sh.w_full[i], 1);
-      mbar_init(&sh.w_empty[i], 1 + kCopyWarps);
+      mbar_init(&sh.w_empty[i], kInfoWarps + kCopyWarps);
     }
     for (int i = 0; i < kBuffers; ++i) {
       mbar_init(&sh.s_full[i][0], 1);
       mbar_init(&sh.s_full[i][1], 1);
-      mbar_init(&sh.s_empty[i], kSumWarps);
+      mbar_init(&sh.s_empty[i][0], 4);
+      mbar_init(&sh.s_empty[i][1], 4);
     }
     mbar_init(&sh.drained, 1);
     for (int i = 0; i < kCopyWarps; ++i) sh.k_asked[i] = sh.q_asked[i] = 0;
@@ -497,13 +483,11 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
   const uint32_t tmem = uniform(sh.tmem);
   bool ok = true;
 
-  // The item at place n of the walk, for a warp that reads it ahead of the products.
-  auto read = [&](int n, Item& it) {
+  // Batch n of the walk, for a warp that works ahead of the products.
+  auto read = [&](int n, Batch& it) {
     const int slot = n % P::kAhead;
     if (!warp_wait(&sh.w_full[slot], (n / P::kAhead) & 1, a.status)) return false;
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(Item) / 16); ++i)
-      reinterpret_cast<int4*>(&it)[i] = reinterpret_cast<const int4*>(&sh.ahead[slot])[i];
+    it = sh.ahead[slot];
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.w_empty[slot]);
     return true;
@@ -519,80 +503,109 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
       row_tok[j] = (j * 32 + lane) / w.heads;
       row_head[j] = j * 32 + lane - row_tok[j] * w.heads;
     }
-    for (int n = turn;; n += kInfoWarps) {
-      Item it;
+    int item = 0;  // all items before
+    for (int n = 0; ok; ++n) {
+      Batch it;
       ok = read(n, it);
       if (!ok) break;
-      const int slot = n % kInfos;
-      auto& info = sh.info[slot];
-      float lse[kPasses], slope[kPasses];
-      RowKeys rk[kPasses];
-      bool have[kPasses];
-      const bool rows = !it.stop && !it.empty;
-      if (rows) {
-        const int c = w.head_parts == 1 ? it.tile : it.tile / w.head_parts;
-        const int first = c * w.tokens, g0 = (it.tile - c * w.head_parts) * w.heads;
-        RowTile t;
-        t.r = t.row0 = t.rows = 0;
-        t.t0 = it.t0;
-        t.n = it.n_all;
-        t.len = it.len;
+      const bool none = it.stop || it.mask == 0;
+      unsigned mask = none ? 1u : it.mask;
+      bool first = it.first != 0;
+      while (mask) {
+        const int tile = it.tile + __ffs(mask) - 1;
+        mask &= mask - 1;
+        const bool now_first = first;
+        first = false;
+        if (item++ % kInfoWarps != turn) continue;
+        const int slot = (item - 1) % kInfos;
+        auto& info = sh.info[slot];
+        float lse[kPasses], slope[kPasses];
+        RowKeys rk[kPasses];
+        bool have[kPasses];
+        if (!none) {
+          const int c = w.head_parts == 1 ? tile : tile / w.head_parts;
+          const int at = c * w.tokens, g0 = (tile - c * w.head_parts) * w.heads;
+          RowTile t;
+          t.r = t.row0 = t.rows = 0;
+          t.t0 = it.t0;
+          t.n = it.n_all;
+          t.len = it.len;
 #pragma unroll
-        for (int j = 0; j < kPasses; ++j) {
-          const int tok = first + row_tok[j], g = g0 + row_head[j];
-          have[j] = j * 32 + lane < used && tok < it.n && g < a.G;
-          lse[j] = slope[j] = 0.f;
-          rk[j] = RowKeys{0, 0, 0};
-          if (have[j]) {
-            lse[j] = w.lse[static_cast<long long>(it.t0 + tok) * a.hq + it.h * a.G + g];
-            if (MODE & 2) slope[j] = a.slopes[it.h * a.G + g];
-            rk[j] = row_keys(a, t, tok);
+          for (int j = 0; j < kPasses; ++j) {
+            const int tok = at + row_tok[j], g = g0 + row_head[j];
+            have[j] = j * 32 + lane < used && tok < it.n && g < a.G;
+            lse[j] = slope[j] = 0.f;
+            rk[j] = RowKeys{0, 0, 0};
+            if (have[j]) {
+              lse[j] = w.lse[static_cast<long long>(it.t0 + tok) * a.hq + it.h * a.G + g];
+              if (MODE & 2) slope[j] = a.slopes[it.h * a.G + g];
+              rk[j] = row_keys(a, t, tok);
+            }
           }
         }
-      }
-      if (n >= kInfos) ok = warp_wait(&sh.i_empty[slot], (n / kInfos - 1) & 1, a.status);
-      if (!ok) break;
-      if (lane == 0) info.item = it;
-      if (rows) {
-        // A row without weight (its log-sum-exp is -inf) sees no key. Rows that only fill up the MMA's are zeros
-        // with a log-sum-exp of infinity.
-        bool odd = false;
+        if (item > kInfos) ok = warp_wait(&sh.i_empty[slot], ((item - 1) / kInfos - 1) & 1, a.status);
+        if (!ok) break;
+        Range g{0x7fffffff, 0, 0, 0x7fffffff};
+        if (!none) {
+          // A row without weight (its log-sum-exp is -inf), or not there, sees no key. Rows that only fill up the
+          // MMA's are zeros with a log-sum-exp of infinity.
 #pragma unroll
-        for (int j = 0; j < kPasses; ++j) {
-          const int row = j * 32 + lane;
-          const bool live = have[j] && lse[j] != neg_inf(), fill = row >= used;
-          odd = odd || (!fill && !live);
-          if (row < P::kRows) {
-            info.neg_lse[row] = live ? -lse[j] * kLog2e : fill ? neg_inf() : 0.f;
-            info.keys[row] = live ? make_int2(rk[j].lo, rk[j].hi) : make_int2(0, 0);
-            if (MODE & 2) info.bias[row] = make_float2(slope[j] * kLog2e, static_cast<float>(rk[j].pos));
+          for (int j = 0; j < kPasses; ++j) {
+            const int row = j * 32 + lane;
+            const bool live = have[j] && lse[j] != neg_inf(), fill = row >= used;
+            const int2 keys = live ? make_int2(rk[j].lo, rk[j].hi) : make_int2(0, 0);
+            if (!fill) {
+              g.all_lo = max(g.all_lo, keys.x);
+              g.all_hi = min(g.all_hi, keys.y);
+            }
+            if (keys.x < keys.y) {
+              g.any_lo = min(g.any_lo, keys.x);
+              g.any_hi = max(g.any_hi, keys.y);
+            }
+            if (row < P::kRows) {
+              info.neg_lse[row] = live ? -lse[j] * kLog2e : fill ? neg_inf() : 0.f;
+              info.keys[row] = keys;
+              if (MODE & 2) info.bias[row] = make_float2(slope[j] * kLog2e, static_cast<float>(rk[j].pos));
+            }
           }
+          g.any_lo = __reduce_min_sync(kFull, g.any_lo);
+          g.any_hi = __reduce_max_sync(kFull, g.any_hi);
+          g.all_lo = __reduce_max_sync(kFull, g.all_lo);
+          g.all_hi = __reduce_min_sync(kFull, g.all_hi);
         }
-        odd = __any_sync(kFull, odd);
-        if (lane == 0) info.odd = odd;
+        if (lane == 0) {
+          Item x;
+          x.h = it.h;
+          x.k0 = it.k0;
+          x.part = it.part;
+          x.room = it.room;
+          x.block0 = it.block0;
+          x.first = now_first;
+          x.last = it.last && mask == 0;
+          x.empty = none;
+          x.stop = it.stop;
+          x.range = g;
+          info.item = x;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.i_full[slot]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.i_full[slot]);
       if (it.stop) break;
     }
   } else if (warp == kSumWarps + 1 + kCopyWarps) {
     // ------------------------------------------------------------ the walk
     Walk<P::kKeys, FEW> walk;
     walk.start(w, lane);
-    Item it;
+    Batch it;
     for (int n = 0;; ++n) {
       walk.next(w, lane, it);
-      // Its end is told to each of the warps that take turns.
-      const int times = it.stop ? kInfoWarps : 1;
-      for (int i = 0; ok && i < times; ++i, n += i < times) {
-        const int slot = n % P::kAhead;
-        if (n >= P::kAhead) ok = warp_wait(&sh.w_empty[slot], (n / P::kAhead - 1) & 1, a.status);
-        if (!ok) break;
-        if (lane == 0) sh.ahead[slot] = it;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.w_full[slot]);
-      }
-      if (!ok || it.stop) break;
+      const int slot = n % P::kAhead;
+      if (n >= P::kAhead) ok = warp_wait(&sh.w_empty[slot], (n / P::kAhead - 1) & 1, a.status);
+      if (!ok) break;
+      if (lane == 0) sh.ahead[slot] = it;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.w_full[slot]);
+      if (it.stop) break;
     }
   } else if (warp > kSumWarps) {
     // ------------------------------------------------------------ copies
@@ -601,11 +614,11 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
     const unsigned ps = a.L.page_size;
     const int bp = min(a.L.page_size, 128), boxes = P::kKeys / bp, ppb = a.L.b / a.L.page_size;
     const uint32_t q_bytes = static_cast<uint32_t>(w.tokens) * w.heads * D * 2;
-    for (int n = 0;; ++n) {
-      Item it;
+    for (int n = 0; ok; ++n) {
+      Batch it;
       ok = read(n, it);
       if (!ok || it.stop) break;
-      if (it.empty || (FEW && it.q % kCopyWarps != turn)) continue;
+      if (it.mask == 0 || (FEW && it.q % kCopyWarps != turn)) continue;
       if (copies_k && it.first) {
         const unsigned key = it.k0 + lane * bp;
         int page = a.pages, y = static_cast<int>(key % ps / 8);
@@ -626,17 +639,20 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
         sh.k_asked[FEW ? turn : 0] = it.k + 1;
       }
       if (copies_q) {
-        const int qs = it.q % P::kQRing;
-        if (it.q >= P::kQRing) ok = warp_wait(&sh.q_empty[qs], (it.q / P::kQRing - 1) & 1, a.status);
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[qs], q_bytes);
-        __syncwarp();
-        const uint32_t dst = uniform(smem_u32(sh.q[qs])), bar = uniform(smem_u32(&sh.q_full[qs]));
-        const int c = w.head_parts == 1 ? it.tile : it.tile / w.head_parts;
-        const int head = uniform(it.h * a.G + (it.tile - c * w.head_parts) * w.heads), token = uniform(it.t0 + c * w.tokens);
+        int q = it.q;
+        for (unsigned mask = it.mask; mask; mask &= mask - 1, ++q) {
+          const int tile = it.tile + __ffs(mask) - 1, qs = q % P::kQRing;
+          if (q >= P::kQRing) ok = warp_wait(&sh.q_empty[qs], (q / P::kQRing - 1) & 1, a.status);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&sh.q_full[qs], q_bytes);
+          __syncwarp();
+          const uint32_t dst = uniform(smem_u32(sh.q[qs])), bar = uniform(smem_u32(&sh.q_full[qs]));
+          const int c = w.head_parts == 1 ? tile : tile / w.head_parts;
+          const int head = uniform(it.h * a.G + (tile - c * w.head_parts) * w.heads), token = uniform(it.t0 + c * w.tokens);
 #pragma unroll
-        for (int half = 0; half < kHalves; ++half) tma_rows(&qmap, dst + half * P::kQHalf, bar, half * 64, head, token);
-        sh.q_asked[FEW ? turn : 0] = it.q + 1;
+          for (int half = 0; half < kHalves; ++half) tma_rows(&qmap, dst + half * P::kQHalf, bar, half * 64, head, token);
+          sh.q_asked[FEW ? turn : 0] = q + 1;
+        }
       }
     }
   } else if (warp == kSumWarps) {
@@ -661,18 +677,23 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
       const int ks = n_k % P::kKRing, qs = n_q % P::kQRing, buf = n_q % kBuffers;
       if (first) ok = warp_wait(&sh.k_full[ks], (n_k / P::kKRing) & 1, a.status);
       ok = ok && warp_wait(&sh.q_full[qs], (n_q / P::kQRing) & 1, a.status);
-      if (ok && n_q >= kBuffers) ok = warp_wait(&sh.s_empty[buf], (n_q / kBuffers - 1) & 1, a.status);
       if (!ok) break;
-      fence_after();
+      const uint32_t kd = uniform(static_cast<uint32_t>(k_desc) + (ks * P::kKBytes >> 4));
+      const uint32_t qd = uniform(static_cast<uint32_t>(q_desc) + (qs * P::kQBytes >> 4));
+      const uint32_t to = uniform(tmem + buf * P::kBufferCols);
 #pragma unroll
       for (int half = 0; half < P::kTiles; ++half) {
-        const uint64_t kd = k_desc + ((ks * P::kKBytes + half * 128 * D * 2) >> 4), qd = q_desc + (qs * P::kQBytes >> 4);
+        if (ok && n_q >= kBuffers) ok = warp_wait(&sh.s_empty[buf][half], (n_q / kBuffers - 1) & 1, a.status);
+        if (!ok) break;
+        fence_after();
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          mma_ss(tmem + buf * P::kBufferCols + half * 128, kd + (((s >> 2) * 1024 + (s & 3) * 32) >> 4),
-                 qd + (((s >> 2) * P::kQHalf + (s & 3) * 32) >> 4), idesc, s > 0);
+          mma_halves(to + half * 128, kd + ((half * 128 * D * 2 + (s >> 2) * 1024 + (s & 3) * 32) >> 4),
+                     static_cast<uint32_t>(k_desc >> 32), qd + (((s >> 2) * P::kQHalf + (s & 3) * 32) >> 4),
+                     static_cast<uint32_t>(q_desc >> 32), idesc, s > 0);
         mma_commit(&sh.s_full[buf][half]);
       }
+      if (!ok) break;
       mma_commit(&sh.q_empty[qs]);
       ++n_q;
       if (last) {
@@ -688,7 +709,7 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
     const int mine = half * 128 + (warp & 3) * 32;  // first of the warp's keys in the job
     const uint32_t ts = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * 128;
     const float c = (MODE & 1) ? a.scale / a.softcap : a.scale * kLog2e, cap2 = a.softcap * kLog2e;
-    const int cols = w.cols, first_half = P::kGroups == 1 ? cols : (cols / kRun + 1) / 2 * kRun;
+    const int cols = w.cols;
     float2 sum = make_float2(0.f, 0.f);
     int n_info = 0, n_s = 0;
     while (true) {
@@ -696,35 +717,39 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
       ok = warp_wait(&sh.i_full[slot], (n_info / kInfos) & 1, a.status);
       if (!ok) break;
       auto& info = sh.info[slot];
-      if (uniform(info.item.stop)) break;
-      if (uniform(info.item.first)) sum = make_float2(0.f, 0.f);
-      const int first_key = uniform(info.item.k0) + mine, key = first_key + lane;
-      if (!uniform(info.item.empty)) {
+      const Item it = info.item;
+      if (it.stop) break;
+      if (it.first) sum = make_float2(0.f, 0.f);
+      const int first_key = it.k0 + mine, key = first_key + lane;
+      // The groups take every second row tile each.
+      const bool own = P::kGroups == 1 || (it.empty ? 0 : n_s & 1) == group;
+      if (!it.empty && !own) {
+        ++n_s;
+      } else if (!it.empty) {
         const int buf = n_s % kBuffers;
         ok = warp_wait(&sh.s_full[buf][half], (n_s / kBuffers) & 1, a.status);
         if (!ok) break;
         fence_after();
-        const Range g = info.item.range;
+        const Range g = it.range;
         const bool none = g.any_lo >= first_key + 32 || g.any_hi <= first_key;
-        const bool whole = !info.odd && g.all_lo <= first_key && g.all_hi >= first_key + 32;
-        // The group's rows [c0, c1): the first and larger half in turn.
-        const bool low = P::kGroups == 1 || ((n_s ^ group) & 1) == 0;
-        const int c0 = low ? 0 : first_half, c1 = low ? first_half : cols;
+        const bool whole = g.all_lo <= first_key && g.all_hi >= first_key + 32;
         auto release = [&]() {  // the warp has read its S
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.s_empty[buf]);
+          if (lane == 0) mbar_arrive(&sh.s_empty[buf][half]);
         };
         float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         auto tile = [&](auto whole_t) {
           constexpr bool WHOLE = decltype(whole_t)::value;
           float2 s[2][kRun / 2];
-          tmem_ld16(ts + buf * P::kBufferCols + c0, reinterpret_cast<uint32_t*>(s[0]));
+          tmem_ld16(ts + buf * P::kBufferCols, reinterpret_cast<uint32_t*>(s[0]));
           auto run = [&](float2 (&x)[kRun / 2], int j) {
             if (MODE & 1) cap_scores(x, c, cap2);
+            float4 l4;
 #pragma unroll
             for (int e = 0; e < kRun / 2; ++e) {
-              const float2 l = *reinterpret_cast<const float2*>(&info.neg_lse[j + 2 * e]);
+              if (e % 2 == 0) l4 = *reinterpret_cast<const float4*>(&info.neg_lse[j + 2 * e]);
+              const float2 l = e % 2 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
               float2 y;
               if (MODE & 2) {
                 const float4 b = *reinterpret_cast<const float4*>(&info.bias[j + 2 * e]);
@@ -746,23 +771,23 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
             }
           };
 #pragma unroll 1
-          for (int j = c0; j < c1; j += 2 * kRun) {
+          for (int j = 0; j < cols; j += 2 * kRun) {
             tmem_wait_ld();
             tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[0]));
-            const bool more = j + kRun < c1;
+            const bool more = j + kRun < cols;
             if (more) tmem_ld16(ts + buf * P::kBufferCols + j + kRun, reinterpret_cast<uint32_t*>(s[1]));
             else release();
             run(s[0], j);
             if (more) {
               tmem_wait_ld();
               tmem_loaded<kRun>(reinterpret_cast<uint32_t*>(s[1]));
-              if (j + 2 * kRun < c1) tmem_ld16(ts + buf * P::kBufferCols + j + 2 * kRun, reinterpret_cast<uint32_t*>(s[0]));
+              if (j + 2 * kRun < cols) tmem_ld16(ts + buf * P::kBufferCols + j + 2 * kRun, reinterpret_cast<uint32_t*>(s[0]));
               else release();
               run(s[1], j + kRun);
             }
           }
         };
-        if (!none && c0 < c1) {
+        if (!none) {
           if (whole) tile(std::true_type{});
           else tile(std::false_type{});
         } else {
@@ -772,20 +797,20 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
         part[0] = add2(part[0], part[1]);
         sum = add2(sum, part[0]);
       }
-      if (P::kGroups == 2 && group == 1) {
-        if (uniform(info.item.last)) info.other[mine + lane] = sum.x + sum.y;
+      if (!own) {
+        if (it.last) info.other[mine + lane] = sum.x + sum.y;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.i_other[slot]);
-      } else if (uniform(info.item.last)) {
+      } else if (it.last) {
         float x = sum.x + sum.y;
         if (P::kGroups == 2) {
           ok = warp_wait(&sh.i_other[slot], (n_info / kInfos) & 1, a.status);
           if (!ok) break;
           x += info.other[mine + lane];
         }
-        if (mine + lane < info.item.room) {
-          const long long at = info.item.h * w.slots + static_cast<long long>(info.item.block0) * a.L.b + key;
-          if (w.partial) w.partial[info.item.part * w.slots * a.L.hkv + at] = x;
+        if (mine + lane < it.room) {
+          const long long at = it.h * w.slots + static_cast<long long>(it.block0) * a.L.b + key;
+          if (w.partial) w.partial[it.part * w.slots * a.L.hkv + at] = x;
           else if (x != 0.f) atomicAdd(w.weights + at, x);  // the key's only one of the call: nothing waits for it
         }
       }

@@ -3,8 +3,14 @@ eviction of the tokens that received least.
 
 ``accumulate_weights`` adds the attention weight that each key receives from a
 call's new tokens (prompts, pieces, drafted or single tokens), from the
-log-sum-exps that ``paged_attention.attention`` returned for them. New: the
-reference keeps every token.
+log-sum-exps that ``paged_attention.attention`` returned for them. ``evict``
+cuts requests back to a number of tokens per KV head by those weights (or any
+others: they are a plain tensor), strictly, ties to the lower place like every
+selection here, and leaves a cache that all other calls read: what stays moves
+to the front of the requests' own pages, in its order. A kept key stays rotated
+by the position it was appended with, so after an eviction append with explicit
+``positions``; attention's distance ``slopes``, ``kv_lo`` and ``kv_hi`` count
+places in the cache. New: the reference keeps every token.
 """
 from __future__ import annotations
 
@@ -103,3 +109,66 @@ def accumulate_weights(weights, q, cache: PagedKVCache, lengths, lse, *, token_o
     if rc:
         L.check(rc, "accumulate_weights")
     return weights
+
+
+@lru_cache(maxsize=1024)
+def _evict_bytes(device, dtype, hkv, block, dim, page, requests, blocks, keep, longest):
+    any_pool = 256
+    kv = L.PACK_KV(any_pool, any_pool, dtype, hkv, 0, block, dim, any_pool, any_pool, page, 0)
+    with torch.cuda.device(device):
+        return L.load().stk_evict_tokens_workspace_bytes(kv, requests, blocks, keep, longest)
+
+
+def evict_workspace(cache: PagedKVCache, keep):
+    """Workspace for ``evict`` down to ``keep`` tokens."""
+    pool = cache.k_pages
+    need = _evict_bytes(pool.get_device(), L.dtype_code(pool), cache.hkv, cache.block_size, cache.dim, cache.page_size,
+                        cache.requests, _slots(cache), int(keep), cache.max_blocks * cache.block_size)
+    return torch.empty((need,), device=pool.device, dtype=torch.uint8)
+
+
+def evict(cache: PagedKVCache, weights, lengths, keep, *, first=0, last=0, weights_out=None, workspace=None):
+    """Cut every request that holds more than ``keep`` of ``lengths[r]`` (int32
+    [R]) tokens back to ``keep``. Per KV head the ``first`` and the ``last``
+    ones stay, and of the others those of the largest ``weights`` (ties to the
+    lower place, NaN above all). Keys, values and weights of what stays move to
+    the front, in their order; lo / hi of the blocks that changed are taken anew
+    (where the cache keeps them), emptied blocks get ``empty_paged_cache``'s.
+    Weights go to ``weights_out`` (None: in place), zeros behind the last token.
+    Pages that requests share are written where their tokens move: protect a
+    shared prefix by ``first``. Requests hold at most 393,216 tokens. Returns the
+    new lengths [R] and the kept places [R, Hkv, keep] int32, ascending, -1
+    behind a shorter request's last."""
+    pool = cache.k_pages
+    pages, hkv, _, d = pool.shape
+    index = pool.get_device()
+    kv = cache.packed_kv(hkv, d)
+    requests, blocks, block = cache.block_offsets.shape[0] - 1, _slots(cache), cache.block_size
+    held = _ints(lengths, (requests,), "lengths", index)
+    keep, longest = int(keep), cache.max_blocks * block
+    if keep < 1 or first < 0 or last < 0 or first + last > keep:
+        raise ValueError(f"keep = {keep} must hold the first {first} and the last {last} tokens")
+    source = _weights(weights, (hkv, blocks, block), "weights", index)
+    goal = source if weights_out is None else _weights(weights_out, (hkv, blocks, block), "weights_out", index)
+    lo = hi = None
+    if cache.lo.shape[1]:
+        for name, x in (("lo", cache.lo), ("hi", cache.hi)):
+            if x.shape != (hkv, blocks, d) or x.dtype is not torch.float32 or x.get_device() != index or \
+                    not x.is_contiguous():
+                raise ValueError(f"{name} must be contiguous FP32 [Hkv, blocks, D] on the cache's device")
+        lo, hi = cache.lo.data_ptr(), cache.hi.data_ptr()
+    if workspace is None:
+        need = _evict_bytes(index, L.dtype_code(pool), hkv, block, d, cache.page_size, requests, blocks, keep, longest)
+        workspace = weights.new_empty((need,), dtype=torch.uint8)
+    else:
+        if workspace.get_device() != index:
+            raise ValueError("workspace must be on the cache's device")
+        need = workspace.numel()
+    kept = lengths.new_empty((requests, hkv, keep))
+    now = lengths.new_empty((requests,))
+    rc = L.on_device(index, L.load().stk_evict_tokens, kv, pages, requests, blocks, held, keep, first, last, longest,
+                     source, goal, lo, hi, kept.data_ptr(), now.data_ptr(), workspace.data_ptr(), need, L.status_ptr(),
+                     L.raw_stream(index))
+    if rc:
+        L.check(rc, "evict")
+    return now, kept

@@ -126,3 +126,100 @@ def test_weights_in_parts():
     """Rows in parts whose sums are joined: the same bits whenever it runs, and within the bounds."""
     _weigh([3001], [3001], 8, 2, 128, 32, 16, BF, 9)
     _weigh([2000, 3], [1500, 3], 4, 1, 64, 32, 16, HALF, 10, mask="documents")
+
+
+def _filled(lengths, hkv, d, block, page, dtype, seed, *, room=0, bounds=True):
+    """A pool with slots that no token fills, its bounds those of the tokens (1e30 where a block has none)."""
+    from strict_topk_overlap_b200 import paged
+    cache = _cache(lengths, hkv, d, block, page, dtype, seed, room=room)
+    if not bounds:
+        return cache
+    off, ppb, total = cache.block_offsets.tolist(), block // page, cache.block_offsets[-1].item()
+    lo, hi = torch.full((hkv, total, d), 1e30, device=DEV), torch.full((hkv, total, d), -1e30, device=DEV)
+    for r, n in enumerate(lengths):
+        k = O.gather(cache.k_pages, cache.page_table, off, block, page, r, n).float()
+        for j in range(-(-n // block)):
+            lo[:, off[r] + j], hi[:, off[r] + j] = k[:, j * block:(j + 1) * block].amin(1), k[:, j * block:(j + 1) * block].amax(1)
+    return paged.PagedKVCache(cache.k_pages, cache.v_pages, cache.page_table, cache.block_offsets, lo, hi, block, page,
+                              cache.max_blocks)
+
+
+def _same(got, want):
+    return torch.equal(got.view(torch.uint8) if got.is_floating_point() else got,
+                       want.view(torch.uint8) if want.is_floating_point() else want)
+
+
+def _evict(lengths, keep, hkv, d, block, page, dtype, seed, *, first=0, last=0, kind="random", in_place=False, room=0, bounds=True):
+    from strict_topk_overlap_b200 import paged_eviction
+    cache = _filled(lengths, hkv, d, block, page, dtype, seed, room=room, bounds=bounds)
+    g = torch.Generator(DEV).manual_seed(seed + 1)
+    weights = paged_eviction.empty_weights(cache)
+    x = torch.exp(2 * torch.randn(weights.shape, generator=g, device=DEV))
+    if kind == "ties":
+        x = (4 * torch.rand(weights.shape, generator=g, device=DEV)).floor()
+    elif kind == "equal":
+        x = torch.zeros_like(x)
+    elif kind == "signs":  # negative ones, zeros of either sign, infinities and NaN
+        x = torch.randn(weights.shape, generator=g, device=DEV)
+        pick = torch.randint(0, 9, weights.shape, generator=g, device=DEV)
+        for i, value in enumerate((0.0, -0.0, float("inf"), float("-inf"), float("nan"))):
+            x[pick == i] = value
+    elif kind == "rising":
+        x = torch.arange(x.numel(), device=DEV).float().view(x.shape)
+    elif kind == "falling":
+        x = -torch.arange(x.numel(), device=DEV).float().view(x.shape)
+    weights.copy_(x)
+    want = E.evict(cache, weights, lengths, keep, first, last)
+    out = None if in_place else torch.full_like(weights, 7.0)
+    now, kept = paged_eviction.evict(cache, weights, _ints(lengths), keep, first=first, last=last, weights_out=out)
+    got = (cache.k_pages, cache.v_pages, cache.lo, cache.hi, weights if in_place else out, now, kept)
+    names = ("k", "v", "lo", "hi", "weights", "lengths", "kept")
+    want = (*want[:5], _ints(want[5]), want[6])
+    if not in_place:
+        assert _same(weights, x)
+    off = cache.block_offsets.tolist()
+    for name, a, b in zip(reversed(names), reversed(got), reversed(want)):
+        if name == "weights":  # slots of no request's blocks are nobody's
+            a, b = a[:, :off[-1]], b[:, :off[-1]]
+        assert _same(a, b), (name, (a != b).nonzero()[:8].tolist())
+    return cache, now, kept
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["random", "ties", "equal", "signs", "rising", "falling"])
+@pytest.mark.parametrize("lengths,keep,first,last", [
+    ([100], 40, 0, 0), ([300, 20, 64, 1], 64, 4, 16), ([513, 700], 512, 0, 1), ([90, 200], 1, 0, 0), ([90, 200], 32, 16, 16),
+    ([33, 1000], 999, 3, 0), ([4100], 300, 10, 50), ([5, 0, 40], 8, 1, 1)])
+def test_evict(kind, lengths, keep, first, last):
+    _evict(lengths, keep, 2, 128, 32, 16, BF, 20, first=first, last=last, kind=kind)
+    _evict(lengths, keep, 3, 64, 64, 32, HALF, 21, first=first, last=last, kind=kind, in_place=True, room=100)
+
+
+@gpu
+@pytest.mark.parametrize("hkv,d,block,page,dtype", [
+    (8, 128, 32, 16, F32), (1, 256, 128, 128, BF), (2, 96, 24, 8, BF), (3, 40, 6, 3, HALF), (2, 33, 12, 4, F32), (2, 33, 7, 7, HALF),
+    (1, 1, 4, 4, BF), (2, 1024, 16, 16, F32), (2, 520, 32, 16, HALF), (16, 64, 256, 16, BF)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_layouts(hkv, d, block, page, dtype, in_place):
+    _evict([200, 77], 60, hkv, d, block, page, dtype, 22, first=2, last=5, in_place=in_place)
+    _evict([200, 77], 70, hkv, d, block, page, dtype, 23, kind="rising", in_place=in_place, bounds=False)
+
+
+@gpu
+def test_evict_long():
+    """Rows that clusters of several CTAs share, and chunks that wait for earlier ones across the whole grid."""
+    _evict([50000], 30000, 2, 64, 32, 16, BF, 24, first=64, last=500)
+    _evict([20000, 9000, 16385], 16384, 1, 64, 64, 16, HALF, 25, kind="ties")
+    _evict([120000], 119000, 1, 64, 32, 16, BF, 26, in_place=True)
+
+
+@gpu
+def test_evict_again():
+    """Evicting what an eviction left: nothing at the same number, and the first part of the first selection below it."""
+    cache, now, kept = _evict([400, 90], 128, 2, 64, 32, 16, BF, 27, last=4)
+    from strict_topk_overlap_b200 import paged_eviction
+    k, lo = cache.k_pages.clone(), cache.lo.clone()
+    w = paged_eviction.empty_weights(cache)
+    now2, kept2 = paged_eviction.evict(cache, w, now, 128)
+    assert torch.equal(now2, now) and _same(cache.k_pages, k) and _same(cache.lo, lo)
+    assert kept2[0, 0].tolist() == list(range(128)) and kept2[1, 1].tolist() == list(range(90)) + [-1] * 38
