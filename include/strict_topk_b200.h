@@ -55,6 +55,7 @@ extern "C" {
 #define STK_STATUS_SHAPE_OVERFLOW 3
 #define STK_STATUS_BAD_POSITION 4 /* a rotary position outside the table */
 #define STK_STATUS_BAD_LENGTH 5   /* a length outside the request's blocks */
+#define STK_STATUS_NO_TOKEN 6     /* a row of logits without one above -inf */
 
 /* block-state job modes */
 #define STK_MODE_FULL 0   /* (m, l, u) per block */
@@ -536,6 +537,26 @@ STK_API int stk_evict_tokens(const stk_kv* kv, int pages, int R, int total_block
                              int first, int last, int max_length, const float* weights, float* weights_out, float* lo,
                              float* hi, int32_t* kept, int32_t* lengths_out, void* workspace, size_t workspace_bytes,
                              int32_t* status, void* stream);
+
+/* Most logits of a row that stk_sample_tokens takes. */
+#define STK_SAMPLE_MAX_LOGITS 393216
+
+/* The next token of each of R rows of V logits (rows row_stride elements
+ * apart), drawn by uniforms [R] in [0, 1). Of the tokens in descending order of
+ * logits (ties: the lower token first) stay the first top_k (0: all), of those
+ * the ones before which less than top_p of their mass exp(x / temperature) lies
+ * (>= 1: all; the first one always stays), of those the ones of at least min_p
+ * times the largest mass; the token is the first, in the vocabulary's order,
+ * whose mass and that of those before it exceed uniforms[r] of what stays.
+ * Temperature 0: the largest logit. Each parameter is one value for all rows
+ * or, where its array [R] is not NULL, one per row (values below 0 count as 0,
+ * NaN turns a filter off). A NaN logit is never chosen; a row without a logit
+ * above -inf gives -1 and STK_STATUS_NO_TOKEN. New: the reference ends at the
+ * attention's output. */
+STK_API int stk_sample_tokens(const void* logits, int dtype, long long row_stride, int R, int V, const float* uniforms,
+                              const float* temperatures, float temperature, const int32_t* top_ks, int top_k,
+                              const float* top_ps, float top_p, const float* min_ps, float min_p, int32_t* tokens,
+                              int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -71,3 +71,41 @@ def evict(cache, weights, lengths, keep, first, last):
                 lo[h, off[r] + j] = torch.full((d,), 1e30, device=k.device) if keys is None else keys.amin(0)
                 hi[h, off[r] + j] = torch.full((d,), -1e30, device=k.device) if keys is None else keys.amax(0)
     return k, v, lo, hi, out, [min(n, keep) for n in lengths], kept
+
+
+def sample(logits, uniform, temperature, top_k, top_p, min_p):
+    """One row: the token drawn, how near a decision that masses make came to its
+    border, and how far sums of masses may be off that are added as whole
+    numbers of 2^-44 (the largest mass is 1), both relative to the whole mass."""
+    import math
+
+    import numpy as np
+    x = logits.double().cpu().numpy()
+    x = np.where(np.isnan(x), -np.inf, x)
+    v = len(x)
+    f = lambda y: float(np.float32(y))  # noqa: E731
+    best = np.lexsort((np.arange(v), -x))
+    if x[best[0]] == -np.inf:
+        return -1, 1.0, 0.0
+    if f(temperature) <= 0:
+        return int(best[0]), 1.0, 0.0
+    with np.errstate(invalid="ignore", over="ignore"):
+        e = np.where(x == x[best[0]], 1.0, np.exp((x - x[best[0]]) / f(temperature)))
+    e = np.where(x == -np.inf, 0.0, e)
+    near, rough = 1.0, e[(e > 0) & (e < 1)]  # (a mass of 1 is exact)
+    off = 2.0 ** -50 + float((2.0 ** -45 + 2e-14 * rough).sum()) / float(e.sum())
+    if 0 < top_k < v:
+        best = best[:top_k]
+    if f(top_p) < 1:
+        before = np.concatenate(([0.0], np.cumsum(e[best], dtype=np.longdouble)))[:-1]
+        total = math.fsum(e[best])
+        near = min(near, float(np.abs(before[1:] - f(top_p) * total).min(initial=total)) / total)
+        best = best[:max(1, int((before < f(top_p) * total).sum()))]
+    if f(min_p) > 0:
+        near = min(near, float(np.abs(e[best] - min(f(min_p), 1.0))[e[best] != 1].min(initial=1.0)))
+        best = best[e[best] >= min(f(min_p), 1.0)]
+    best = np.sort(best)
+    sums = np.cumsum(e[best], dtype=np.longdouble)
+    at = f(uniform) * sums[-1]
+    near = min(near, float(np.abs(sums[:-1] - at).min(initial=1.0)) / float(sums[-1]))
+    return int(best[min(int(np.searchsorted(sums, at, side="right")), len(best) - 1)]), near, off

@@ -38,7 +38,7 @@ SYMBOLS = (
     "stk_group_attention_workspace_bytes", "stk_group_attention", "stk_touch_kv",
     "stk_append_tokens", "stk_paged_attention_workspace_bytes", "stk_paged_attention",
     "stk_accumulate_weights_workspace_bytes", "stk_accumulate_weights",
-    "stk_evict_tokens_workspace_bytes", "stk_evict_tokens",
+    "stk_evict_tokens_workspace_bytes", "stk_evict_tokens", "stk_sample_tokens",
 )
 
 
@@ -130,6 +130,7 @@ _SIGS = {
     "stk_accumulate_weights_workspace_bytes": (_SZ, [_B, _I, _I, _I, _I, _I, _I, _I, _I]),
     "stk_accumulate_weights": (_I, [_B, _I, _P, _LL, _LL, _I, _I, _I, _I, _P, _P, _I, _I, _B, _P, _P, _P, _SZ, _P, _P]),
     "stk_evict_tokens_workspace_bytes": (_SZ, [_B, _I, _I, _I, _I]),
+    "stk_sample_tokens": (_I, [_P, _I, _LL, _I, _I, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]),
     "stk_evict_tokens": (_I, [_B, _I, _I, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _P]),
 }
 

@@ -14,6 +14,7 @@
 #include "internal.cuh"
 #include "paged_ops.cuh"
 #include "evict.cuh"
+#include "sample.cuh"
 #include "weigh.cuh"
 #include "../../include/strict_topk_b200.h"
 
@@ -1242,4 +1243,27 @@ extern "C" int stk_evict_tokens(const stk_kv* kv, int pages, int R, int total_bl
   int r2 = launch_evict_select(a, sm_count_current(), st);
   if (r2 == 0 && keep < max_length) r2 = launch_evict_move(a, kv->kv_dtype, piece, sm_count_current(), st);
   return cuda_status(r2, "evict_tokens");
+}
+
+// ----------------------------------------------------------------------------- sampling
+
+extern "C" int stk_sample_tokens(const void* logits, int dtype, long long row_stride, int R, int V, const float* uniforms,
+                                 const float* temperatures, float temperature, const int32_t* top_ks, int top_k,
+                                 const float* top_ps, float top_p, const float* min_ps, float min_p, int32_t* tokens,
+                                 int32_t* status, void* stream) {
+  if (!valid_dtype(dtype)) return fail(STK_EINVAL, "unsupported logits dtype %d", dtype);
+  if (R < 0 || V <= 0 || (R > 1 && row_stride < 0)) return fail(STK_EINVAL, "bad sampling shape R=%d V=%d", R, V);
+  if (V > kSampleMost) return fail(STK_ESMEM, "rows of up to %d logits can be sampled, not of %d", kSampleMost, V);
+  if (!(temperature >= 0.f) || top_k < 0 || !(top_p >= 0.f) || !(min_p >= 0.f))
+    return fail(STK_EINVAL, "temperature, top_k, top_p and min_p must not be negative");
+  if (R == 0) return 0;
+  if (!logits || !uniforms || !tokens) return fail(STK_EINVAL, "null pointer");
+  SampleArgs a{};
+  a.logits = logits; a.stride = row_stride; a.R = R; a.V = V; a.uniforms = uniforms;
+  a.temperature = {temperatures, temperature};
+  a.top_k = {top_ks, top_k};
+  a.top_p = {top_ps, top_p};
+  a.min_p = {min_ps, min_p};
+  a.tokens = tokens; a.status = status;
+  return cuda_status(launch_sample(a, dtype, sm_count_current(), static_cast<cudaStream_t>(stream)), "sample_tokens");
 }

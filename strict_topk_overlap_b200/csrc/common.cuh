@@ -26,6 +26,7 @@ enum DeviceStatus : int {
   kStatusWaitTimeout = 1,    // a bounded mbarrier wait ran out
   kStatusBadBlockId = 2,     // a block id outside [0, N) was met
   kStatusShapeOverflow = 3,  // a per-row size exceeded the kernel's static bound
+  kStatusNoToken = 6,        // a row of logits without one above -inf (4, 5: paged_ops.cuh)
 };
 
 constexpr unsigned kFull = 0xffffffffu;
