@@ -9,9 +9,13 @@
 // neighbouring tokens, so sums must not depend on the order of additions nor
 // lose what lies between two tokens of a large vocabulary: e is computed in FP64
 // (2^t by a degree-9 polynomial, relative error 2e-14) and added as a 64-bit
-// whole number of 2^-44. Thresholds are then found digit by digit of the
-// logits' order keys (11, 11 and 10 bits), by counts for top_k and by masses
-// for top_p, exactly and the same on every run.
+// whole number of 2^-44. A threshold (by counts for top_k, by masses for top_p)
+// is found in a histogram over the distance from the largest logit, 32 bins to a
+// unit, whose one bin that holds it is sorted by a CTA, a token to a thread; a
+// bin of too many tokens is cut by a second histogram. What even that leaves
+// crowded (many equal logits), or lies beyond its range, is found digit by digit
+// of the logits' order keys (11, 11 and 10 bits). All of it is exact and the same
+// on every run.
 //
 // A row is read once, into the shared memory of a cluster of up to eight CTAs.
 
@@ -25,8 +29,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024, kBins = 2048;
-constexpr double kUnit = 17592186044416.0;  // 2^44
+constexpr int kThreads = 1024, kBins = 1024;  // bins of a histogram: one to a thread
+constexpr float kBinsPerUnit = 32.f;
 
 using u64 = unsigned long long;
 
@@ -64,23 +68,63 @@ struct Row {
     const double t = (static_cast<double>(x) - static_cast<double>(max)) * rate;
     return t < -60.0 ? 0.0 : mass_of(t);
   }
-  // In units; 0 for a token of too little mass.
+  // In units; 0 for a token of too little mass. (The last bits of e + 256 are e's in units of 2^-44, rounded to nearest.)
   __device__ __forceinline__ u64 units(float x) const {
     const double e = mass(x);
-    return e >= least ? __double2ull_rn(e * kUnit) : 0ull;
+    return e >= least ? static_cast<u64>(__double_as_longlong(e + 256.0) - __double_as_longlong(256.0)) : 0ull;
   }
 };
 
+struct Hist {
+  uint32_t count[kBins], low[kBins], high[kBins];  // tokens, and the two halves of their mass
+};
+
 struct Shared {
-  uint32_t low[2][kBins], high[2][kBins];  // of two digits by turns: counts, or the two halves of masses
+  Hist hist;
+  u64 list[kThreads];  // tokens of a bin: order key, and the token's complement
   int warp_ints[32];
   u64 warp_sums[32];
-  u64 best;   // of the CTA: the largest logit's key, and the lowest token that has it
-  int equal;  // tokens at the limit
-  u64 sum;    // mass of what stays
-  int digit;
-  u64 above, inside;
+  u64 best;    // of the CTA: the largest logit's key, and the lowest token that has it
+  int equal;   // tokens at the limit
+  u64 sum;     // mass of what stays
+  int listed;  // tokens asked into the list
+  int bin;
+  u64 above;         // of the goal, before the bin
+  int upto, crowd;   // tokens up to the bin, and in it
+  uint32_t limit;  // the threshold found
+  int take;
 };
+
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+__device__ __forceinline__ void add_mass(Hist& h, int bin, u64 e) {
+  const uint32_t e_low = static_cast<uint32_t>(e), old = atomicAdd(&h.low[bin], e_low);
+  const uint32_t e_high = static_cast<uint32_t>(e >> 32) + (old + e_low < old ? 1u : 0u);
+  if (e_high) atomicAdd(&h.high[bin], e_high);
+}
+
+// Sorts the CTA's values in descending order, one to a thread.
+__device__ __forceinline__ u64 sort_descending(u64 x, int n, u64* list) {
+  const int tid = threadIdx.x;
+  for (int k = 2; k < 2 * n; k *= 2) {
+    for (int j = k / 2; j > 0; j /= 2) {
+      u64 y;
+      if (j >= 32) {
+        __syncthreads();
+        list[tid] = x;
+        __syncthreads();
+        y = list[tid ^ j];
+      } else {
+        y = __shfl_xor_sync(kFull, x, j);
+      }
+      const bool keep_large = ((tid & k) == 0) == ((tid & j) == 0);
+      x = (x > y) == keep_large ? x : y;
+    }
+  }
+  return x;
+}
 
 template <typename T>
 __device__ __forceinline__ T scan_add(T v, T* warp_sums, T& total) {
@@ -107,7 +151,8 @@ __device__ __forceinline__ T scan_add(T v, T* warp_sums, T& total) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a) {
-  extern __shared__ float row[];
+  extern __shared__ __align__(16) unsigned char slice_bytes[];
+  T* row = reinterpret_cast<T*>(slice_bytes);
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
@@ -115,30 +160,51 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   const int r = static_cast<int>(blockIdx.x) / parts;
   const int slice = ((a.V + parts - 1) / parts + 31) / 32 * 32;
   const int begin = min(a.V, part * slice), n = min(a.V, begin + slice) - begin;
+  auto clean = [](float x) { return x == x ? x : neg_inf(); };  // NaN is never chosen
+  auto logit = [&](int i) { return clean(to_f32(row[i])); };
+  constexpr int kVec = 16 / sizeof(T);
+  // f(i, logit) for the slice's tokens from `from` on, in any order, 16 bytes of them to each of `threads` threads.
+  auto for_each = [&](int from, int to, int me, int threads, auto f) {
+    int i = from + me * kVec;
+    for (; i + kVec <= to; i += threads * kVec) {
+      const uint4 v = *reinterpret_cast<const uint4*>(row + i);
+      const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) f(i + j, clean(to_f32(e[j])));
+    }
+    for (; i < to; ++i) f(i, logit(i));
+  };
+  auto all_tokens = [&](auto f) { for_each(0, n, tid, kThreads, f); };
 
-  // ---- the slice, and its largest logit (NaN is never chosen)
+  // ---- the slice, and its largest logit
   const T* src = static_cast<const T*>(a.logits) + r * a.stride + begin;
   u64 best = 0;
-  auto take_in = [&](int i, float x) {
+  auto look = [&](int i, T v) {
+    float x = to_f32(v);
     if (x != x) x = neg_inf();
-    row[i] = x;
     const u64 b = static_cast<u64>(order_key(x)) << 32 | static_cast<uint32_t>(~(begin + i));
     best = b > best ? b : best;
   };
-  constexpr int kVec = 16 / sizeof(T);
   int done = 0;
   if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
     done = n / kVec * kVec;
 #pragma unroll 4
     for (int i = tid * kVec; i < done; i += kThreads * kVec) {
       const uint4 v = *reinterpret_cast<const uint4*>(src + i);
+      *reinterpret_cast<uint4*>(row + i) = v;
       const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) take_in(i + j, to_f32(e[j]));
+      for (int j = 0; j < kVec; ++j) look(i + j, e[j]);
     }
   }
-  for (int i = done + tid; i < n; i += kThreads) take_in(i, to_f32(src[i]));
-  for (int i = tid; i < kBins; i += kThreads) sh.low[0][i] = sh.high[0][i] = 0;
+#pragma unroll 4
+  for (int i = done + tid; i < n; i += kThreads) {
+    const T v = src[i];
+    row[i] = v;
+    look(i, v);
+  }
+  sh.hist.count[tid] = sh.hist.low[tid] = sh.hist.high[tid] = 0;
+  if (tid == 0) sh.listed = 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const u64 y = __shfl_xor_sync(kFull, best, o);
@@ -171,85 +237,235 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     return;
   }
   Row w;
-  w.max = __uint_as_float(top & 0x80000000u ? top ^ 0x80000000u : ~top);
+  w.max = value_of(top);
   w.rate = 1.4426950408889634 / static_cast<double>(temperature);
   w.least = 0.0;
   w.limit = 0;
-  w.take = 0x7fffffff;
+  w.take = 0x7fffffff;  // (all above)
   const int top_k = a.top_k.rows ? a.top_k.rows[r] : a.top_k.all;
   const float top_p = a.top_p.rows ? a.top_p.rows[r] : a.top_p.all;
   const float min_p = a.min_p.rows ? a.min_p.rows[r] : a.min_p.all;
 
+  // The mass that the draw has to pass, of all that stays.
+  const double uniform = static_cast<double>(a.uniforms[r]);
+  auto drawn = [&](u64 all) {
+    const double g = uniform > 0.0 ? floor(uniform * static_cast<double>(all)) : 0.0;
+    const u64 x = g >= static_cast<double>(all) ? all - 1 : static_cast<u64>(g);
+    return x < all ? x : all - 1;
+  };
+  // The rest, by one CTA, for the first m tokens in descending order (in its list, in any order) among which everything
+  // that stays is: the first k of them, of those the ones before which less than `goal` lies (0: of top_p of these).
+  auto finish = [&](int m, int k, u64 goal) {
+    u64 x = tid < m ? sh.list[tid] : 0;
+    x = sort_descending(x, m, sh.list);
+    const int token = static_cast<int>(~static_cast<uint32_t>(x));
+    const float logit_of = value_of(static_cast<uint32_t>(x >> 32));
+    u64 e = tid < min(m, k) ? w.units(logit_of) : 0, total;
+    const u64 before = scan_add<u64>(e, sh.warp_sums, total);
+    if (goal == 0) {
+      const double g = top_p < 1.f ? ceil(static_cast<double>(top_p > 0.f ? top_p : 0.f) * static_cast<double>(total)) : 0.0;
+      goal = top_p < 1.f ? static_cast<u64>(g) : total;
+      goal = goal < 1 ? 1 : goal;
+    }
+    if (min_p > 0.f) w.least = fmin(static_cast<double>(min_p), 1.0);
+    e = before < goal && e ? w.units(logit_of) : 0;
+    // In the vocabulary's order.
+    u64* masses = reinterpret_cast<u64*>(&sh.hist);
+    __syncthreads();
+    masses[tid] = e;
+    const int kept = __syncthreads_count(e != 0);  // (the first ones)
+    u64 y = e ? ~(static_cast<u64>(token) << 10 | tid) : 0;
+    y = ~sort_descending(y, kept, sh.list);
+    e = tid < kept ? masses[y & 1023] : 0;
+    u64 all;
+    const u64 sum = scan_add<u64>(e, sh.warp_sums, all) + e;
+    const u64 number = drawn(all);
+    if (sum > number && sum - e <= number) a.tokens[r] = static_cast<int>(y >> 10);
+  };
+
   // ---- thresholds: first by counts (top_k), then by masses (top_p)
-  int turn = 0;  // of the histograms
+  // Of the cluster's histograms, the thread's bin (in the order of descending logits).
+  auto cluster_bin = [&](int bin, u64& count, u64& mass) {
+    count = mass = 0;
+    for (int p = 0; p < parts; ++p) {
+      const Hist* h = cluster.map_shared_rank(&sh.hist, p);
+      count += h->count[bin];
+      mass += static_cast<u64>(h->high[bin]) << 32 | h->low[bin];
+    }
+  };
+  auto clear = [&]() {  // once all have read
+    cluster.sync();
+    sh.hist.count[tid] = sh.hist.low[tid] = sh.hist.high[tid] = 0;
+    __syncthreads();
+  };
   for (int mode = 0; mode < 2; ++mode) {
     const bool counts = mode == 0;
     if (counts ? top_k <= 0 || top_k >= a.V : !(top_p < 1.f)) continue;
-    u64 goal = counts ? static_cast<u64>(top_k) : 0;
-    uint32_t limit = 0;
-    for (int digit = 0; digit < 3; ++digit, turn ^= 1) {
-      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
-      uint32_t *low = sh.low[turn], *high = sh.high[turn];
-      for (int i = tid; i < n; i += kThreads) {
-        const float x = row[i];
-        const uint32_t key = order_key(x);
-        if (digit > 0 && (key >> (shift + bits)) != (limit >> (shift + bits))) continue;
-        const int bin = (key >> shift) & ((1u << bits) - 1);
-        if (counts) {
-          atomicAdd(&low[bin], 1u);
-        } else {
-          if (key <= w.limit) continue;  // those at top_k's limit follow below
-          const u64 e = w.units(x);
-          const uint32_t e_low = static_cast<uint32_t>(e), old = atomicAdd(&low[bin], e_low);
-          const uint32_t e_high = static_cast<uint32_t>(e >> 32) + (old + e_low < old ? 1u : 0u);
-          if (e_high) atomicAdd(&high[bin], e_high);
-        }
+    // What of a token counts towards the goal; tokens at top_k's limit that do not all stay are told apart in the list.
+    const bool some_at_limit = !counts && w.take != 0x7fffffff;
+    u64 goal = counts ? static_cast<u64>(top_k) : 0, start = 0;  // start: the goal of the whole row
+    auto weigh = [&](float x, uint32_t key, int bin) {
+      if (!counts) {
+        if (key <= w.limit) return;  // (those at it that stay are added below)
+        add_mass(sh.hist, bin, w.units(x));
       }
-      // (All that stay at top_k's limit weigh alike.)
-      if (!counts && part == 0 && tid == 0 && w.take != 0x7fffffff &&
-          (digit == 0 || (w.limit >> (shift + bits)) == (limit >> (shift + bits)))) {
-        const float x = __uint_as_float(w.limit & 0x80000000u ? w.limit ^ 0x80000000u : ~w.limit);
-        const u64 e = w.units(x) * static_cast<u64>(w.take);
-        const int bin = (w.limit >> shift) & ((1u << bits) - 1);
-        const uint32_t e_low = static_cast<uint32_t>(e), old = atomicAdd(&low[bin], e_low);
-        const uint32_t e_high = static_cast<uint32_t>(e >> 32) + (old + e_low < old ? 1u : 0u);
-        if (e_high) atomicAdd(&high[bin], e_high);
-      }
-      cluster.sync();
-      for (int i = tid; i < kBins; i += kThreads) sh.low[turn ^ 1][i] = sh.high[turn ^ 1][i] = 0;
-      const int b0 = kBins - 1 - 2 * tid;  // two bins per thread, the highest first
-      u64 c0 = 0, c1 = 0;
-      for (int p = 0; p < parts; ++p) {
-        const uint32_t *l = cluster.map_shared_rank(low, p), *u = cluster.map_shared_rank(high, p);
-        c0 += static_cast<u64>(u[b0]) << 32 | l[b0];
-        c1 += static_cast<u64>(u[b0 - 1]) << 32 | l[b0 - 1];
-      }
+      atomicAdd(&sh.hist.count[bin], 1u);
+    };
+    // All that stay at top_k's limit weigh alike.
+    auto weigh_limit = [&](int bin) {
+      if (!some_at_limit || part != 0 || tid != 0) return;
+      add_mass(sh.hist, bin, w.units(value_of(w.limit)) * static_cast<u64>(w.take));
+      atomicAdd(&sh.hist.count[bin], static_cast<uint32_t>(w.take));
+    };
+    // The bin that holds the goal: `bin` is the thread's place in descending order.
+    auto choose = [&](u64 count, u64 mass, bool whole) {
+      const u64 v = counts ? count : mass;
       u64 total;
-      const u64 before = scan_add<u64>(c0 + c1, sh.warp_sums, total);
-      if (!counts && digit == 0) {
+      const u64 before = scan_add<u64>(v, sh.warp_sums, total);
+      int all;
+      const int ahead = counts ? 0 : scan_add<int>(static_cast<int>(count), sh.warp_ints, all);
+      if (whole && !counts) {
         // The least whole number that is not below top_p of the mass; the first token always stays.
         const double g = ceil(static_cast<double>(top_p > 0.f ? top_p : 0.f) * static_cast<double>(total));
         goal = static_cast<u64>(g);
         goal = goal < 1 ? 1 : goal > total ? total : goal;
       }
-      if (before < goal && before + c0 + c1 >= goal) {
-        const bool first = before + c0 >= goal;
-        sh.digit = first ? b0 : b0 - 1;
-        sh.above = first ? before : before + c0;
-        sh.inside = first ? c0 : c1;
+      if (whole) start = goal;
+      if (before < goal && before + v >= goal) {
+        sh.bin = tid;
+        sh.above = before;
+        sh.crowd = static_cast<int>(count);
+        sh.upto = (counts ? static_cast<int>(before) : ahead) + static_cast<int>(count);
       }
       __syncthreads();
-      limit |= static_cast<uint32_t>(sh.digit) << shift;
       goal -= sh.above;
-      __syncthreads();
+    };
+    bool found = false, lost = false;
+    int crowded = 0;  // level 1: the bin of level 0 that is cut
+    for (int level = 0; level < 2 && !found && !lost; ++level) {
+      // Monotone in the logit, so that equal logits share a bin and a lower one's is never before a higher one's; the
+      // last bin has no end. -1: not of the bin that is cut.
+      auto bin_of = [&](float x) {
+        const float d = x == w.max ? 0.f : w.max - x;
+        const int bin = static_cast<int>(fminf(d * kBinsPerUnit, static_cast<float>(kBins - 1)));
+        if (level == 0) return bin;
+        const float in = (d - static_cast<float>(crowded) / kBinsPerUnit) * (kBinsPerUnit * kBins);
+        return bin != crowded ? -1 : static_cast<int>(fminf(fmaxf(in, 0.f), static_cast<float>(kBins - 1)));
+      };
+      all_tokens([&](int, float x) {
+        const int bin = bin_of(x);
+        if (bin >= 0) weigh(x, order_key(x), bin);
+      });
+      if (some_at_limit && bin_of(value_of(w.limit)) >= 0) weigh_limit(bin_of(value_of(w.limit)));
+      cluster.sync();
+      u64 count, mass;
+      cluster_bin(tid, count, mass);
+      choose(count, mass, level == 0);
+      const int bin = sh.bin, crowd = sh.crowd, upto = sh.upto;
+      clear();
+      u64* list = cluster.map_shared_rank(sh.list, 0);
+      int* listed = cluster.map_shared_rank(&sh.listed, 0);
+      auto enlist = [&](int i, uint32_t key) {
+        const int at = atomicAdd(listed, 1);
+        if (at < kThreads) list[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(begin + i));
+      };
+      if (level == 0 && upto <= kThreads && !some_at_limit) {
+        // ---- few: all of them go to the first CTA, which does the rest
+        all_tokens([&](int i, float x) {
+          if (bin_of(x) <= bin) enlist(i, order_key(x));
+        });
+        cluster.sync();
+        if (part != 0) return;
+        finish(upto, counts ? top_k : 0x7fffffff, counts ? 0 : start);
+        return;
+      }
+      if (crowd > kThreads) {  // its tokens alone, in finer bins
+        lost = bin == kBins - 1 || level == 1;
+        crowded = bin;
+        continue;
+      }
+      // ---- its tokens to the first CTA, sorted there
+      all_tokens([&](int i, float x) {
+        if (bin_of(x) != bin) return;
+        const uint32_t key = order_key(x);
+        if (counts || key > w.limit || (some_at_limit && key == w.limit)) enlist(i, key);
+      });
+      cluster.sync();
+      if (part == 0) {
+        const int m = sh.listed;
+        if (m <= kThreads) {  // (more where some at top_k's limit do not stay)
+          u64 x = tid < m ? sh.list[tid] : 0;
+          x = sort_descending(x, m, sh.list);
+          __syncthreads();
+          sh.list[tid] = x;
+          __syncthreads();
+          const uint32_t key = static_cast<uint32_t>(x >> 32);
+          // Tokens of the same logit before this one.
+          int first = tid;
+          if (tid < m) {
+            int lo = 0;  // the first place with the key
+            while (lo < first) {
+              const int mid = (lo + first) >> 1;
+              if (static_cast<uint32_t>(sh.list[mid] >> 32) > key) lo = mid + 1; else first = mid;
+            }
+          }
+          const int same = tid - first;
+          u64 v = 0;
+          if (tid < m && !(some_at_limit && key == w.limit && same >= w.take)) v = counts ? 1ull : w.units(value_of(key));
+          u64 total;
+          const u64 before = scan_add<u64>(v, sh.warp_sums, total);
+          if (before < goal && before + v >= goal) {
+            // The last of its logit: all of that logit stay, and need not be told apart.
+            const bool whole = !(some_at_limit && key == w.limit) &&
+                               (tid + 1 == m || static_cast<uint32_t>(sh.list[tid + 1] >> 32) != key);
+            sh.limit = whole ? key - 1 : key;
+            sh.take = whole ? 0x7fffffff : same + 1;
+          }
+        } else if (tid == 0) {
+          sh.take = 0;
+        }
+        __syncthreads();
+        if (tid == 0) sh.listed = 0;
+      }
+      cluster.sync();
+      const uint32_t limit = *cluster.map_shared_rank(&sh.limit, 0);
+      const int take = *cluster.map_shared_rank(&sh.take, 0);
+      if (take == 0) {
+        lost = true;
+      } else {
+        w.limit = limit;
+        w.take = take;
+        found = true;
+      }
+      cluster.sync();  // read before the first CTA writes them again
+    }
+    if (found) continue;
+    // ---- digit by digit
+    goal = start;
+    uint32_t limit = 0;
+    constexpr int kBits = 10;
+    for (int digit = 0; digit < 4; ++digit) {
+      const int shift = digit == 3 ? 0 : 22 - kBits * digit, bits = digit == 3 ? 2 : kBits;
+      auto digit_of = [&](uint32_t key) { return static_cast<int>((key >> shift) & ((1u << bits) - 1)); };
+      auto within = [&](uint32_t key) { return digit == 0 || (key >> (shift + bits)) == (limit >> (shift + bits)); };
+      all_tokens([&](int, float x) {
+        const uint32_t key = order_key(x);
+        if (within(key)) weigh(x, key, kBins - 1 - digit_of(key));
+      });
+      if (some_at_limit && within(w.limit)) weigh_limit(kBins - 1 - digit_of(w.limit));
+      cluster.sync();
+      u64 count, mass;
+      cluster_bin(tid, count, mass);
+      choose(count, mass, false);
+      limit |= static_cast<uint32_t>(kBins - 1 - sh.bin) << shift;
+      clear();
     }
     // What is left of the goal is taken at the limit, token by token.
     if (counts) {
       w.take = static_cast<int>(goal);
     } else {
-      const float x = __uint_as_float(limit & 0x80000000u ? limit ^ 0x80000000u : ~limit);
-      const u64 e = w.units(x), some = (goal + e - 1) / e;
-      const int available = limit == w.limit && w.take != 0x7fffffff ? w.take : 0x7fffffff;
+      const u64 e = w.units(value_of(limit)), some = (goal + e - 1) / e;
+      const int available = limit == w.limit && some_at_limit ? w.take : 0x7fffffff;
       w.take = some < static_cast<u64>(available) ? static_cast<int>(some) : available;
     }
     w.limit = limit;
@@ -262,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   const bool ties = w.take != 0x7fffffff;  // only then do tokens at the limit differ
   if (ties) {
     for (int i0 = w0; i0 < w1; i0 += 32)
-      equal += __popc(__ballot_sync(kFull, i0 + lane < w1 && order_key(row[i0 + lane]) == w.limit));
+      equal += __popc(__ballot_sync(kFull, i0 + lane < w1 && order_key(logit(i0 + lane)) == w.limit));
     int all_equal;
     equal = scan_add<int>(lane == 0 ? equal : 0, sh.warp_ints, all_equal);
     equal = __shfl_sync(kFull, equal, 0);
@@ -270,23 +486,23 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     cluster.sync();
     for (int p = 0; p < part; ++p) equal += *cluster.map_shared_rank(&sh.equal, p);
   }
-  // Mass of token i of the slice, with `e` tokens at the limit before it.
-  auto stays = [&](int i, int e) {
-    if (i >= w1) return 0ull;
-    const uint32_t key = order_key(row[i]);
-    return key > w.limit || (key == w.limit && e < w.take) ? w.units(row[i]) : 0ull;
-  };
-  auto equal_before = [&](int i, int e, unsigned& at) {
-    at = ties ? __ballot_sync(kFull, i < w1 && order_key(row[i]) == w.limit) : 0u;
-    return e + __popc(at & ((1u << lane) - 1));
+  // Mass of a token, with `e` tokens at the limit before it.
+  auto stays = [&](float x, int e) {
+    const uint32_t key = order_key(x);
+    return key > w.limit || (key == w.limit && e < w.take) ? w.units(x) : 0ull;
   };
   u64 sum = 0;
-  int e = equal;
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    unsigned at;
-    const int mine = equal_before(i0 + lane, e, at);
-    sum += stays(i0 + lane, mine);
-    e += __popc(at);
+  if (!ties) {
+    for_each(w0, w1, lane, 32, [&](int, float x) { sum += order_key(x) > w.limit ? w.units(x) : 0ull; });
+  } else {
+    int e = equal;
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+      const bool in = i0 + lane < w1;
+      const float x = in ? logit(i0 + lane) : neg_inf();
+      const unsigned at = __ballot_sync(kFull, in && order_key(x) == w.limit);
+      if (in) sum += stays(x, e + __popc(at & ((1u << lane) - 1)));
+      e += __popc(at);
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
@@ -301,42 +517,44 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     if (p < part) mine += y;
   }
   cluster.sync();  // the sums have been read: a sibling may leave
-  // The first token whose mass and that of those before it exceed u of all.
-  const double u = static_cast<double>(a.uniforms[r]);
-  const double g = u > 0.0 ? floor(u * static_cast<double>(all)) : 0.0;
-  u64 goal = g >= static_cast<double>(all) ? all - 1 : static_cast<u64>(g);
-  goal = goal < all ? goal : all - 1;
-  if (mine > goal || mine + sum <= goal) return;
-  e = equal;
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    unsigned at;
-    const int eq = equal_before(i0 + lane, e, at);
-    u64 x = stays(i0 + lane, eq);
-    e += __popc(at);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 y = __shfl_up_sync(kFull, x, o);
-      if (lane >= o) x += y;
-    }
-    const unsigned passed = __ballot_sync(kFull, mine + x > goal);
-    if (passed) {
-      if (lane == 0) a.tokens[r] = begin + i0 + __ffs(passed) - 1;
-      return;
-    }
-    mine += __shfl_sync(kFull, x, 31);
+  // The first token whose mass and that of those before it exceed the draw: in the stretch of one of the warps.
+  const u64 number = drawn(all);
+  const bool here = mine <= number && mine + sum > number;
+  if (here && lane == 0) {
+    sh.above = mine;
+    sh.bin = warp;
+    sh.equal = equal;
+  }
+  if (!__syncthreads_or(here)) return;
+  const int s0 = min(n, sh.bin * stretch), s1 = min(n, s0 + stretch);
+  u64 passed = sh.above;
+  int at_limit = sh.equal;
+  for (int i0 = s0; i0 < s1; i0 += kThreads) {
+    const int i = i0 + tid;
+    const float x = i < s1 ? logit(i) : neg_inf();
+    int some = 0;
+    const int e = ties ? scan_add<int>(i < s1 && order_key(x) == w.limit, sh.warp_ints, some) : 0;
+    const u64 v = i < s1 ? stays(x, at_limit + e) : 0;
+    u64 step;
+    const u64 up_to = passed + scan_add<u64>(v, sh.warp_sums, step) + v;
+    if (up_to > number && up_to - v <= number) a.tokens[r] = begin + i;
+    passed += step;
+    at_limit += some;
   }
 }
 
 template <typename T>
 int launch(const SampleArgs& a, int sms, cudaStream_t stream) {
-  // CTAs of a row: as many as its logits need, more while they find SMs and a few thousand logits each.
+  // CTAs of a row: as many as its logits need, more while they find SMs and 16 K logits each (fewer pay less for a
+  // pass than they pay for meeting).
+  constexpr int kSlice = kSampleBytes / static_cast<int>(sizeof(T));
   int parts = 1;
-  while (parts * kSampleSlice < a.V) parts *= 2;
-  while (parts < kSampleCluster && static_cast<long long>(a.R) * parts * 2 <= sms && a.V / parts > 4096) parts *= 2;
+  while (parts * kSlice < a.V) parts *= 2;
+  while (parts < kSampleCluster && static_cast<long long>(a.R) * parts * 2 <= sms && a.V / parts > 16384) parts *= 2;
   if (static_cast<long long>(a.R) * parts > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
-  const int bytes = static_cast<int>(sizeof(float)) * (((a.V + parts - 1) / parts + 31) / 32 * 32);
+  const int bytes = static_cast<int>(sizeof(T)) * (((a.V + parts - 1) / parts + 31) / 32 * 32);
   auto kern = sample_kernel<T>;
-  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleSlice * 4));
+  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleBytes));
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.R * parts));

@@ -23,9 +23,9 @@ struct SampleArgs {
   int* status;
 };
 
-constexpr int kSampleCluster = 8;    // CTAs that share a row at most
-constexpr int kSampleSlice = 49152;  // logits that one of them holds in shared memory
-constexpr int kSampleMost = kSampleCluster * kSampleSlice;
+constexpr int kSampleCluster = 8;         // CTAs that share a row at most
+constexpr int kSampleBytes = 4 * 49152;   // of its logits that one of them holds in shared memory
+constexpr int kSampleMost = kSampleCluster * kSampleBytes / 4;
 
 int launch_sample(const SampleArgs& a, int dtype, int sms, cudaStream_t stream);
 
