@@ -9,13 +9,16 @@
 // neighbouring tokens, so sums must not depend on the order of additions nor
 // lose what lies between two tokens of a large vocabulary: e is computed in FP64
 // (2^t by a degree-9 polynomial, relative error 2e-14) and added as a 64-bit
-// whole number of 2^-44. A threshold (by counts for top_k, by masses for top_p)
-// is found in a histogram over the distance from the largest logit, 32 bins to a
-// unit, whose one bin that holds it is sorted by a CTA, a token to a thread; a
-// bin of too many tokens is cut by a second histogram. What even that leaves
-// crowded (many equal logits), or lies beyond its range, is found digit by digit
-// of the logits' order keys (11, 11 and 10 bits). All of it is exact and the same
-// on every run.
+// whole number of 2^-44. A threshold is found in a histogram over the distance
+// from the largest logit, 32 bins to a unit, whose bins that may hold it are
+// sorted by one CTA, a token to a thread. top_k counts. For top_p a bin's count
+// bounds its mass from both sides (by 3 % at T = 1), which leaves a few bins; the
+// exact masses before them, and of all, are then added in registers (a mass
+// added to a histogram costs three atomics, more than the exponential). Where
+// the tokens up to top_k's bin are few, that CTA does the rest as well. Bins of too
+// many tokens are cut by a second histogram, and what even that leaves crowded
+// (many equal logits), or lies beyond its range, is found digit by digit of the
+// logits' order keys. All of it is exact and the same on every run.
 //
 // A row is read once, into the shared memory of a cluster of up to eight CTAs.
 
@@ -39,39 +42,41 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return x == 0.f ? 0x80000000u : u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
-// 2^t for t <= 0 as a whole number of 2^-44: t = n + f with |f| <= 1/2, 2^f by
-// a polynomial fitted for the least relative error.
-__device__ __forceinline__ double mass_of(double t) {
-  const double m = t + 6755399441055744.0;  // 1.5 * 2^52: n in the low bits
-  const double f = t - (m - 6755399441055744.0);
-  double p = fma(f, 1.0148587078171632e-07, 1.325834013445892e-06);
-  p = fma(p, f, 1.5252988727215495e-05);
-  p = fma(p, f, 0.00015403440864986972);
-  p = fma(p, f, 0.0013333557627726357);
-  p = fma(p, f, 0.0096181291811879843);
-  p = fma(p, f, 0.055504108668400408);
-  p = fma(p, f, 0.24022650695722783);
-  p = fma(p, f, 0.69314718055988556);
-  p = fma(p, f, 1.0);
-  return __hiloint2double(__double2hiint(p) + (__double2loint(m) << 20), __double2loint(p));
-}
-
 struct Row {
-  float max;
-  double rate;   // log2 e / T
-  double least;  // mass below which a token does not stay
+  float max, rate32;
+  double top, rate;  // the largest logit, log2 e / T
+  double least;      // mass below which a token does not stay
   // Tokens above `limit` stay, of those at it the first `take`.
   uint32_t limit;
   int take;
+  // exp((x - max) / T) = 2^t: t = n + f with |f| <= 1/2, 2^f by a polynomial
+  // fitted for the least relative error, n added to the exponent. 14 FP64
+  // operations, the last of them in_units', bound a pass over the masses.
   __device__ __forceinline__ double mass(float x) const {
-    if (x == max) return 1.0;
-    const double t = (static_cast<double>(x) - static_cast<double>(max)) * rate;
-    return t < -60.0 ? 0.0 : mass_of(t);
+    const double d = static_cast<double>(x) - top;
+    const double m = fma(d, rate, 6755399441055744.0);  // 1.5 * 2^52: n in the low bits
+    const double f = fma(d, rate, 6755399441055744.0 - m);
+    double p = fma(f, 1.0148587078171632e-07, 1.325834013445892e-06);
+    p = fma(p, f, 1.5252988727215495e-05);
+    p = fma(p, f, 0.00015403440864986972);
+    p = fma(p, f, 0.0013333557627726357);
+    p = fma(p, f, 0.0096181291811879843);
+    p = fma(p, f, 0.055504108668400408);
+    p = fma(p, f, 0.24022650695722783);
+    p = fma(p, f, 0.69314718055988556);
+    p = fma(p, f, 1.0);
+    const double e = __hiloint2double(__double2hiint(p) + (__double2loint(m) << 20), __double2loint(p));
+    // Nothing below 2^-60, nor of -inf at an infinite temperature (no number); infinities weigh alike.
+    return x == max ? 1.0 : (max - x) * rate32 <= 60.f ? e : 0.0;
   }
-  // In units; 0 for a token of too little mass. (The last bits of e + 256 are e's in units of 2^-44, rounded to nearest.)
+  // As a whole number of 2^-44: the last bits of e + 256.
+  static __device__ __forceinline__ u64 in_units(double e) {
+    return static_cast<u64>(__double_as_longlong(e + 256.0) - __double_as_longlong(256.0));
+  }
+  // 0 for a token of too little mass.
   __device__ __forceinline__ u64 units(float x) const {
     const double e = mass(x);
-    return e >= least ? static_cast<u64>(__double_as_longlong(e + 256.0) - __double_as_longlong(256.0)) : 0ull;
+    return e >= least ? in_units(e) : 0ull;
   }
 };
 
@@ -84,10 +89,16 @@ struct Shared {
   u64 list[kThreads];  // tokens of a bin: order key, and the token's complement
   int warp_ints[32];
   u64 warp_sums[32];
-  u64 best;    // of the CTA: the largest logit's key, and the lowest token that has it
+  float best;  // of the CTA: the largest logit
+  int token;   // and the lowest token that has the row's
+  int warp_min[32];
+  double warp_doubles[32];
+  int from, to;      // bins that may hold the threshold
+  u64 whole;         // mass of all tokens
   int equal;   // tokens at the limit
   u64 sum;     // mass of what stays
   int listed;  // tokens asked into the list
+  int owned;   // and into the CTA's own
   int bin;
   u64 above;         // of the goal, before the bin
   int upto, crowd;   // tokens up to the bin, and in it
@@ -105,22 +116,32 @@ __device__ __forceinline__ void add_mass(Hist& h, int bin, u64 e) {
   if (e_high) atomicAdd(&h.high[bin], e_high);
 }
 
-// Sorts the CTA's values in descending order, one to a thread.
+// Sorts the first n of the CTA's values, one to a thread, in descending order
+// (the others are 0 and stay behind them). Warps without values only meet.
 __device__ __forceinline__ u64 sort_descending(u64 x, int n, u64* list) {
   const int tid = threadIdx.x;
-  for (int k = 2; k < 2 * n; k *= 2) {
-    for (int j = k / 2; j > 0; j /= 2) {
-      u64 y;
-      if (j >= 32) {
-        __syncthreads();
-        list[tid] = x;
-        __syncthreads();
-        y = list[tid ^ j];
-      } else {
-        y = __shfl_xor_sync(kFull, x, j);
+  int size = 32;
+  while (size < n) size *= 2;
+  const bool active = tid < size;
+  for (int k = 2; k <= size; k *= 2) {
+    int j = k / 2;
+    for (; j >= 32; j /= 2) {
+      __syncthreads();
+      if (active) list[tid] = x;
+      __syncthreads();
+      if (active) {
+        const u64 y = list[tid ^ j];
+        const bool keep_large = ((tid & k) == 0) == ((tid & j) == 0);
+        x = (x > y) == keep_large ? x : y;
       }
-      const bool keep_large = ((tid & k) == 0) == ((tid & j) == 0);
-      x = (x > y) == keep_large ? x : y;
+    }
+    if (active) {
+#pragma unroll 1
+      for (; j > 0; j /= 2) {
+        const u64 y = __shfl_xor_sync(kFull, x, j);
+        const bool keep_large = ((tid & k) == 0) == ((tid & j) == 0);
+        x = (x > y) == keep_large ? x : y;
+      }
     }
   }
   return x;
@@ -178,67 +199,62 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
 
   // ---- the slice, and its largest logit
   const T* src = static_cast<const T*>(a.logits) + r * a.stride + begin;
-  u64 best = 0;
-  auto look = [&](int i, T v) {
-    float x = to_f32(v);
-    if (x != x) x = neg_inf();
-    const u64 b = static_cast<u64>(order_key(x)) << 32 | static_cast<uint32_t>(~(begin + i));
-    best = b > best ? b : best;
-  };
+  float best = neg_inf();  // (fmaxf passes NaN over)
   int done = 0;
   if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
     done = n / kVec * kVec;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = tid * kVec; i < done; i += kThreads * kVec) {
       const uint4 v = *reinterpret_cast<const uint4*>(src + i);
       *reinterpret_cast<uint4*>(row + i) = v;
       const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) look(i + j, e[j]);
+      for (int j = 0; j < kVec; ++j) best = fmaxf(best, to_f32(e[j]));
     }
   }
-#pragma unroll 4
+#pragma unroll 8
   for (int i = done + tid; i < n; i += kThreads) {
     const T v = src[i];
     row[i] = v;
-    look(i, v);
+    best = fmaxf(best, to_f32(v));
   }
-  sh.hist.count[tid] = sh.hist.low[tid] = sh.hist.high[tid] = 0;
-  if (tid == 0) sh.listed = 0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 y = __shfl_xor_sync(kFull, best, o);
-    best = y > best ? y : best;
-  }
-  if (lane == 0) sh.warp_sums[warp] = best;
+  for (int i = tid; i < kBins; i += kThreads) sh.hist.count[i] = sh.hist.low[i] = sh.hist.high[i] = 0;
+  if (tid == 0) sh.listed = sh.owned = 0;
+  best = warp_max(best);
+  if (lane == 0) sh.warp_doubles[warp] = best;
   __syncthreads();
-  best = sh.warp_sums[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 y = __shfl_xor_sync(kFull, best, o);
-    best = y > best ? y : best;
-  }
+  best = warp_max(static_cast<float>(sh.warp_doubles[lane]));
   if (tid == 0) sh.best = best;
   cluster.sync();
-  for (int p = 0; p < parts; ++p) {
-    const u64 y = *cluster.map_shared_rank(&sh.best, p);
-    best = y > best ? y : best;
-  }
-  const int greedy = static_cast<int>(~static_cast<uint32_t>(best));
-  const uint32_t top = static_cast<uint32_t>(best >> 32);
+  for (int p = 0; p < parts; ++p) best = fmaxf(best, *cluster.map_shared_rank(&sh.best, p));
   const float temperature = a.temperature.rows ? a.temperature.rows[r] : a.temperature.all;
-  const bool nothing = top <= order_key(neg_inf());
+  const bool nothing = best == neg_inf();
   if (nothing || !(temperature > 0.f)) {
-    if (part == 0 && tid == 0) {
-      a.tokens[r] = nothing ? -1 : greedy;
-      if (nothing) report(a.status, kStatusNoToken);
+    // ---- greedy: the lowest token with the largest logit
+    int token = 0x7fffffff;
+    if (!nothing)
+      all_tokens([&](int i, float x) {
+        if (x == best) token = min(token, begin + i);
+      });
+    token = __reduce_min_sync(kFull, token);
+    if (lane == 0) sh.warp_min[warp] = token;
+    __syncthreads();
+    token = __reduce_min_sync(kFull, sh.warp_min[lane]);
+    if (tid == 0) sh.token = token;
+    cluster.sync();
+    if (part == 0) {
+      for (int p = 0; p < parts; ++p) token = min(token, *cluster.map_shared_rank(&sh.token, p));
+      if (tid == 0) a.tokens[r] = nothing ? -1 : token;
+      if (tid == 0 && nothing) report(a.status, kStatusNoToken);
     }
-    cluster.sync();  // siblings may still read this CTA's best
+    cluster.sync();  // the first CTA has read
     return;
   }
   Row w;
-  w.max = value_of(top);
+  w.max = best;
+  w.top = static_cast<double>(best);
   w.rate = 1.4426950408889634 / static_cast<double>(temperature);
+  w.rate32 = static_cast<float>(w.rate);
   w.least = 0.0;
   w.limit = 0;
   w.take = 0x7fffffff;  // (all above)
@@ -246,6 +262,30 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   const float top_p = a.top_p.rows ? a.top_p.rows[r] : a.top_p.all;
   const float min_p = a.min_p.rows ? a.min_p.rows[r] : a.min_p.all;
 
+  // f(i, logit, mass) for a stretch's tokens; the masses of several are computed side by side, whether they are used or
+  // not (one after the other, behind a branch, each waits for its chain of FP64 products: three times as long).
+  auto with_masses = [&](int from, int to, auto f) {
+    int i = from + lane * kVec;
+    for (; i + kVec <= to; i += 32 * kVec) {
+      const uint4 v = *reinterpret_cast<const uint4*>(row + i);
+      const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int j = 0; j < kVec; j += 4) {
+        float x[4];
+        double m[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = clean(to_f32(e[j + q]));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m[q] = w.mass(x[q]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) f(i + j + q, x[q], m[q]);
+      }
+    }
+    for (; i < to; ++i) {
+      const float x = logit(i);
+      f(i, x, w.mass(x));
+    }
+  };
   // The mass that the draw has to pass, of all that stays.
   const double uniform = static_cast<double>(a.uniforms[r]);
   auto drawn = [&](u64 all) {
@@ -283,14 +323,62 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     if (sum > number && sum - e <= number) a.tokens[r] = static_cast<int>(y >> 10);
   };
 
-  // ---- thresholds: first by counts (top_k), then by masses (top_p)
+  // The bin of a logit: its distance from the largest, rounded to whole bins (by adding 2^23); the last has no end.
+  auto coarse_bin = [&](float x) {
+    const float d = fminf(x == w.max ? 0.f : w.max - x, static_cast<float>(kBins - 1) / kBinsPerUnit);
+    return __float_as_int(fmaf(d, kBinsPerUnit, 8388608.f)) - 0x4b000000;
+  };
+  u64* list = cluster.map_shared_rank(sh.list, 0);
+  int* listed = cluster.map_shared_rank(&sh.listed, 0);
+  // Tokens into the first CTA's list: first into an own one (over the histogram, which is clear before and after).
+  u64* own = reinterpret_cast<u64*>(&sh.hist);
+  auto enlist = [&](int i, uint32_t key) {
+    const int at = atomicAdd(&sh.owned, 1);
+    if (at < kThreads) own[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(begin + i));
+  };
+  auto hand_over = [&]() {
+    __syncthreads();
+    const int m = min(sh.owned, kThreads);
+    if (tid == 0) sh.bin = atomicAdd(listed, sh.owned);
+    __syncthreads();
+    if (tid < m && sh.bin + tid < kThreads) list[sh.bin + tid] = own[tid];
+    __syncthreads();
+    if (tid == 0) sh.owned = 0;
+    sh.hist.count[tid] = sh.hist.low[tid] = sh.hist.high[tid] = 0;
+    cluster.sync();
+  };
+  // Each warp's stretch of the slice.
+  const int stretch = (n + 32 * 32 - 1) / (32 * 32) * 32, w0 = min(n, warp * stretch), w1 = min(n, w0 + stretch);
+  // In the first CTA: of its sorted list's m tokens, the thread's one weighs v; the one that reaches the goal sets the
+  // threshold. `partly`: of its logit do not all tokens stay that could.
+  auto set_limit = [&](uint32_t key, int same, bool partly) {
+    // The last of its logit: all of that logit stay, and need not be told apart.
+    sh.limit = partly ? key : key - 1;
+    sh.take = partly ? same + 1 : 0x7fffffff;
+  };
+  auto sorted = [&](int m) {  // the list in descending order; the thread's token, and its place among those of its logit
+    u64 x = tid < m ? sh.list[tid] : 0;
+    x = sort_descending(x, m, sh.list);
+    __syncthreads();
+    sh.list[tid] = x;
+    __syncthreads();
+    const uint32_t key = static_cast<uint32_t>(x >> 32);
+    int first = tid, lo = 0;  // the first place with the key
+    while (tid < m && lo < first) {
+      const int mid = (lo + first) >> 1;
+      if (static_cast<uint32_t>(sh.list[mid] >> 32) > key) lo = mid + 1; else first = mid;
+    }
+    return make_uint2(key, static_cast<uint32_t>(tid - first));
+  };
+  auto last_of_logit = [&](int m, uint32_t key) { return tid + 1 == m || static_cast<uint32_t>(sh.list[tid + 1] >> 32) != key; };
+
   // Of the cluster's histograms, the thread's bin (in the order of descending logits).
-  auto cluster_bin = [&](int bin, u64& count, u64& mass) {
+  auto cluster_bin = [&](int bin, u64& count, u64& mass, bool masses) {
     count = mass = 0;
     for (int p = 0; p < parts; ++p) {
       const Hist* h = cluster.map_shared_rank(&sh.hist, p);
       count += h->count[bin];
-      mass += static_cast<u64>(h->high[bin]) << 32 | h->low[bin];
+      if (masses) mass += static_cast<u64>(h->high[bin]) << 32 | h->low[bin];
     }
   };
   auto clear = [&]() {  // once all have read
@@ -298,9 +386,101 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     sh.hist.count[tid] = sh.hist.low[tid] = sh.hist.high[tid] = 0;
     __syncthreads();
   };
+
+  // ---- top_p alone: bounds on the bins' masses, then the exact ones where it matters
+  bool before_known = false;  // the mass of what stays of the stretch in the bins before `from`
+  u64 before_mass = 0;
+  int from = 0, to = 0;
+  if ((top_k <= 0 || top_k >= a.V) && top_p < 1.f) {
+    all_tokens([&](int, float x) { atomicAdd(&sh.hist.count[coarse_bin(x)], 1u); });
+    cluster.sync();
+    u64 count, none;
+    cluster_bin(tid, count, none, false);
+    // A distance is off by 2^-24 of 32 at most, a mass by half a unit.
+    const double near = fmax(0.0, (tid - 0.5) / kBinsPerUnit - 4e-6), far = (tid + 0.5) / kBinsPerUnit + 4e-6;
+    const double most = count ? static_cast<double>(count) * exp2(-near * w.rate) : 0.0;
+    const double least = count && tid < kBins - 1 ? static_cast<double>(count) * exp2(-far * w.rate) : 0.0;
+    double all_most, all_least;
+    const double up_to = scan_add<double>(most, sh.warp_doubles, all_most) + most;
+    const double down_to = scan_add<double>(least, sh.warp_doubles, all_least) + least;
+    const double share = top_p > 0.f ? static_cast<double>(top_p) : 0.0;
+    const double goal_least = fmax(share * all_least * (1 - 1e-6), 1e-300), goal_most = share * all_most * (1 + 1e-6) + 1e-6;
+    if (tid == 0) sh.from = sh.to = kBins - 1;
+    __syncthreads();
+    from = __reduce_min_sync(kFull, up_to >= goal_least ? tid : kBins - 1);
+    to = __reduce_min_sync(kFull, down_to >= goal_most ? tid : kBins - 1);
+    if (lane == 0) {
+      atomicMin(&sh.from, from);
+      atomicMin(&sh.to, to);
+    }
+    __syncthreads();
+    from = sh.from;
+    to = max(from, sh.to);
+    // ---- the exact mass of all, of the bins before, and of each that may hold the threshold
+    const double bar = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+    u64 whole = 0, above = 0;
+    with_masses(w0, w1, [&](int, float x, double m) {
+      const int bin = coarse_bin(x);
+      const u64 e = Row::in_units(m);
+      whole += e;
+      if (bin < from) {
+        above += e;
+        before_mass += bar == 0.0 || m >= bar ? e : 0ull;
+      } else if (bin <= to) {
+        add_mass(sh.hist, bin, e);
+      }
+    });
+    u64 total;
+    scan_add<u64>(whole, sh.warp_sums, total);
+    if (tid == 0) sh.whole = total;
+    scan_add<u64>(above, sh.warp_sums, total);
+    if (tid == 0) sh.sum = total;
+    cluster.sync();
+    whole = above = 0;
+    for (int p = 0; p < parts; ++p) {
+      whole += *cluster.map_shared_rank(&sh.whole, p);
+      above += *cluster.map_shared_rank(&sh.sum, p);
+    }
+    // The least whole number that is not below top_p of the mass; the first token always stays.
+    u64 goal = static_cast<u64>(ceil(share * static_cast<double>(whole)));
+    goal = goal < 1 ? 1 : goal > whole ? whole : goal;
+    u64 again, mass;
+    cluster_bin(tid, again, mass, true);
+    if (tid == 0) sh.crowd = kThreads + 1;
+    const u64 before = above + scan_add<u64>(mass, sh.warp_sums, total);
+    if (tid >= from && tid <= to && before < goal && before + mass >= goal) {
+      sh.bin = tid;
+      sh.above = before;
+      sh.crowd = static_cast<int>(count);
+    }
+    clear();
+    const int bin = sh.bin;
+    if (sh.crowd <= kThreads) {
+      // ---- the bin's tokens, sorted by the first CTA
+      all_tokens([&](int i, float x) {
+        if (coarse_bin(x) == bin) enlist(i, order_key(x));
+      });
+      hand_over();
+      if (part == 0) {
+        const int m = sh.listed;
+        const uint2 at = sorted(m);
+        const u64 v = tid < m ? w.units(value_of(at.x)) : 0;
+        const u64 up_to = sh.above + scan_add<u64>(v, sh.warp_sums, total);
+        if (up_to < goal && up_to + v >= goal) set_limit(at.x, static_cast<int>(at.y), !last_of_logit(m, at.x));
+        if (tid == 0) sh.listed = 0;
+      }
+      cluster.sync();
+      w.limit = *cluster.map_shared_rank(&sh.limit, 0);
+      w.take = *cluster.map_shared_rank(&sh.take, 0);
+      before_known = true;
+      to = bin;
+    }
+  }
+
+  // ---- thresholds: first by counts (top_k), then by masses (top_p)
   for (int mode = 0; mode < 2; ++mode) {
     const bool counts = mode == 0;
-    if (counts ? top_k <= 0 || top_k >= a.V : !(top_p < 1.f)) continue;
+    if (counts ? top_k <= 0 || top_k >= a.V : !(top_p < 1.f) || before_known) continue;
     // What of a token counts towards the goal; tokens at top_k's limit that do not all stay are told apart in the list.
     const bool some_at_limit = !counts && w.take != 0x7fffffff;
     u64 goal = counts ? static_cast<u64>(top_k) : 0, start = 0;  // start: the goal of the whole row
@@ -346,10 +526,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
       // Monotone in the logit, so that equal logits share a bin and a lower one's is never before a higher one's; the
       // last bin has no end. -1: not of the bin that is cut.
       auto bin_of = [&](float x) {
-        const float d = x == w.max ? 0.f : w.max - x;
-        const int bin = static_cast<int>(fminf(d * kBinsPerUnit, static_cast<float>(kBins - 1)));
+        const int bin = coarse_bin(x);
         if (level == 0) return bin;
-        const float in = (d - static_cast<float>(crowded) / kBinsPerUnit) * (kBinsPerUnit * kBins);
+        const float d = x == w.max ? 0.f : w.max - x;
+        const float in = (d - (static_cast<float>(crowded) - 0.5f) / kBinsPerUnit) * (kBinsPerUnit * kBins);
         return bin != crowded ? -1 : static_cast<int>(fminf(fmaxf(in, 0.f), static_cast<float>(kBins - 1)));
       };
       all_tokens([&](int, float x) {
@@ -359,22 +539,16 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
       if (some_at_limit && bin_of(value_of(w.limit)) >= 0) weigh_limit(bin_of(value_of(w.limit)));
       cluster.sync();
       u64 count, mass;
-      cluster_bin(tid, count, mass);
+      cluster_bin(tid, count, mass, !counts);
       choose(count, mass, level == 0);
       const int bin = sh.bin, crowd = sh.crowd, upto = sh.upto;
       clear();
-      u64* list = cluster.map_shared_rank(sh.list, 0);
-      int* listed = cluster.map_shared_rank(&sh.listed, 0);
-      auto enlist = [&](int i, uint32_t key) {
-        const int at = atomicAdd(listed, 1);
-        if (at < kThreads) list[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(begin + i));
-      };
       if (level == 0 && upto <= kThreads && !some_at_limit) {
         // ---- few: all of them go to the first CTA, which does the rest
         all_tokens([&](int i, float x) {
           if (bin_of(x) <= bin) enlist(i, order_key(x));
         });
-        cluster.sync();
+        hand_over();
         if (part != 0) return;
         finish(upto, counts ? top_k : 0x7fffffff, counts ? 0 : start);
         return;
@@ -390,37 +564,18 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
         const uint32_t key = order_key(x);
         if (counts || key > w.limit || (some_at_limit && key == w.limit)) enlist(i, key);
       });
-      cluster.sync();
+      hand_over();
       if (part == 0) {
         const int m = sh.listed;
         if (m <= kThreads) {  // (more where some at top_k's limit do not stay)
-          u64 x = tid < m ? sh.list[tid] : 0;
-          x = sort_descending(x, m, sh.list);
-          __syncthreads();
-          sh.list[tid] = x;
-          __syncthreads();
-          const uint32_t key = static_cast<uint32_t>(x >> 32);
-          // Tokens of the same logit before this one.
-          int first = tid;
-          if (tid < m) {
-            int lo = 0;  // the first place with the key
-            while (lo < first) {
-              const int mid = (lo + first) >> 1;
-              if (static_cast<uint32_t>(sh.list[mid] >> 32) > key) lo = mid + 1; else first = mid;
-            }
-          }
-          const int same = tid - first;
+          const uint2 at = sorted(m);
+          const int same = static_cast<int>(at.y);
           u64 v = 0;
-          if (tid < m && !(some_at_limit && key == w.limit && same >= w.take)) v = counts ? 1ull : w.units(value_of(key));
+          if (tid < m && !(some_at_limit && at.x == w.limit && same >= w.take)) v = counts ? 1ull : w.units(value_of(at.x));
           u64 total;
           const u64 before = scan_add<u64>(v, sh.warp_sums, total);
-          if (before < goal && before + v >= goal) {
-            // The last of its logit: all of that logit stay, and need not be told apart.
-            const bool whole = !(some_at_limit && key == w.limit) &&
-                               (tid + 1 == m || static_cast<uint32_t>(sh.list[tid + 1] >> 32) != key);
-            sh.limit = whole ? key - 1 : key;
-            sh.take = whole ? 0x7fffffff : same + 1;
-          }
+          if (before < goal && before + v >= goal)
+            set_limit(at.x, same, (some_at_limit && at.x == w.limit) || !last_of_logit(m, at.x));
         } else if (tid == 0) {
           sh.take = 0;
         }
@@ -455,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
       if (some_at_limit && within(w.limit)) weigh_limit(kBins - 1 - digit_of(w.limit));
       cluster.sync();
       u64 count, mass;
-      cluster_bin(tid, count, mass);
+      cluster_bin(tid, count, mass, !counts);
       choose(count, mass, false);
       limit |= static_cast<uint32_t>(kBins - 1 - sh.bin) << shift;
       clear();
@@ -473,7 +628,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   w.least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
 
   // ---- what stays, in order: each warp a stretch
-  const int stretch = (n + 32 * 32 - 1) / (32 * 32) * 32, w0 = min(n, warp * stretch), w1 = min(n, w0 + stretch);
   int equal = 0;
   const bool ties = w.take != 0x7fffffff;  // only then do tokens at the limit differ
   if (ties) {
@@ -492,8 +646,16 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     return key > w.limit || (key == w.limit && e < w.take) ? w.units(x) : 0ull;
   };
   u64 sum = 0;
-  if (!ties) {
-    for_each(w0, w1, lane, 32, [&](int, float x) { sum += order_key(x) > w.limit ? w.units(x) : 0ull; });
+  if (before_known && !ties) {
+    sum = before_mass;
+    with_masses(w0, w1, [&](int, float x, double m) {
+      const int bin = coarse_bin(x);
+      if (bin >= from && bin <= to && order_key(x) > w.limit && (w.least == 0.0 || m >= w.least)) sum += Row::in_units(m);
+    });
+  } else if (!ties) {
+    with_masses(w0, w1, [&](int, float x, double m) {
+      if (order_key(x) > w.limit && (w.least == 0.0 || m >= w.least)) sum += Row::in_units(m);
+    });
   } else {
     int e = equal;
     for (int i0 = w0; i0 < w1; i0 += 32) {
