@@ -421,14 +421,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     u64 whole = 0, above = 0;
     with_masses(w0, w1, [&](int, float x, double m) {
       const int bin = coarse_bin(x);
-      const u64 e = Row::in_units(m);
+      const u64 e = Row::in_units(m), early = bin < from ? e : 0ull;
       whole += e;
-      if (bin < from) {
-        above += e;
-        before_mass += bar == 0.0 || m >= bar ? e : 0ull;
-      } else if (bin <= to) {
-        add_mass(sh.hist, bin, e);
-      }
+      above += early;
+      before_mass += m >= bar ? early : 0ull;
+      if (bin >= from && bin <= to) add_mass(sh.hist, bin, e);
     });
     u64 total;
     scan_add<u64>(whole, sh.warp_sums, total);
@@ -650,11 +647,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     sum = before_mass;
     with_masses(w0, w1, [&](int, float x, double m) {
       const int bin = coarse_bin(x);
-      if (bin >= from && bin <= to && order_key(x) > w.limit && (w.least == 0.0 || m >= w.least)) sum += Row::in_units(m);
+      const bool in = (static_cast<unsigned>(bin - from) <= static_cast<unsigned>(to - from)) & (order_key(x) > w.limit) &
+                      (m >= w.least);
+      sum += in ? Row::in_units(m) : 0ull;
     });
   } else if (!ties) {
     with_masses(w0, w1, [&](int, float x, double m) {
-      if (order_key(x) > w.limit && (w.least == 0.0 || m >= w.least)) sum += Row::in_units(m);
+      sum += (order_key(x) > w.limit) & (m >= w.least) ? Row::in_units(m) : 0ull;
     });
   } else {
     int e = equal;
