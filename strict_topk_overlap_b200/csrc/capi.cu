@@ -1225,6 +1225,8 @@ extern "C" int stk_evict_tokens(const stk_kv* kv, int pages, int R, int total_bl
   if (!lengths || !weights || !weights_out || !kept || !lengths_out || pages <= 0)
     return fail(STK_EINVAL, "null pointer or empty pool");
   if ((lo == nullptr) != (hi == nullptr)) return fail(STK_EINVAL, "lo and hi go together");
+  if (static_cast<long long>(pages) * kv->hkv * kv->page_size >= 0x7fffffff)
+    return fail(STK_EINVAL, "a pool of %d pages has too many rows", pages);
   if (lengths == lengths_out) return fail(STK_EINVAL, "lengths_out must not be lengths: both are read and written");
   EvictArgs a{};
   const int piece = evict_piece(kv->kv_dtype, kv->d, kv->k, kv->v);

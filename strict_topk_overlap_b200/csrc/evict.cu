@@ -3,23 +3,27 @@
 // protected), in their order, at the front of the request's own pages.
 //
 // Selection: a row (request, KV head) lies in the shared memory of a cluster
-// of up to eight CTAs, read once. The threshold is found digit by digit (11, 11
-// and 10 bits of the weights' order keys), the histograms summed over the
-// cluster; then every warp counts and writes its stretch in order: IDs, weights
-// and, for the move, how many kept tokens lie before each chunk.
+// of up to eight CTAs, read once. The threshold's bin is found in a histogram over
+// the distance of the weights' order keys from the largest one, 32 bins to an
+// octave, and its tokens are sorted by one CTA, one to a thread. What is left
+// crowded (equal weights), or lies 32 octaves down, is found digit by digit of
+// the order keys. Then every warp counts and writes its stretch in order: IDs,
+// weights and, for the move, how many kept tokens lie before each chunk.
 //
 // Move: kept token i goes to place i <= its own. Moving in place saves half the
 // bytes of a way through a copy, but a place may be overwritten only after it
 // has been read. A warp reads a chunk into registers, announces that, waits for
 // the (at most two) earlier chunks that read the places it writes, and writes.
 // The warps of a co-resident grid take chunks in ascending order, so each waits
-// for earlier ones only and some warp can always go on. A block's key bounds are
-// taken on the way by the warp that moves its keys.
+// for earlier ones only and some warp can always go on. A warp's next chunk is on
+// its way into shared memory while one is written. A block's key bounds are taken
+// by the warp that moves its keys.
 
 #include <cooperative_groups.h>
 
 #include <type_traits>
 
+#include "cta_select.cuh"
 #include "evict.cuh"
 
 namespace stk {
@@ -30,16 +34,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024, kBins = 2048;
-constexpr float kNothing = 1e30f;  // lo, and minus hi, of a block without tokens
+constexpr int kThreads = 1024, kBins = 1024;  // one bin to a thread
+constexpr int kBinShift = 18;                 // 32 bins to an octave
+constexpr float kNothing = 1e30f;             // lo, and minus hi, of a block without tokens
 
 // Weights in ascending order, NaN above all, zeros of either sign alike.
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t u = __float_as_uint(x);
-  if (x != x) return 0xffffffffu;
-  if (x == 0.f) return 0x80000000u;
-  return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
-}
+__device__ __forceinline__ uint32_t weight_key(float x) { return x == x ? order_key(x) : 0xffffffffu; }
 
 // Tokens of request r, at most as many as its blocks hold.
 __device__ __forceinline__ int held_tokens(const EvictArgs& a, int r) {
@@ -48,38 +48,21 @@ __device__ __forceinline__ int held_tokens(const EvictArgs& a, int r) {
   return max(0, min(n, min(room, a.longest)));
 }
 
-// Exclusive prefix sums of v over the CTA's threads, and its total. Two barriers.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(kFull, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  int s = warp_sums[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(kFull, s, o);
-    if (lane >= o) s += y;
-  }
-  total = __shfl_sync(kFull, s, 31);
-  const int before = warp ? __shfl_sync(kFull, s, warp - 1) : 0;
-  return before + x - v;
-}
-
 struct SelectShared {
-  int hist[2][kBins];  // of two digits by turns: a sibling may still read the last one's
+  int hist[2][kBins];   // of two passes by turns: a sibling may still read the last one's
+  u64 list[kThreads];   // tokens of a bin: weight key, and the place's complement
+  uint2 kinds[kEvictSlice / 32];  // of each 32 tokens: which stay, which are at the threshold
   int warp_sums[32];
-  int2 count;          // of the CTA: tokens above the threshold (or protected), tokens at it
-  int digit, above, inside;
+  uint32_t warp_top[32];
+  uint32_t top;         // of the CTA: the largest key
+  int2 count;           // tokens above the threshold (or protected), tokens at it
+  int bin, above, crowd, listed;
+  uint32_t limit;
+  int take;
 };
 
 __global__ void __launch_bounds__(kThreads, 1) evict_select_kernel(const EvictArgs a) {
-  extern __shared__ float row[];
+  extern __shared__ __align__(16) float row[];
   __shared__ SelectShared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
@@ -106,56 +89,126 @@ __global__ void __launch_bounds__(kThreads, 1) evict_select_kernel(const EvictAr
   // ---- the CTA's slice [begin, end) of the row, whole groups of 32
   const int slice = ((len + parts - 1) / parts + 31) / 32 * 32;
   const int begin = min(len, part * slice), end = min(len, begin + slice), n = end - begin;
-  for (int i = tid; i < n; i += kThreads) row[i] = weights[begin + i];
-  for (int i = tid; i < kBins; i += kThreads) sh.hist[0][i] = 0;
+  const int lo = a.first, hi = len - a.last;  // the others of the row are protected
+  uint32_t top = 0;
+  auto look = [&](int i, float x) {
+    if (begin + i >= lo && begin + i < hi) top = max(top, weight_key(x));
+  };
+  const int four = reinterpret_cast<uintptr_t>(weights + begin) % 16 == 0 ? n / 4 * 4 : 0;
+#pragma unroll 8
+  for (int i = tid * 4; i < four; i += kThreads * 4) {
+    const float4 x = *reinterpret_cast<const float4*>(weights + begin + i);
+    *reinterpret_cast<float4*>(row + i) = x;
+    look(i, x.x);
+    look(i + 1, x.y);
+    look(i + 2, x.z);
+    look(i + 3, x.w);
+  }
+  for (int i = four + tid; i < n; i += kThreads) {
+    row[i] = weights[begin + i];
+    look(i, row[i]);
+  }
+  // Blocks that lose all their tokens (the stores run beside what follows).
+  if (a.lo != nullptr) {
+    const int b0 = (now + a.L.b - 1) / a.L.b, b1 = (len + a.L.b - 1) / a.L.b;
+    const long long d = a.L.d, from = (base / a.L.b + b0) * d, count = (b1 - b0) * d;
+    if ((from | d) % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.lo) | reinterpret_cast<uintptr_t>(a.hi)) & 15) == 0) {
+      const float4 none = make_float4(kNothing, kNothing, kNothing, kNothing), no = make_float4(-kNothing, -kNothing, -kNothing, -kNothing);
+      for (long long i = at; i < count / 4; i += all) {
+        reinterpret_cast<float4*>(a.lo + from)[i] = none;
+        reinterpret_cast<float4*>(a.hi + from)[i] = no;
+      }
+    } else {
+      for (long long i = at; i < count; i += all) {
+        a.lo[from + i] = kNothing;
+        a.hi[from + i] = -kNothing;
+      }
+    }
+  }
+  sh.hist[0][tid] = sh.hist[1][tid] = 0;
+  if (tid == 0) sh.listed = 0;
+  top = __reduce_max_sync(kFull, top);
+  if (lane == 0) sh.warp_top[warp] = top;
   __syncthreads();
+  top = __reduce_max_sync(kFull, sh.warp_top[lane]);
+  if (tid == 0) sh.top = top;
+  cluster.sync();
+  for (int p = 0; p < parts; ++p) top = max(top, *cluster.map_shared_rank(&sh.top, p));
 
   // ---- the threshold: `take` tokens whose key is `limit` stay, and all above
-  const int lo = a.first, hi = len - a.last;  // the others of the row are protected
   uint32_t limit = 0;
   int take = a.keep - a.first - a.last;
-  bool found = take == 0;  // (then nothing unprotected stays)
-  if (found) limit = 0xffffffffu;
-  for (int digit = 0; digit < 3; ++digit) {
-    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
-    int* hist = sh.hist[digit & 1];
-    if (!found) {
-      for (int i = tid; i < n; i += kThreads) {
-        const uint32_t key = order_key(row[i]);
-        const bool in = begin + i >= lo && begin + i < hi && (digit == 0 || (key >> (shift + bits)) == (limit >> (shift + bits)));
-        if (in) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1);
-      }
-    }
+  const bool none = take == 0;  // nothing unprotected stays
+  int turn = 0;
+  // The thread's bin, over the cluster; the one that reaches the goal is told to all, and the goal left in it.
+  auto choose = [&](int& goal) {
     cluster.sync();
-    if (digit < 2)
-      for (int i = tid; i < kBins; i += kThreads) sh.hist[(digit & 1) ^ 1][i] = 0;  // (read by siblings before the last sync)
-    // Two bins per thread, the highest first.
-    const int top = kBins - 1 - 2 * tid;
-    int c0 = 0, c1 = 0;
-    for (int p = 0; p < parts; ++p) {
-      const int* other = cluster.map_shared_rank(hist, p);
-      c0 += other[top];
-      c1 += other[top - 1];
-    }
+    sh.hist[turn ^ 1][tid] = 0;  // (read by siblings before the last meeting)
+    int count = 0;
+    for (int p = 0; p < parts; ++p) count += cluster.map_shared_rank(sh.hist[turn], p)[tid];
     int total;
-    const int before = block_scan(c0 + c1, sh.warp_sums, total);
-    if (!found) {
-      if (before < take && before + c0 >= take) {
-        sh.digit = top;
-        sh.above = before;
-        sh.inside = c0;
-      } else if (before + c0 < take && before + c0 + c1 >= take) {
-        sh.digit = top - 1;
-        sh.above = before + c0;
-        sh.inside = c1;
+    const int before = scan_add<int>(count, sh.warp_sums, total);
+    if (before < goal && before + count >= goal) {
+      sh.bin = tid;
+      sh.above = before;
+      sh.crowd = count;
+    }
+    __syncthreads();
+    goal -= sh.above;
+    turn ^= 1;
+  };
+  auto bin_of = [&](uint32_t key) { return static_cast<int>(min((top - key) >> kBinShift, static_cast<uint32_t>(kBins - 1))); };
+  auto middle = [&](auto f) {
+    const int i1 = min(n, hi - begin);
+    for (int i = max(0, lo - begin) + tid; i < i1; i += kThreads) f(i, weight_key(row[i]));
+  };
+  bool found = none;
+  if (!none) {
+    int goal = take;
+    middle([&](int, uint32_t key) { atomicAdd(&sh.hist[turn][bin_of(key)], 1); });
+    choose(goal);
+    const int bin = sh.bin, crowd = sh.crowd;
+    if (crowd <= kThreads && bin < kBins - 1) {
+      u64* list = cluster.map_shared_rank(sh.list, 0);
+      int* listed = cluster.map_shared_rank(&sh.listed, 0);
+      middle([&](int i, uint32_t key) {
+        if (bin_of(key) == bin) list[atomicAdd(listed, 1)] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(begin + i));
+      });
+      cluster.sync();
+      if (part == 0) {
+        u64 x = tid < crowd ? sh.list[tid] : 0;
+        x = sort_descending(x, crowd, sh.list);
+        __syncthreads();
+        sh.list[tid] = x;
+        __syncthreads();
+        if (tid == goal - 1) {  // the last one that stays, and how many of its weight do
+          const uint32_t key = static_cast<uint32_t>(x >> 32);
+          int first = tid, l = 0;
+          while (l < first) {
+            const int mid = (l + first) >> 1;
+            if (static_cast<uint32_t>(sh.list[mid] >> 32) > key) l = mid + 1; else first = mid;
+          }
+          sh.limit = key;
+          sh.take = tid - first + 1;
+        }
       }
+      cluster.sync();
+      limit = *cluster.map_shared_rank(&sh.limit, 0);
+      take = *cluster.map_shared_rank(&sh.take, 0);
+      found = true;
     }
-    __syncthreads();
-    if (!found) {
-      limit |= static_cast<uint32_t>(sh.digit) << shift;
-      take -= sh.above;
+  }
+  if (!found) {
+    for (int digit = 0; digit < 4; ++digit) {  // 10, 10, 10 and 2 bits
+      const int shift = digit == 3 ? 0 : 22 - 10 * digit, bits = digit == 3 ? 2 : 10;
+      middle([&](int, uint32_t key) {
+        if (digit == 0 || (key >> (shift + bits)) == (limit >> (shift + bits)))
+          atomicAdd(&sh.hist[turn][kBins - 1 - static_cast<int>((key >> shift) & ((1u << bits) - 1))], 1);
+      });
+      choose(take);
+      limit |= static_cast<uint32_t>(kBins - 1 - sh.bin) << shift;
+      __syncthreads();
     }
-    __syncthreads();
   }
 
   // ---- each warp's stretch: tokens above, and at, the threshold
@@ -163,18 +216,21 @@ __global__ void __launch_bounds__(kThreads, 1) evict_select_kernel(const EvictAr
   auto kind = [&](int i) {  // 2: stays, 1: at the threshold
     const int place = begin + i;
     if (place < lo || place >= hi) return 2;
-    const uint32_t key = order_key(row[i]);
-    return found ? 0 : key > limit ? 2 : key == limit ? 1 : 0;
+    const uint32_t key = weight_key(row[i]);
+    return none ? 0 : key > limit ? 2 : key == limit ? 1 : 0;
   };
   int above = 0, equal = 0;
+#pragma unroll 4
   for (int i0 = w0; i0 < w1; i0 += 32) {
     const int k = i0 + lane < w1 ? kind(i0 + lane) : 0;
-    above += __popc(__ballot_sync(kFull, k == 2));
-    equal += __popc(__ballot_sync(kFull, k == 1));
+    const unsigned a2 = __ballot_sync(kFull, k == 2), a1 = __ballot_sync(kFull, k == 1);
+    if (lane == 0) sh.kinds[i0 / 32] = make_uint2(a2, a1);
+    above += __popc(a2);
+    equal += __popc(a1);
   }
   int all_above, all_equal;
-  above = block_scan(lane == 0 ? above : 0, sh.warp_sums, all_above);
-  equal = block_scan(lane == 0 ? equal : 0, sh.warp_sums, all_equal);
+  above = scan_add<int>(lane == 0 ? above : 0, sh.warp_sums, all_above);
+  equal = scan_add<int>(lane == 0 ? equal : 0, sh.warp_sums, all_equal);
   above = __shfl_sync(kFull, above, 0);
   equal = __shfl_sync(kFull, equal, 0);
   if (tid == 0) sh.count = make_int2(all_above, all_equal);
@@ -184,18 +240,21 @@ __global__ void __launch_bounds__(kThreads, 1) evict_select_kernel(const EvictAr
     above += c.x;
     equal += c.y;
   }
+  __syncwarp();
+  const unsigned below = (1u << lane) - 1;
+  const int chunk_shift = __ffs(a.chunk) - 1;
+#pragma unroll 4
   for (int i0 = w0; i0 < w1; i0 += 32) {
+    const uint2 kinds = sh.kinds[i0 / 32];
     const int i = i0 + lane, place = begin + i;
-    const int k = i < w1 ? kind(i) : 0;
-    const unsigned a2 = __ballot_sync(kFull, k == 2), a1 = __ballot_sync(kFull, k == 1), below = (1u << lane) - 1;
-    const int e = equal + __popc(a1 & below), goal = above + __popc(a2 & below) + min(e, take);
-    if (k == 2 || (k == 1 && e < take)) {
+    const int e = equal + __popc(kinds.y & below), goal = above + __popc(kinds.x & below) + min(e, take);
+    if ((kinds.x >> lane & 1) || ((kinds.y >> lane & 1) && e < take)) {
       kept[goal] = place;
       out[goal] = row[i];
     }
-    if (i < w1 && place % a.chunk == 0 && place / a.chunk <= a.chunks) rank[place / a.chunk] = goal;
-    above += __popc(a2);
-    equal += __popc(a1);
+    if ((place & (a.chunk - 1)) == 0 && i < w1 && place <= a.chunk * a.chunks) rank[place >> chunk_shift] = goal;
+    above += __popc(kinds.x);
+    equal += __popc(kinds.y);
   }
   for (int i = at; i <= a.chunks; i += all)
     if (i * a.chunk >= len) rank[i] = a.keep;
@@ -225,145 +284,296 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-constexpr int kMoveThreads = 256, kSteps = 16;
+constexpr int kMoveWarps = 12, kSteps = 16, kStage = 2;  // a warp's chunks in shared memory
+constexpr int kStageBytes = kSteps * 32 * 16;
+constexpr int kMoveBytes = kMoveWarps * kStage * kStageBytes;
 
-// PIECE: bytes that a lane moves at once. An item is one block of a row (all
-// its chunks in order), of K or of V, one segment of up to 32 pieces.
+template <int PIECE>
+__device__ __forceinline__ void copy_piece(void* to, const void* from) {
+  if constexpr (PIECE == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+  else if constexpr (PIECE == 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+  else
+    *static_cast<unsigned short*>(to) = *static_cast<const unsigned short*>(from);
+}
+
+// Least and largest of the values of a piece, NaN where any is: 16-bit ones in pairs.
 template <typename T, int PIECE>
-__global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const EvictArgs a, long long items) {
-  using P = typename Piece<PIECE>::type;
-  constexpr int E = PIECE / static_cast<int>(sizeof(T));
-  const int lane = threadIdx.x & 31;
-  const int rows = a.R * a.L.hkv, per = rows * 2 * a.segments;
-  const int pieces = a.L.d / E, ps = a.L.page_size, chunks_per_block = a.L.b / a.chunk;
-  bool ok = true;
-  const long long warps = static_cast<long long>(gridDim.x) * (kMoveThreads / 32);
-  for (long long item = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); item < items && ok; item += warps) {
-    const int block = static_cast<int>(item / per);
-    int rest = static_cast<int>(item - static_cast<long long>(block) * per);
-    const int id = rest % rows;
-    rest /= rows;
-    const bool keys = rest % 2 == 0;
-    const int segment = rest / 2, r = id / a.L.hkv, h = id - r * a.L.hkv;
-    const int len = held_tokens(a, r);
-    if (len <= a.keep || block * a.L.b >= len) continue;
-    const int now = a.keep, b0 = a.L.block_offsets[r], t0 = block * a.L.b;
-    const int p0 = segment * 32, np = min(32, pieces - p0);  // the segment's pieces
-    const int at_once = 32 / np, group = lane / np, column = lane - group * np;
-    const bool active = group < at_once;
-    const bool bounds = keys && a.lo != nullptr;
-    const long long bound_at = (h * (a.slots / a.L.b) + b0 + block) * static_cast<long long>(a.L.d) + (p0 + column) * E;
-    if (t0 >= now) {  // a block that holds nothing any more
-      if (bounds && group == 0)
+struct Bounds {
+  static constexpr bool kPairs = sizeof(T) == 2 && PIECE >= 4;
+  static constexpr int E = PIECE / static_cast<int>(sizeof(T)), N = kPairs ? E / 2 : E;
+  using V = typename std::conditional<!kPairs, float, typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type>::type;
+  V low[N], high[N];
+  static __device__ __forceinline__ V least(V a, V b) {
+    if constexpr (kPairs) return __hmin2_nan(a, b);
+    else return min_nan(a, b);
+  }
+  static __device__ __forceinline__ V most(V a, V b) {
+    if constexpr (kPairs) return __hmax2_nan(a, b);
+    else return max_nan(a, b);
+  }
+  static __device__ __forceinline__ V shuffle(V x, int lane) {
+    uint32_t u = __shfl_sync(kFull, *reinterpret_cast<const uint32_t*>(&x), lane);
+    return *reinterpret_cast<const V*>(&u);
+  }
+  __device__ __forceinline__ void take(const void* piece, bool first) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          a.lo[bound_at + e] = kNothing;
-          a.hi[bound_at + e] = -kNothing;
-        }
-      continue;
+    for (int i = 0; i < N; ++i) {
+      V v;
+      if constexpr (kPairs) v = static_cast<const V*>(piece)[i];
+      else v = to_f32(static_cast<const T*>(piece)[i]);
+      low[i] = first ? v : least(low[i], v);
+      high[i] = first ? v : most(high[i], v);
     }
-    const int* kept = a.kept + static_cast<long long>(id) * a.keep;
-    const int tokens = min(a.L.b, now - t0);
-    // A full block whose last token stays in place is what it was.
-    if (tokens == a.L.b && kept[t0 + tokens - 1] == t0 + tokens - 1) continue;
-    T* pool = static_cast<T*>(const_cast<void*>(keys ? a.L.k : a.L.v));
-    const int* table = a.L.page_table + static_cast<long long>(b0) * (a.L.b / ps);
-    const int* rank = a.rank + static_cast<long long>(id) * (a.chunks + 1);
-    int* read = a.read + (static_cast<long long>(id) * 2 * a.segments + segment * 2 + (keys ? 0 : 1)) * a.chunks;
-    float low[E], high[E];
+  }
+  __device__ __forceinline__ void put(float* lo, float* hi) const {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      low[e] = __int_as_float(0x7f800000);
-      high[e] = -low[e];
-    }
-    for (int c = t0 / a.chunk; c * a.chunk < t0 + tokens && ok; ++c) {
-      const int first = c * a.chunk, count = min(a.chunk, t0 + tokens - first);
-      // The lane's token of the chunk: where it is, and where it goes.
-      const int to = first + min(lane, count - 1), from = kept[to];
-      auto place = [&](int token) {
-        int page = table[token / ps];
-        if (page < 0 || page >= a.pages) {
-          report(a.status, kStatusBadBlockId);
-          page = -1;
-        }
-        return page < 0 ? -1ll : (static_cast<long long>(page) * a.L.hkv + h) * ps + token % ps;
-      };
-      const long long source = place(from), goal = place(to);
-      const bool moves = __any_sync(kFull, from != to);
-      P x[kSteps];
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int t = i * at_once + group;
-        const long long s = __shfl_sync(kFull, source, min(t, 31));
-        if (active && t < count && s >= 0) x[i] = *reinterpret_cast<const P*>(pool + s * a.L.d + (p0 + column) * E);
-      }
-      if (moves) {
-        __threadfence();  // the chunk has been read before this is seen
-        __syncwarp();
-        if (lane == 0) *reinterpret_cast<volatile int*>(read + c) = 1;
-        // The earlier chunks of kept tokens that lie in this chunk's places.
-        const int i0 = rank[c], i1 = min(rank[c + 1], first);
-        if (i0 < i1) {
-          const int c0 = i0 / a.chunk, c1 = (i1 - 1) / a.chunk;
-          const volatile int* flag = read + min(c0 + lane, c1);
-          const unsigned long long began = global_ns();
-          // (A chunk that does not move reads its own places alone: nobody waits for it.)
-          while (!__all_sync(kFull, *flag != 0)) {
-            if (global_ns() - began > c_wait_ns) {
-              report(a.status, kStatusWaitTimeout);
-              ok = false;
-            }
-            if (__any_sync(kFull, !ok)) {
-              ok = false;
-              break;
-            }
-          }
-          __threadfence();
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int t = i * at_once + group;
-        const long long s = __shfl_sync(kFull, source, min(t, 31)), g = __shfl_sync(kFull, goal, min(t, 31));
-        if (!active || t >= count || s < 0 || g < 0 || !ok) continue;
-        if (s != g) *reinterpret_cast<P*>(pool + g * a.L.d + (p0 + column) * E) = x[i];
-        if (bounds) {
-          const T* v = reinterpret_cast<const T*>(&x[i]);
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            low[e] = min_nan(low[e], to_f32(v[e]));
-            high[e] = max_nan(high[e], to_f32(v[e]));
-          }
-        }
-      }
-    }
-    if (bounds && ok) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float l = low[e], u = high[e];
-        for (int g = 1; g < at_once; ++g) {
-          l = min_nan(l, __shfl_sync(kFull, low[e], (column + g * np) & 31));
-          u = max_nan(u, __shfl_sync(kFull, high[e], (column + g * np) & 31));
-        }
-        if (group == 0) {
-          a.lo[bound_at + e] = l;
-          a.hi[bound_at + e] = u;
-        }
+    for (int i = 0; i < N; ++i) {
+      if constexpr (kPairs) {
+        lo[2 * i] = to_f32(low[i].x);
+        lo[2 * i + 1] = to_f32(low[i].y);
+        hi[2 * i] = to_f32(high[i].x);
+        hi[2 * i + 1] = to_f32(high[i].y);
+      } else {
+        lo[i] = low[i];
+        hi[i] = high[i];
       }
     }
   }
+};
+
+// A chunk on its way: the rows of the pool that the lane's token of it is in and goes to, and its block.
+struct Chunk {
+  uint32_t source, goal;
+  int c, first, count, id, block;
+  bool keys, moves, opens, closes;  // of the block's chunks
+  int segment;
+};
+constexpr uint32_t kNoRow = 0xffffffffu;  // its page lies outside the pool
+
+// PIECE: bytes that a lane moves at once. PIECES: of a row (one segment), 0: any
+// number, in segments of 32. An item is one block of a row (all its chunks in
+// order), of K or of V, one segment.
+template <typename T, int PIECE, int PIECES>
+__global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const EvictArgs a, int items) {
+  using P = typename Piece<PIECE>::type;
+  constexpr int E = PIECE / static_cast<int>(sizeof(T));
+  extern __shared__ __align__(16) unsigned char stages[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned char* stage = stages + warp * kStage * kStageBytes;
+  const int rows = a.R * a.L.hkv, per = rows * 2 * a.segments;
+  const int pieces = a.L.d / E, ps = a.L.page_size, ppb = a.L.b / ps, row_bytes = pieces * PIECE;
+  const int ps_shift = (ps & (ps - 1)) == 0 ? __ffs(ps) - 1 : -1, chunk_shift = __ffs(a.chunk) - 1;
+  const int warps = static_cast<int>(gridDim.x) * kMoveWarps;
+  int item = static_cast<int>(blockIdx.x) * kMoveWarps + warp - warps;
+  // The item's block.
+  int id = 0, h = 0, segment = 0, t0 = 0, tokens = 0, next = 0, at_block = 0;
+  bool keys = false;
+  const int* kept = nullptr;
+  const int* table = nullptr;
+  // The lane's place in a step: which of the rows at once, which piece.
+  int np = PIECES, at_once = PIECES ? 32 / (PIECES ? PIECES : 1) : 0, group = PIECES ? lane / (PIECES ? PIECES : 1) : 0;
+  int column = PIECES ? lane % (PIECES ? PIECES : 1) : 0, set = -1;
+  auto lanes_of = [&](int seg) {
+    if (PIECES || seg == set) return;
+    set = seg;
+    np = min(32, pieces - seg * 32);
+    at_once = 32 / np;
+    group = lane / np;
+    column = lane - group * np;
+  };
+  // The next chunk that has something to do: its tokens' places.
+  auto fetch = [&](Chunk& x) {
+    while (next >= t0 + tokens) {
+      item += warps;
+      if (item >= items) return false;
+      const int block = item / per;
+      int rest = item - block * per;
+      const int line = rest / rows;
+      id = rest - line * rows;
+      keys = line % 2 == 0;
+      segment = line / 2;
+      const int r = id / a.L.hkv;
+      h = id - r * a.L.hkv;
+      tokens = 0;
+      next = t0 = block * a.L.b;
+      const int b0 = a.L.block_offsets[r];
+      if (held_tokens(a, r) <= a.keep) continue;
+      kept = a.kept + static_cast<long long>(id) * a.keep;
+      const int most = min(a.L.b, a.keep - t0);
+      // A full block whose last token stays in place is what it was.
+      if (most == a.L.b && kept[t0 + most - 1] == t0 + most - 1) continue;
+      tokens = most;
+      at_block = b0 + block;
+      table = a.L.page_table + static_cast<long long>(b0) * ppb;
+    }
+    x.first = next;
+    x.c = next >> chunk_shift;
+    x.count = min(a.chunk, t0 + tokens - next);
+    x.id = id;
+    x.block = at_block;
+    x.segment = segment;
+    x.keys = keys;
+    x.opens = next == t0;
+    next += x.count;
+    x.closes = next >= t0 + tokens;
+    const int to = x.first + min(lane, x.count - 1), from = kept[to];
+    auto place = [&](int token) {
+      const int in = ps_shift >= 0 ? token >> ps_shift : token / ps;
+      const int page = table[in];
+      if (page < 0 || page >= a.pages) {
+        report(a.status, kStatusBadBlockId);
+        return kNoRow;
+      }
+      return static_cast<uint32_t>((page * a.L.hkv + h) * ps + (token - in * ps));
+    };
+    x.source = place(from);
+    x.goal = place(to);
+    x.moves = __any_sync(kFull, from != to);
+    return true;
+  };
+  auto pool_of = [&](const Chunk& x) {
+    return static_cast<unsigned char*>(const_cast<void*>(x.keys ? a.L.k : a.L.v)) + (x.segment * 32 + column) * PIECE;
+  };
+  auto load = [&](const Chunk& x, unsigned char* to) {
+    lanes_of(x.segment);
+    const unsigned char* pool = pool_of(x);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if (i * at_once >= x.count) break;
+      const int t = i * at_once + group;
+      const uint32_t s = __shfl_sync(kFull, x.source, t & 31);
+      if ((PIECES || group < at_once) && t < x.count && s != kNoRow)
+        copy_piece<PIECE>(to + (i * 32 + lane) * PIECE, pool + static_cast<unsigned long long>(s) * row_bytes);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  Bounds<T, PIECE> bounds;
+  bool started = false;  // the lane has seen a value of the block
+  bool ok = true;
+  auto store = [&](const Chunk& x, const unsigned char* from) {
+    lanes_of(x.segment);
+    if (x.moves) {
+      int* read = a.read + (static_cast<long long>(x.id) * 2 * a.segments + x.segment * 2 + (x.keys ? 0 : 1)) * a.chunks;
+      const int* rank = a.rank + static_cast<long long>(x.id) * (a.chunks + 1);
+      // The earlier chunks of kept tokens that lie in this chunk's places.
+      const int i0 = rank[x.c], i1 = min(rank[x.c + 1], x.first);
+      asm volatile("fence.acq_rel.gpu;" ::: "memory");  // the chunk has been read before this is seen
+      __syncwarp();
+      if (lane == 0) asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(read + x.c) : "memory");
+      if (i0 < i1) {
+        const int* flag = read + min((i0 >> chunk_shift) + lane, (i1 - 1) >> chunk_shift);
+        auto seen = [&]() {
+          int f;
+          asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(f) : "l"(flag) : "memory");
+          return f != 0;
+        };
+        // (A chunk that does not move reads its own places alone: nobody waits for it.)
+        if (!__all_sync(kFull, seen())) {
+          const unsigned long long began = global_ns();
+          while (!__all_sync(kFull, seen())) {
+            if (__any_sync(kFull, global_ns() - began > c_wait_ns)) {
+              report(a.status, kStatusWaitTimeout);
+              ok = false;
+              return;
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+    const bool bounded = x.keys && a.lo != nullptr;
+    if (x.opens) started = false;
+    unsigned char* pool = pool_of(x);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if (i * at_once >= x.count) break;
+      const int t = i * at_once + group;
+      const uint32_t s = __shfl_sync(kFull, x.source, t & 31), g = __shfl_sync(kFull, x.goal, t & 31);
+      if ((!PIECES && group >= at_once) || t >= x.count || s == kNoRow || g == kNoRow) continue;
+      const P v = *reinterpret_cast<const P*>(from + (i * 32 + lane) * PIECE);
+      if (s != g) *reinterpret_cast<P*>(pool + static_cast<unsigned long long>(g) * row_bytes) = v;
+      if (bounded) {
+        bounds.take(&v, !started);
+        started = true;
+      }
+    }
+    if (bounded && x.closes) {
+      // Lanes of the same pieces: those without a value (fewer rows than lanes) take another's.
+      const unsigned have = __ballot_sync(kFull, started);
+      unsigned peers = 0;
+      for (int g = 0; g < at_once; ++g) peers |= 1u << (column + g * np);
+      peers &= have;
+      for (int g = 0; g < at_once; ++g) {
+        const int other = (column + g * np) & 31;
+        Bounds<T, PIECE> y = bounds;
+#pragma unroll
+        for (int i = 0; i < Bounds<T, PIECE>::N; ++i) {
+          y.low[i] = Bounds<T, PIECE>::shuffle(bounds.low[i], other);
+          y.high[i] = Bounds<T, PIECE>::shuffle(bounds.high[i], other);
+        }
+        if (group == 0 && g > 0 && (peers >> other & 1)) {
+#pragma unroll
+          for (int i = 0; i < Bounds<T, PIECE>::N; ++i) {
+            bounds.low[i] = started ? Bounds<T, PIECE>::least(bounds.low[i], y.low[i]) : y.low[i];
+            bounds.high[i] = started ? Bounds<T, PIECE>::most(bounds.high[i], y.high[i]) : y.high[i];
+          }
+          started = true;
+        }
+      }
+      if (group == 0 && started) {
+        const int hh = x.id % a.L.hkv;
+        const long long at = (hh * (a.slots / a.L.b) + x.block) * static_cast<long long>(a.L.d) + (x.segment * 32 + column) * E;
+        bounds.put(a.lo + at, a.hi + at);
+      }
+    }
+  };
+  Chunk x[2];
+  bool more = fetch(x[0]);
+  if (more) load(x[0], stage);
+  while (more) {  // two states by turns
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (!more) break;
+      more = fetch(x[s ^ 1]);
+      if (more) load(x[s ^ 1], stage + (s ^ 1) * kStageBytes);
+      if (more) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+      store(x[s], stage + s * kStageBytes);
+      __syncwarp();
+      if (!ok) more = false;
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <typename T, int PIECE, int PIECES>
+int launch_pieces(const EvictArgs& a, int sms, cudaStream_t stream) {
+  EvictArgs args = a;
+  const long long all = static_cast<long long>((a.keep + a.L.b - 1) / a.L.b) * a.R * a.L.hkv * 2 * a.segments;
+  if (all > 0x7fffffff - sms * kMoveWarps) return static_cast<int>(cudaErrorInvalidValue);
+  int items = static_cast<int>(all);
+  auto kern = evict_move_kernel<T, PIECE, PIECES>;
+  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoveBytes));
+  if (rc) return rc;
+  const int ctas = (items + kMoveWarps - 1) / kMoveWarps;
+  const int grid = ctas < sms ? ctas : sms;  // all of them resident: they wait for one another
+  void* params[] = {&args, &items};
+  return static_cast<int>(
+      cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kern), dim3(grid), dim3(kMoveWarps * 32), params, kMoveBytes, stream));
 }
 
 template <typename T, int PIECE>
 int launch_move(const EvictArgs& a, int sms, cudaStream_t stream) {
-  EvictArgs args = a;
-  long long items = static_cast<long long>((a.longest + a.L.b - 1) / a.L.b) * a.R * a.L.hkv * 2 * a.segments;
-  if (static_cast<long long>(a.R) * a.L.hkv * 2 * a.segments > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
-  auto kern = evict_move_kernel<T, PIECE>;
-  const long long ctas = (items + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
-  const int grid = static_cast<int>(ctas < 2ll * sms ? ctas : 2ll * sms);  // all of them resident: they wait for one another
-  void* params[] = {&args, &items};
-  return static_cast<int>(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kern), dim3(grid), dim3(kMoveThreads), params, 0, stream));
+  if (PIECE == 16) {
+    const int pieces = a.L.d * static_cast<int>(sizeof(T)) / 16;
+    if (pieces == 8) return launch_pieces<T, PIECE, PIECE == 16 ? 8 : 0>(a, sms, stream);
+    if (pieces == 16) return launch_pieces<T, PIECE, PIECE == 16 ? 16 : 0>(a, sms, stream);
+    if (pieces == 32) return launch_pieces<T, PIECE, PIECE == 16 ? 32 : 0>(a, sms, stream);
+  }
+  return launch_pieces<T, PIECE, 0>(a, sms, stream);
 }
 
 }  // namespace

@@ -24,6 +24,7 @@
 
 #include <cooperative_groups.h>
 
+#include "cta_select.cuh"
 #include "sample.cuh"
 
 namespace stk {
@@ -34,13 +35,6 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024, kBins = 1024;  // bins of a histogram: one to a thread
 constexpr float kBinsPerUnit = 32.f;
-
-using u64 = unsigned long long;
-
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return x == 0.f ? 0x80000000u : u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
-}
 
 struct Row {
   float max, rate32;
@@ -106,68 +100,10 @@ struct Shared {
   int take;
 };
 
-__device__ __forceinline__ float value_of(uint32_t key) {
-  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-}
-
 __device__ __forceinline__ void add_mass(Hist& h, int bin, u64 e) {
   const uint32_t e_low = static_cast<uint32_t>(e), old = atomicAdd(&h.low[bin], e_low);
   const uint32_t e_high = static_cast<uint32_t>(e >> 32) + (old + e_low < old ? 1u : 0u);
   if (e_high) atomicAdd(&h.high[bin], e_high);
-}
-
-// Sorts the first n of the CTA's values, one to a thread, in descending order
-// (the others are 0 and stay behind them). Warps without values only meet.
-__device__ __forceinline__ u64 sort_descending(u64 x, int n, u64* list) {
-  const int tid = threadIdx.x;
-  int size = 32;
-  while (size < n) size *= 2;
-  const bool active = tid < size;
-  for (int k = 2; k <= size; k *= 2) {
-    int j = k / 2;
-    for (; j >= 32; j /= 2) {
-      __syncthreads();
-      if (active) list[tid] = x;
-      __syncthreads();
-      if (active) {
-        const u64 y = list[tid ^ j];
-        const bool keep_large = ((tid & k) == 0) == ((tid & j) == 0);
-        x = (x > y) == keep_large ? x : y;
-      }
-    }
-    if (active) {
-#pragma unroll 1
-      for (; j > 0; j /= 2) {
-        const u64 y = __shfl_xor_sync(kFull, x, j);
-        const bool keep_large = ((tid & k) == 0) == ((tid & j) == 0);
-        x = (x > y) == keep_large ? x : y;
-      }
-    }
-  }
-  return x;
-}
-
-template <typename T>
-__device__ __forceinline__ T scan_add(T v, T* warp_sums, T& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(kFull, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  T s = warp_sums[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(kFull, s, o);
-    if (lane >= o) s += y;
-  }
-  total = __shfl_sync(kFull, s, 31);
-  const T before = __shfl_sync(kFull, s, max(warp - 1, 0));
-  return (warp ? before : T{0}) + x - v;
 }
 
 template <typename T>
