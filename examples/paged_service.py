@@ -3,8 +3,11 @@ prompts' tokens enter the page pool rotated, attend over it, and are followed
 by a few decode steps, each one an append, a dense attention and a strict Top-K
 selection whose block-sparse attention reads the same pages. Behind a system
 prompt that all requests share, its pages are stored and attended once.
+Requests that outgrow their share of the pool are cut back to the tokens that
+are attended most, and tokens are drawn from a head's logits on the way
+(``serve_within``).
 
-    python examples/paged_service.py [--requests 8] [--system 1024] [--steps 4]
+    python examples/paged_service.py [--requests 8] [--system 1024] [--steps 4] [--budget 96]
 """
 from __future__ import annotations
 
@@ -16,7 +19,7 @@ sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
 
 import torch  # noqa: E402
 
-from strict_topk_overlap_b200 import paged, paged_append, paged_attention, rotary  # noqa: E402
+from strict_topk_overlap_b200 import paged, paged_append, paged_attention, paged_eviction, rotary, sampling  # noqa: E402
 
 HQ, HKV, D, BLOCK, PAGE, TOPK = 32, 8, 128, 32, 16, 8
 
@@ -85,10 +88,60 @@ def serve(requests=8, system=1024, steps=4, seed=0, say=print):
     return worst
 
 
+def serve_within(budget=96, slack=32, prompts=(200, 40, 130), steps=80, sinks=4, recent=16, vocabulary=500, seed=0, say=print):
+    """Decodes with at most budget + slack tokens of a request in the pool: whenever that many are there, what was
+    attended least is evicted down to the budget. Each step's token is drawn from the logits of a random head and fed
+    back as the next step's embedding. Returns the cache, its lengths, the places in the sequence of the cached tokens
+    of each KV head, and the drawn tokens."""
+    gen = torch.Generator("cuda").manual_seed(seed)
+    requests = len(prompts)
+    room = max(max(prompts), budget + slack)
+    cache = paged_append.empty_paged_cache([room] * requests, HKV, D, BLOCK, PAGE, generator=torch.Generator().manual_seed(seed))
+    turn = rotary.build_rotary(max(prompts) + steps, D)
+    weights = paged_eviction.empty_weights(cache)
+    embeddings = torch.randn((vocabulary, (HQ + 2 * HKV) * D), generator=gen, device="cuda").to(torch.bfloat16)
+    head = torch.randn((HQ * D, vocabulary), generator=gen, device="cuda").to(torch.bfloat16)
+
+    # The prompts; their last tokens' attention is the first word on what is kept.
+    offsets = ints([sum(prompts[:r]) for r in range(requests + 1)])
+    q, k, v = projections(sum(prompts), gen)
+    q = paged_append.append_tokens(cache, k, v, ints([0] * requests), token_offsets=offsets, q=q, rotary=turn)
+    lengths = ints(prompts)
+    out, lse = paged_attention.attention(q, cache, lengths, token_offsets=offsets, max_tokens=max(prompts), return_lse=True)
+    paged_eviction.accumulate_weights(weights, q, cache, lengths, lse, token_offsets=offsets, max_tokens=max(prompts))
+    places = torch.arange(room, device="cuda").expand(requests, HKV, room)
+    out = out[offsets[1:].long() - 1]
+    seen, tokens = list(prompts), []
+    held = list(prompts)  # lengths, as the host knows them
+    for _ in range(steps):
+        if max(held) >= budget + slack:
+            lengths, kept = paged_eviction.evict(cache, weights, lengths, budget, first=sinks, last=recent)
+            held = [min(n, budget) for n in held]
+            moved = torch.gather(places, 2, kept.long().clamp(min=0))
+            places = torch.cat((torch.where(kept < 0, 0, moved), places[..., budget:]), -1)
+        logits = out.flatten(1) @ head
+        tokens.append(sampling.sample(logits, torch.rand((requests,), generator=gen, device="cuda"), temperature=0.8, top_k=40,
+                                      top_p=0.95))
+        qkv = embeddings[tokens[-1].long()].view(requests, HQ + 2 * HKV, D)
+        # The kept keys stay rotated as they were: a new token has its place in the sequence, not the one in the pool.
+        q = paged_append.append_tokens(cache, qkv[:, HQ:HQ + HKV], qkv[:, HQ + HKV:], lengths, q=qkv[:, :HQ], rotary=turn,
+                                       positions=ints(seen))
+        places = places.scatter(2, lengths.long()[:, None, None].expand(requests, HKV, 1),
+                                ints(seen).long()[:, None, None].expand(requests, HKV, 1))
+        lengths = lengths + 1
+        seen, held = [n + 1 for n in seen], [n + 1 for n in held]
+        out, lse = paged_attention.attention(q, cache, lengths, return_lse=True)
+        paged_eviction.accumulate_weights(weights, q, cache, lengths, lse)
+    say(f"{steps} steps within {budget} + {slack} tokens a request: {held} of {seen} tokens are kept")
+    return cache, lengths, places, torch.stack(tokens)
+
+
 if __name__ == "__main__":
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--requests", type=int, default=8)
     ap.add_argument("--system", type=int, default=1024)
     ap.add_argument("--steps", type=int, default=4)
+    ap.add_argument("--budget", type=int, default=96)
     a = ap.parse_args()
     serve(a.requests, a.system, a.steps)
+    serve_within(a.budget)
