@@ -5,9 +5,9 @@
 // Selection: a row (request, KV head) lies in the shared memory of a cluster
 // of up to eight CTAs, read once. The threshold's bin is found in a histogram over
 // the distance of the weights' order keys from the largest one, 32 bins to an
-// octave, and its tokens are sorted by one CTA, one to a thread. What is left
-// crowded (equal weights), or lies 32 octaves down, is found digit by digit of
-// the order keys. Then every warp counts and writes its stretch in order: IDs,
+// octave, and its tokens are sorted by one CTA, one to a thread (zeros have a bin
+// of their own and need no sorting). What is left crowded (equal weights) is
+// found digit by digit of the order keys. Then every warp counts and writes its stretch in order: IDs,
 // weights and, for the move, how many kept tokens lie before each chunk.
 //
 // Move: kept token i goes to place i <= its own. Moving in place saves half the
@@ -157,7 +157,12 @@ __global__ void __launch_bounds__(kThreads, 1) evict_select_kernel(const EvictAr
     goal -= sh.above;
     turn ^= 1;
   };
-  auto bin_of = [&](uint32_t key) { return static_cast<int>(min((top - key) >> kBinShift, static_cast<uint32_t>(kBins - 1))); };
+  // Zeros, the weights of tokens that nothing has seen, have a bin of their own before the last, the negative ones'.
+  constexpr uint32_t kZero = 0x80000000u;
+  auto bin_of = [&](uint32_t key) {
+    return key > kZero ? static_cast<int>(min((top - key) >> kBinShift, static_cast<uint32_t>(kBins - 3)))
+                       : key == kZero ? kBins - 2 : kBins - 1;
+  };
   auto middle = [&](auto f) {
     const int i1 = min(n, hi - begin);
     for (int i = max(0, lo - begin) + tid; i < i1; i += kThreads) f(i, weight_key(row[i]));
@@ -168,7 +173,11 @@ __global__ void __launch_bounds__(kThreads, 1) evict_select_kernel(const EvictAr
     middle([&](int, uint32_t key) { atomicAdd(&sh.hist[turn][bin_of(key)], 1); });
     choose(goal);
     const int bin = sh.bin, crowd = sh.crowd;
-    if (crowd <= kThreads && bin < kBins - 1) {
+    if (bin == kBins - 2) {
+      limit = kZero;
+      take = goal;
+      found = true;
+    } else if (crowd <= kThreads) {
       u64* list = cluster.map_shared_rank(sh.list, 0);
       int* listed = cluster.map_shared_rank(&sh.listed, 0);
       middle([&](int i, uint32_t key) {
@@ -581,10 +590,10 @@ int launch_move(const EvictArgs& a, int sms, cudaStream_t stream) {
 int launch_evict_select(const EvictArgs& a, int sms, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.R) * a.L.hkv;
   // CTAs of a row: as many as its tokens need, more while they find SMs and a
-  // few thousand tokens each.
+  // 16 K tokens each (fewer pay less for a pass than they pay for meeting).
   int parts = 1;
   while (parts * kEvictSlice < a.longest) parts *= 2;
-  while (parts < kEvictCluster && rows * parts * 2 <= sms && a.longest / parts > 4096) parts *= 2;
+  while (parts < kEvictCluster && rows * parts * 2 <= sms && a.longest / parts > 16384) parts *= 2;
   if (rows * parts > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
   const int bytes = static_cast<int>(sizeof(float)) * (((a.longest + parts - 1) / parts + 31) / 32 * 32);
   auto kern = evict_select_kernel;
