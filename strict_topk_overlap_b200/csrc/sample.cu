@@ -11,10 +11,10 @@
 // (2^t by a degree-9 polynomial, relative error 2e-14) and added as a 64-bit
 // whole number of 2^-44. A threshold is found in a histogram over the distance
 // from the largest logit, 32 bins to a unit, whose bins that may hold it are
-// sorted by one CTA, a token to a thread. top_k counts. For top_p a bin's count
-// bounds its mass from both sides (by 3 % at T = 1), which leaves a few bins; the
-// exact masses before them, and of all, are then added in registers (a mass
-// added to a histogram costs three atomics, more than the exponential). Where
+// sorted by one CTA, a token to a thread. top_k counts. For top_p the bins' counts
+// give a guess; the exact masses before the bins around it, and of all, are
+// then added in registers and theirs in a few counters of each warp (a mass added to
+// a histogram costs three atomics, more than the exponential). Where
 // the tokens up to top_k's bin are few, that CTA does the rest as well. Bins of too
 // many tokens are cut by a second histogram, and what even that leaves crowded
 // (many equal logits), or lies beyond its range, is found digit by digit of the
@@ -35,6 +35,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024, kBins = 1024;  // bins of a histogram: one to a thread
 constexpr float kBinsPerUnit = 32.f;
+constexpr int kNear = 8;  // bins around the guessed one that are looked at
 
 struct Row {
   float max, rate32;
@@ -86,9 +87,11 @@ struct Shared {
   float best;  // of the CTA: the largest logit
   int token;   // and the lowest token that has the row's
   int warp_min[32];
+  uint32_t part_low[32][2 * kNear + 1], part_high[32][2 * kNear + 1];  // mass of each warp's stretch in each of the bins that may hold the threshold
   double warp_doubles[32];
-  int from, to;      // bins that may hold the threshold
+  int from;          // the bin that is guessed to hold the threshold
   u64 whole;         // mass of all tokens
+  double bound, last;
   int equal;   // tokens at the limit
   u64 sum;     // mass of what stays
   int listed;  // tokens asked into the list
@@ -100,11 +103,12 @@ struct Shared {
   int take;
 };
 
-__device__ __forceinline__ void add_mass(Hist& h, int bin, u64 e) {
-  const uint32_t e_low = static_cast<uint32_t>(e), old = atomicAdd(&h.low[bin], e_low);
+__device__ __forceinline__ void add_mass(uint32_t* low, uint32_t* high, u64 e) {
+  const uint32_t e_low = static_cast<uint32_t>(e), old = atomicAdd(low, e_low);
   const uint32_t e_high = static_cast<uint32_t>(e >> 32) + (old + e_low < old ? 1u : 0u);
-  if (e_high) atomicAdd(&h.high[bin], e_high);
+  if (e_high) atomicAdd(high, e_high);
 }
+__device__ __forceinline__ void add_mass(Hist& h, int bin, u64 e) { add_mass(&h.low[bin], &h.high[bin], e); }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a) {
@@ -323,46 +327,77 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     __syncthreads();
   };
 
-  // ---- top_p alone: bounds on the bins' masses, then the exact ones where it matters
+  // ---- top_p alone: a guess from the bins' counts, then the exact masses around it
+  bool narrow = false;        // the bins that may hold it are few, and each warp knows their masses in its stretch
   bool before_known = false;  // the mass of what stays of the stretch in the bins before `from`
   u64 before_mass = 0;
   int from = 0, to = 0;
-  if ((top_k <= 0 || top_k >= a.V) && top_p < 1.f) {
+  const bool searched = (top_k <= 0 || top_k >= a.V) && top_p < 1.f;
+  bool decided = false;       // top_p leaves all that min_p does
+  u64 count = 0;              // tokens of the thread's bin
+  if (searched) {
     all_tokens([&](int, float x) { atomicAdd(&sh.hist.count[coarse_bin(x)], 1u); });
     cluster.sync();
-    u64 count, none;
+    u64 none;
     cluster_bin(tid, count, none, false);
-    // A distance is off by 2^-24 of 32 at most, a mass by half a unit.
-    const double near = fmax(0.0, (tid - 0.5) / kBinsPerUnit - 4e-6), far = (tid + 0.5) / kBinsPerUnit + 4e-6;
-    const double most = count ? static_cast<double>(count) * exp2(-near * w.rate) : 0.0;
-    const double least = count && tid < kBins - 1 ? static_cast<double>(count) * exp2(-far * w.rate) : 0.0;
-    double all_most, all_least;
-    const double up_to = scan_add<double>(most, sh.warp_doubles, all_most) + most;
-    const double down_to = scan_add<double>(least, sh.warp_doubles, all_least) + least;
+    // Were all of a bin at its middle, the threshold would be in bin `guess`; the masses within bins are even enough that
+    // it is at most a few bins away (if not, it is searched for below).
+    const double about = count ? static_cast<double>(count) * exp2(-tid / static_cast<double>(kBinsPerUnit) * w.rate) : 0.0;
+    double all_about;
+    const double up_to = scan_add<double>(about, sh.warp_doubles, all_about) + about;
     const double share = top_p > 0.f ? static_cast<double>(top_p) : 0.0;
-    const double goal_least = fmax(share * all_least * (1 - 1e-6), 1e-300), goal_most = share * all_most * (1 + 1e-6) + 1e-6;
-    if (tid == 0) sh.from = sh.to = kBins - 1;
+    if (tid == 0) sh.from = kBins - 1;
     __syncthreads();
-    from = __reduce_min_sync(kFull, up_to >= goal_least ? tid : kBins - 1);
-    to = __reduce_min_sync(kFull, down_to >= goal_most ? tid : kBins - 1);
-    if (lane == 0) {
-      atomicMin(&sh.from, from);
-      atomicMin(&sh.to, to);
-    }
+    const int guess = __reduce_min_sync(kFull, up_to >= share * all_about ? tid : kBins - 1);
+    if (lane == 0) atomicMin(&sh.from, guess);
     __syncthreads();
-    from = sh.from;
-    to = max(from, sh.to);
-    // ---- the exact mass of all, of the bins before, and of each that may hold the threshold
+    from = max(0, sh.from - kNear);
+    to = min(kBins - 1, sh.from + kNear);
+    // min_p decides alone where everything before `from` surely stays by top_p and nothing from there on does by min_p: a
+    // mass is off its bin's middle by half a bin and what rounding moves a distance by.
     const double bar = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+    const double half = 0.5 / kBinsPerUnit + 4e-6, factor = exp2(half * w.rate);
+    if (tid == max(from, 1) - 1) sh.bound = up_to;
+    if (tid == kBins - 1) sh.last = about;
+    __syncthreads();
+    decided = from > 0 && exp2(-(from / static_cast<double>(kBinsPerUnit) - half) * w.rate) < bar * (1 - 1e-9) &&
+              sh.bound * factor * factor < share * (all_about - sh.last) * (1 - 1e-6);
+    if (decided) clear();
+  }
+  if (searched && !decided) {
+    const double bar = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+    const double share = top_p > 0.f ? static_cast<double>(top_p) : 0.0;
+    // ---- the exact mass of all, of the bins before, and of each that may hold the threshold
     u64 whole = 0, above = 0;
-    with_masses(w0, w1, [&](int, float x, double m) {
-      const int bin = coarse_bin(x);
-      const u64 e = Row::in_units(m), early = bin < from ? e : 0ull;
-      whole += e;
-      above += early;
-      before_mass += m >= bar ? early : 0ull;
-      if (bin >= from && bin <= to) add_mass(sh.hist, bin, e);
-    });
+    narrow = bar == 0.0;
+    if (narrow) {  // by warps as well, whose stretches' masses need no second look then
+      if (lane <= 2 * kNear) sh.part_low[warp][lane] = sh.part_high[warp][lane] = 0;
+      __syncwarp();
+      with_masses(w0, w1, [&](int, float x, double m) {
+        const int bin = coarse_bin(x);
+        const u64 e = Row::in_units(m);
+        whole += e;
+        above += bin < from ? e : 0ull;
+        if (bin >= from && bin <= to) add_mass(&sh.part_low[warp][bin - from], &sh.part_high[warp][bin - from], e);
+      });
+      before_mass = above;
+      __syncthreads();
+      if (tid <= to - from) {
+        u64 e = 0;
+        for (int i = 0; i < 32; ++i) e += static_cast<u64>(sh.part_high[i][tid]) << 32 | sh.part_low[i][tid];
+        sh.hist.low[from + tid] = static_cast<uint32_t>(e);
+        sh.hist.high[from + tid] = static_cast<uint32_t>(e >> 32);
+      }
+    } else {
+      with_masses(w0, w1, [&](int, float x, double m) {
+        const int bin = coarse_bin(x);
+        const u64 e = Row::in_units(m), early = bin < from ? e : 0ull;
+        whole += e;
+        above += early;
+        before_mass += m >= bar ? early : 0ull;
+        if (bin >= from && bin <= to) add_mass(sh.hist, bin, e);
+      });
+    }
     u64 total;
     scan_add<u64>(whole, sh.warp_sums, total);
     if (tid == 0) sh.whole = total;
@@ -413,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   // ---- thresholds: first by counts (top_k), then by masses (top_p)
   for (int mode = 0; mode < 2; ++mode) {
     const bool counts = mode == 0;
-    if (counts ? top_k <= 0 || top_k >= a.V : !(top_p < 1.f) || before_known) continue;
+    if (counts ? top_k <= 0 || top_k >= a.V : !(top_p < 1.f) || before_known || decided) continue;
     // What of a token counts towards the goal; tokens at top_k's limit that do not all stay are told apart in the list.
     const bool some_at_limit = !counts && w.take != 0x7fffffff;
     u64 goal = counts ? static_cast<u64>(top_k) : 0, start = 0;  // start: the goal of the whole row
@@ -581,7 +616,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   u64 sum = 0;
   if (before_known && !ties) {
     sum = before_mass;
-    with_masses(w0, w1, [&](int, float x, double m) {
+    if (narrow) {
+      if (lane < to - from) sum += static_cast<u64>(sh.part_high[warp][lane]) << 32 | sh.part_low[warp][lane];
+      for_each(w0, w1, lane, 32, [&](int, float x) {
+        if (coarse_bin(x) == to && order_key(x) > w.limit) sum += w.units(x);
+      });
+    } else with_masses(w0, w1, [&](int, float x, double m) {
       const int bin = coarse_bin(x);
       const bool in = (static_cast<unsigned>(bin - from) <= static_cast<unsigned>(to - from)) & (order_key(x) > w.limit) &
                       (m >= w.least);
