@@ -10,7 +10,7 @@
 // lose what lies between two tokens of a large vocabulary: e is computed in FP64
 // (2^t by a degree-9 polynomial, relative error 2e-14) and added as a 64-bit
 // whole number of 2^-44. A threshold is found in a histogram over the distance
-// from the largest logit, 32 bins to a unit, whose bins that may hold it are
+// from the largest logit, 64 bins to a unit, whose bins that may hold it are
 // sorted by one CTA, a token to a thread. top_k counts. For top_p the bins' counts
 // give a guess; the exact masses before the bins around it, and of all, are
 // then added in registers and theirs in a few counters of each warp (a mass added to
@@ -34,7 +34,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024, kBins = 1024;  // bins of a histogram: one to a thread
-constexpr float kBinsPerUnit = 32.f;
+constexpr float kBinsPerUnit = 64.f;
 constexpr int kNear = 8;  // bins around the guessed one that are looked at
 
 struct Row {
