@@ -21,6 +21,15 @@
 // logits' order keys. All of it is exact and the same on every run.
 //
 // A row is read once, into the shared memory of a cluster of up to eight CTAs.
+//
+// Far from bound by HBM (64 rows of 131,072 FP32 logits: 5 us of bytes): a pass
+// over the masses is 14 FP64 operations and some fifty instructions a token, one
+// over the histogram an atomic. Measured (B200): one row of 32,001, top_k 50 and
+// top_p 0.9: 16 us; those 64 rows with top_p 0.95: 78 us, with top_k 50: 38, with
+// neither: 37 (two rounds of CTAs, one to an SM: their slices fill its shared
+// memory); 256 rows of 50,257 bf16 logits with parameters of their own: 104 us.
+// The three passes of digits over counts and masses that the rest falls back to
+// took 86, 173 and 173 us.
 
 #include <cooperative_groups.h>
 

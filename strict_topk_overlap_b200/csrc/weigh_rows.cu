@@ -14,7 +14,8 @@
 // shared memory: a warp's lanes share a key's dims, eight keys are on their way
 // at once, and the 8 x 4 sums of eight keys and four rows are transposed into
 // one per lane (31 shuffles). 5 requests of 700 to 9,000 tokens, 32 / 8 heads,
-// FP32: 58 us in the form above, whose CTAs live for one chain of loads.
+// FP32 (82 MB): 36 us, 2.3 TB/s (58 in the form above), of which a CTA's chain of
+// loads (offsets, lengths, table, keys) is most: it lives for 256 keys.
 
 #include "weigh.cuh"
 

@@ -5,8 +5,8 @@
 //   S^T = K Q^T        128 keys x up to 112 rows, FP32 in tensor memory
 //   sum += 2^(c S - lse)   one thread per key; a row's log-sum-exp, known
 //                          beforehand, is the same for all of a warp's keys
-// No running maximum, no reduction across threads, no atomics: a key's sum is
-// taken in the order of its rows.
+// No running maximum, no sums across lanes: a key's sum is taken in the order of
+// its rows, and reaches the weights by one reduction, the key's only one.
 //
 // A job is 256 keys (128 where the rows are few) of one request's KV head and a
 // part of its rows. The CTAs of a persistent grid (one per SM) take the jobs in
@@ -24,6 +24,26 @@
 // rows every second job), one that walks over jobs and row tiles ahead of all
 // others, and four for the log-sum-exps and key intervals of the row tiles'
 // rows, in turn.
+//
+// HBM-bound for single tokens: K is read once. 64 requests of 8-32 K tokens, 16 /
+// 8 heads, bf16 (2.6 GB): 396 us, 6.7 TB/s; 16 requests of 4-12 K: 49 us, 80 %
+// of a copy's rate. What it took: whole pages of a head in one copy each (a
+// 5-dimensional map puts the halves of 8 keys next to each other), issued as
+// predicates of uniform code (128-dim boxes lane by lane cost 130 clocks each
+// and held the kernel at 58 %), and results added by reductions that nobody
+// waits for.
+//
+// With prompts bound by the exponentials in principle: 16 per SM and clock, 1,792
+// clocks for 256 keys x 112 rows, whose products are 960. In fact about 3,000:
+// a warp's waits and the tile's bookkeeping, some 1,100 clocks, run under the
+// other group's exponentials only in part. Three prompts of 1.5-8 K tokens, 16 / 8
+// heads, D 128: 180 us (69 at the tensor cores' rate), capped 261; the last 64
+// tokens of 4 prompts of 17-32 K: 102; 15 K tokens in a window of 1,024, D 64,
+// biased: 339. On the plain prompts, in the order tried: every load warp
+// walking over all items 194-243 us, one walking warp 194, batches of its row tiles
+// 184, row tiles by turns instead of halves of each 180; row tiles of 64 with four
+// S buffers 199, exponentials on the FMA units 188-228 (the issue slots, not the
+// special function unit alone, are short), waits with long suspensions 241.
 //
 // Rows that see none of a warp's keys are skipped tile by tile, tiles whose
 // rows all see all of a warp's keys need no mask. Unseen keys may hold
