@@ -47,7 +47,7 @@ constexpr float kBinsPerUnit = 64.f;
 constexpr int kNear = 8;  // bins around the guessed one that are looked at
 
 struct Row {
-  float max, rate32;
+  float max, half, rate32;  // half of the largest logit
   double top, rate;  // the largest logit, log2 e / T
   double least;      // mass below which a token does not stay
   // Tokens above `limit` stay, of those at it the first `take`.
@@ -71,7 +71,8 @@ struct Row {
     p = fma(p, f, 1.0);
     const double e = __hiloint2double(__double2hiint(p) + (__double2loint(m) << 20), __double2loint(p));
     // Nothing below 2^-60, nor of -inf at an infinite temperature (no number); infinities weigh alike.
-    return x == max ? 1.0 : (max - x) * rate32 <= 60.f ? e : 0.0;
+    // (Half the distance: the whole one may pass FP32's largest number.)
+    return x == max ? 1.0 : fmaf(x, -0.5f, half) * rate32 <= 30.f ? e : 0.0;
   }
   // As a whole number of 2^-44: the last bits of e + 256.
   static __device__ __forceinline__ u64 in_units(double e) {
@@ -201,6 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   }
   Row w;
   w.max = best;
+  w.half = 0.5f * best;
   w.top = static_cast<double>(best);
   w.rate = 1.4426950408889634 / static_cast<double>(temperature);
   w.rate32 = static_cast<float>(w.rate);

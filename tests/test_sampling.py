@@ -96,6 +96,15 @@ def test_odd_logits(more):
 
 
 @gpu
+@pytest.mark.parametrize("more", [dict(), dict(top_k=3), dict(top_p=0.9), dict(min_p=0.2)])
+def test_distances_beyond_the_largest_number(more):
+    """Logits whose difference FP32 cannot hold, at temperatures that make masses of it all the same."""
+    x = torch.tensor([[3e38, -3e38, 1e38, 0.0, -2e38]], device=DEV).expand(64, 5)
+    u = torch.arange(64, device=DEV).float() / 64 + 1 / 200
+    _check(x, u, temperature=3e38, **more)
+
+
+@gpu
 def test_numbers_at_the_ends():
     """0, the last number below 1, and numbers outside [0, 1), which count as its ends."""
     x, _ = _rows(1, 700, torch.float32, 5)
