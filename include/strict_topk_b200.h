@@ -526,7 +526,7 @@ STK_API size_t stk_evict_tokens_workspace_bytes(const stk_kv* kv, int R, int tot
  * and the last `last` ones stay, and of the others those of the largest weights
  * [hkv, total_blocks, b] (ties to the lower place, NaN above all). What stays
  * moves to the front of the request's own pages, in its order: K, V and the
- * weights (to weights_out, which may be weights; zeros behind the last token),
+ * weights (to weights_out: weights, or apart from them; zeros behind the last token),
  * and the bounds lo / hi (NULL: none kept) of the blocks that changed, 1e30 and
  * -1e30 where a block is left without tokens. kept [R, hkv, keep] names the
  * tokens (ascending; -1 behind the last one of a shorter request), lengths_out

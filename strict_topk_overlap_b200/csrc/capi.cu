@@ -1228,6 +1228,9 @@ extern "C" int stk_evict_tokens(const stk_kv* kv, int pages, int R, int total_bl
   if (static_cast<long long>(pages) * kv->hkv * kv->page_size >= 0x7fffffff)
     return fail(STK_EINVAL, "a pool of %d pages has too many rows", pages);
   if (lengths == lengths_out) return fail(STK_EINVAL, "lengths_out must not be lengths: both are read and written");
+  const uintptr_t in = reinterpret_cast<uintptr_t>(weights), out = reinterpret_cast<uintptr_t>(weights_out);
+  if (in != out && (in < out ? out - in : in - out) < static_cast<uintptr_t>(total_blocks) * kv->b * kv->hkv * sizeof(float))
+    return fail(STK_EINVAL, "weights_out must be weights or lie apart from them");
   EvictArgs a{};
   const int piece = evict_piece(kv->kv_dtype, kv->d, kv->k, kv->v);
   const size_t need = plan_evict(a, kv, R, total_blocks, keep, max_length, piece);

@@ -100,8 +100,8 @@ def accumulate_weights(weights, q, cache: PagedKVCache, lengths, lse, *, token_o
         if need:
             workspace = q.new_empty((need,), dtype=torch.uint8)
     else:
-        if workspace.get_device() != index:
-            raise ValueError("workspace must be on the cache's device")
+        if workspace.get_device() != index or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous and on the cache's device")
         need = workspace.numel()
     rc = L.on_device(index, L.load().stk_accumulate_weights, kv, pages, qp, qt, qh, requests, t, hq, blocks, held, offsets,
                      most, longest, options, lse.data_ptr(), to, L.ptr(workspace), need, L.status_ptr(),
@@ -134,7 +134,8 @@ def evict(cache: PagedKVCache, weights, lengths, keep, *, first=0, last=0, weigh
     lower place, NaN above all). Keys, values and weights of what stays move to
     the front, in their order; lo / hi of the blocks that changed are taken anew
     (where the cache keeps them), emptied blocks get ``empty_paged_cache``'s.
-    Weights go to ``weights_out`` (None: in place), zeros behind the last token.
+    Weights go to ``weights_out`` (None: in place; memory that overlaps
+    theirs in part is refused), zeros behind the last token.
     Pages that requests share are written where their tokens move: protect a
     shared prefix by ``first``. Requests hold at most 393,216 tokens. Returns the
     new lengths [R] and the kept places [R, Hkv, keep] int32, ascending, -1
@@ -161,8 +162,8 @@ def evict(cache: PagedKVCache, weights, lengths, keep, *, first=0, last=0, weigh
         need = _evict_bytes(index, L.dtype_code(pool), hkv, block, d, cache.page_size, requests, blocks, keep, longest)
         workspace = weights.new_empty((need,), dtype=torch.uint8)
     else:
-        if workspace.get_device() != index:
-            raise ValueError("workspace must be on the cache's device")
+        if workspace.get_device() != index or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous and on the cache's device")
         need = workspace.numel()
     kept = lengths.new_empty((requests, hkv, keep))
     now = lengths.new_empty((requests,))

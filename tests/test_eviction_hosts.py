@@ -90,6 +90,14 @@ def test_arguments_of_eviction(untouched, change):
         _evict(_cache(_on_device), a["weights"], a["lengths"], **more)
 
 
+def test_workspaces_without_memory_of_their_own(untouched):
+    a, spread = _args(), _on_device(torch.zeros(1, dtype=torch.uint8).expand(1 << 20))
+    with pytest.raises(ValueError, match="workspace"):
+        _weigh(_cache(_on_device), **a, workspace=spread)
+    with pytest.raises(ValueError, match="workspace"):
+        _evict(_cache(_on_device), a["weights"], a["lengths"], workspace=spread)
+
+
 def test_bounds_of_eviction(untouched):
     a, cache = _args(), _cache(_on_device)
     cache.hi = _on_device(torch.zeros(2, 4, 32))
@@ -186,6 +194,7 @@ def test_library_refusals_of_eviction(lib):
                       (dict(now=None), b"null"), (dict(pages=0), b"pool"), (dict(R=0), b"shape"), (dict(total=0), b"shape"),
                       (dict(longest=0), b"shape"), (dict(keep=0), b"kept"), (dict(first=5, last=4), b"kept"), (dict(first=-1), b"kept"),
                       (dict(first=2 ** 31 - 1, last=2 ** 31 - 1), b"kept"), (dict(hi=None), b"together"), (dict(now=256), b"lengths_out"),
+                      (dict(out=256 + 4), b"apart"), (dict(weights=256 + 64 * 4), b"apart"),
                       (dict(kv=_kv(table=0)), b"paged"), (dict(ws=264), b"boundary"), (dict(pages=2 ** 31 - 1), b"rows")):
         assert call(**bad) == -1 and word in lib.stk_last_error(), (bad, lib.stk_last_error())
     assert call(longest=400000) == -2 and b"393216" in lib.stk_last_error()
