@@ -305,6 +305,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 constexpr int kMoveWarps = 12, kSteps = 16, kStage = 2;  // a warp's chunks in shared memory
+static_assert(32 / kEvictSegment * kSteps >= 32, "a chunk is 32 rows at most");
 constexpr int kStageBytes = kSteps * 32 * 16;
 constexpr int kMoveBytes = kMoveWarps * kStage * kStageBytes;
 
@@ -372,8 +373,8 @@ struct Chunk {
 };
 constexpr uint32_t kNoRow = 0xffffffffu;  // its page lies outside the pool
 
-// PIECE: bytes that a lane moves at once. PIECES: of a row (one segment), 0: any
-// number, in segments of 32. An item is one block of a row (all its chunks in
+// PIECE: bytes that a lane moves at once. PIECES: of each segment of a row, 0: any
+// number. An item is one block of a row (all its chunks in
 // order), of K or of V, one segment.
 template <typename T, int PIECE, int PIECES>
 __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const EvictArgs a, int items) {
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const Ev
   auto lanes_of = [&](int seg) {
     if (PIECES || seg == set) return;
     set = seg;
-    np = min(32, pieces - seg * 32);
+    np = min(kEvictSegment, pieces - seg * kEvictSegment);
     at_once = 32 / np;
     group = lane / np;
     column = lane - group * np;
@@ -454,7 +455,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const Ev
     return true;
   };
   auto pool_of = [&](const Chunk& x) {
-    return static_cast<unsigned char*>(const_cast<void*>(x.keys ? a.L.k : a.L.v)) + (x.segment * 32 + column) * PIECE;
+    return static_cast<unsigned char*>(const_cast<void*>(x.keys ? a.L.k : a.L.v)) + (x.segment * kEvictSegment + column) * PIECE;
   };
   auto load = [&](const Chunk& x, unsigned char* to) {
     lanes_of(x.segment);
@@ -479,8 +480,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const Ev
       const int* rank = a.rank + static_cast<long long>(x.id) * (a.chunks + 1);
       // The earlier chunks of kept tokens that lie in this chunk's places.
       const int i0 = rank[x.c], i1 = min(rank[x.c + 1], x.first);
-      asm volatile("fence.acq_rel.gpu;" ::: "memory");  // the chunk has been read before this is seen
-      __syncwarp();
+      __syncwarp();  // all lanes have read the chunk before the release
       if (lane == 0) asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(read + x.c) : "memory");
       if (i0 < i1) {
         const int* flag = read + min((i0 >> chunk_shift) + lane, (i1 - 1) >> chunk_shift);
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const Ev
       }
       if (group == 0 && started) {
         const int hh = x.id % a.L.hkv;
-        const long long at = (hh * (a.slots / a.L.b) + x.block) * static_cast<long long>(a.L.d) + (x.segment * 32 + column) * E;
+        const long long at = (hh * (a.slots / a.L.b) + x.block) * static_cast<long long>(a.L.d) + (x.segment * kEvictSegment + column) * E;
         bounds.put(a.lo + at, a.hi + at);
       }
     }
@@ -590,8 +590,7 @@ int launch_move(const EvictArgs& a, int sms, cudaStream_t stream) {
   if (PIECE == 16) {
     const int pieces = a.L.d * static_cast<int>(sizeof(T)) / 16;
     if (pieces == 8) return launch_pieces<T, PIECE, PIECE == 16 ? 8 : 0>(a, sms, stream);
-    if (pieces == 16) return launch_pieces<T, PIECE, PIECE == 16 ? 16 : 0>(a, sms, stream);
-    if (pieces == 32) return launch_pieces<T, PIECE, PIECE == 16 ? 32 : 0>(a, sms, stream);
+    if (pieces % 16 == 0) return launch_pieces<T, PIECE, PIECE == 16 ? 16 : 0>(a, sms, stream);
   }
   return launch_pieces<T, PIECE, 0>(a, sms, stream);
 }

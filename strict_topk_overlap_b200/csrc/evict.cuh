@@ -22,7 +22,7 @@ struct EvictArgs {
   // Between the two kernels: tokens are moved in chunks, each announced once it
   // has been read.
   int chunk, chunks;     // tokens of a chunk (a power of two that divides b), chunks of `keep` tokens
-  int segments;          // parts of a row (of 32 pieces) that are moved apart
+  int segments;          // parts of a row (of kEvictSegment pieces) that are moved apart
   int* rank;             // [R * hkv, chunks + 1] kept tokens before each chunk's first place
   int* read;             // [R * hkv, 2 * segments, chunks] flags
   int* status;
@@ -30,6 +30,7 @@ struct EvictArgs {
 
 constexpr int kEvictCluster = 8;        // CTAs that share a row at most
 constexpr int kEvictSlice = 49152;      // its tokens that one of them holds in shared memory
+constexpr int kEvictSegment = 16;       // pieces of a row that are moved together: a chunk of 32 rows in 16 steps of a warp
 constexpr int kEvictMost = kEvictCluster * kEvictSlice;
 
 // Bytes of the pieces that rows of the pools are moved in.
@@ -39,15 +40,12 @@ inline int evict_piece(int kv_dtype, int d, const void* k, const void* v) {
   return any % 16 == 0 ? 16 : any % 4 == 0 ? 4 : 2;
 }
 
-// Tokens of a chunk: at most 16 pieces a lane, of 32 / (pieces of a row) rows at once.
+// Tokens of a chunk: one to a lane, if they divide the block.
 inline void evict_plan(EvictArgs& a, int kv_dtype, int piece) {
   const int row = a.L.d * (kv_dtype == kF32 ? 4 : 2) / piece;
-  a.segments = (row + 31) / 32;
-  const int lanes = row < 32 ? row : 32;
-  int most = 32 / lanes * 16;
-  most = most < 32 ? most : 32;
+  a.segments = (row + kEvictSegment - 1) / kEvictSegment;
   a.chunk = 1;
-  while (2 * a.chunk <= most && a.L.b % (2 * a.chunk) == 0) a.chunk *= 2;
+  while (a.chunk < 32 && a.L.b % (2 * a.chunk) == 0) a.chunk *= 2;
   a.chunks = (a.keep + a.chunk - 1) / a.chunk;
 }
 
