@@ -7,28 +7,31 @@
 // the distance of the weights' order keys from the largest one, 32 bins to an
 // octave, and its tokens are sorted by one CTA, one to a thread (zeros have a bin
 // of their own and need no sorting). What is left crowded (equal weights) is
-// found digit by digit of the order keys. Then every warp counts and writes its stretch in order: IDs,
-// weights and, for the move, how many kept tokens lie before each chunk.
+// found digit by digit of the order keys. Then every warp counts and writes its
+// stretch in order: IDs, weights and, for the move, how many kept tokens lie
+// before each chunk.
 //
 // Move: kept token i goes to place i <= its own. Moving in place saves half the
 // bytes of a way through a copy, but a place may be overwritten only after it
-// has been read. A warp reads a chunk into registers, announces that, waits for
-// the (at most two) earlier chunks that read the places it writes, and writes.
+// has been read. A warp copies a chunk into shared memory, announces that, waits
+// for the (at most two) earlier chunks that read the places it writes, and writes.
 // The warps of a co-resident grid take chunks in ascending order, so each waits
-// for earlier ones only and some warp can always go on. A warp's next chunk is on
-// its way into shared memory while one is written. A block's key bounds are taken
-// by the warp that moves its keys.
+// for earlier ones only and some warp can always go on. As many warps as shared
+// memory holds chunks for: each is a chain of latencies (places, rows, the
+// announcement, the wait). A block's key bounds are taken by the warp that moves
+// its keys.
 //
 // Measured (B200, D 128, calls in a row): 16 prompts of 1.5-32 K tokens cut to
-// 2 K each, 8 heads, bf16 (268 MB moved, 120 MB of bounds reset): 129 us, 52 of
+// 2 K each, 8 heads, bf16 (268 MB moved, 120 MB of bounds reset): 114 us, 52 of
 // them the selection, whose CTAs hold 32 K weights each; 6 requests of 20-60 K
-// tokens cut to 16 K, f16 (800 MB moved): 246 us, 3.4 TB/s. Read and written
-// rows are single ones of 256 bytes wherever the kept tokens lie, and about a
-// thousand instructions a chunk of 32 rows. On the same calls: chunks in
-// registers instead of shared memory and one item for every block of the cache,
-// kept or not, 199 and 309 us; three passes of digits instead of one histogram
-// in the selection, 48 against 30 us for the selection without the bounds. A
-// copy to other pages and back would move twice the bytes.
+// tokens cut to 16 K, f16 (800 MB moved): 212 us, 4 TB/s; 6 requests of 8-9 K
+// to 4 K, FP32: 131. Read and written rows are single ones of 256 bytes wherever
+// the kept tokens lie. The first two calls with 12 warps an SM of two chunks each
+// took 126 and 240 us, 14: 118 and 224, chunks of 16 rows 146 and 268, chunks in
+// registers and one item for every block of the cache, kept or not, 199 and 309;
+// the selection by three passes of digits instead of one histogram 48 instead of
+// 30 us (without the bounds), by twice the CTAs, two to an SM, the same. A copy
+// to other pages and back would move twice the bytes.
 
 #include <cooperative_groups.h>
 
@@ -304,10 +307,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-constexpr int kMoveWarps = 12, kSteps = 16, kStage = 2;  // a warp's chunks in shared memory
+constexpr int kMoveWarps = 28, kSteps = 16;  // warps of a CTA at most, steps of a chunk
 static_assert(32 / kEvictSegment * kSteps >= 32, "a chunk is 32 rows at most");
-constexpr int kStageBytes = kSteps * 32 * 16;
-constexpr int kMoveBytes = kMoveWarps * kStage * kStageBytes;
+constexpr int kStageBytes = kSteps * 32 * 16;  // a warp's chunk in shared memory
 
 template <int PIECE>
 __device__ __forceinline__ void copy_piece(void* to, const void* from) {
@@ -382,12 +384,12 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const Ev
   constexpr int E = PIECE / static_cast<int>(sizeof(T));
   extern __shared__ __align__(16) unsigned char stages[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned char* stage = stages + warp * kStage * kStageBytes;
+  unsigned char* stage = stages + warp * kStageBytes;
   const int rows = a.R * a.L.hkv, per = rows * 2 * a.segments;
   const int pieces = a.L.d / E, ps = a.L.page_size, ppb = a.L.b / ps, row_bytes = pieces * PIECE;
   const int ps_shift = (ps & (ps - 1)) == 0 ? __ffs(ps) - 1 : -1, chunk_shift = __ffs(a.chunk) - 1;
-  const int warps = static_cast<int>(gridDim.x) * kMoveWarps;
-  int item = static_cast<int>(blockIdx.x) * kMoveWarps + warp - warps;
+  const int warps = static_cast<int>(gridDim.x) * (static_cast<int>(blockDim.x) >> 5);
+  int item = static_cast<int>(blockIdx.x) + warp * static_cast<int>(gridDim.x) - warps;
   // The item's block.
   int id = 0, h = 0, segment = 0, t0 = 0, tokens = 0, next = 0, at_block = 0;
   bool keys = false;
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const Ev
   auto pool_of = [&](const Chunk& x) {
     return static_cast<unsigned char*>(const_cast<void*>(x.keys ? a.L.k : a.L.v)) + (x.segment * kEvictSegment + column) * PIECE;
   };
-  auto load = [&](const Chunk& x, unsigned char* to) {
+  auto load = [&](const Chunk& x) {
     lanes_of(x.segment);
     const unsigned char* pool = pool_of(x);
 #pragma unroll
@@ -466,14 +468,14 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const Ev
       const int t = i * at_once + group;
       const uint32_t s = __shfl_sync(kFull, x.source, t & 31);
       if ((PIECES || group < at_once) && t < x.count && s != kNoRow)
-        copy_piece<PIECE>(to + (i * 32 + lane) * PIECE, pool + static_cast<unsigned long long>(s) * row_bytes);
+        copy_piece<PIECE>(stage + (i * 32 + lane) * PIECE, pool + static_cast<unsigned long long>(s) * row_bytes);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   Bounds<T, PIECE> bounds;
   bool started = false;  // the lane has seen a value of the block
   bool ok = true;
-  auto store = [&](const Chunk& x, const unsigned char* from) {
+  auto store = [&](const Chunk& x) {
     lanes_of(x.segment);
     if (x.moves) {
       int* read = a.read + (static_cast<long long>(x.id) * 2 * a.segments + x.segment * 2 + (x.keys ? 0 : 1)) * a.chunks;
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const Ev
       const int t = i * at_once + group;
       const uint32_t s = __shfl_sync(kFull, x.source, t & 31), g = __shfl_sync(kFull, x.goal, t & 31);
       if ((!PIECES && group >= at_once) || t >= x.count || s == kNoRow || g == kNoRow) continue;
-      const P v = *reinterpret_cast<const P*>(from + (i * 32 + lane) * PIECE);
+      const P v = *reinterpret_cast<const P*>(stage + (i * 32 + lane) * PIECE);
       if (s != g) *reinterpret_cast<P*>(pool + static_cast<unsigned long long>(g) * row_bytes) = v;
       if (bounded) {
         bounds.take(&v, !started);
@@ -551,22 +553,19 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 1) evict_move_kernel(const Ev
   };
   Chunk x[2];
   bool more = fetch(x[0]);
-  if (more) load(x[0], stage);
-  while (more) {  // two states by turns
+  while (more) {  // two states by turns: the next chunk's places are looked up while one's rows are on their way
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       if (!more) break;
+      load(x[s]);
       more = fetch(x[s ^ 1]);
-      if (more) load(x[s ^ 1], stage + (s ^ 1) * kStageBytes);
-      if (more) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncwarp();
-      store(x[s], stage + s * kStageBytes);
+      store(x[s]);
       __syncwarp();
       if (!ok) more = false;
     }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 template <typename T, int PIECE, int PIECES>
@@ -576,13 +575,13 @@ int launch_pieces(const EvictArgs& a, int sms, cudaStream_t stream) {
   if (all > 0x7fffffff - sms * kMoveWarps) return static_cast<int>(cudaErrorInvalidValue);
   int items = static_cast<int>(all);
   auto kern = evict_move_kernel<T, PIECE, PIECES>;
-  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoveBytes));
+  const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoveWarps * kStageBytes));
   if (rc) return rc;
-  const int ctas = (items + kMoveWarps - 1) / kMoveWarps;
-  const int grid = ctas < sms ? ctas : sms;  // all of them resident: they wait for one another
+  const int grid = items < sms ? items : sms;  // all of them resident: they wait for one another
+  const int each = (items + grid - 1) / grid, warps = each < kMoveWarps ? each : kMoveWarps;
   void* params[] = {&args, &items};
-  return static_cast<int>(
-      cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kern), dim3(grid), dim3(kMoveWarps * 32), params, kMoveBytes, stream));
+  return static_cast<int>(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kern), dim3(grid), dim3(warps * 32), params,
+                                                      static_cast<size_t>(warps) * kStageBytes, stream));
 }
 
 template <typename T, int PIECE>
