@@ -523,9 +523,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
       const int bin = sh.bin, crowd = sh.crowd, upto = sh.upto;
       clear();
       if (level == 0 && upto <= kThreads && !some_at_limit) {
-        // ---- few: all of them go to the first CTA, which does the rest
+        // ---- few: all of them (those that top_k left: `upto` counts no others) go to the first CTA, which does the rest
         all_tokens([&](int i, float x) {
-          if (bin_of(x) <= bin) enlist(i, order_key(x));
+          const uint32_t key = order_key(x);
+          if (bin_of(x) <= bin && (counts || key > w.limit)) enlist(i, key);
         });
         hand_over();
         if (part != 0) return;
