@@ -620,10 +620,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     cluster.sync();
     for (int p = 0; p < part; ++p) equal += *cluster.map_shared_rank(&sh.equal, p);
   }
-  // Mass of a token, with `e` tokens at the limit before it.
+  // Mass of a token, with `e` tokens at the limit before it. (Without ties the limit is the order key below the last
+  // logit that stays: a logit one unit in its last place lower does not.)
   auto stays = [&](float x, int e) {
     const uint32_t key = order_key(x);
-    return key > w.limit || (key == w.limit && e < w.take) ? w.units(x) : 0ull;
+    return key > w.limit || (ties && key == w.limit && e < w.take) ? w.units(x) : 0ull;
   };
   u64 sum = 0;
   if (before_known && !ties) {

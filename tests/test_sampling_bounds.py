@@ -1,6 +1,6 @@
 """Sampling where the thresholds of top_k and top_p meet: in one bin of the
-kernel's histogram, among more tokens than one CTA sorts, behind masked tokens.
-Each row is drawn from with many numbers and
+kernel's histogram, among neighbouring numbers, among more tokens than one CTA
+sorts, behind masked tokens. Each row is drawn from with many numbers and
 compared with the definition in 64 bits; a decision that lies within four times
 what the masses' sums may be off by (whole numbers of 2^-44, 2e-14 relative)
 from its border is left out."""
@@ -89,6 +89,31 @@ def test_top_k_with_top_p(dtype, v, spread):
         for top_p in (0.5, 0.9, 0.99, 0.999):
             check(x, numbers(64, i), least=0.5, temperature=(1.0, 1.3)[i % 2], top_k=top_k, top_p=top_p,
                   min_p=0.01 if i % 3 == 2 else 0.0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_crowded_bins(dtype):
+    """Thousands of tokens within one bin, different ones and equal ones, at a small top_k."""
+    g = torch.Generator(DEV).manual_seed(1)
+    for v in (5000, 70000):
+        x = (1 + torch.rand((v,), generator=g, device=DEV) / 100).to(dtype)
+        for top_k in (1, 50, 1023, 1025, 3000):
+            for top_p in (1.0, 0.999, 0.6):
+                check(x, numbers(128), least=0.5, top_k=top_k, top_p=top_p)
+
+
+@gpu
+@pytest.mark.parametrize("more", [dict(top_k=1500), dict(top_k=1100), dict(top_k=1500, top_p=0.97), dict(top_p=0.9), dict(top_p=0.6)])
+@pytest.mark.parametrize("v", [4000, 60000])
+def test_neighbouring_numbers(v, more):
+    """Logits one unit in the last place apart: the first one that does not stay is the next number below the last that does."""
+    x = torch.full((v,), -40.0)
+    place = torch.randperm(v, generator=torch.Generator().manual_seed(2))[:1800]
+    ulp = 2.0 ** -24
+    x[place[:900]] = 1.0
+    x[place[900:]] = 0.75 - torch.arange(900) * ulp
+    check(x.to(DEV), numbers(8192), **more)
 
 
 @gpu
