@@ -41,6 +41,11 @@ inline void weigh_plan(WeighArgs& w, int sms) {
   const int fit = kWeighRows / w.heads;
   const int chunks = (w.most + fit - 1) / fit;
   w.tokens = (w.most + chunks - 1) / chunks;  // chunks of even sizes: a short last one costs as much as a full one
+  // Where more tokens fill up the MMA's rows they cost nothing.
+  int unit = 16;
+  while (unit > 1 && unit / 2 * w.heads % 16 == 0) unit /= 2;
+  const int full = (w.tokens + unit - 1) / unit * unit;
+  if (full <= w.most && full * w.heads <= kWeighRows) w.tokens = full;
   w.cols = (w.tokens * w.heads + 15) / 16 * 16;
   const long long tiles = static_cast<long long>((w.most + w.tokens - 1) / w.tokens) * w.head_parts;
   // Jobs of (keys, part of the rows): enough to even out the SMs, each of at

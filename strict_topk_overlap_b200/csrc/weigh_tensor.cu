@@ -448,8 +448,10 @@ __device__ __forceinline__ void cap_scores(float2 (&s)[kRun / 2], float c1, floa
   }
 }
 
-// MODE: 1 capped scores, 2 biased by distance, 3 both.
-template <typename T, int D, int MODE, bool FEW>
+// MODE: 1 capped scores, 2 biased by distance, 3 both. RAGGED: a tile's rows do not fill the MMA's, which takes them by
+// sixteens. The rows that fill it up are zeros, whose product with an infinite key is NaN: they must not be added.
+// (In one kernel for both, the second form of the sums costs tiles without such rows 4 to 6 %.)
+template <typename T, int D, int MODE, bool FEW, bool RAGGED>
 __global__ void __launch_bounds__(Plan<D, FEW>::kThreads, 1)
 weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap qmap) {
   using P = Plan<D, FEW>;
@@ -567,8 +569,7 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
         if (!ok) break;
         Range g{0x7fffffff, 0, 0, 0x7fffffff};
         if (!none) {
-          // A row without weight (its log-sum-exp is -inf), or not there, sees no key. Rows that only fill up the
-          // MMA's are zeros with a log-sum-exp of infinity.
+          // A row without weight (its log-sum-exp is -inf), or not there, sees no key.
 #pragma unroll
           for (int j = 0; j < kPasses; ++j) {
             const int row = j * 32 + lane;
@@ -729,7 +730,7 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
     const int mine = half * 128 + (warp & 3) * 32;  // first of the warp's keys in the job
     const uint32_t ts = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * 128;
     const float c = (MODE & 1) ? a.scale / a.softcap : a.scale * kLog2e, cap2 = a.softcap * kLog2e;
-    const int cols = w.cols;
+    const int cols = w.cols, used = w.tokens * w.heads;
     float2 sum = make_float2(0.f, 0.f);
     int n_info = 0, n_s = 0;
     while (true) {
@@ -764,10 +765,18 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
           float2 s[2][kRun / 2];
           tmem_ld16(ts + buf * P::kBufferCols, reinterpret_cast<uint32_t*>(s[0]));
           auto run = [&](float2 (&x)[kRun / 2], int j) {
+            if (RAGGED && !FEW && WHOLE && j + kRun > used) {  // rows that fill up: scores of 0, log-sum-exps of infinity
+#pragma unroll
+              for (int e = 0; e < kRun / 2; ++e) {
+                x[e].x = j + 2 * e < used ? x[e].x : 0.f;
+                x[e].y = j + 2 * e + 1 < used ? x[e].y : 0.f;
+              }
+            }
             if (MODE & 1) cap_scores(x, c, cap2);
             float4 l4;
 #pragma unroll
             for (int e = 0; e < kRun / 2; ++e) {
+              if (RAGGED && FEW && 2 * e >= used) break;
               if (e % 2 == 0) l4 = *reinterpret_cast<const float4*>(&info.neg_lse[j + 2 * e]);
               const float2 l = e % 2 ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
               float2 y;
@@ -786,6 +795,8 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
                 const int4 k = *reinterpret_cast<const int4*>(&info.keys[j + 2 * e]);
                 y.x = key >= k.x && key < k.y ? y.x : 0.f;
                 y.y = key >= k.z && key < k.w ? y.y : 0.f;
+              } else if (RAGGED && FEW) {
+                y.y = 2 * e + 1 < used ? y.y : 0.f;
               }
               part[e & 1] = add2(part[e & 1], y);
             }
@@ -949,15 +960,21 @@ int encode_query_map(CUtensorMap* map, const WeighArgs& w, int kv_dtype) {
   return r == CUDA_SUCCESS ? 0 : 1;
 }
 
-template <typename T, int D, int MODE, bool FEW>
-int launch_mode(const WeighArgs& w, int sms, const CUtensorMap& km, const CUtensorMap& qm, cudaStream_t stream) {
+template <typename T, int D, int MODE, bool FEW, bool RAGGED>
+int launch_kernel(const WeighArgs& w, int sms, const CUtensorMap& km, const CUtensorMap& qm, cudaStream_t stream) {
   constexpr int bytes = sizeof(Shared<D, FEW>);
   static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
-  auto kern = weigh_tensor_kernel<T, D, MODE, FEW>;
+  auto kern = weigh_tensor_kernel<T, D, MODE, FEW, RAGGED>;
   const int rc = static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   if (rc) return rc;
   kern<<<sms, Plan<D, FEW>::kThreads, bytes, stream>>>(w, km, qm);
   return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, int D, int MODE, bool FEW>
+int launch_mode(const WeighArgs& w, int sms, const CUtensorMap& km, const CUtensorMap& qm, cudaStream_t stream) {
+  if (FEW || w.tokens * w.heads < w.cols) return launch_kernel<T, D, MODE, FEW, true>(w, sms, km, qm, stream);
+  return launch_kernel<T, D, MODE, FEW, FEW>(w, sms, km, qm, stream);
 }
 
 template <typename T, int D, bool FEW>

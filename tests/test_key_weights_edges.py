@@ -1,0 +1,57 @@
+"""Key weights at single infinite elements of keys."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import eviction as E
+from oracle import paged_dense as O
+from test_paged_attention import _cache, _ints
+
+gpu = pytest.mark.gpu
+DEV = "cuda"
+BF, HALF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HALF, 64), (F32, 128), (F32, 96)])
+@pytest.mark.parametrize("hq", [2, 8, 14, 32])
+@pytest.mark.parametrize("new", [1, 3, 30, 200])
+@pytest.mark.parametrize("more", [dict(), dict(softcap=20.0), dict(slopes=True), dict(softcap=20.0, slopes=True)])
+def test_one_infinite_element(dtype, d, hq, new, more):
+    """A key with one infinite element weighs nothing where all scores are -inf, infinitely much where some are +inf, and what
+    the cap says where there is one. Bounds as in test_paged_eviction.py; an infinite score is capped without an error."""
+    from strict_topk_overlap_b200 import paged_eviction
+    hkv, n = 2, 400
+    cache = _cache([n], hkv, d, 32, 16, dtype, 5)
+    g = torch.Generator(DEV).manual_seed(6)
+    q = torch.randn((new, hq, d), generator=g, device=DEV)
+    q[..., 0] = -q[..., 0].abs() - 0.1  # all below zero, all above, some of either sign
+    q[..., 1] = q[..., 1].abs() + 0.1
+    q[..., 2] = torch.where(q[..., 2] == 0, 1.0, q[..., 2])
+    q = q.to(dtype)
+    infinite = {5: (0, 1.0), 40: (1, 1.0), 77: (2, 1.0), 100: (2, -1.0), 130: (1, -1.0), 190: (0, -1.0)}
+    for key, (dim, sign) in infinite.items():
+        cache.k_pages[cache.page_table[key // 16].long(), :, key % 16, dim] = sign * float("inf")
+    lse = 5 + torch.rand((new, hq), generator=g, device=DEV)
+    args = dict(softcap=more.get("softcap", 0.0),
+                slopes=torch.tensor([2.0 ** (-8.0 * (h + 1) / hq) for h in range(hq)], device=DEV) if more.get("slopes") else None)
+    offsets = dict(token_offsets=_ints([0, new]), max_tokens=new) if new > 1 else {}
+    got = paged_eviction.accumulate_weights(paged_eviction.empty_weights(cache), q, cache, _ints([n]), lse, **args, **offsets)
+    k = O.gather(cache.k_pages, cache.page_table, cache.block_offsets.tolist(), 32, 16, 0, n)
+    pos = list(range(n - new, n))
+    want, by_size, by_score = E.key_weights(q, k, lse, [0] * new, [p + 1 for p in pos], pos, scale=d ** -0.5, **args)
+    got = got.view(hkv, -1)[:, :n].double()
+    keys = list(infinite)
+    assert torch.equal(got.isnan(), want.isnan()) and not bool(want.isnan().any())
+    assert torch.equal(got.isinf(), want.isinf())
+    if args["softcap"]:
+        by_size[:, keys] = 0
+        assert bool((want[:, keys] > 0).all())
+    else:
+        assert bool((got[:, [5, 130]] == 0).all()) and bool(got[:, [40, 190]].isinf().all())
+    live = want.isfinite() & (want != 0)
+    tol = (d + 16) * 2.0 ** -24 * by_size + (8 if args["softcap"] else 4) * 2.0 ** -24 * by_score + (2.0 ** -21 + 128 * 2.0 ** -24) * want
+    off_by = (got - want).abs()
+    assert bool((off_by <= tol)[live].all()), (off_by / want)[live].max()
+    assert torch.equal(got == 0, want == 0)
