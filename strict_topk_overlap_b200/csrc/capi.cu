@@ -36,6 +36,7 @@ int fail(int code, const char* fmt, ...) {
 
 int cuda_status(int rc, const char* what) {
   if (rc > 0) {
+    cudaGetLastError();  // not left for the next call's launch to report
     g_err = std::string(what) + ": " + cudaGetErrorString(static_cast<cudaError_t>(rc));
   } else if (rc < 0) {
     g_err = std::string(what) + ": per-row sizes exceed the kernel plan";
@@ -1167,10 +1168,10 @@ extern "C" int stk_accumulate_weights(const stk_kv* kv, int pages, const void* q
   }
   if (w.parts > 1) w.partial = reinterpret_cast<float*>(at);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int r2 = 1;
+  int r2 = kWeighNoMap;
   if (weigh_tensor_takes(kv->kv_dtype, kv->d, kv->page_size, kv->k, q, q_token_stride, q_head_stride))
     r2 = launch_weigh_tensor(w, kv->kv_dtype, sm_count_current(), st);
-  if (r2 == 1) r2 = launch_weigh_rows(w, kv->kv_dtype, st);
+  if (r2 == kWeighNoMap) r2 = launch_weigh_rows(w, kv->kv_dtype, st);
   return cuda_status(r2, "accumulate_weights");
 }
 

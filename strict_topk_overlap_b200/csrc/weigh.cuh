@@ -74,7 +74,7 @@ __host__ __device__ inline long long weigh_range_at(int t0, int r, int tokens) {
 
 int launch_weigh_rows(const WeighArgs& w, int kv_dtype, cudaStream_t stream);
 bool weigh_tensor_takes(int kv_dtype, int d, int page_size, const void* k, const void* q, long long q_ts, long long q_hs);
-// 1: the queries' strides do not fit a tensor map, nothing was launched.
+constexpr int kWeighNoMap = -1000;  // (no CUDA error's number) the queries' strides do not fit a tensor map, nothing was launched
 int launch_weigh_tensor(const WeighArgs& w, int kv_dtype, int sms, cudaStream_t stream);
 int set_wait_limit_weigh(unsigned long long ns);
 

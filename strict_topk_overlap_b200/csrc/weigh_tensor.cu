@@ -957,7 +957,7 @@ int encode_query_map(CUtensorMap* map, const WeighArgs& w, int kv_dtype) {
                         const_cast<void*>(a.q), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : 1;
+  return r == CUDA_SUCCESS ? 0 : kWeighNoMap;
 }
 
 template <typename T, int D, int MODE, bool FEW, bool RAGGED>
@@ -1010,20 +1010,18 @@ int launch_weigh_tensor(const WeighArgs& w, int kv_dtype, int sms, cudaStream_t 
   if (rc) return rc;
   rc = encode_query_map(&qm, w, kv_dtype);
   if (rc) return rc;
+  const int tiles = (w.longest + 255) / 256;
+  const long long ctas = static_cast<long long>(w.a.R) * w.parts, joins = static_cast<long long>(tiles) * w.a.L.hkv * w.a.R;
+  if ((w.partial && joins > 0x7fffffff) || (w.ranges && ctas > 0x7fffffff)) return static_cast<int>(cudaErrorInvalidValue);
   if (w.ranges) {
-    const long long ctas = static_cast<long long>(w.a.R) * w.parts;
-    if (ctas > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
     weigh_ranges_kernel<<<static_cast<unsigned>(ctas), 256, 0, stream>>>(w);
     rc = static_cast<int>(cudaGetLastError());
     if (rc) return rc;
   }
   rc = kv_dtype == kBF16 ? launch_t<__nv_bfloat16>(w, sms, km, qm, stream) : launch_t<__half>(w, sms, km, qm, stream);
   if (rc || !w.partial) return rc;
-  const int tiles = (w.longest + 255) / 256;
-  const long long ctas = static_cast<long long>(tiles) * w.a.L.hkv * w.a.R;
-  if (ctas > 0x7fffffff) return static_cast<int>(cudaErrorInvalidValue);
   const auto join = w.few ? weigh_join_kernel<128> : weigh_join_kernel<256>;
-  join<<<static_cast<unsigned>(ctas), 256, 0, stream>>>(w, tiles);
+  join<<<static_cast<unsigned>(joins), 256, 0, stream>>>(w, tiles);
   return static_cast<int>(cudaGetLastError());
 }
 

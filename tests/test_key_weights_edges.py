@@ -1,4 +1,4 @@
-"""Key weights at single infinite elements of keys."""
+"""Key weights at single infinite elements of keys, and what the calls return."""
 from __future__ import annotations
 
 import pytest
@@ -55,3 +55,34 @@ def test_one_infinite_element(dtype, d, hq, new, more):
     off_by = (got - want).abs()
     assert bool((off_by <= tol)[live].all()), (off_by / want)[live].max()
     assert torch.equal(got == 0, want == 0)
+
+
+@gpu
+def test_errors_are_returned():
+    """A call that CUDA refuses (here: a pool of more rows than a tensor map takes) is not run by another kernel instead."""
+    from strict_topk_overlap_b200 import _lib as L
+    cache = _cache([100], 4, 64, 32, 16, BF, 3)
+    kv = cache.packed_kv(4, 64)
+    q = torch.randn((1, 8, 64), device=DEV).to(BF)
+    lse, weights = torch.zeros((1, 8), device=DEV), torch.zeros((4, 4, 32), device=DEV)
+    lengths, lib = _ints([100]), L.load()
+
+    def call(pages):
+        return lib.stk_accumulate_weights(kv, pages, q.data_ptr(), 512, 64, 1, 1, 8, 4, lengths.data_ptr(), None, 1, 128, None,
+                                          lse.data_ptr(), weights.data_ptr(), None, 0, None, L.raw_stream(0))
+
+    assert call(2 ** 31 - 1) != 0  # (the table names pages of the real pool)
+    assert lib.stk_last_error() and not bool(weights.any())
+    assert call(cache.k_pages.shape[0]) == 0 and bool(weights.any())
+
+
+@gpu
+def test_queries_that_no_tensor_map_takes():
+    """Tokens further apart than a tensor map's strides: the same weights by the other kernel."""
+    from strict_topk_overlap_b200 import paged_eviction
+    cache = _cache([100], 2, 64, 32, 16, BF, 4)
+    q = torch.randn((1, 8, 64), generator=torch.Generator(DEV).manual_seed(2), device=DEV).to(BF)
+    lse = torch.full((1, 8), 4.0, device=DEV)
+    weigh = lambda x: paged_eviction.accumulate_weights(paged_eviction.empty_weights(cache), x, cache, _ints([100]), lse)  # noqa: E731
+    want, got = weigh(q), weigh(q.as_strided((1, 8, 64), (2 ** 40, 64, 1)))
+    assert bool(want.any()) and bool(((got - want).abs() <= 1e-5 * want).all())
