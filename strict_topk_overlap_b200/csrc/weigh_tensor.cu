@@ -643,14 +643,15 @@ weigh_tensor_kernel(const WeighArgs w, const __grid_constant__ CUtensorMap kmap,
       if (copies_k && it.first) {
         const unsigned key = it.k0 + lane * bp;
         int page = a.pages, y = static_cast<int>(key % ps / 8);
-        if (lane < boxes && static_cast<int>(key) < it.keys_hi && static_cast<int>(key) + bp > it.keys_lo)
+        const bool named = lane < boxes && static_cast<int>(key) < it.keys_hi && static_cast<int>(key) + bp > it.keys_lo;
+        if (named)
           page = a.L.page_table[static_cast<long long>(it.block0) * ppb + key / ps];
         const int ks = it.k % P::kKRing;
         if (it.k >= P::kKRing) ok = warp_wait(&sh.k_empty[ks], (it.k / P::kKRing - 1) & 1, a.status);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&sh.k_full[ks], P::kKBytes);
         __syncwarp();
-        if (page < 0 || page > a.pages) {  // reads as zeros
+        if (named && (page < 0 || page >= a.pages)) {  // reads as zeros
           report(a.status, kStatusBadBlockId);
           page = a.pages;
         }

@@ -1,4 +1,5 @@
-"""Key weights at single infinite elements of keys, and what the calls return."""
+"""Key weights at single infinite elements of keys, and what the calls return
+and report."""
 from __future__ import annotations
 
 import pytest
@@ -11,6 +12,15 @@ from test_paged_attention import _cache, _ints
 gpu = pytest.mark.gpu
 DEV = "cuda"
 BF, HALF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture
+def status():
+    from strict_topk_overlap_b200 import _lib as L
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    L.set_status_tensor(word)
+    yield word
+    L.set_status_tensor(None)
 
 
 @gpu
@@ -86,3 +96,24 @@ def test_queries_that_no_tensor_map_takes():
     weigh = lambda x: paged_eviction.accumulate_weights(paged_eviction.empty_weights(cache), x, cache, _ints([100]), lse)  # noqa: E731
     want, got = weigh(q), weigh(q.as_strided((1, 8, 64), (2 ** 40, 64, 1)))
     assert bool(want.any()) and bool(((got - want).abs() <= 1e-5 * want).all())
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new", [1, 40])
+def test_the_first_page_behind_the_pool(status, dtype, new):
+    """A table entry that equals the number of pages is outside the pool like any other."""
+    from strict_topk_overlap_b200 import paged_eviction
+    cache = _cache([100, 70], 2, 128, 32, 16, dtype, 2)
+    q = torch.randn((2 * new, 8, 128), generator=torch.Generator(DEV).manual_seed(1), device=DEV).to(dtype)
+    lse = torch.full((2 * new, 8), 8.0, device=DEV)
+    more = dict(token_offsets=_ints([0, new, 2 * new]), max_tokens=new) if new > 1 else {}
+
+    def weigh():
+        return paged_eviction.accumulate_weights(paged_eviction.empty_weights(cache), q, cache, _ints([100, 70]), lse, **more)
+
+    good = weigh()
+    assert status.item() == 0
+    cache.page_table[1] = cache.k_pages.shape[0]
+    got = weigh()
+    assert status.item() == 2
+    assert torch.equal(got[:, 4:], good[:, 4:]) and torch.equal(got[:, 0, :16], good[:, 0, :16])
