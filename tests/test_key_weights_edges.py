@@ -1,5 +1,5 @@
-"""Key weights at single infinite elements of keys, and what the calls return
-and report."""
+"""Key weights at single infinite elements of keys and in long sums, and what the
+calls return and report."""
 from __future__ import annotations
 
 import pytest
@@ -117,3 +117,20 @@ def test_the_first_page_behind_the_pool(status, dtype, new):
     got = weigh()
     assert status.item() == 2
     assert torch.equal(got[:, 4:], good[:, 4:]) and torch.equal(got[:, 0, :16], good[:, 0, :16])
+
+@gpu
+@pytest.mark.parametrize("hq,hkv,d", [(12, 1, 64), (4, 2, 72)])
+def test_long_sums(hq, hkv, d):
+    """Thousands of rows on the FP32 units: sums of 64 rows of a warp, then in FP64. Rows that all weigh 0.1 are what a single
+    FP32 sum is worst at: its roundings all go the same way."""
+    from strict_topk_overlap_b200 import paged_eviction
+    n = 4100
+    cache = _cache([n], hkv, d, 32, 16, F32, 7)
+    q = torch.zeros((n, hq, d), device=DEV)
+    lse = torch.full((n, hq), 2.302585, device=DEV)
+    got = paged_eviction.accumulate_weights(paged_eviction.empty_weights(cache), q, cache, _ints([n]), lse,
+                                            token_offsets=_ints([0, n]), max_tokens=n).view(hkv, -1)[:, :n].double()
+    want = (hq // hkv) * torch.arange(n, 0, -1, device=DEV).double() * torch.exp(-lse[0, 0].double())
+    # 4 roundings of |s| + |lse|, the exponential, 64 additions of a run, and 4 roundings of what the warps' sums become.
+    tol = (4 * 2.302585 * 2.0 ** -24 + 2.0 ** -21 + 68 * 2.0 ** -24) * want
+    assert bool(((got - want).abs() <= tol).all()), ((got - want).abs() / want).max()
