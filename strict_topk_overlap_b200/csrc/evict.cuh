@@ -46,7 +46,7 @@ inline void evict_plan(EvictArgs& a, int kv_dtype, int piece) {
   a.segments = (row + kEvictSegment - 1) / kEvictSegment;
   a.chunk = 1;
   while (a.chunk < 32 && a.L.b % (2 * a.chunk) == 0) a.chunk *= 2;
-  a.chunks = (a.keep + a.chunk - 1) / a.chunk;
+  a.chunks = a.keep / a.chunk + (a.keep % a.chunk != 0);
 }
 
 int launch_evict_select(const EvictArgs& a, int sms, cudaStream_t stream);

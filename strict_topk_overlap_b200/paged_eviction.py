@@ -111,6 +111,14 @@ def accumulate_weights(weights, q, cache: PagedKVCache, lengths, lse, *, token_o
     return weights
 
 
+def _kept(keep):
+    """The number of tokens that stay, as the library takes it."""
+    keep = int(keep)
+    if not 1 <= keep < 2 ** 31:
+        raise ValueError(f"keep = {keep} must be positive and fit into 32 bits")
+    return keep
+
+
 @lru_cache(maxsize=1024)
 def _evict_bytes(device, dtype, hkv, block, dim, page, requests, blocks, keep, longest):
     any_pool = 256
@@ -121,9 +129,9 @@ def _evict_bytes(device, dtype, hkv, block, dim, page, requests, blocks, keep, l
 
 def evict_workspace(cache: PagedKVCache, keep):
     """Workspace for ``evict`` down to ``keep`` tokens."""
-    pool = cache.k_pages
+    pool, keep = cache.k_pages, _kept(keep)
     need = _evict_bytes(pool.get_device(), L.dtype_code(pool), cache.hkv, cache.block_size, cache.dim, cache.page_size,
-                        cache.requests, _slots(cache), int(keep), cache.max_blocks * cache.block_size)
+                        cache.requests, _slots(cache), keep, cache.max_blocks * cache.block_size)
     return torch.empty((need,), device=pool.device, dtype=torch.uint8)
 
 
@@ -146,8 +154,8 @@ def evict(cache: PagedKVCache, weights, lengths, keep, *, first=0, last=0, weigh
     kv = cache.packed_kv(hkv, d)
     requests, blocks, block = cache.block_offsets.shape[0] - 1, _slots(cache), cache.block_size
     held = _ints(lengths, (requests,), "lengths", index)
-    keep, longest = int(keep), cache.max_blocks * block
-    if keep < 1 or first < 0 or last < 0 or first + last > keep:
+    keep, longest = _kept(keep), cache.max_blocks * block
+    if first < 0 or last < 0 or first + last > keep:
         raise ValueError(f"keep = {keep} must hold the first {first} and the last {last} tokens")
     source = _weights(weights, (hkv, blocks, block), "weights", index)
     goal = source if weights_out is None else _weights(weights_out, (hkv, blocks, block), "weights_out", index)
