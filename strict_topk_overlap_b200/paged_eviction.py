@@ -32,7 +32,7 @@ def _slots(cache):
 def empty_weights(cache: PagedKVCache) -> torch.Tensor:
     """Zero weights for every token slot of the cache: FP32 [Hkv, blocks, block_size], block
     block_offsets[r] + j // block_size holding the key j of request r."""
-    return torch.zeros((cache.hkv, _slots(cache), cache.block_size), device=cache.k_pages.device)
+    return torch.zeros((cache.hkv, _slots(cache), cache.block_size), dtype=torch.float32, device=cache.k_pages.device)
 
 
 def _weights(x, shape, name, index):

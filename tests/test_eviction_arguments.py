@@ -23,3 +23,14 @@ def test_more_tokens_than_32_bits_hold(monkeypatch, keep):
         paged_eviction.evict(_cache(_on_device), weights, lengths, keep)
     with pytest.raises(ValueError, match="keep"):
         paged_eviction.evict_workspace(_cache(_on_device), keep)
+
+
+@pytest.mark.parametrize("kind", [torch.float64, torch.bfloat16])
+def test_weights_are_fp32_whatever_the_default(kind):
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(kind)
+    try:
+        weights = paged_eviction.empty_weights(_cache())
+    finally:
+        torch.set_default_dtype(before)
+    assert weights.dtype is torch.float32 and weights.shape == (2, 4, 32)
