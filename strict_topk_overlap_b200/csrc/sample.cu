@@ -695,8 +695,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
 
 template <typename T>
 int launch(const SampleArgs& a, int sms, cudaStream_t stream) {
-  // CTAs of a row: as many as its logits need, more while they find SMs and 16 K logits each (fewer pay less for a
-  // pass than they pay for meeting).
+  // CTAs of a row: as many as its logits need, more while they find SMs and 16 K logits each. One FP32 row of 32,001
+  // takes 16.4 us by the two CTAs of this rule (by one 20.5, four 14.4, eight 14.4 to 17.0) with top_k 50 and top_p 0.9,
+  // 28.7 (36.9, 24.6, 25.5) with top_p 0.95 alone; one of 131,072 33 to 34 by its eight (39 by four).
   constexpr int kSlice = kSampleBytes / static_cast<int>(sizeof(T));
   int parts = 1;
   while (parts * kSlice < a.V) parts *= 2;

@@ -49,6 +49,9 @@
 // rows all see all of a warp's keys need no mask. Unseen keys may hold
 // anything: each key is a lane of its own, selected, never multiplied. Boxes
 // of keys that no row of the job sees are not looked up and read as zeros.
+// Rows that only fill up the MMA's sixteens are left out of the sums, by kernels
+// of their own (drafts of 5 tokens of 4 heads: 64 us with them, NaN at infinite
+// keys, 68.5 without; where more tokens fit into these rows there are none).
 
 #include "paged_tensor.cuh"
 #include "tcgen05.cuh"
@@ -407,8 +410,11 @@ struct Walk {
   }
 };
 
-// tanh for capped scores: odd polynomials (fitted for the least relative
-// error: 2.5e-9 up to 0.25, 4.2e-9 up to 1), 1 - 2 / (1 + e^2x) beyond, whose
+// tanh for capped scores. A score's error is the weight's relative error, and
+// weights are FP32: attention's shorter polynomials (4e-7, for 16-bit outputs)
+// would add up to 2e-5 of a weight under a cap of 50 to what the log-sum-exps
+// carry of theirs. Odd polynomials (fitted for
+// the least relative error: 2.5e-9 up to 0.25, 4.2e-9 up to 1), 1 - 2 / (1 + e^2x) beyond, whose
 // absolute error of about 2^-23 is a rounding of the result there.
 __device__ constexpr float kTanh4[4] = {0.999999998f, -0.333332066f, 0.133231367f, -0.0513280764f};
 __device__ constexpr float kTanh8[8] = {0.999999996f,  -0.333332787f,  0.133321604f,  -0.0538709451f,
