@@ -97,6 +97,7 @@ def test_queries_that_no_tensor_map_takes():
     want, got = weigh(q), weigh(q.as_strided((1, 8, 64), (2 ** 40, 64, 1)))
     assert bool(want.any()) and bool(((got - want).abs() <= 1e-5 * want).all())
 
+
 @gpu
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("new", [1, 40])
@@ -117,6 +118,7 @@ def test_the_first_page_behind_the_pool(status, dtype, new):
     got = weigh()
     assert status.item() == 2
     assert torch.equal(got[:, 4:], good[:, 4:]) and torch.equal(got[:, 0, :16], good[:, 0, :16])
+
 
 @gpu
 @pytest.mark.parametrize("hq,hkv,d", [(12, 1, 64), (4, 2, 72)])
